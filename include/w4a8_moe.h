@@ -51,6 +51,7 @@ extern "C" {
 /* x dtype selector for w4a8_moe_apply. */
 #define W4A8_DTYPE_F16 0
 #define W4A8_DTYPE_BF16 1
+#define W4A8_DTYPE_E4M3 2   /* block-scaled fp8 operators only */
 
 /* Version of this ABI (bumped on any signature change). */
 W4A8_API int w4a8_abi_version(void);
@@ -333,6 +334,75 @@ W4A8_API int w4a8_moe_mxfp4_apply(const void* x, int x_dtype, int64_t T, int64_t
                                   const int32_t* topk_ids, const int32_t* expert_map,
                                   int64_t num_global_experts, void* out, int out_dtype,
                                   void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---------------------------------------------------------------------------------
+ * Block-scaled fp8 (W8A8) operators: e4m3 weights (E, N, K) with one fp32 scale per 128 x 128
+ * block, (E, ceil(N / 128), ceil(K / 128)), against e4m3 rows (rows, K) with one fp32 scale per
+ * row and 128 values, (rows, ceil(K / 128)). No reference counterpart (the reference serves int4
+ * and E2M1 weights only): the same layers for checkpoints that hold block-scaled fp8 weights.
+ *
+ * Rows are quantised as s = max(absmax / 448, 1e-8), q = e4m3(x * (1 / s)) in fp32 (a NaN counts
+ * for no absmax and stays NaN). Strides are in elements; the last dimension is contiguous.
+ */
+
+/* RMS norm with an optional residual and e4m3 output. z = x + residual rounded to x's type (x
+ * without a residual), y = z / sqrt(mean(z^2) + eps) * weight in fp32. Writes q and scales of y
+ * (one scale per 128 values, or with scale_per_row one a row: (rows, 1)), z to residual_out
+ * (rows, H; with a residual only) and y rounded to x's type to norm_out (rows, H; may be NULL).
+ * weight (H,) has x's type, or fp32 when weight_is_f32. residual_out may be residual or x, and
+ * norm_out x, where their strides are H. */
+W4A8_API int w4a8_rms_norm_quant_fp8(const void* x, int x_dtype, int64_t rows, int64_t H,
+                                     int64_t x_stride, const void* residual,
+                                     int64_t residual_stride, const void* weight,
+                                     int weight_is_f32, float eps, int scale_per_row,
+                                     void* residual_out, void* norm_out, uint8_t* q,
+                                     float* scales, void* stream);
+
+/* e4m3 rows and scales of x (rows, K) fp16 / bf16, or with silu_gate_up of silu(gate) * up of
+ * x = [gate | up] (rows, 2 K), computed in fp32. */
+W4A8_API int w4a8_act_quant_fp8_block(const void* x, int x_dtype, int64_t rows, int64_t K,
+                                      int64_t x_stride, int silu_gate_up, uint8_t* q,
+                                      float* scales, void* stream);
+
+/* Dense product: out (M, N) = rows x weights^T with the block scales, fp32 accumulation. x is e4m3
+ * with x_scales, or fp16 / bf16 rows, which the call quantises as w4a8_act_quant_fp8_block does
+ * (x_scales NULL). K a multiple of 16, rows and weights aligned to 16 bytes; any N.
+ * The workspace may be NULL where its size is 0. */
+W4A8_API size_t w4a8_fp8_block_gemm_workspace_size(int x_dtype, int64_t M, int64_t K);
+W4A8_API int w4a8_fp8_block_gemm(const void* x, int x_dtype, const float* x_scales, int64_t M,
+                                 int64_t K, int64_t x_stride, const uint8_t* w,
+                                 const float* w_scales, int64_t N, void* out, int out_dtype,
+                                 void* workspace, size_t workspace_bytes, void* stream);
+
+/* The product grouped by expert, in the padded sorted layout of w4a8_moe_align_block_size: row r
+ * with slot s = sorted_token_ids[r] < num_slots (and r < num_tokens_post_padded) is x[s / top_k]
+ * (gather != 0; needs num_slots <= x_rows * top_k) or x[r], times the weights of expert
+ * expert_ids[r / block_m], out (P, N). Other rows, and rows of x or experts that do not exist, are
+ * not written. block_m: a multiple of 16 up to 128. */
+W4A8_API int w4a8_moe_fp8_block_gemm(const void* x, const float* x_scales, int64_t x_rows,
+                                     int64_t K, int64_t x_stride, const uint8_t* w,
+                                     const float* w_scales, int64_t E, int64_t N,
+                                     const int32_t* sorted_token_ids, int64_t P,
+                                     const int32_t* expert_ids,
+                                     const int32_t* num_tokens_post_padded, int64_t num_slots,
+                                     int64_t top_k, int64_t block_m, int gather, void* out,
+                                     int out_dtype, void* stream);
+
+/* A whole gated expert layer: align, quantise x (skipped for e4m3 x with x_scales), gemm1 with
+ * SiLU * mul and quantisation of h (fp32 in between), gemm2, reduce over the slots in order with
+ * topk_weights. x (T, H) contiguous -> out (T, H). w13 (E, 2 inter, H) = [gate | up], w2
+ * (E, H, inter); H and inter multiples of 128. topk_ids, expert_map and num_global_experts as in
+ * w4a8_moe_apply. */
+W4A8_API size_t w4a8_moe_fp8_block_workspace_size(int64_t T, int64_t H, int64_t inter, int64_t E,
+                                                  int64_t top_k);
+W4A8_API int w4a8_moe_fp8_block_apply(const void* x, int x_dtype, const float* x_scales,
+                                      int64_t T, int64_t H, int64_t inter, int64_t E,
+                                      int64_t top_k, const uint8_t* w13, const float* w13_scales,
+                                      const uint8_t* w2, const float* w2_scales,
+                                      const float* topk_weights, const int32_t* topk_ids,
+                                      const int32_t* expert_map, int64_t num_global_experts,
+                                      void* out, int out_dtype, void* workspace,
+                                      size_t workspace_bytes, void* stream);
 
 /* Optional per-stage timing of the whole-layer calls on the calling thread: when count >= 8,
  * the next w4a8_moe_apply / _fragments / w4a8_moe_forward calls record events[0] before the

@@ -27,6 +27,14 @@ from ._ops import (  # noqa: F401
     silu_and_mul,
 )
 
+from .fp8_block import (  # noqa: E402,F401  block-scaled fp8 (W8A8) layers
+    act_quant_fp8_block,
+    fp8_block_gemm,
+    moe_fp8_block_apply,
+    moe_fp8_block_gemm,
+    rms_norm_quant_fp8,
+)
+
 _MOE_KERNELS = {"scalar": 0, "wmma": 6, "gemv": 7}
 
 _DENSE_KERNELS = {
@@ -126,4 +134,6 @@ __all__ = [
     "fused_topk",
     "moe_align_block_size", "moe_apply", "moe_forward", "repack_fragments", "set_decode_fused",
     "set_prefill_pair", "silu_and_mul",
+    "act_quant_fp8_block", "fp8_block_gemm", "moe_fp8_block_apply", "moe_fp8_block_gemm",
+    "rms_norm_quant_fp8",
 ]

@@ -81,6 +81,24 @@ SIGNATURES = {
                                     ctypes.c_float, ctypes.c_float, _c_void_p, _c_void_p,
                                     _c_void_p, _i64, _c_void_p, _int, _c_void_p, _size,
                                     _c_void_p]),
+    "w4a8_rms_norm_quant_fp8": (_int, [_c_void_p, _int, _i64, _i64, _i64, _c_void_p, _i64,
+                                       _c_void_p, _int, ctypes.c_float, _int, _c_void_p,
+                                       _c_void_p, _c_void_p, _c_void_p, _c_void_p]),
+    "w4a8_act_quant_fp8_block": (_int, [_c_void_p, _int, _i64, _i64, _i64, _int, _c_void_p,
+                                        _c_void_p, _c_void_p]),
+    "w4a8_fp8_block_gemm_workspace_size": (_size, [_int, _i64, _i64]),
+    "w4a8_fp8_block_gemm": (_int, [_c_void_p, _int, _c_void_p, _i64, _i64, _i64, _c_void_p,
+                                   _c_void_p, _i64, _c_void_p, _int, _c_void_p, _size,
+                                   _c_void_p]),
+    "w4a8_moe_fp8_block_gemm": (_int, [_c_void_p, _c_void_p, _i64, _i64, _i64, _c_void_p,
+                                       _c_void_p, _i64, _i64, _c_void_p, _i64, _c_void_p,
+                                       _c_void_p, _i64, _i64, _i64, _int, _c_void_p, _int,
+                                       _c_void_p]),
+    "w4a8_moe_fp8_block_workspace_size": (_size, [_i64, _i64, _i64, _i64, _i64]),
+    "w4a8_moe_fp8_block_apply": (_int, [_c_void_p, _int, _c_void_p, _i64, _i64, _i64, _i64,
+                                        _i64, _c_void_p, _c_void_p, _c_void_p, _c_void_p,
+                                        _c_void_p, _c_void_p, _c_void_p, _i64, _c_void_p, _int,
+                                        _c_void_p, _size, _c_void_p]),
     "w4a8_set_decode_fused": (_int, [_int]),
     "w4a8_set_prefill_pair": (_int, [_int]),
     "w4a8_decode_fused_test_fault": (_int, [_int]),
