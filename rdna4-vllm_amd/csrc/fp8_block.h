@@ -66,6 +66,7 @@ struct BlockParams {
     int64_t ldx, ldo;
     int P, K, N, G, NB, E;
     int x_rows, top_k, num_valid, block_m, gather;
+    int out8;                    // out is aligned to 8 bytes
 };
 
 inline BlockParams block_params(const BlockArgs& a) {
@@ -78,6 +79,7 @@ inline BlockParams block_params(const BlockArgs& a) {
     p.NB = (int)blk_groups(a.N); p.E = (int)a.E;
     p.x_rows = (int)a.x_rows; p.top_k = (int)a.top_k; p.num_valid = (int)a.num_valid;
     p.block_m = (int)a.block_m; p.gather = a.gather ? 1 : 0;
+    p.out8 = reinterpret_cast<uintptr_t>(a.out) % 8 == 0 ? 1 : 0;
     return p;
 }
 

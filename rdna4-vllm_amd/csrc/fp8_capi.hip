@@ -207,14 +207,13 @@ int w4a8_moe_fp8_block_apply(const void* x, int x_dtype, const float* x_scales, 
     if (int rc = launch_align(topk_ids, T * top_k, E, pl.block_m, expert_map, n_global, m.sti, pl.P, m.eid, m.ntp,
                               m.align_ws, m.align_bytes, s))
         return rc;
-    if (quantise)
-        if (int rc = launch_act_quant_block(x, x_dtype == W4A8_DTYPE_BF16, T, H, H, false, m.xq, m.xs, s)) return rc;
+    // (few rows are quantised in the registers that hold them; so no row is prepared for it here)
     BlockArgs g1{};
-    g1.x = quantise ? m.xq : x; g1.xs = quantise ? m.xs : x_scales; g1.x_rows = T; g1.K = H; g1.ldx = H;
+    g1.x = x; g1.xs = x_scales; g1.x_rows = T; g1.K = H; g1.ldx = H;
     g1.w = w13; g1.ws = w13_scales; g1.E = E; g1.N = 2 * inter;
     g1.sorted_ids = m.sti; g1.expert_ids = m.eid; g1.ntp = m.ntp; g1.P = pl.P;
     g1.top_k = top_k; g1.num_valid = T * top_k; g1.block_m = pl.block_m; g1.gather = true;
-    g1.src = Src::kFp8; g1.dst = Dst::kSiluF32; g1.out = m.h; g1.ldo = inter;
+    g1.src = src_of(x_dtype); g1.dst = Dst::kSiluF32; g1.out = m.h; g1.ldo = inter;
     if (int rc = launch_block_stream(g1, s)) return rc;
     BlockArgs g2 = g1;
     g2.x = m.h; g2.xs = nullptr; g2.x_rows = pl.P; g2.K = inter; g2.ldx = inter;

@@ -1,13 +1,15 @@
-// Block-scaled fp8 products that stream the weights (gfx950 fp8 MFMA): few rows, dense or grouped.
+// Block-scaled fp8 products of few rows (gfx950): the weights are streamed once, dense or grouped.
 //
-// A work-group owns 16 FT rows and 16 FN columns; its waves take the K groups in turn (wave w the
-// groups w, w + waves, ...: what they read at one time is contiguous along K) and add their sums in
-// LDS, in wave order. Weights and e4m3 rows go from memory to the MFMA operands' registers with no
-// detour: of each group of 128 values, lane (q, c) = (lane / 16, lane % 16) holds the 16-byte pieces
-// q and q + 4 of row c, for rows and weights alike, so a load instruction touches 64 contiguous bytes
-// of sixteen rows. Weights are the first operand: a lane ends up with four adjacent columns of one row,
-// and the scale xs[row, g] * ws[block, g] is one number a lane and group.
-// Bound: HBM (every weight once per 16 FT rows).
+// Bound: HBM, every weight once per 16 FT rows. Weights go from memory to the MFMA operands' registers
+// with no detour: of each group of 128 values, lane (q, c) = (lane / 16, lane % 16) holds the 16-byte
+// pieces q and q + 4 of row c, for rows and weights alike, so a load instruction touches 64 contiguous
+// bytes of sixteen rows. Weights are the first operand: a lane ends up with four adjacent columns of
+// one row, and the scale xs[row, g] * ws[block, g] is one number a lane and group.
+//
+// block_rows_kernel holds its rows in registers (16 FT rows by GPW groups a wave, quantised there
+// where they come in 16 or 32 bits) and walks over column fragments with D of them in flight; KS
+// waves share K and add their sums in LDS, one barrier per D fragments. block_stream_kernel takes any
+// K and reads the rows again for each column fragment.
 #include <algorithm>
 #include <type_traits>
 
@@ -16,25 +18,313 @@
 namespace w4a8 {
 namespace {
 
-constexpr int kRing = 3;          // groups of a wave in flight
+using v8h = _Float16 __attribute__((ext_vector_type(8)));
 
-template <int FT, int FN, int KS, Src SRC, Dst DST, bool TAIL>
-__global__ void __launch_bounds__(64 * KS) block_stream_kernel(BlockParams p, int slices) {
-    // kSiluF32: the column fragments are FN / 2 of the gate half and the matching ones of the up half
+// The row operand of one group: a lane's 32 values as e4m3 bytes, or (EXACT) as fp16.
+template <bool EXACT>
+struct RowOp {
+    v8i b;
+};
+template <>
+struct RowOp<true> {
+    v8h h[4];
+};
+
+__device__ __forceinline__ v8h e4m3_to_half8(int lo, int hi) {
+    typedef _Float16 v2h __attribute__((ext_vector_type(2)));
+    const v2h a = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.0f, false);
+    const v2h b = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.0f, true);
+    const v2h c = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.0f, false);
+    const v2h d = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.0f, true);
+    return v8h{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+
+// Sum over one group of 128 k. The fp8 matrix core cuts products of eight neighbouring k to 2^-13 of
+// their largest; EXACT feeds the fp16 one (every e4m3 number is an fp16 number), which adds them as
+// fp32 numbers, at a quarter of the rate and for sixteen conversions. It is for sums that are
+// quantised again: an error of 1e-4 there moves values across a border between two e4m3 numbers, and
+// the layer's output by 1e-3 (one token up to 6e-3), three times what the rounding to bf16 does.
+template <bool EXACT>
+__device__ __forceinline__ v4f group_dot(const u32x4& w0, const u32x4& w1, const RowOp<EXACT>& x) {
+    const v4f zero{0.f, 0.f, 0.f, 0.f};
+    if constexpr (EXACT) {
+        v4f t = __builtin_amdgcn_mfma_f32_16x16x32_f16(e4m3_to_half8(w0[0], w0[1]), x.h[0], zero, 0, 0, 0);
+        t = __builtin_amdgcn_mfma_f32_16x16x32_f16(e4m3_to_half8(w0[2], w0[3]), x.h[1], t, 0, 0, 0);
+        t = __builtin_amdgcn_mfma_f32_16x16x32_f16(e4m3_to_half8(w1[0], w1[1]), x.h[2], t, 0, 0, 0);
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(e4m3_to_half8(w1[2], w1[3]), x.h[3], t, 0, 0, 0);
+    } else {
+        const v8i w{(int)w0[0], (int)w0[1], (int)w0[2], (int)w0[3], (int)w1[0], (int)w1[1], (int)w1[2], (int)w1[3]};
+        return mfma_16x16x128(w, x.b, zero);
+    }
+}
+
+// Raw bytes of a row's 32 values of one group, as loaded.
+template <Src SRC>
+constexpr int kSrcBytes = SRC == Src::kFp8 ? 1 : SRC == Src::kF32 ? 4 : 2;
+template <Src SRC>
+struct RowRaw {
+    u32x4 v[2 * kSrcBytes<SRC>];
+};
+// xp: the lane's row; absent pieces read the last one and are zeroed in row_operand.
+template <Src SRC>
+__device__ __forceinline__ void row_load(RowRaw<SRC>& r, const uint8_t* xp, int g, int q, int K) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const int k = min(g * kBlk + h * 64 + q * 16, K - 16);
+#pragma unroll
+        for (int b = 0; b < kSrcBytes<SRC>; ++b)
+            r.v[h * kSrcBytes<SRC> + b] = *reinterpret_cast<const u32x4*>(xp + (int64_t)k * kSrcBytes<SRC> + 16 * b);
+    }
+}
+// The MFMA operand; rows in 16 or 32 bits are quantised (the group's absmax lies in four lanes).
+template <Src SRC, bool EXACT>
+__device__ __forceinline__ RowOp<EXACT> row_operand(const RowRaw<SRC>& r, int g, int q, int K, float& xs) {
+    const bool in[2] = {g * kBlk + q * 16 < K, g * kBlk + 64 + q * 16 < K};
+    int o[8];
+    if constexpr (SRC == Src::kFp8) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int d = 0; d < 4; ++d) o[4 * h + d] = in[h] ? (int)r.v[h][d] : 0;
+    } else {
+        float f[2][16];
+        float m = 0.f;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+#pragma unroll
+            for (int t = 0; t < 16; ++t) {
+                if constexpr (SRC == Src::kF32) {
+                    f[h][t] = __uint_as_float(r.v[h * 4 + t / 4][t % 4]);
+                } else {
+                    const uint32_t u = r.v[h * 2 + t / 8][(t / 2) % 4];
+                    if constexpr (SRC == Src::kBf16)
+                        f[h][t] = __uint_as_float((t & 1) ? u & 0xFFFF0000u : u << 16);
+                    else
+                        f[h][t] = __half2float(__ushort_as_half((uint16_t)((t & 1) ? u >> 16 : u & 0xFFFF)));
+                }
+                f[h][t] = in[h] ? f[h][t] : 0.f;
+                m = fmaxf(m, fabsf(f[h][t]));
+            }
+        }
+        xs = act_scale_from_absmax(rows4_max(m));
+        const float inv = 1.0f / xs;
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int d = 0; d < 4; ++d)
+                o[4 * h + d] = (int)pack4_e4m3(f[h][4 * d] * inv, f[h][4 * d + 1] * inv, f[h][4 * d + 2] * inv,
+                                               f[h][4 * d + 3] * inv);
+    }
+    RowOp<EXACT> x;
+    if constexpr (EXACT) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x.h[i] = e4m3_to_half8(o[2 * i], o[2 * i + 1]);
+    } else {
+        x.b = v8i{o[0], o[1], o[2], o[3], o[4], o[5], o[6], o[7]};
+    }
+    return x;
+}
+
+// Four adjacent columns of one row.
+template <Dst DST>
+__device__ __forceinline__ void store4(const BlockParams& p, int64_t orow, int col, int cols, const v4f& t) {
+    if constexpr (DST == Dst::kSlotF32 || DST == Dst::kSiluF32) {
+        // (whole layers: multiples of 128 columns)
+        *reinterpret_cast<v4f*>(reinterpret_cast<float*>(p.out) + orow * p.ldo + col) = t;
+    } else {
+        uint16_t* o = reinterpret_cast<uint16_t*>(p.out) + orow * p.ldo + col;
+        constexpr bool bf16 = DST == Dst::kBf16;
+        const uint32_t a = pack_out16(t[0], t[1], bf16), b = pack_out16(t[2], t[3], bf16);
+        if (p.ldo % 4 == 0 && p.out8) {
+            *reinterpret_cast<uint2*>(o) = make_uint2(a, b);
+        } else {
+            const uint32_t v[4] = {a & 0xFFFF, a >> 16, b & 0xFFFF, b >> 16};
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                if (col + r < cols) o[r] = (uint16_t)v[r];
+        }
+    }
+}
+
+// The expert and the end of the rows in use of the rows from row0; false: nothing to do.
+__device__ __forceinline__ bool block_expert(const BlockParams& p, int row0, int& e, int& end) {
+    e = 0;
+    end = p.P;
+    if (p.sorted_ids != nullptr) {
+        end = min(p.ntp[0], p.P);
+        if (row0 >= end) return false;
+        e = __builtin_amdgcn_readfirstlane(p.expert_ids[row0 / p.block_m]);
+        if (e < 0 || e >= p.E) return false;
+    }
+    return true;
+}
+
+// CG groups of KS waves; a group walks over its own `per` column fragments (kSiluF32: fragments of
+// the gate half, each with its up fragment), D in flight. part: [2][CG][D][FT][KS][64] v4f in LDS.
+template <int FT, int GPW, int KS, int CG, int D, Src SRC, Dst DST>
+__global__ void __launch_bounds__(64 * KS * CG) block_rows_kernel(BlockParams p, int slices, int per) {
     constexpr bool kSilu = DST == Dst::kSiluF32;
+    constexpr bool EXACT = kSilu;
+    constexpr int kPair = kSilu ? 2 : 1;                       // fragments of one output fragment
+    static_assert(D % kPair == 0, "an output fragment's parts are in flight together");
+    constexpr int kUnits = D / kPair * FT;                     // output fragments of one round
+    __shared__ __attribute__((aligned(16))) v4f part[KS > 1 ? 2 : 1][KS > 1 ? CG : 1][KS > 1 ? D * FT : 1]
+                                                    [KS > 1 ? KS : 1][64];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int ks = wave % KS, cg = wave / KS;
+    const int q = lane >> 4, c = lane & 15;
+    const int tb = blockIdx.x / slices, sl = blockIdx.x % slices;
+    const int row0 = tb * (16 * FT);
+    int e, end;
+    if (!block_expert(p, row0, e, end)) return;
+    const int half = p.N / 2;
+    const int cols = kSilu ? half : p.N;
+    const int K = p.K, G = p.G;
+    const int frags = (cols + 15) / 16;
+    const int f0 = (sl * CG + cg) * per;                       // first output fragment of this group
+    const int g0 = ks * GPW;                                   // first K group of this wave
+
+    // ---- weights: step i is fragment f0 + i / kPair of the gate (i even) or the up half ----
+    const uint8_t* we = p.w + (int64_t)e * p.N * K;
+    const float* wse = p.ws + (int64_t)e * p.NB * G;
+    struct Stage {
+        u32x4 w[GPW][2];
+        float ws[GPW];
+    };
+    auto load = [&](Stage& s, int i) __attribute__((always_inline)) {
+        const int f = min(f0 + i / kPair, frags - 1);
+        const int up = kSilu && (i & 1) ? half : 0;
+        // (columns past the end read the last one; never stored)
+        const uint8_t* wr = we + (int64_t)(up + min(f * 16 + c, cols - 1)) * K;
+        const float* sr = wse + (int64_t)((up + f * 16) / kBlk) * G;
+#pragma unroll
+        for (int i = 0; i < GPW; ++i) {
+            const int g = min(g0 + i, G - 1);
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+                s.w[i][h] = *reinterpret_cast<const u32x4*>(wr + min(g * kBlk + h * 64 + q * 16, K - 16));
+            s.ws[i] = sr[g];
+        }
+    };
+    Stage ring[D];
+#pragma unroll
+    for (int d = 0; d < D; ++d) load(ring[d], d);
+    __builtin_amdgcn_sched_barrier(0);
+
+    // ---- rows, held ----
+    int slot[FT];
+    RowOp<EXACT> x[FT][GPW];
+    float xs[FT][GPW];
+#pragma unroll
+    for (int i = 0; i < FT; ++i) {
+        int xrow;
+        slot[i] = block_slot(p, row0 + 16 * i + c, end, xrow);
+        const uint8_t* xp = reinterpret_cast<const uint8_t*>(p.x) + (int64_t)xrow * p.ldx * kSrcBytes<SRC>;
+        // (some groups' raw bytes at a time: all of them beside the ring would not fit the registers)
+        constexpr int kAt = SRC == Src::kF32 ? (GPW < 2 ? GPW : 2) : GPW < 4 ? GPW : 4;
+        static_assert(GPW % kAt == 0, "groups divide");
+#pragma unroll
+        for (int j0 = 0; j0 < GPW; j0 += kAt) {
+            RowRaw<SRC> raw[kAt];
+#pragma unroll
+            for (int j = 0; j < kAt; ++j) {
+                const int g = min(g0 + j0 + j, G - 1);
+                row_load(raw[j], xp, g, q, K);
+                xs[i][j0 + j] = 0.f;
+                if constexpr (SRC == Src::kFp8) xs[i][j0 + j] = p.xs[(int64_t)xrow * G + g];
+            }
+#pragma unroll
+            for (int j = 0; j < kAt; ++j) {
+                // groups past the end: zero rows and a zero scale (what the clamped addresses hold
+                // counts in its own group)
+                const int g = g0 + j0 + j;
+                x[i][j0 + j] = row_operand<SRC, EXACT>(raw[j], g, q, K, xs[i][j0 + j]);
+                if (g >= G) xs[i][j0 + j] = 0.f;
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    }
+
+    const int mine = min(per, frags - f0);                     // output fragments of this group (may be <= 0)
+    const int rounds = (per * kPair + D - 1) / D;              // of the work-group: the barriers agree
+    for (int it = 0; it < rounds; ++it) {
+        v4f run[D][FT];
+#pragma unroll
+        for (int d = 0; d < D; ++d) {
+#pragma unroll
+            for (int i = 0; i < FT; ++i) {
+                run[d][i] = v4f{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int j = 0; j < GPW; ++j) {
+                    const v4f t = group_dot<EXACT>(ring[d].w[j][0], ring[d].w[j][1], x[i][j]);
+                    const float s = xs[i][j] * ring[d].ws[j];
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) run[d][i][r] = fmaf(t[r], s, run[d][i][r]);
+                }
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            load(ring[d], (it + 1) * D + d);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        // unit u of the round: output fragment u / FT, row fragment u % FT
+        auto put = [&](int u, v4f t, const v4f& up, int sl_id) __attribute__((always_inline)) {
+            const int of = it * (D / kPair) + u / FT;
+            const int col = (f0 + of) * 16 + 4 * q;
+            if constexpr (kSilu) {
+#pragma unroll
+                for (int r = 0; r < 4; ++r) t[r] = silu_mul_f32(t[r], up[r]);
+            }
+            if (of >= mine || sl_id < 0 || col >= cols) return;
+            store4<DST>(p, DST == Dst::kSlotF32 ? sl_id : row0 + 16 * (u % FT) + c, col, cols, t);
+        };
+        if constexpr (KS == 1) {
+#pragma unroll
+            for (int u = 0; u < kUnits; ++u)
+                put(u, run[u / FT * kPair][u % FT], run[u / FT * kPair + kPair - 1][u % FT], slot[u % FT]);
+        } else {
+            auto& buf = part[it & 1][cg];
+#pragma unroll
+            for (int d = 0; d < D; ++d)
+#pragma unroll
+                for (int i = 0; i < FT; ++i) buf[d * FT + i][ks][lane] = run[d][i];
+            lds_barrier();
+            // (the next round writes the other buffer; this one is written again behind its barrier)
+#pragma unroll
+            for (int u0 = 0; u0 < kUnits; u0 += KS) {
+                const int u = u0 + ks;
+                if (kUnits % KS != 0 && u >= kUnits) break;
+                auto total = [&](int d) __attribute__((always_inline)) {
+                    v4f t = buf[d * FT + u % FT][0][lane];
+#pragma unroll
+                    for (int w = 1; w < KS; ++w) t += buf[d * FT + u % FT][w][lane];
+                    return t;
+                };
+                const v4f t = total(u / FT * kPair);
+                int sl_id = slot[0];
+#pragma unroll
+                for (int i = 1; i < FT; ++i)
+                    if (u % FT == i) sl_id = slot[i];
+                if constexpr (kSilu) put(u, t, total(u / FT * kPair + 1), sl_id);
+                else put(u, t, t, sl_id);
+            }
+        }
+    }
+}
+
+// Any K: KS waves take the K groups in turn (what they read at one time is contiguous along K).
+constexpr int kRing = 3;          // groups of a wave in flight
+template <int FT, int FN, int KS, Src SRC, Dst DST>
+__global__ void __launch_bounds__(64 * KS) block_stream_kernel(BlockParams p, int slices) {
+    constexpr bool kSilu = DST == Dst::kSiluF32;
+    constexpr bool EXACT = kSilu;
     constexpr int kCols = kSilu ? FN / 2 : FN;                 // column fragments of the output
     __shared__ __attribute__((aligned(16))) v4f part[KS][FT * FN][64];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int q = lane >> 4, c = lane & 15;
     const int tb = blockIdx.x / slices, sl = blockIdx.x % slices;
     const int row0 = tb * (16 * FT);
-    int e = 0, end = p.P;
-    if (p.sorted_ids != nullptr) {
-        end = min(p.ntp[0], p.P);
-        if (row0 >= end) return;
-        e = p.expert_ids[row0 / p.block_m];
-        if (e < 0 || e >= p.E) return;
-    }
+    int e, end;
+    if (!block_expert(p, row0, e, end)) return;
     const int half = p.N / 2;
     const int cols = kSilu ? half : p.N;
     const int K = p.K, G = p.G;
@@ -43,99 +333,40 @@ __global__ void __launch_bounds__(64 * KS) block_stream_kernel(BlockParams p, in
     const float* wsp[FN];
 #pragma unroll
     for (int j = 0; j < FN; ++j) {
-        // columns past the end read the last one (never stored)
-        const int col = min((sl * kCols + j % kCols) * 16 + c, cols - 1) + (kSilu && j >= kCols ? half : 0);
-        const int blk = min((sl * kCols + j % kCols) * 16, cols - 1) + (kSilu && j >= kCols ? half : 0);
-        wp[j] = p.w + ((int64_t)e * p.N + col) * K;
-        // (kSiluF32 takes halves of whole blocks, and blocks are a multiple of 16 columns)
-        wsp[j] = p.ws + ((int64_t)e * p.NB + blk / kBlk) * G;
+        const int f = (sl * kCols + j % kCols) * 16, up = kSilu && j >= kCols ? half : 0;
+        wp[j] = p.w + ((int64_t)e * p.N + up + min(f + c, cols - 1)) * K;
+        wsp[j] = p.ws + ((int64_t)e * p.NB + (up + min(f, cols - 1)) / kBlk) * G;
     }
-    int slot[FT];
     const uint8_t* xp[FT];
     const float* xsp[FT];
-    constexpr int kBytes = SRC == Src::kFp8 ? 1 : SRC == Src::kF32 ? 4 : 2;
 #pragma unroll
     for (int i = 0; i < FT; ++i) {
         int xrow;
-        slot[i] = block_slot(p, row0 + 16 * i + c, end, xrow);
-        xp[i] = reinterpret_cast<const uint8_t*>(p.x) + (int64_t)xrow * p.ldx * kBytes;
+        block_slot(p, row0 + 16 * i + c, end, xrow);
+        xp[i] = reinterpret_cast<const uint8_t*>(p.x) + (int64_t)xrow * p.ldx * kSrcBytes<SRC>;
         xsp[i] = p.xs + (SRC == Src::kFp8 ? (int64_t)xrow * G : 0);
     }
-
     struct Stage {
         u32x4 w[FN][2];
-        u32x4 x[FT][2 * kBytes];
+        RowRaw<SRC> x[FT];
         float ws[FN];
         float xs[FT];
     };
-    // the group of step i; past the end the last one, whose result is scaled by 0
     auto load = [&](Stage& s, int step) __attribute__((always_inline)) {
         const int g = min(step * KS + wave, G - 1);
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            int k = g * kBlk + h * 64 + q * 16;
-            if constexpr (TAIL) k = min(k, K - 16);
-#pragma unroll
-            for (int j = 0; j < FN; ++j) s.w[j][h] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(wp[j] + k));
-#pragma unroll
-            for (int i = 0; i < FT; ++i)
-#pragma unroll
-                for (int b = 0; b < kBytes; ++b)
-                    s.x[i][h * kBytes + b] = *reinterpret_cast<const u32x4*>(xp[i] + (int64_t)k * kBytes + 16 * b);
-        }
-#pragma unroll
-        for (int j = 0; j < FN; ++j) s.ws[j] = wsp[j][g];
-        if constexpr (SRC == Src::kFp8) {
-#pragma unroll
-            for (int i = 0; i < FT; ++i) s.xs[i] = xsp[i][g];
-        }
-    };
-    // a row's 32 values of this lane as an MFMA operand, and their scale
-    auto operand = [&](const Stage& s, int i, int g, float& xs) __attribute__((always_inline)) {
-        bool in[2] = {true, true};
-        if constexpr (TAIL) {
-            in[0] = g * kBlk + q * 16 < K;
-            in[1] = g * kBlk + 64 + q * 16 < K;
-        }
-        v8i o;
-        if constexpr (SRC == Src::kFp8) {
+        for (int j = 0; j < FN; ++j) {
 #pragma unroll
             for (int h = 0; h < 2; ++h)
-#pragma unroll
-                for (int d = 0; d < 4; ++d) o[4 * h + d] = in[h] ? (int)s.x[i][h][d] : 0;
-            xs = s.xs[i];
-        } else {
-            float f[2][16];
-            float m = 0.f;
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-#pragma unroll
-                for (int t = 0; t < 16; ++t) {
-                    if constexpr (SRC == Src::kF32) {
-                        f[h][t] = __uint_as_float(s.x[i][h * 4 + t / 4][t % 4]);
-                    } else {
-                        const uint32_t u = s.x[i][h * 2 + t / 8][(t / 2) % 4];
-                        if constexpr (SRC == Src::kBf16)
-                            f[h][t] = __uint_as_float((t & 1) ? u & 0xFFFF0000u : u << 16);
-                        else
-                            f[h][t] = __half2float(__ushort_as_half((uint16_t)((t & 1) ? u >> 16 : u & 0xFFFF)));
-                    }
-                    if constexpr (TAIL) f[h][t] = in[h] ? f[h][t] : 0.f;
-                    m = fmaxf(m, fabsf(f[h][t]));
-                }
-            }
-            xs = act_scale_from_absmax(rows4_max(m));
-            const float inv = 1.0f / xs;
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-#pragma unroll
-                for (int d = 0; d < 4; ++d)
-                    o[4 * h + d] = (int)pack4_e4m3(as_f32(f[h][4 * d] * inv), as_f32(f[h][4 * d + 1] * inv),
-                                                   as_f32(f[h][4 * d + 2] * inv), as_f32(f[h][4 * d + 3] * inv));
+                s.w[j][h] = *reinterpret_cast<const u32x4*>(wp[j] + min(g * kBlk + h * 64 + q * 16, K - 16));
+            s.ws[j] = wsp[j][g];
         }
-        return o;
+#pragma unroll
+        for (int i = 0; i < FT; ++i) {
+            row_load(s.x[i], xp[i], g, q, K);
+            if constexpr (SRC == Src::kFp8) s.xs[i] = xsp[i][g];
+        }
     };
-
     v4f run[FT][FN];
 #pragma unroll
     for (int i = 0; i < FT; ++i)
@@ -143,29 +374,20 @@ __global__ void __launch_bounds__(64 * KS) block_stream_kernel(BlockParams p, in
         for (int j = 0; j < FN; ++j) run[i][j] = v4f{0.f, 0.f, 0.f, 0.f};
     auto consume = [&](const Stage& s, int step) __attribute__((always_inline)) {
         const int g = step * KS + wave;
-        v8i wv[FN];
-#pragma unroll
-        for (int j = 0; j < FN; ++j)
-#pragma unroll
-            for (int d = 0; d < 8; ++d) {
-                wv[j][d] = (int)s.w[j][d / 4][d % 4];
-                // both operands of absent pieces are zero: what the clamped address holds may be NaN
-                if constexpr (TAIL) wv[j][d] = g * kBlk + (d / 4) * 64 + q * 16 < K ? wv[j][d] : 0;
-            }
 #pragma unroll
         for (int i = 0; i < FT; ++i) {
-            float xs;
-            const v8i xv = operand(s, i, g, xs);
+            float xs = s.xs[i];
+            const RowOp<EXACT> xv = row_operand<SRC, EXACT>(s.x[i], g, q, K, xs);   // zero past the end
+            if (g >= G) xs = 0.f;
 #pragma unroll
             for (int j = 0; j < FN; ++j) {
-                const v4f t = mfma_16x16x128(wv[j], xv, v4f{0.f, 0.f, 0.f, 0.f});
-                const float sc = g < G ? xs * s.ws[j] : 0.f;
+                const v4f t = group_dot<EXACT>(s.w[j][0], s.w[j][1], xv);
+                const float sc = xs * s.ws[j];
 #pragma unroll
-                for (int r = 0; r < 4; ++r) run[i][j][r] = g < G ? fmaf(t[r], sc, run[i][j][r]) : run[i][j][r];
+                for (int r = 0; r < 4; ++r) run[i][j][r] = fmaf(t[r], sc, run[i][j][r]);
             }
         }
     };
-
     const int steps = (G + KS - 1) / KS;
     Stage ring[kRing];
 #pragma unroll
@@ -179,14 +401,12 @@ __global__ void __launch_bounds__(64 * KS) block_stream_kernel(BlockParams p, in
             __builtin_amdgcn_sched_barrier(0);
         }
     }
-
 #pragma unroll
     for (int i = 0; i < FT; ++i)
 #pragma unroll
         for (int j = 0; j < FN; ++j) part[wave][i * FN + j][lane] = run[i][j];
     __syncthreads();
-    // one unit: four adjacent columns of a row
-    for (int u = tid; u < FT * kCols * 64; u += 64 * KS) {
+    for (int u = tid; u < FT * kCols * 64; u += 64 * KS) {     // four adjacent columns of a row
         const int ln = u & 63, f = u >> 6, i = f / kCols, j = f % kCols;
         auto total = [&](int frag) __attribute__((always_inline)) {
             v4f t = part[0][frag][ln];
@@ -200,48 +420,62 @@ __global__ void __launch_bounds__(64 * KS) block_stream_kernel(BlockParams p, in
 #pragma unroll
             for (int r = 0; r < 4; ++r) t[r] = silu_mul_f32(t[r], up[r]);
         }
-        // the lane that holds row 16 i + ln % 16 in every wave knows its slot
         int xrow;
         const int row = row0 + 16 * i + (ln & 15);
         const int sl_id = block_slot(p, row, end, xrow);
-        if (sl_id < 0) continue;
         const int col = (sl * kCols + j) * 16 + 4 * (ln >> 4);
-        if (col >= cols) continue;
-        const int64_t orow = DST == Dst::kSlotF32 ? sl_id : row;
-        if constexpr (DST == Dst::kSlotF32 || kSilu) {
-            float* o = reinterpret_cast<float*>(p.out) + orow * p.ldo + col;
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-                if (col + r < cols) o[r] = t[r];
-        } else {
-            uint16_t* o = reinterpret_cast<uint16_t*>(p.out) + orow * p.ldo + col;
-            constexpr bool bf16 = DST == Dst::kBf16;
-            const uint32_t a = pack_out16(t[0], t[1], bf16), b = pack_out16(t[2], t[3], bf16);
-            if (col + 3 < cols && p.ldo % 4 == 0) {
-                *reinterpret_cast<uint2*>(o) = make_uint2(a, b);
-            } else {
-                const uint32_t v[4] = {a & 0xFFFF, a >> 16, b & 0xFFFF, b >> 16};
-#pragma unroll
-                for (int r = 0; r < 4; ++r)
-                    if (col + r < cols) o[r] = (uint16_t)v[r];
-            }
-        }
+        if (sl_id < 0 || col >= cols) continue;
+        store4<DST>(p, DST == Dst::kSlotF32 ? sl_id : row, col, cols, t);
     }
 }
 
+int too_many() {
+    set_error("fp8 block product: too many tiles");
+    return W4A8_ERR_INVALID;
+}
+
 template <int FT, int FN, int KS, Src SRC, Dst DST>
-int go(const BlockParams& p, hipStream_t s) {
+int go_any(const BlockParams& p, hipStream_t s) {
     constexpr bool silu = DST == Dst::kSiluF32;
     const int cols = silu ? p.N / 2 : p.N, per = 16 * (silu ? FN / 2 : FN);
     const int slices = (cols + per - 1) / per;
     const int64_t grid = (int64_t)((p.P + 16 * FT - 1) / (16 * FT)) * slices;
-    if (grid >= (int64_t)1 << 31) {
-        set_error("fp8 block product: too many tiles");
-        return W4A8_ERR_INVALID;
-    }
-    if (p.K % kBlk != 0) launch_kernel(&block_stream_kernel<FT, FN, KS, SRC, DST, true>, dim3((unsigned)grid), dim3(64 * KS), 0, s, p, slices);
-    else launch_kernel(&block_stream_kernel<FT, FN, KS, SRC, DST, false>, dim3((unsigned)grid), dim3(64 * KS), 0, s, p, slices);
+    if (grid >= (int64_t)1 << 31) return too_many();
+    launch_kernel(&block_stream_kernel<FT, FN, KS, SRC, DST>, dim3((unsigned)grid), dim3(64 * KS), 0, s, p, slices);
     return check_launch("block_stream_kernel");
+}
+
+// blocks: row blocks expected to hold rows
+template <int FT, int GPW, int KS, int CG, int D, Src SRC, Dst DST>
+int go_rows(const BlockParams& p, int64_t blocks, hipStream_t s) {
+    constexpr bool silu = DST == Dst::kSiluF32;
+    const int frags = ((silu ? p.N / 2 : p.N) + 15) / 16;
+    // a work-group a CU and round where there are fewer fragments than that, else some rounds' worth
+    // of groups, each with whole rounds of D
+    constexpr int unit = D / (silu ? 2 : 1);
+    const int64_t want = (int64_t)device_cu_count() * (8 / (KS * CG) > 0 ? 8 / (KS * CG) : 1) * 2;
+    int64_t per = (blocks * frags + want * CG - 1) / (want * CG);
+    per = std::max<int64_t>(unit, std::min<int64_t>((per + unit - 1) / unit * unit, 4 * unit));
+    const int slices = (int)((frags + per * CG - 1) / (per * CG));
+    const int64_t grid = (int64_t)((p.P + 16 * FT - 1) / (16 * FT)) * slices;
+    if (grid >= (int64_t)1 << 31) return too_many();
+    launch_kernel(&block_rows_kernel<FT, GPW, KS, CG, D, SRC, DST>, dim3((unsigned)grid), dim3(64 * KS * CG), 0, s, p,
+                  slices, (int)per);
+    return check_launch("block_rows_kernel");
+}
+
+// FT row fragments: the wave split by the number of K groups.
+template <Src SRC, Dst DST>
+int rows1(const BlockParams& p, int64_t blocks, hipStream_t s) {
+    if (p.G <= 1) return go_rows<1, 1, 1, 4, 4, SRC, DST>(p, blocks, s);
+    if (p.G <= 2) return go_rows<1, 2, 1, 4, 4, SRC, DST>(p, blocks, s);
+    if (p.G <= 4) return go_rows<1, 4, 1, 4, 2, SRC, DST>(p, blocks, s);
+    if (p.G <= 8) return go_rows<1, 2, 4, 1, 4, SRC, DST>(p, blocks, s);
+    if (p.G <= 16) return go_rows<1, 4, 4, 1, 2, SRC, DST>(p, blocks, s);
+    if (p.G <= 32) return go_rows<1, 4, 8, 1, 2, SRC, DST>(p, blocks, s);
+    if constexpr (DST != Dst::kSiluF32)
+        if (p.G <= 64) return go_rows<1, 8, 8, 1, 1, SRC, DST>(p, blocks, s);
+    return go_any<1, 2, 4, SRC, DST>(p, s);
 }
 
 }  // namespace
@@ -249,24 +483,25 @@ int go(const BlockParams& p, hipStream_t s) {
 int launch_block_stream(const BlockArgs& a, hipStream_t s) {
     const BlockParams p = block_params(a);
     if (p.P == 0) return W4A8_OK;
-    auto dst = [&](auto src) -> int {
+    const int64_t blocks = a.sorted_ids != nullptr ? std::min<int64_t>(std::min(a.P / 16, a.num_valid), a.E + a.num_valid / 16)
+                                                   : (a.P + 15) / 16;
+    auto out16 = [&](auto src) -> int {
         constexpr Src S = decltype(src)::value;
-        switch (a.dst) {
-            case Dst::kF16: return go<1, 2, 4, S, Dst::kF16>(p, s);
-            case Dst::kBf16: return go<1, 2, 4, S, Dst::kBf16>(p, s);
-            case Dst::kSiluF32: return go<1, 2, 4, S, Dst::kSiluF32>(p, s);
-            case Dst::kSlotF32: return go<1, 2, 4, S, Dst::kSlotF32>(p, s);
-            default: break;
-        }
+        if (a.dst == Dst::kF16) return rows1<S, Dst::kF16>(p, blocks, s);
+        if (a.dst == Dst::kBf16) return rows1<S, Dst::kBf16>(p, blocks, s);
+        if (a.dst == Dst::kSiluF32) return rows1<S, Dst::kSiluF32>(p, blocks, s);
         set_error("fp8 block product: output form not taken by the streaming kernel");
         return W4A8_ERR_INVALID;
     };
     switch (a.src) {
-        case Src::kFp8: return dst(std::integral_constant<Src, Src::kFp8>{});
-        case Src::kF16: return dst(std::integral_constant<Src, Src::kF16>{});
-        case Src::kBf16: return dst(std::integral_constant<Src, Src::kBf16>{});
-        default: return dst(std::integral_constant<Src, Src::kF32>{});
+        case Src::kFp8: return out16(std::integral_constant<Src, Src::kFp8>{});
+        case Src::kF16: return out16(std::integral_constant<Src, Src::kF16>{});
+        case Src::kBf16: return out16(std::integral_constant<Src, Src::kBf16>{});
+        default: break;
     }
+    if (a.dst == Dst::kSlotF32) return rows1<Src::kF32, Dst::kSlotF32>(p, blocks, s);
+    set_error("fp8 block product: fp32 rows are the layer's second product's");
+    return W4A8_ERR_INVALID;
 }
 
 }  // namespace w4a8
