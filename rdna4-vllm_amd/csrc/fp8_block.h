@@ -144,5 +144,7 @@ int launch_act_quant_block(const void* x, bool bf16, int64_t rows, int64_t K, in
                            uint8_t* q, float* scales, hipStream_t s);
 // Weight-streaming product (fp8_stream.hip): any sizes.
 int launch_block_stream(const BlockArgs& a, hipStream_t s);
+// Tiles (fp8_tiles.hip): e4m3 rows.
+int launch_block_tiles(const BlockArgs& a, hipStream_t s);
 
 }  // namespace w4a8

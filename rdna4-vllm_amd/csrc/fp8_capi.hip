@@ -138,6 +138,7 @@ int w4a8_fp8_block_gemm(const void* x, int x_dtype, const float* x_scales, int64
     a.w = w; a.ws = w_scales; a.E = 1; a.N = N;
     a.P = M; a.top_k = 1; a.num_valid = M; a.block_m = 16; a.gather = false;
     a.src = src_of(x_dtype); a.dst = dst_of(out_dtype); a.out = out; a.ldo = N;
+    if (a.src == Src::kFp8 && M > 64) return launch_block_tiles(a, as_stream(stream));
     return launch_block_stream(a, as_stream(stream));
 }
 

@@ -13,50 +13,10 @@
 #include <algorithm>
 #include <type_traits>
 
-#include "fp8_block.h"
+#include "fp8_mfma.h"
 
 namespace w4a8 {
 namespace {
-
-using v8h = _Float16 __attribute__((ext_vector_type(8)));
-
-// The row operand of one group: a lane's 32 values as e4m3 bytes, or (EXACT) as fp16.
-template <bool EXACT>
-struct RowOp {
-    v8i b;
-};
-template <>
-struct RowOp<true> {
-    v8h h[4];
-};
-
-__device__ __forceinline__ v8h e4m3_to_half8(int lo, int hi) {
-    typedef _Float16 v2h __attribute__((ext_vector_type(2)));
-    const v2h a = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.0f, false);
-    const v2h b = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.0f, true);
-    const v2h c = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.0f, false);
-    const v2h d = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.0f, true);
-    return v8h{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
-}
-
-// Sum over one group of 128 k. The fp8 matrix core cuts products of eight neighbouring k to 2^-13 of
-// their largest; EXACT feeds the fp16 one (every e4m3 number is an fp16 number), which adds them as
-// fp32 numbers, at a quarter of the rate and for sixteen conversions. It is for sums that are
-// quantised again: an error of 1e-4 there moves values across a border between two e4m3 numbers, and
-// the layer's output by 1e-3 (one token up to 6e-3), three times what the rounding to bf16 does.
-template <bool EXACT>
-__device__ __forceinline__ v4f group_dot(const u32x4& w0, const u32x4& w1, const RowOp<EXACT>& x) {
-    const v4f zero{0.f, 0.f, 0.f, 0.f};
-    if constexpr (EXACT) {
-        v4f t = __builtin_amdgcn_mfma_f32_16x16x32_f16(e4m3_to_half8(w0[0], w0[1]), x.h[0], zero, 0, 0, 0);
-        t = __builtin_amdgcn_mfma_f32_16x16x32_f16(e4m3_to_half8(w0[2], w0[3]), x.h[1], t, 0, 0, 0);
-        t = __builtin_amdgcn_mfma_f32_16x16x32_f16(e4m3_to_half8(w1[0], w1[1]), x.h[2], t, 0, 0, 0);
-        return __builtin_amdgcn_mfma_f32_16x16x32_f16(e4m3_to_half8(w1[2], w1[3]), x.h[3], t, 0, 0, 0);
-    } else {
-        const v8i w{(int)w0[0], (int)w0[1], (int)w0[2], (int)w0[3], (int)w1[0], (int)w1[1], (int)w1[2], (int)w1[3]};
-        return mfma_16x16x128(w, x.b, zero);
-    }
-}
 
 // Raw bytes of a row's 32 values of one group, as loaded.
 template <Src SRC>
@@ -78,14 +38,14 @@ __device__ __forceinline__ void row_load(RowRaw<SRC>& r, const uint8_t* xp, int 
 }
 // The MFMA operand; rows in 16 or 32 bits are quantised (the group's absmax lies in four lanes).
 template <Src SRC, bool EXACT>
-__device__ __forceinline__ RowOp<EXACT> row_operand(const RowRaw<SRC>& r, int g, int q, int K, float& xs) {
+__device__ __forceinline__ GroupOp<EXACT> row_operand(const RowRaw<SRC>& r, int g, int q, int K, float& xs) {
     const bool in[2] = {g * kBlk + q * 16 < K, g * kBlk + 64 + q * 16 < K};
-    int o[8];
+    uint32_t o[8];
     if constexpr (SRC == Src::kFp8) {
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
-            for (int d = 0; d < 4; ++d) o[4 * h + d] = in[h] ? (int)r.v[h][d] : 0;
+            for (int d = 0; d < 4; ++d) o[4 * h + d] = in[h] ? r.v[h][d] : 0u;
     } else {
         float f[2][16];
         float m = 0.f;
@@ -112,38 +72,10 @@ __device__ __forceinline__ RowOp<EXACT> row_operand(const RowRaw<SRC>& r, int g,
         for (int h = 0; h < 2; ++h)
 #pragma unroll
             for (int d = 0; d < 4; ++d)
-                o[4 * h + d] = (int)pack4_e4m3(f[h][4 * d] * inv, f[h][4 * d + 1] * inv, f[h][4 * d + 2] * inv,
+                o[4 * h + d] = pack4_e4m3(f[h][4 * d] * inv, f[h][4 * d + 1] * inv, f[h][4 * d + 2] * inv,
                                                f[h][4 * d + 3] * inv);
     }
-    RowOp<EXACT> x;
-    if constexpr (EXACT) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) x.h[i] = e4m3_to_half8(o[2 * i], o[2 * i + 1]);
-    } else {
-        x.b = v8i{o[0], o[1], o[2], o[3], o[4], o[5], o[6], o[7]};
-    }
-    return x;
-}
-
-// Four adjacent columns of one row.
-template <Dst DST>
-__device__ __forceinline__ void store4(const BlockParams& p, int64_t orow, int col, int cols, const v4f& t) {
-    if constexpr (DST == Dst::kSlotF32 || DST == Dst::kSiluF32) {
-        // (whole layers: multiples of 128 columns)
-        *reinterpret_cast<v4f*>(reinterpret_cast<float*>(p.out) + orow * p.ldo + col) = t;
-    } else {
-        uint16_t* o = reinterpret_cast<uint16_t*>(p.out) + orow * p.ldo + col;
-        constexpr bool bf16 = DST == Dst::kBf16;
-        const uint32_t a = pack_out16(t[0], t[1], bf16), b = pack_out16(t[2], t[3], bf16);
-        if (p.ldo % 4 == 0 && p.out8) {
-            *reinterpret_cast<uint2*>(o) = make_uint2(a, b);
-        } else {
-            const uint32_t v[4] = {a & 0xFFFF, a >> 16, b & 0xFFFF, b >> 16};
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-                if (col + r < cols) o[r] = (uint16_t)v[r];
-        }
-    }
+    return group_op<EXACT>(u32x4{o[0], o[1], o[2], o[3]}, u32x4{o[4], o[5], o[6], o[7]});
 }
 
 // The expert and the end of the rows in use of the rows from row0; false: nothing to do.
@@ -213,7 +145,7 @@ __global__ void __launch_bounds__(64 * KS * CG) block_rows_kernel(BlockParams p,
 
     // ---- rows, held ----
     int slot[FT];
-    RowOp<EXACT> x[FT][GPW];
+    GroupOp<EXACT> x[FT][GPW];
     float xs[FT][GPW];
 #pragma unroll
     for (int i = 0; i < FT; ++i) {
@@ -256,7 +188,7 @@ __global__ void __launch_bounds__(64 * KS * CG) block_rows_kernel(BlockParams p,
                 run[d][i] = v4f{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int j = 0; j < GPW; ++j) {
-                    const v4f t = group_dot<EXACT>(ring[d].w[j][0], ring[d].w[j][1], x[i][j]);
+                    const v4f t = group_mfma<EXACT>(group_op<EXACT>(ring[d].w[j][0], ring[d].w[j][1]), x[i][j]);
                     const float s = xs[i][j] * ring[d].ws[j];
 #pragma unroll
                     for (int r = 0; r < 4; ++r) run[d][i][r] = fmaf(t[r], s, run[d][i][r]);
@@ -377,11 +309,11 @@ __global__ void __launch_bounds__(64 * KS) block_stream_kernel(BlockParams p, in
 #pragma unroll
         for (int i = 0; i < FT; ++i) {
             float xs = s.xs[i];
-            const RowOp<EXACT> xv = row_operand<SRC, EXACT>(s.x[i], g, q, K, xs);   // zero past the end
+            const GroupOp<EXACT> xv = row_operand<SRC, EXACT>(s.x[i], g, q, K, xs);   // zero past the end
             if (g >= G) xs = 0.f;
 #pragma unroll
             for (int j = 0; j < FN; ++j) {
-                const v4f t = group_dot<EXACT>(s.w[j][0], s.w[j][1], xv);
+                const v4f t = group_mfma<EXACT>(group_op<EXACT>(s.w[j][0], s.w[j][1]), xv);
                 const float sc = xs * s.ws[j];
 #pragma unroll
                 for (int r = 0; r < 4; ++r) run[i][j][r] = fmaf(t[r], sc, run[i][j][r]);
