@@ -67,6 +67,7 @@ struct BlockParams {
     int P, K, N, G, NB, E;
     int x_rows, top_k, num_valid, block_m, gather;
     int out8;                    // out is aligned to 8 bytes
+    int out_bf16;                // Dst::kBf16
 };
 
 inline BlockParams block_params(const BlockArgs& a) {
@@ -79,6 +80,7 @@ inline BlockParams block_params(const BlockArgs& a) {
     p.NB = (int)blk_groups(a.N); p.E = (int)a.E;
     p.x_rows = (int)a.x_rows; p.top_k = (int)a.top_k; p.num_valid = (int)a.num_valid;
     p.block_m = (int)a.block_m; p.gather = a.gather ? 1 : 0;
+    p.out_bf16 = a.dst == Dst::kBf16 ? 1 : 0;
     p.out8 = reinterpret_cast<uintptr_t>(a.out) % 8 == 0 ? 1 : 0;
     return p;
 }
@@ -144,7 +146,12 @@ int launch_act_quant_block(const void* x, bool bf16, int64_t rows, int64_t K, in
                            uint8_t* q, float* scales, hipStream_t s);
 // Weight-streaming product (fp8_stream.hip): any sizes.
 int launch_block_stream(const BlockArgs& a, hipStream_t s);
-// Tiles (fp8_tiles.hip): e4m3 rows.
+// Tiles (fp8_tiles.hip): e4m3 rows, sizes that 32-bit offsets reach.
+bool block_tiles_supported(const BlockArgs& a);
 int launch_block_tiles(const BlockArgs& a, hipStream_t s);
+// out[t, n] = sum over the slots j in order of tw[t, j] * y[slot_to_row[t, j], n] in fp32, rounded to
+// 16 bits; y (rows, N) in out's type, rows < 0 contribute nothing. N % 8 == 0.
+int launch_block_reduce(const void* y, const int32_t* slot_to_row, const float* tw, int64_t T, int64_t N,
+                        int64_t top_k, void* out, bool bf16, hipStream_t s);
 
 }  // namespace w4a8

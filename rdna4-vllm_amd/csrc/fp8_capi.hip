@@ -1,5 +1,6 @@
 // C ABI entry points of the block-scaled fp8 operators (include/w4a8_moe.h): argument checks,
 // workspace carving, the choice of kernel and the whole-layer composition.
+#include <algorithm>
 #include <string>
 
 #include "fp8_block.h"
@@ -21,6 +22,7 @@ bool is16(int dt) { return dt == W4A8_DTYPE_F16 || dt == W4A8_DTYPE_BF16; }
 
 constexpr int64_t kMaxSide = (int64_t)1 << 24;    // rows of a weight, values of a row
 constexpr int64_t kMaxRows = ((int64_t)1 << 31) - 256;
+constexpr int64_t kStreamRows = 64;               // dense rows up to which the weights are streamed
 
 // Sizes and pointers that every product shares.
 int check_product(const void* x, int x_dtype, const float* xs, int64_t rows, int64_t K, int64_t ldx, const uint8_t* w,
@@ -44,37 +46,55 @@ Src src_of(int x_dtype) {
 Dst dst_of(int dt) { return dt == W4A8_DTYPE_BF16 ? Dst::kBf16 : Dst::kF16; }
 
 // ---- the gated layer ----
+// Few rows an expert: blocks of 16 rows on the streaming kernels (rows quantised in registers, h and
+// the slots' rows in fp32). Else tiles: rows quantised beforehand, h by gemm1, the slots' rows in the
+// output's type, blocks of the 64 rows that a tile's wave takes.
 struct LayerPlan {
+    bool tiles;
     int64_t block_m, P, nblk;
 };
-LayerPlan plan_layer(int64_t T, int64_t E, int64_t top_k) {
+LayerPlan plan_layer(int64_t T, int64_t H, int64_t inter, int64_t E, int64_t top_k) {
     LayerPlan pl;
-    pl.block_m = 16;
+    const int64_t lim = (int64_t)1 << 32;
+    pl.tiles = T * top_k > 16 * E;
+    pl.block_m = pl.tiles ? 64 : 16;
     pl.P = w4a8_moe_align_sorted_len(T * top_k, E, pl.block_m);
+    if (pl.tiles && (T * H >= lim || pl.P * inter >= lim || 2 * inter * H >= lim)) {
+        pl.tiles = false;
+        pl.block_m = 16;
+        pl.P = w4a8_moe_align_sorted_len(T * top_k, E, pl.block_m);
+    }
     pl.nblk = pl.P / pl.block_m;
     return pl;
 }
 struct LayerScratch {
-    int32_t *sti, *eid, *ntp;
+    int32_t *sti, *eid, *ntp, *s2r;
     void* align_ws;
     size_t align_bytes;
-    uint8_t* xq;
-    float* xs;
-    float* h;
-    float* y;
+    uint8_t *xq, *hq;
+    float *xs, *hs, *h, *y32;
+    uint16_t* y16;
 };
 template <typename WS>
 void carve_layer(WS& w, const LayerPlan& pl, int64_t T, int64_t H, int64_t inter, int64_t E, int64_t top_k,
                  bool quantise, LayerScratch& m) {
+    m = LayerScratch{};
     m.sti = w.template take<int32_t>((size_t)pl.P);
     m.eid = w.template take<int32_t>((size_t)pl.nblk);
     m.ntp = w.template take<int32_t>(1);
     m.align_bytes = align_workspace_bytes(T * top_k, E);
     m.align_ws = w.template take<uint8_t>(m.align_bytes);
+    if (!pl.tiles) {
+        m.h = w.template take<float>((size_t)(pl.P * inter));
+        m.y32 = w.template take<float>((size_t)(T * top_k * H));
+        return;
+    }
+    m.s2r = w.template take<int32_t>((size_t)(T * top_k));
     m.xq = w.template take<uint8_t>(quantise ? (size_t)(T * H) : 0);
     m.xs = w.template take<float>(quantise ? (size_t)(T * blk_groups(H)) : 0);
-    m.h = w.template take<float>((size_t)(pl.P * inter));
-    m.y = w.template take<float>((size_t)(T * top_k * H));
+    m.hq = w.template take<uint8_t>((size_t)(pl.P * inter));
+    m.hs = w.template take<float>((size_t)(pl.P * blk_groups(inter)));
+    m.y16 = w.template take<uint16_t>((size_t)(pl.P * H));
 }
 struct SizeProbe {
     WorkspaceSize s;
@@ -120,25 +140,40 @@ int w4a8_act_quant_fp8_block(const void* x, int x_dtype, int64_t rows, int64_t K
 }
 
 size_t w4a8_fp8_block_gemm_workspace_size(int x_dtype, int64_t M, int64_t K) {
-    (void)x_dtype; (void)M; (void)K;
-    return 0;
+    if (x_dtype == W4A8_DTYPE_E4M3 || M <= kStreamRows || K <= 0) return 0;
+    WorkspaceSize s;
+    s.take<uint8_t>((size_t)(M * K));
+    s.take<float>((size_t)(M * blk_groups(K)));
+    return s.used;
 }
 
 int w4a8_fp8_block_gemm(const void* x, int x_dtype, const float* x_scales, int64_t M, int64_t K, int64_t x_stride,
                         const uint8_t* w, const float* w_scales, int64_t N, void* out, int out_dtype, void* workspace,
                         size_t workspace_bytes, void* stream) {
     clear_error();
-    (void)workspace; (void)workspace_bytes;
     if (int rc = check_product(x, x_dtype, x_scales, M, K, x_stride, w, w_scales, 1, N)) return rc;
     W4A8_REQUIRE(is16(out_dtype), "fp8_block_gemm: out must be fp16 or bf16");
     if (M == 0) return W4A8_OK;
     W4A8_REQUIRE(out, "fp8_block_gemm: null pointer");
+    const bool quantise = x_dtype != W4A8_DTYPE_E4M3;
     BlockArgs a{};
     a.x = x; a.xs = x_scales; a.x_rows = M; a.K = K; a.ldx = x_stride;
     a.w = w; a.ws = w_scales; a.E = 1; a.N = N;
     a.P = M; a.top_k = 1; a.num_valid = M; a.block_m = 16; a.gather = false;
     a.src = src_of(x_dtype); a.dst = dst_of(out_dtype); a.out = out; a.ldo = N;
-    if (a.src == Src::kFp8 && M > 64) return launch_block_tiles(a, as_stream(stream));
+    if (M > kStreamRows && quantise) {
+        Workspace w(workspace, workspace_bytes);
+        uint8_t* xq = w.take<uint8_t>((size_t)(M * K));
+        float* xs = w.take<float>((size_t)(M * blk_groups(K)));
+        if (workspace == nullptr || !w.ok()) {
+            set_error("fp8_block_gemm: workspace smaller than w4a8_fp8_block_gemm_workspace_size()");
+            return W4A8_ERR_WORKSPACE;
+        }
+        if (int rc = launch_act_quant_block(x, x_dtype == W4A8_DTYPE_BF16, M, K, x_stride, false, xq, xs, as_stream(stream)))
+            return rc;
+        a.x = xq; a.xs = xs; a.ldx = K; a.src = Src::kFp8;
+    }
+    if (M > kStreamRows && block_tiles_supported(a)) return launch_block_tiles(a, as_stream(stream));
     return launch_block_stream(a, as_stream(stream));
 }
 
@@ -164,6 +199,7 @@ int w4a8_moe_fp8_block_gemm(const void* x, const float* x_scales, int64_t x_rows
     a.sorted_ids = sorted_token_ids; a.expert_ids = expert_ids; a.ntp = num_tokens_post_padded;
     a.P = P; a.top_k = top_k; a.num_valid = num_slots; a.block_m = block_m; a.gather = gather != 0;
     a.src = Src::kFp8; a.dst = dst_of(out_dtype); a.out = out; a.ldo = N;
+    if (std::min(P, num_slots) > 16 * E && block_tiles_supported(a)) return launch_block_tiles(a, as_stream(stream));
     return launch_block_stream(a, as_stream(stream));
 }
 
@@ -171,7 +207,7 @@ size_t w4a8_moe_fp8_block_workspace_size(int64_t T, int64_t H, int64_t inter, in
     if (T <= 0 || H <= 0 || inter <= 0 || E <= 0 || top_k <= 0) return 0;
     SizeProbe p;
     LayerScratch m;
-    carve_layer(p, plan_layer(T, E, top_k), T, H, inter, E, top_k, true, m);
+    carve_layer(p, plan_layer(T, H, inter, E, top_k), T, H, inter, E, top_k, true, m);
     return p.s.used;
 }
 
@@ -194,7 +230,7 @@ int w4a8_moe_fp8_block_apply(const void* x, int x_dtype, const float* x_scales, 
     if (T == 0) return W4A8_OK;
     W4A8_REQUIRE(w2 && w2_scales && topk_weights && topk_ids && out, "moe_fp8_block_apply: null pointer");
     W4A8_REQUIRE(aligned16(w2) && aligned16(out), "moe_fp8_block_apply: w2 and out must be aligned to 16 bytes");
-    const LayerPlan pl = plan_layer(T, E, top_k);
+    const LayerPlan pl = plan_layer(T, H, inter, E, top_k);
     W4A8_REQUIRE(pl.P <= kMaxRows, "moe_fp8_block_apply: too many slots");
     const bool quantise = x_dtype != W4A8_DTYPE_E4M3;
     Workspace w(workspace, workspace_bytes);
@@ -205,24 +241,36 @@ int w4a8_moe_fp8_block_apply(const void* x, int x_dtype, const float* x_scales, 
         return W4A8_ERR_WORKSPACE;
     }
     hipStream_t s = as_stream(stream);
+    const bool bf16 = out_dtype == W4A8_DTYPE_BF16;
     if (int rc = launch_align(topk_ids, T * top_k, E, pl.block_m, expert_map, n_global, m.sti, pl.P, m.eid, m.ntp,
-                              m.align_ws, m.align_bytes, s))
+                              m.align_ws, m.align_bytes, s, m.s2r))
         return rc;
-    // (few rows are quantised in the registers that hold them; so no row is prepared for it here)
+    if (pl.tiles && quantise)
+        if (int rc = launch_act_quant_block(x, x_dtype == W4A8_DTYPE_BF16, T, H, H, false, m.xq, m.xs, s)) return rc;
     BlockArgs g1{};
-    g1.x = x; g1.xs = x_scales; g1.x_rows = T; g1.K = H; g1.ldx = H;
+    g1.x = pl.tiles && quantise ? m.xq : x;
+    g1.xs = pl.tiles && quantise ? m.xs : x_scales;
+    g1.x_rows = T; g1.K = H; g1.ldx = H;
     g1.w = w13; g1.ws = w13_scales; g1.E = E; g1.N = 2 * inter;
     g1.sorted_ids = m.sti; g1.expert_ids = m.eid; g1.ntp = m.ntp; g1.P = pl.P;
     g1.top_k = top_k; g1.num_valid = T * top_k; g1.block_m = pl.block_m; g1.gather = true;
-    g1.src = src_of(x_dtype); g1.dst = Dst::kSiluF32; g1.out = m.h; g1.ldo = inter;
-    if (int rc = launch_block_stream(g1, s)) return rc;
+    g1.src = pl.tiles ? Src::kFp8 : src_of(x_dtype);
+    g1.dst = pl.tiles ? Dst::kSiluFp8 : Dst::kSiluF32;
+    g1.out = pl.tiles ? (void*)m.hq : (void*)m.h; g1.out_scales = m.hs; g1.ldo = inter;
     BlockArgs g2 = g1;
-    g2.x = m.h; g2.xs = nullptr; g2.x_rows = pl.P; g2.K = inter; g2.ldx = inter;
+    g2.x = pl.tiles ? (const void*)m.hq : (const void*)m.h; g2.xs = m.hs; g2.x_rows = pl.P; g2.K = inter; g2.ldx = inter;
     g2.w = w2; g2.ws = w2_scales; g2.N = H; g2.gather = false;
-    g2.src = Src::kF32; g2.dst = Dst::kSlotF32; g2.out = m.y; g2.ldo = H;
+    g2.src = pl.tiles ? Src::kFp8 : Src::kF32;
+    g2.dst = pl.tiles ? dst_of(out_dtype) : Dst::kSlotF32;
+    g2.out = pl.tiles ? (void*)m.y16 : (void*)m.y32; g2.ldo = H;
+    if (pl.tiles) {
+        if (int rc = launch_block_tiles(g1, s)) return rc;
+        if (int rc = launch_block_tiles(g2, s)) return rc;
+        return launch_block_reduce(m.y16, m.s2r, topk_weights, T, H, top_k, out, bf16, s);
+    }
+    if (int rc = launch_block_stream(g1, s)) return rc;
     if (int rc = launch_block_stream(g2, s)) return rc;
-    return launch_slot_reduce(m.y, topk_weights, topk_ids, expert_map, n_global, E, T, H, top_k, out,
-                              out_dtype == W4A8_DTYPE_BF16, s);
+    return launch_slot_reduce(m.y32, topk_weights, topk_ids, expert_map, n_global, E, T, H, top_k, out, bf16, s);
 }
 
 }  // extern "C"

@@ -59,24 +59,26 @@ __device__ __forceinline__ v4f group_mfma(const GroupOp<EXACT>& w, const GroupOp
     }
 }
 
-// Four adjacent columns of one row.
+// Four adjacent columns of one row, rounded to 16 bits.
+__device__ __forceinline__ void store16(const BlockParams& p, int64_t orow, int col, int cols, const v4f& t, bool bf16) {
+    uint16_t* o = reinterpret_cast<uint16_t*>(p.out) + orow * p.ldo + col;
+    const uint32_t a = pack_out16(t[0], t[1], bf16), b = pack_out16(t[2], t[3], bf16);
+    if (p.ldo % 4 == 0 && p.out8) {
+        *reinterpret_cast<uint2*>(o) = make_uint2(a, b);
+    } else {
+        const uint32_t v[4] = {a & 0xFFFF, a >> 16, b & 0xFFFF, b >> 16};
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+            if (col + r < cols) o[r] = (uint16_t)v[r];
+    }
+}
 template <Dst DST>
 __device__ __forceinline__ void store4(const BlockParams& p, int64_t orow, int col, int cols, const v4f& t) {
     if constexpr (DST == Dst::kSlotF32 || DST == Dst::kSiluF32) {
         // (whole layers: multiples of 128 columns)
         *reinterpret_cast<v4f*>(reinterpret_cast<float*>(p.out) + orow * p.ldo + col) = t;
     } else {
-        uint16_t* o = reinterpret_cast<uint16_t*>(p.out) + orow * p.ldo + col;
-        constexpr bool bf16 = DST == Dst::kBf16;
-        const uint32_t a = pack_out16(t[0], t[1], bf16), b = pack_out16(t[2], t[3], bf16);
-        if (p.ldo % 4 == 0 && p.out8) {
-            *reinterpret_cast<uint2*>(o) = make_uint2(a, b);
-        } else {
-            const uint32_t v[4] = {a & 0xFFFF, a >> 16, b & 0xFFFF, b >> 16};
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-                if (col + r < cols) o[r] = (uint16_t)v[r];
-        }
+        store16(p, orow, col, cols, t, DST == Dst::kBf16);
     }
 }
 

@@ -286,6 +286,41 @@ __global__ void __launch_bounds__(256) act_quant_groups_any_kernel(const void* _
     if (lane == 0) scales[row * G + g] = s;
 }
 
+// Eight columns a lane; a token's rows are requested together, eight at a time.
+template <bool BF16>
+__global__ void __launch_bounds__(256) block_reduce_kernel(const void* __restrict__ y, const int32_t* __restrict__ s2r,
+                                                           const float* __restrict__ tw, int N, int top_k,
+                                                           void* __restrict__ out) {
+    const int64_t t = blockIdx.x;
+    const int n = (blockIdx.y * 256 + threadIdx.x) * 8;
+    if (n >= N) return;
+    float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    for (int j0 = 0; j0 < top_k; j0 += 8) {
+        int32_t r[8];
+        u32x4 v[8];
+        float w[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            r[j] = j0 + j < top_k ? s2r[t * top_k + j0 + j] : -1;
+            w[j] = j0 + j < top_k ? tw[t * top_k + j0 + j] : 0.f;
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            v[j] = u32x4{0, 0, 0, 0};
+            if (r[j] >= 0) v[j] = *reinterpret_cast<const u32x4*>(reinterpret_cast<const uint16_t*>(y) + (int64_t)r[j] * N + n);
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            if (r[j] < 0) continue;
+            float f[8];
+            unpack8<BF16>(v[j], f);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) acc[i] = fmaf(w[j], f[i], acc[i]);
+        }
+    }
+    *reinterpret_cast<u32x4*>(reinterpret_cast<uint16_t*>(out) + t * N + n) = pack8<BF16>(acc);
+}
+
 template <int W, int NV, bool BF16, bool RES, bool KEEP, bool WF32>
 void norm_go(const NormParams& p, bool per_row, hipStream_t s) {
     const unsigned grid = (unsigned)(W == 1 ? (p.rows + 3) / 4 : p.rows);
@@ -333,6 +368,15 @@ int launch_rms_norm_quant(const NormArgs& a, hipStream_t s) {
     if (a.bf16) rms_norm_quant_any_kernel<true><<<(unsigned)a.rows, 256, 0, s>>>(p, a.weight_f32, a.per_row);
     else rms_norm_quant_any_kernel<false><<<(unsigned)a.rows, 256, 0, s>>>(p, a.weight_f32, a.per_row);
     return check_launch("rms_norm_quant_any_kernel");
+}
+
+int launch_block_reduce(const void* y, const int32_t* slot_to_row, const float* tw, int64_t T, int64_t N,
+                        int64_t top_k, void* out, bool bf16, hipStream_t s) {
+    if (T == 0) return W4A8_OK;
+    const dim3 grid((unsigned)T, (unsigned)((N / 8 + 255) / 256));
+    if (bf16) block_reduce_kernel<true><<<grid, 256, 0, s>>>(y, slot_to_row, tw, (int)N, (int)top_k, out);
+    else block_reduce_kernel<false><<<grid, 256, 0, s>>>(y, slot_to_row, tw, (int)N, (int)top_k, out);
+    return check_launch("block_reduce_kernel");
 }
 
 int launch_act_quant_block(const void* x, bool bf16, int64_t rows, int64_t K, int64_t ldx, bool silu, uint8_t* q,

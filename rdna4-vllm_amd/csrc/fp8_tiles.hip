@@ -1,13 +1,15 @@
 // Block-scaled fp8 products of many rows (gfx950 MFMA), dense or grouped.
 //
 // A work-group owns BT rows by BN weight rows (columns); per group of 128 k both come straight from
-// memory to LDS (16 bytes a lane, no registers), S slots deep. Weights are the first MFMA operand: a
+// memory to LDS (16 bytes a lane, no registers), S groups deep. Weights are the first MFMA operand: a
 // lane ends up with four adjacent columns of one row, so the scale xs[row, g] * ws[block, g] is one
 // number a row fragment, lane and group (a wave's columns lie in one 128-block of the weights).
+//
+// A tile takes any rows of the padded layout: it passes over the experts of its 16-row fragments one
+// by one, so blocks of any multiple of 16 rows do.
 #include <algorithm>
 #include <type_traits>
 
-#include "fp8_block.h"
 #include "fp8_mfma.h"
 
 namespace w4a8 {
@@ -17,13 +19,13 @@ using lds_void_ptr = __attribute__((address_space(3))) void*;
 using global_cvoid_ptr = const __attribute__((address_space(1))) void*;
 
 constexpr int kTileXcds = 8;
-constexpr int kRunRows = 8;       // row tiles of an XCD's run
+constexpr int kRunRows = 4;       // row tiles of an XCD's run
 
 // What pieces past the end of K are read from.
 __device__ __attribute__((aligned(16))) uint32_t g_zero_piece[4];
 
-// s_waitcnt operand: at most n vector-memory loads in flight, the other counters ignored.
-constexpr int wait_vm(int n) { return 0x0F70 | (n & 0xF) | ((n >> 4) << 14); }
+// s_waitcnt operand: at most n vector-memory loads and no LDS operation in flight.
+constexpr int wait_vm(int n) { return 0x0070 | (n & 0xF) | ((n >> 4) << 14); }
 
 // Work-group barrier that no load or store may be moved across and that waits for none of them.
 __device__ __forceinline__ void group_barrier() {
@@ -34,222 +36,405 @@ __device__ __forceinline__ void group_barrier() {
     __builtin_amdgcn_sched_barrier(0);
 }
 
+// WT x WN waves of FT row fragments x FN column fragments of 16, S groups in LDS.
 template <int WT_, int WN_, int FT_, int FN_, int S_>
 struct TileCfg {
     static constexpr int WT = WT_, WN = WN_, FT = FT_, FN = FN_, S = S_;
     static constexpr int kWaves = WT * WN, kThreads = 64 * kWaves;
     static constexpr int BT = WT * FT * 16, BN = WN * FN * 16;
-    static constexpr int kSlot = (BT + BN) * kBlk + BT * 4;      // rows, weights, row scales
+    static constexpr int kW = BT * kBlk;                         // weights behind the rows
+    static constexpr int kSlot = kW + BN * kBlk;
     static constexpr int PX = BT * 8 / kThreads, PW = BN * 8 / kThreads;   // 16-byte pieces a thread
+    static constexpr int kLoads = PX + PW;                       // of a wave and group
+    static constexpr int kChunk = 6;                             // groups whose row scales are loaded at once
+    static constexpr int PT = (BT * kChunk + kThreads - 1) / kThreads;   // entries a thread
     static_assert(PX * kThreads == BT * 8 && PW * kThreads == BN * 8, "pieces divide");
     static_assert(FN * 16 <= kBlk && kBlk % (FN * 16) == 0, "a wave's columns lie in one block");
-    static_assert(BT % 64 == 0, "row scales come 64 at a time");
+    static_assert(kChunk % S == 0, "rounds divide");
+    static_assert((S == 2 || S == 3) && kLoads < 64, "slots; loads in flight can be counted");
 };
 
-template <typename C, Dst DST, bool EXACT>
-__global__ void __launch_bounds__(C::kThreads) block_tiles_kernel(BlockParams p, int mtiles, int ntiles) {
-    constexpr int FT = C::FT, FN = C::FN, BT = C::BT, BN = C::BN;
+template <typename C, Dst DST, bool EXACT, bool TAIL, bool GROUPED>
+__global__ void __launch_bounds__(C::kThreads, C::kWaves >= 8 || C::S == 2 ? 2 : 1) block_tiles_kernel(BlockParams p, int ntiles) {
+    constexpr int FT = C::FT, FN = C::FN, BT = C::BT, BN = C::BN, S = C::S;
+    constexpr bool kSilu = DST == Dst::kSiluFp8;
+    static_assert(!kSilu || BN == 256, "SiLU tiles hold 128 gate and 128 up columns");
+    // arrays of their own: the compiler then sees that reads of one do not wait for loads into another
     __shared__ __attribute__((aligned(1024))) uint8_t slot0[C::kSlot];
     __shared__ __attribute__((aligned(1024))) uint8_t slot1[C::kSlot];
-    __shared__ __attribute__((aligned(1024))) uint8_t slot2[C::S > 2 ? C::kSlot : 16];
+    __shared__ __attribute__((aligned(1024))) uint8_t slot2[S > 2 ? C::kSlot : 16];
+    __shared__ float s_xs[2 * C::kChunk * BT];                   // row scales [group][row] of two chunks
 
-    // ---- the tile: an XCD takes a contiguous run, eight row tiles by all column tiles ----
+    // ---- the tile: an XCD takes a contiguous run of those in use, kRunRows row tiles by all columns ----
+    const int end = GROUPED ? min(p.ntp[0], p.P) : p.P;
+    const int mtiles = (end + BT - 1) / BT;
     const int items = mtiles * ntiles, perx = (items + kTileXcds - 1) / kTileXcds;
     const int jx = blockIdx.x / kTileXcds, item = (int)(blockIdx.x % kTileXcds) * perx + jx;
     if (jx >= perx || item >= items) return;
     const int run_items = kRunRows * ntiles;
     const int m0 = item / run_items * kRunRows, rem = item % run_items;
     const int rows_here = min(kRunRows, mtiles - m0);
-    const int row0 = (m0 + rem % rows_here) * BT, col0 = rem / rows_here * BN;
-
-    int e = 0, end = p.P;
-    if (p.sorted_ids != nullptr) {
-        end = min(p.ntp[0], p.P);
-        if (row0 >= end) return;
-        e = __builtin_amdgcn_readfirstlane(p.expert_ids[row0 / p.block_m]);
-        if (e < 0 || e >= p.E) return;
-        end = min(end, (row0 / p.block_m + 1) * p.block_m);     // (a tile of rows lies in one block)
-    }
+    const int row0 = (m0 + rem % rows_here) * BT, ct = rem / rows_here;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int wt = wave / C::WN, wn = wave % C::WN;
     const int q = lane >> 4, c = lane & 15;
     const int K = p.K, G = p.G, N = p.N;
 
-    // ---- staging: piece i of a thread is row (tid + i kThreads) / 8 of the slot, slot piece tid % 8.
-    // Row r lies at place r ^ ((r >> 3) & 1), its piece j at j ^ (r & 7): equal pieces of sixteen rows
-    // in different banks.
-    const uint8_t* xb = reinterpret_cast<const uint8_t*>(p.x);
-    const uint8_t* wb = p.w + ((int64_t)e * N + col0) * K;
-    uint32_t xoff[C::PX], woff[C::PW];
-    int kx[C::PX], kw[C::PW];                                  // the piece's first k within a group
-#pragma unroll
-    for (int i = 0; i < C::PX; ++i) {
-        const int pr = (tid + i * C::kThreads) >> 3, r = pr ^ ((pr >> 3) & 1);
-        int xrow;
-        block_slot(p, row0 + r, end, xrow);
-        kx[i] = ((tid & 7) ^ (r & 7)) * 16;
-        xoff[i] = (uint32_t)xrow * (uint32_t)p.ldx + (uint32_t)kx[i];
-    }
-#pragma unroll
-    for (int i = 0; i < C::PW; ++i) {
-        const int pr = (tid + i * C::kThreads) >> 3, r = pr ^ ((pr >> 3) & 1);
-        kw[i] = ((tid & 7) ^ (r & 7)) * 16;
-        woff[i] = (uint32_t)min(r, N - 1 - col0) * (uint32_t)K + (uint32_t)kw[i];
-    }
-    int srow;
-    block_slot(p, row0 + (wave * 64 + lane) % BT, end, srow);
-    const uint32_t soff = (uint32_t)srow * (uint32_t)G * 4u;
-    auto put = [&](const uint8_t* src, uint8_t* dst) __attribute__((always_inline)) {
-        __builtin_amdgcn_global_load_lds((global_cvoid_ptr)src, (lds_void_ptr)dst, 16, 0, 0);
+    // the expert of fragment f's rows (-1: none)
+    auto expert_of = [&](int f) __attribute__((always_inline)) {
+        const int r = row0 + 16 * f;
+        if (r >= end) return -1;
+        if constexpr (!GROUPED) return 0;
+        const int e = __builtin_amdgcn_readfirstlane(p.expert_ids[r / p.block_m]);
+        return e >= 0 && e < p.E ? e : -1;
     };
-    // whole: the group is not the last one
-    auto issue = [&](uint8_t* slot, int g, auto whole) __attribute__((always_inline)) {
-        const uint8_t *xg = xb + g * kBlk, *wg = wb + g * kBlk;
-        if (decltype(whole)::value || (g + 1) * kBlk <= K) {
-#pragma unroll
-            for (int i = 0; i < C::PX; ++i) put(xg + opaque_u32(xoff[i]), slot + (wave * 64 + i * C::kThreads) * 16);
-#pragma unroll
-            for (int i = 0; i < C::PW; ++i) put(wg + opaque_u32(woff[i]), slot + BT * kBlk + (wave * 64 + i * C::kThreads) * 16);
+    const int wt = wave / C::WN, wn = wave % C::WN;
+    // the weight row behind row r of the slot's BN: fragment r / 16 belongs to wave r / (16 FN); kSilu
+    // takes FN / 2 fragments of the gate half and the same of the up half
+    const int half = N / 2;
+    auto col_of = [&](int r) __attribute__((always_inline)) {
+        if constexpr (kSilu) {
+            const int w = r / (FN * 16), j = r / 16 % FN;
+            return ct * kBlk + (w * (FN / 2) + j % (FN / 2)) * 16 + r % 16 + (j >= FN / 2 ? half : 0);
         } else {
-            // the last, partial group: pieces past the end are zero in both operands
-            const uint8_t* zero = reinterpret_cast<const uint8_t*>(g_zero_piece);
+            return ct * BN + r;
+        }
+    };
+
+    uint32_t todo = 0;                                           // row fragments not yet done
+#pragma unroll 1
+    for (int f = 0; f < BT / 16; ++f)
+        if (expert_of(f) >= 0) todo |= 1u << f;
+    while (todo != 0) {
+        const int e = expert_of(__builtin_ctz(todo));
+        uint32_t now = 0;
+#pragma unroll 1
+        for (int f = 0; f < BT / 16; ++f)
+            if ((todo >> f & 1) && expert_of(f) == e) now |= 1u << f;
+        todo &= ~now;
+        // row r of the tile: the row of x it reads (a row that exists, for rows of no use)
+        auto xrow_of = [&](int r) __attribute__((always_inline)) {
+            int xrow;
+            block_slot(p, row0 + r, (now >> (r >> 4) & 1) ? end : 0, xrow);
+            return (uint32_t)xrow;
+        };
+
+        // ---- staging: piece i of a thread is row (tid + i kThreads) / 8 of the slot, slot piece tid % 8.
+        // Row r lies at place r ^ ((r >> 3) & 1), its piece j at (2 (j % 4) + j / 4) ^ (r & 7): the sixteen
+        // lanes that a 16-byte LDS read serves at once then read different banks.
+        const uint8_t* xb = reinterpret_cast<const uint8_t*>(p.x);
+        const uint8_t* wb = p.w + (int64_t)e * N * K;
+        uint32_t xoff[C::PX], woff[C::PW];
+        auto piece_k = [&](int r) __attribute__((always_inline)) {     // the piece's first k within a group
+            const int j = (tid & 7) ^ (r & 7);
+            return ((j >> 1) | (j & 1) << 2) * 16;
+        };
+        auto piece_row = [&](int i) __attribute__((always_inline)) {
+            const int pr = (tid + i * C::kThreads) >> 3;
+            return pr ^ ((pr >> 3) & 1);
+        };
 #pragma unroll
-            for (int i = 0; i < C::PX; ++i) put(g * kBlk + kx[i] < K ? xg + xoff[i] : zero, slot + (wave * 64 + i * C::kThreads) * 16);
+        for (int i = 0; i < C::PX; ++i) xoff[i] = xrow_of(piece_row(i)) * (uint32_t)p.ldx + (uint32_t)piece_k(piece_row(i));
+#pragma unroll
+        for (int i = 0; i < C::PW; ++i)
+            woff[i] = (uint32_t)min(col_of(piece_row(i)), N - 1) * (uint32_t)K + (uint32_t)piece_k(piece_row(i));
+        auto dma = [&](const uint8_t* src, uint8_t* dst) __attribute__((always_inline)) {
+            __builtin_amdgcn_global_load_lds((global_cvoid_ptr)src, (lds_void_ptr)dst, 16, 0, 0);
+        };
+        // Past the last group every lane reads one piece (nobody reads the slot). TAIL: absent pieces of
+        // the last, partial group are zero in both operands.
+        auto issue_part = [&](uint8_t* slot, int g, int part, int parts) __attribute__((always_inline)) {
+            const uint32_t on = g < G ? ~0u : 0u;
+            const int gg = min(g, G - 1);
+            const uint8_t *xg = xb + (int64_t)gg * kBlk, *wg = wb + (int64_t)gg * kBlk;
+            asm volatile("" : "+s"(xg), "+s"(wg));               // (scalar bases, 32-bit offsets)
+            uint8_t *xd = slot + wave * 1024, *wd = slot + C::kW + wave * 1024;
+            auto src = [&](const uint8_t* base, uint32_t off, int i) __attribute__((always_inline)) {
+                const uint8_t* at = base + opaque_u32(off & on);
+                if constexpr (TAIL)
+                    if (gg * kBlk + piece_k(piece_row(i)) >= K) at = reinterpret_cast<const uint8_t*>(g_zero_piece);
+                return at;
+            };
+#pragma unroll
+            for (int i = 0; i < C::PX; ++i)
+                if (i * parts / C::kLoads == part) dma(src(xg, xoff[i], i), xd + i * C::kThreads * 16);
 #pragma unroll
             for (int i = 0; i < C::PW; ++i)
-                put(g * kBlk + kw[i] < K ? wg + woff[i] : zero, slot + BT * kBlk + (wave * 64 + i * C::kThreads) * 16);
+                if ((C::PX + i) * parts / C::kLoads == part) dma(src(wg, woff[i], i), wd + i * C::kThreads * 16);
+        };
+        auto issue = [&](uint8_t* slot, int g) __attribute__((always_inline)) { issue_part(slot, g, 0, 1); };
+        // Row scales: kChunk groups at a time, through registers to a table (read group by group, each
+        // row's scale is a request of its own: more of them than the rows and weights make together).
+        // (entries past the last one are the last one again)
+        auto entry = [&](int i) __attribute__((always_inline)) { return min(tid + i * C::kThreads, BT * C::kChunk - 1); };
+        uint32_t toff[C::PT];
+#pragma unroll
+        for (int i = 0; i < C::PT; ++i) toff[i] = xrow_of(entry(i) / C::kChunk) * (uint32_t)G;
+        float tv[C::PT];
+        auto load_scales = [&](int g0) __attribute__((always_inline)) {
+#pragma unroll
+            for (int i = 0; i < C::PT; ++i)
+                tv[i] = p.xs[toff[i] + (uint32_t)min(g0 + entry(i) % C::kChunk, G - 1)];
+        };
+        auto store_scales = [&](int at) __attribute__((always_inline)) {
+#pragma unroll
+            for (int i = 0; i < C::PT; ++i) s_xs[at + entry(i) % C::kChunk * BT + entry(i) / C::kChunk] = tv[i];
+        };
+        const float* wsb = p.ws + (int64_t)e * p.NB * G;
+        const float* wsg = wsb + (int64_t)(min(col_of(wn * FN * 16), N - 1) / kBlk) * G;
+        const float* wsu = kSilu ? wsb + (int64_t)(min(col_of((wn * FN + FN - 1) * 16), N - 1) / kBlk) * G : wsg;
+
+        v4f run[FT][FN];
+#pragma unroll
+        for (int i = 0; i < FT; ++i)
+#pragma unroll
+            for (int j = 0; j < FN; ++j) run[i][j] = v4f{0.f, 0.f, 0.f, 0.f};
+
+        const int cr = (c ^ (c >> 3)) * kBlk;
+        const int p0 = cr + (((2 * q) ^ (c & 7)) << 4), p1 = cr + (((2 * q + 1) ^ (c & 7)) << 4);
+        const bool mine = !GROUPED || (now >> (wt * FT) & ((1u << FT) - 1)) != 0;   // this wave has rows in the pass
+        // One group: the rows' fragments against the columns', of which the next is read while one is
+        // multiplied and the one before is folded.
+        // next, gn: the slot and group whose loads are issued between the fragments, so that no wave waits
+        // for the address unit to take all of them (2048 x 4096 x 12288: 132 -> NN us)
+        auto compute = [&](const uint8_t* slot, uint8_t* next, int gn, int xs_at, float wg, float wu) __attribute__((always_inline)) {
+            auto frag = [&](int at, u32x4 (&f)[2]) __attribute__((always_inline)) {
+                f[0] = *reinterpret_cast<const u32x4*>(slot + at + p0);
+                f[1] = *reinterpret_cast<const u32x4*>(slot + at + p1);
+            };
+            u32x4 wf[2][2], xr[FT][2];
+            float xs[FT];
+            GroupOp<EXACT> xf[FT];
+            v4f pend[2][FT];
+            auto fold = [&](int j) __attribute__((always_inline)) {
+#pragma unroll
+                for (int i = 0; i < FT; ++i) {
+                    const float s = xs[i] * (kSilu && j >= FN / 2 ? wu : wg);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) run[i][j][r] = fmaf(pend[j & 1][i][r], s, run[i][j][r]);
+                }
+            };
+            if (mine) {
+                frag(C::kW + wn * FN * 16 * kBlk, wf[0]);
+#pragma unroll
+                for (int i = 0; i < FT; ++i) frag((wt * FT + i) * 16 * kBlk, xr[i]);
+#pragma unroll
+                for (int i = 0; i < FT; ++i) xs[i] = s_xs[xs_at + i * 16];
+#pragma unroll
+                for (int i = 0; i < FT; ++i) xf[i] = group_op<EXACT>(xr[i][0], xr[i][1]);
+            }
+#pragma unroll
+            for (int j = 0; j < FN; ++j) {
+                if (mine) {
+                    if (j + 1 < FN) frag(C::kW + (wn * FN + j + 1) * 16 * kBlk, wf[(j + 1) & 1]);
+                    __builtin_amdgcn_sched_barrier(0);
+                    const GroupOp<EXACT> w = group_op<EXACT>(wf[j & 1][0], wf[j & 1][1]);
+#pragma unroll
+                    for (int i = 0; i < FT; ++i) pend[j & 1][i] = group_mfma<EXACT>(w, xf[i]);
+                }
+                // (outside the branch: the same loads in flight along every path)
+                if (S > 2) issue_part(next, gn, j, FN);
+                if (mine && j > 0) fold(j - 1);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            if (mine) fold(FN - 1);
+        };
+
+        // Group g. Its stage has landed for this wave when no more than the next one's loads are in
+        // flight, and for all waves behind the barrier. With three slots the barrier also says that
+        // nobody reads group g - 1's slot, which the next loads go to; with two a second one does. Loads
+        // are issued in every step, past the last group too: the compiler counts those in flight along
+        // every path, and would wait for all of them where some path issues none.
+        auto step = [&](uint8_t* slot, uint8_t* next, int g, int xs_at, float wg, float wu) __attribute__((always_inline)) {
+            __builtin_amdgcn_s_waitcnt(wait_vm(C::kLoads));
+            group_barrier();
+            compute(slot, next, g + 2, xs_at, wg, wu);
+            __builtin_amdgcn_sched_barrier(0);
+            if constexpr (S == 2) {
+                group_barrier();
+                issue(slot, g + 2);
+            }
+        };
+        constexpr int kSpan = 64 * S / C::kChunk * C::kChunk;     // groups of a table of weight scales
+        float wgv[S], wuv[S];                                    // lane l: groups base + l S + t
+        int g = 0, base = 0;
+        auto ws_table = [&]() __attribute__((always_inline)) {
+            base = g;
+#pragma unroll
+            for (int t = 0; t < S; ++t) {
+                const int k = min(base + lane * S + t, G - 1);
+                wgv[t] = wsg[k];
+                wuv[t] = kSilu ? wsu[k] : 0.f;
+            }
+            // (waited for here: at their first use, in the loop, the wait would be every round's)
+#pragma unroll
+            for (int t = 0; t < S; ++t) asm volatile("" : "+v"(wgv[t]), "+v"(wuv[t]));
+        };
+        const int xs_lane = wt * FT * 16 + c;
+        // A chunk's table is written behind the first round of the chunk before: its last readers are past
+        // a barrier by then, and the chunk's own first barrier shows it to everybody.
+        load_scales(0);
+        ws_table();
+        store_scales(0);
+        issue(slot0, 0);
+        issue(slot1, 1);
+        load_scales(C::kChunk);
+        // (the ways out of the loop are jumps: with a flag the compiler counts loads in flight along paths
+        // from there back into the loop)
+        for (int at = 0;; at ^= C::kChunk * BT) {
+            if (g - base >= kSpan) ws_table();
+            int l = (g - base) / S, xa = at + xs_lane;
+            auto pick = [&](float v) __attribute__((always_inline)) {
+                return __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(v), l));
+            };
+            // S groups
+            auto round0 = [&]() __attribute__((always_inline)) { step(slot0, S > 2 ? slot2 : slot0, g, xa, pick(wgv[0]), pick(wuv[0])); };
+            auto round1 = [&]() __attribute__((always_inline)) { step(slot1, slot0, g, xa + BT, pick(wgv[1]), pick(wuv[1])); };
+            auto round2 = [&]() __attribute__((always_inline)) {
+                if constexpr (S > 2) step(slot2, slot1, g, xa + 2 * BT, pick(wgv[S > 2 ? 2 : 0]), pick(wuv[S > 2 ? 2 : 0]));
+            };
+            round0();
+            if (++g == G) goto summed;
+            round1();
+            if (++g == G) goto summed;
+            if constexpr (S > 2) {
+                round2();
+                if (++g == G) goto summed;
+            }
+            store_scales(at ^ (C::kChunk * BT));
+            load_scales(g - S + 2 * C::kChunk);
+            ++l;
+            xa += S * BT;
+            round0();
+            if (++g == G) goto summed;
+            round1();
+            if (++g == G) goto summed;
+            if constexpr (S > 2) {
+                round2();
+                if (++g == G) goto summed;
+            } else {
+                ++l;
+                xa += S * BT;
+                round0();
+                if (++g == G) goto summed;
+                round1();
+                if (++g == G) goto summed;
+            }
         }
-        // (waves past BT / 64 write what another one writes: every wave has the same count in flight)
-        __builtin_amdgcn_global_load_lds((global_cvoid_ptr)(reinterpret_cast<const uint8_t*>(p.xs + g) + opaque_u32(soff)),
-                                         (lds_void_ptr)(slot + (BT + BN) * kBlk + (wave * 64 % BT) * 4), 4, 0, 0);
-    };
-    constexpr int kOps = C::PX + C::PW + 1;
+    summed:
+        __builtin_amdgcn_s_waitcnt(wait_vm(0));                  // (the loads past the last group)
 
-    const float* wsb = p.ws + ((int64_t)e * p.NB + min(col0 + wn * FN * 16, N - 1) / kBlk) * G;
-
-    v4f run[FT][FN];
+        // ---- epilogue: lane (q, c) holds row 16 i + c, columns 4 q .. 4 q + 3 of each fragment ----
+        auto live = [&](int i, int& row) __attribute__((always_inline)) {
+            const int f = wt * FT + i;
+            row = row0 + f * 16 + c;
+            int xrow;
+            return (now >> f & 1) != 0 && block_slot(p, row, end, xrow) >= 0;
+        };
+        if constexpr (kSilu) {
+            // h of this wave's columns; a row's absmax over the 128 is joined over the waves in LDS
+            float* s_max = reinterpret_cast<float*>(slot0);      // [WN][BT]
+            float top[FT];
 #pragma unroll
-    for (int i = 0; i < FT; ++i)
+            for (int i = 0; i < FT; ++i) {
+                float m = 0.f;
 #pragma unroll
-        for (int j = 0; j < FN; ++j) run[i][j] = v4f{0.f, 0.f, 0.f, 0.f};
-
-    const int cr = c ^ (c >> 3);
-    const int p0 = (q ^ (c & 7)) << 4, p1 = ((q + 4) ^ (c & 7)) << 4;
-    const int x_lane = (wt * FT * 16 + cr) * kBlk, w_lane = BT * kBlk + (wn * FN * 16 + cr) * kBlk;
-    const int s_lane = (BT + BN) * kBlk + (wt * FT * 16 + c) * 4;
-    auto compute = [&](const uint8_t* slot, float ws) __attribute__((always_inline)) {
-        GroupOp<EXACT> xf[FT];
-        float s[FT];
+                for (int j = 0; j < FN / 2; ++j)
 #pragma unroll
-        for (int i = 0; i < FT; ++i) {
-            xf[i] = group_op<EXACT>(*reinterpret_cast<const u32x4*>(slot + x_lane + i * 16 * kBlk + p0),
-                                    *reinterpret_cast<const u32x4*>(slot + x_lane + i * 16 * kBlk + p1));
-            s[i] = *reinterpret_cast<const float*>(slot + s_lane + i * 64) * ws;
-        }
-        v4f pend[2][FT];
-        auto fold = [&](int j) __attribute__((always_inline)) {
+                    for (int r = 0; r < 4; ++r) {
+                        run[i][j][r] = silu_mul_f32(run[i][j][r], run[i][j + FN / 2][r]);
+                        m = fmaxf(m, fabsf(run[i][j][r]));
+                    }
+                top[i] = rows4_max(m);
+            }
+            group_barrier();                                     // (nobody reads slot 0 any more)
 #pragma unroll
             for (int i = 0; i < FT; ++i)
+                if (q == 0) s_max[wn * BT + (wt * FT + i) * 16 + c] = top[i];
+            lds_barrier();
 #pragma unroll
-                for (int r = 0; r < 4; ++r) run[i][j][r] = fmaf(pend[j & 1][i][r], s[i], run[i][j][r]);
-        };
+            for (int i = 0; i < FT; ++i) {
+                float m = s_max[(wt * FT + i) * 16 + c];
 #pragma unroll
-        for (int j = 0; j < FN; ++j) {
-            const GroupOp<EXACT> wf = group_op<EXACT>(*reinterpret_cast<const u32x4*>(slot + w_lane + j * 16 * kBlk + p0),
-                                                      *reinterpret_cast<const u32x4*>(slot + w_lane + j * 16 * kBlk + p1));
+                for (int w = 1; w < C::WN; ++w) m = fmaxf(m, s_max[w * BT + (wt * FT + i) * 16 + c]);
+                const float sc = act_scale_from_absmax(m), inv = 1.0f / sc;
+                int row;
+                if (!live(i, row)) continue;
 #pragma unroll
-            for (int i = 0; i < FT; ++i) pend[j & 1][i] = group_mfma<EXACT>(wf, xf[i]);
-            if (j > 0) fold(j - 1);
+                for (int j = 0; j < FN / 2; ++j)
+                    *reinterpret_cast<uint32_t*>(reinterpret_cast<uint8_t*>(p.out) + (int64_t)row * p.ldo +
+                                                 col_of((wn * FN + j) * 16) + 4 * q) =
+                        pack4_e4m3(run[i][j][0] * inv, run[i][j][1] * inv, run[i][j][2] * inv, run[i][j][3] * inv);
+                if (wn == 0 && q == 0) p.out_scales[(int64_t)row * (half / kBlk) + ct] = sc;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < FT; ++i) {
+                int row;
+                if (!live(i, row)) continue;
+#pragma unroll
+                for (int j = 0; j < FN; ++j) {
+                    const int col = col_of((wn * FN + j) * 16) + 4 * q;
+                    if (col < N) store16(p, row, col, N, run[i][j], p.out_bf16 != 0);
+                }
+            }
         }
-        fold(FN - 1);
-    };
-    // One group. Its stage has landed for this wave when no more than the later ones' loads are in
-    // flight, and for all waves behind the barrier. With three slots the barrier also says that
-    // nobody reads the slot of the group before, which the next loads go to; with two a second one does.
-    // LAST: the loads may end before the group does (the compiler counts loads in flight along every
-    // path: with the branches in the main loop it would wait for all of them in each round).
-    constexpr int kAhead = C::S == 2 ? 1 : C::S - 2;           // later stages in flight at the wait
-    auto step = [&](uint8_t* slot, uint8_t* next, int g, float ws, auto last) __attribute__((always_inline)) {
-        constexpr bool LAST = decltype(last)::value;
-        if (!LAST || g + kAhead < G) __builtin_amdgcn_s_waitcnt(wait_vm(kAhead * kOps));
-        else __builtin_amdgcn_s_waitcnt(wait_vm(0));
-        group_barrier();
-        if constexpr (C::S > 2)
-            if (!LAST || g + C::S - 1 < G) issue(next, g + C::S - 1, std::integral_constant<bool, !LAST>{});
-        __builtin_amdgcn_sched_barrier(0);
-        compute(slot, ws);
-        __builtin_amdgcn_sched_barrier(0);
-        if constexpr (C::S == 2) {
-            group_barrier();
-            if (!LAST || g + 2 < G) issue(slot, g + 2, std::integral_constant<bool, !LAST>{});
-        }
-    };
-    issue(slot0, 0, std::false_type{});
-    if (G > 1) issue(slot1, 1, std::false_type{});
-    constexpr int kIssued = C::S == 2 ? 2 : C::S - 1;          // a step issues the group this far on
-    constexpr int kSpan = 62 * C::S;                           // groups of a table of weight scales
-    int g = 0;
-    float wsv[C::S];                                           // lane l: groups base + l S + t
-    auto round = [&](int l, auto last) __attribute__((always_inline)) {
-        constexpr bool LAST = decltype(last)::value;
-        auto ws_of = [&](int t) __attribute__((always_inline)) {
-            return __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(wsv[t]), l));
-        };
-        step(slot0, C::S > 2 ? slot2 : slot0, g, ws_of(0), last);
-        if (!LAST || g + 1 < G) step(slot1, slot0, g + 1, ws_of(1), last);
-        if constexpr (C::S > 2)
-            if (!LAST || g + 2 < G) step(slot2, slot1, g + 2, ws_of(2), last);
-    };
-    int base;
-    do {
-        base = g;
-#pragma unroll
-        for (int t = 0; t < C::S; ++t) wsv[t] = wsb[min(base + lane * C::S + t, G - 1)];
-        for (; g + C::S + kIssued < G && g < base + kSpan; g += C::S) round((g - base) / C::S, std::false_type{});
-    } while (g + C::S + kIssued < G);
-    // (at most two rounds are left, and the table reaches two past its span)
-    for (; g < G; g += C::S) round((g - base) / C::S, std::true_type{});
-
-    // ---- epilogue: lane (q, c) holds row 16 i + c, columns 4 q .. 4 q + 3 of each fragment ----
-#pragma unroll
-    for (int i = 0; i < FT; ++i) {
-        const int row = row0 + (wt * FT + i) * 16 + c;
-        int xrow;
-        const int sl = block_slot(p, row, end, xrow);
-        if (sl < 0) continue;
-#pragma unroll
-        for (int j = 0; j < FN; ++j) {
-            const int col = col0 + (wn * FN + j) * 16 + 4 * q;
-            if (col >= N) continue;
-            store4<DST>(p, row, col, N, run[i][j]);
-        }
+        group_barrier();                                         // the slots are free for the next pass
     }
 }
 
-template <typename C, Dst DST, bool EXACT>
+template <typename C, Dst DST, bool GROUPED>
 int tiles_go(const BlockParams& p, hipStream_t s) {
-    const int ntiles = (p.N + C::BN - 1) / C::BN, mtiles = (p.P + C::BT - 1) / C::BT;
+    constexpr bool silu = DST == Dst::kSiluFp8;
+    const int ntiles = silu ? p.N / 2 / kBlk : (p.N + C::BN - 1) / C::BN, mtiles = (p.P + C::BT - 1) / C::BT;
     const int64_t items = (int64_t)mtiles * ntiles;
     if (items >= (int64_t)1 << 30) {
         set_error("fp8 block product: too many tiles");
         return W4A8_ERR_INVALID;
     }
-    launch_kernel(&block_tiles_kernel<C, DST, EXACT>, dim3((unsigned)((items + kTileXcds - 1) / kTileXcds * kTileXcds)),
-                  dim3(C::kThreads), 0, s, p, mtiles, ntiles);
+    const dim3 grid((unsigned)((items + kTileXcds - 1) / kTileXcds * kTileXcds));
+    if constexpr (!silu)
+        if (p.K % kBlk != 0) {
+            launch_kernel(&block_tiles_kernel<C, DST, silu, true, GROUPED>, grid, dim3(C::kThreads), 0, s, p, ntiles);
+            return check_launch("block_tiles_kernel");
+        }
+    launch_kernel(&block_tiles_kernel<C, DST, silu, false, GROUPED>, grid, dim3(C::kThreads), 0, s, p, ntiles);
     return check_launch("block_tiles_kernel");
 }
 
-#ifndef TILE
-#define TILE 4, 1, 4, 8, 3
-#endif
-using Tile256x256 = TileCfg<TILE>;
+using Tile64x64 = TileCfg<1, 4, 4, 1, 3>;       // four waves, three work-groups a CU
+using Tile64x128 = TileCfg<1, 4, 4, 2, 3>;      // four, two
+using Tile128x128 = TileCfg<2, 2, 4, 4, 2>;     // four, two
+using Tile256x128 = TileCfg<4, 2, 4, 4, 3>;     // eight, one
+using TileSilu = TileCfg<2, 4, 4, 4, 3>;        // 128 x 256: eight, one
 
 }  // namespace
+
+bool block_tiles_supported(const BlockArgs& a) {
+    // rows, scales and an expert's weights are addressed in 32 bits
+    const int64_t lim = (int64_t)1 << 32;
+    return a.src == Src::kFp8 && a.x_rows * a.ldx < lim && a.x_rows * blk_groups(a.K) * 4 < lim && a.N * a.K < lim &&
+           (a.dst == Dst::kF16 || a.dst == Dst::kBf16 ||
+            (a.dst == Dst::kSiluFp8 && a.sorted_ids != nullptr && a.K % kBlk == 0 && a.N % (2 * kBlk) == 0));
+}
 
 int launch_block_tiles(const BlockArgs& a, hipStream_t s) {
     const BlockParams p = block_params(a);
     if (p.P == 0) return W4A8_OK;
-    return a.dst == Dst::kBf16 ? tiles_go<Tile256x256, Dst::kBf16, false>(p, s) : tiles_go<Tile256x256, Dst::kF16, false>(p, s);
+    if (!block_tiles_supported(a)) {
+        set_error("fp8 block product: sizes not taken by the tiles");
+        return W4A8_ERR_INVALID;
+    }
+    if (a.dst == Dst::kSiluFp8) return tiles_go<TileSilu, Dst::kSiluFp8, true>(p, s);
+    if (a.sorted_ids != nullptr) {
+#ifndef GT
+#define GT Tile128x128
+#endif
+        return tiles_go<GT, Dst::kF16, true>(p, s);
+    }
+#ifdef DT
+    return tiles_go<DT, Dst::kF16, false>(p, s);
+#endif
+    return tiles_go<Tile256x128, Dst::kF16, false>(p, s);
 }
 
 }  // namespace w4a8
