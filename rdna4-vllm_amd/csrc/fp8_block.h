@@ -30,6 +30,8 @@ enum class Dst : int {
     kSiluF32 = 2,   // out[row, n] = silu(gate) * up in fp32, N = [gate | up] halves
     kSlotF32 = 3,   // out[slot, n] in fp32
     kSiluFp8 = 4,   // silu(gate) * up quantised: e4m3 rows (out) and their scales (out_scales)
+    kRowF16 = 5,    // out[row, n] in fp16 with a power of two per row and 32 columns (out_scales), so that
+                    // no value overflows and none loses bits to a fixed range
 };
 
 struct BlockArgs {
@@ -48,8 +50,9 @@ struct BlockArgs {
     Src src;
     Dst dst;
     void* out;
-    float* out_scales;           // kSiluFp8: (P, inter / 128)
+    float* out_scales;           // kSiluFp8: (P, inter / 128); kRowF16: (P, N / 32)
     int64_t ldo;
+    bool all_rows;               // padding rows of out may be written (tiles)
 };
 
 // The same on the device, sizes in 32 bits where they fit.
@@ -68,6 +71,7 @@ struct BlockParams {
     int x_rows, top_k, num_valid, block_m, gather;
     int out8;                    // out is aligned to 8 bytes
     int out_bf16;                // Dst::kBf16
+    int all_rows;
 };
 
 inline BlockParams block_params(const BlockArgs& a) {
@@ -80,6 +84,7 @@ inline BlockParams block_params(const BlockArgs& a) {
     p.NB = (int)blk_groups(a.N); p.E = (int)a.E;
     p.x_rows = (int)a.x_rows; p.top_k = (int)a.top_k; p.num_valid = (int)a.num_valid;
     p.block_m = (int)a.block_m; p.gather = a.gather ? 1 : 0;
+    p.all_rows = a.all_rows ? 1 : 0;
     p.out_bf16 = a.dst == Dst::kBf16 ? 1 : 0;
     p.out8 = reinterpret_cast<uintptr_t>(a.out) % 8 == 0 ? 1 : 0;
     return p;
@@ -150,8 +155,8 @@ int launch_block_stream(const BlockArgs& a, hipStream_t s);
 bool block_tiles_supported(const BlockArgs& a);
 int launch_block_tiles(const BlockArgs& a, hipStream_t s);
 // out[t, n] = sum over the slots j in order of tw[t, j] * y[slot_to_row[t, j], n] in fp32, rounded to
-// 16 bits; y (rows, N) in out's type, rows < 0 contribute nothing. N % 8 == 0.
-int launch_block_reduce(const void* y, const int32_t* slot_to_row, const float* tw, int64_t T, int64_t N,
+// 16 bits; y as kRowF16 leaves it, rows < 0 contribute nothing. N % 32 == 0.
+int launch_block_reduce(const void* y, const float* ys, const int32_t* slot_to_row, const float* tw, int64_t T, int64_t N,
                         int64_t top_k, void* out, bool bf16, hipStream_t s);
 
 }  // namespace w4a8

@@ -47,8 +47,9 @@ Dst dst_of(int dt) { return dt == W4A8_DTYPE_BF16 ? Dst::kBf16 : Dst::kF16; }
 
 // ---- the gated layer ----
 // Few rows an expert: blocks of 16 rows on the streaming kernels (rows quantised in registers, h and
-// the slots' rows in fp32). Else tiles: rows quantised beforehand, h by gemm1, the slots' rows in the
-// output's type, blocks of the 64 rows that a tile's wave takes.
+// the slots' rows in fp32). Else tiles: rows quantised beforehand, h by gemm1, the slots' rows in fp16
+// with scales (in the output's type they would add as much error as its own rounding: 1.5 times the
+// layer's in all), blocks of the 64 rows that a tile's wave takes.
 struct LayerPlan {
     bool tiles;
     int64_t block_m, P, nblk;
@@ -72,7 +73,7 @@ struct LayerScratch {
     void* align_ws;
     size_t align_bytes;
     uint8_t *xq, *hq;
-    float *xs, *hs, *h, *y32;
+    float *xs, *hs, *h, *y32, *ys;
     uint16_t* y16;
 };
 template <typename WS>
@@ -95,6 +96,7 @@ void carve_layer(WS& w, const LayerPlan& pl, int64_t T, int64_t H, int64_t inter
     m.hq = w.template take<uint8_t>((size_t)(pl.P * inter));
     m.hs = w.template take<float>((size_t)(pl.P * blk_groups(inter)));
     m.y16 = w.template take<uint16_t>((size_t)(pl.P * H));
+    m.ys = w.template take<float>((size_t)(pl.P * (H / 32)));
 }
 struct SizeProbe {
     WorkspaceSize s;
@@ -253,7 +255,7 @@ int w4a8_moe_fp8_block_apply(const void* x, int x_dtype, const float* x_scales, 
     g1.x_rows = T; g1.K = H; g1.ldx = H;
     g1.w = w13; g1.ws = w13_scales; g1.E = E; g1.N = 2 * inter;
     g1.sorted_ids = m.sti; g1.expert_ids = m.eid; g1.ntp = m.ntp; g1.P = pl.P;
-    g1.top_k = top_k; g1.num_valid = T * top_k; g1.block_m = pl.block_m; g1.gather = true;
+    g1.top_k = top_k; g1.num_valid = T * top_k; g1.block_m = pl.block_m; g1.gather = true; g1.all_rows = true;
     g1.src = pl.tiles ? Src::kFp8 : src_of(x_dtype);
     g1.dst = pl.tiles ? Dst::kSiluFp8 : Dst::kSiluF32;
     g1.out = pl.tiles ? (void*)m.hq : (void*)m.h; g1.out_scales = m.hs; g1.ldo = inter;
@@ -261,12 +263,12 @@ int w4a8_moe_fp8_block_apply(const void* x, int x_dtype, const float* x_scales, 
     g2.x = pl.tiles ? (const void*)m.hq : (const void*)m.h; g2.xs = m.hs; g2.x_rows = pl.P; g2.K = inter; g2.ldx = inter;
     g2.w = w2; g2.ws = w2_scales; g2.N = H; g2.gather = false;
     g2.src = pl.tiles ? Src::kFp8 : Src::kF32;
-    g2.dst = pl.tiles ? dst_of(out_dtype) : Dst::kSlotF32;
-    g2.out = pl.tiles ? (void*)m.y16 : (void*)m.y32; g2.ldo = H;
+    g2.dst = pl.tiles ? Dst::kRowF16 : Dst::kSlotF32;
+    g2.out = pl.tiles ? (void*)m.y16 : (void*)m.y32; g2.out_scales = m.ys; g2.ldo = H;
     if (pl.tiles) {
         if (int rc = launch_block_tiles(g1, s)) return rc;
         if (int rc = launch_block_tiles(g2, s)) return rc;
-        return launch_block_reduce(m.y16, m.s2r, topk_weights, T, H, top_k, out, bf16, s);
+        return launch_block_reduce(m.y16, m.ys, m.s2r, topk_weights, T, H, top_k, out, bf16, s);
     }
     if (int rc = launch_block_stream(g1, s)) return rc;
     if (int rc = launch_block_stream(g2, s)) return rc;

@@ -288,7 +288,8 @@ __global__ void __launch_bounds__(256) act_quant_groups_any_kernel(const void* _
 
 // Eight columns a lane; a token's rows are requested together, eight at a time.
 template <bool BF16>
-__global__ void __launch_bounds__(256) block_reduce_kernel(const void* __restrict__ y, const int32_t* __restrict__ s2r,
+__global__ void __launch_bounds__(256) block_reduce_kernel(const void* __restrict__ y, const float* __restrict__ ys,
+                                                           const int32_t* __restrict__ s2r,
                                                            const float* __restrict__ tw, int N, int top_k,
                                                            void* __restrict__ out) {
     const int64_t t = blockIdx.x;
@@ -307,13 +308,16 @@ __global__ void __launch_bounds__(256) block_reduce_kernel(const void* __restric
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             v[j] = u32x4{0, 0, 0, 0};
-            if (r[j] >= 0) v[j] = *reinterpret_cast<const u32x4*>(reinterpret_cast<const uint16_t*>(y) + (int64_t)r[j] * N + n);
+            if (r[j] >= 0) {
+                v[j] = *reinterpret_cast<const u32x4*>(reinterpret_cast<const uint16_t*>(y) + (int64_t)r[j] * N + n);
+                w[j] *= ys[(int64_t)r[j] * (N / 32) + n / 32];
+            }
         }
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             if (r[j] < 0) continue;
             float f[8];
-            unpack8<BF16>(v[j], f);
+            unpack8<false>(v[j], f);
 #pragma unroll
             for (int i = 0; i < 8; ++i) acc[i] = fmaf(w[j], f[i], acc[i]);
         }
@@ -370,12 +374,12 @@ int launch_rms_norm_quant(const NormArgs& a, hipStream_t s) {
     return check_launch("rms_norm_quant_any_kernel");
 }
 
-int launch_block_reduce(const void* y, const int32_t* slot_to_row, const float* tw, int64_t T, int64_t N,
+int launch_block_reduce(const void* y, const float* ys, const int32_t* slot_to_row, const float* tw, int64_t T, int64_t N,
                         int64_t top_k, void* out, bool bf16, hipStream_t s) {
     if (T == 0) return W4A8_OK;
     const dim3 grid((unsigned)T, (unsigned)((N / 8 + 255) / 256));
-    if (bf16) block_reduce_kernel<true><<<grid, 256, 0, s>>>(y, slot_to_row, tw, (int)N, (int)top_k, out);
-    else block_reduce_kernel<false><<<grid, 256, 0, s>>>(y, slot_to_row, tw, (int)N, (int)top_k, out);
+    if (bf16) block_reduce_kernel<true><<<grid, 256, 0, s>>>(y, ys, slot_to_row, tw, (int)N, (int)top_k, out);
+    else block_reduce_kernel<false><<<grid, 256, 0, s>>>(y, ys, slot_to_row, tw, (int)N, (int)top_k, out);
     return check_launch("block_reduce_kernel");
 }
 

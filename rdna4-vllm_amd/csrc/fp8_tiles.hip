@@ -20,6 +20,7 @@ using global_cvoid_ptr = const __attribute__((address_space(1))) void*;
 
 constexpr int kTileXcds = 8;
 constexpr int kRunRows = 4;       // row tiles of an XCD's run
+constexpr int kGroupedRuns = 64;  // grouped: runs at least, where there are that many row tiles
 
 // What pieces past the end of K are read from.
 __device__ __attribute__((aligned(16))) uint32_t g_zero_piece[4];
@@ -55,7 +56,7 @@ struct TileCfg {
 };
 
 template <typename C, Dst DST, bool EXACT, bool TAIL, bool GROUPED>
-__global__ void __launch_bounds__(C::kThreads, C::kWaves >= 8 || C::S == 2 ? 2 : 1) block_tiles_kernel(BlockParams p, int ntiles) {
+__global__ void __launch_bounds__(C::kThreads, 2) block_tiles_kernel(BlockParams p, int ntiles, int run_rows) {
     constexpr int FT = C::FT, FN = C::FN, BT = C::BT, BN = C::BN, S = C::S;
     constexpr bool kSilu = DST == Dst::kSiluFp8;
     static_assert(!kSilu || BN == 256, "SiLU tiles hold 128 gate and 128 up columns");
@@ -65,28 +66,63 @@ __global__ void __launch_bounds__(C::kThreads, C::kWaves >= 8 || C::S == 2 ? 2 :
     __shared__ __attribute__((aligned(1024))) uint8_t slot2[S > 2 ? C::kSlot : 16];
     __shared__ float s_xs[2 * C::kChunk * BT];                   // row scales [group][row] of two chunks
 
-    // ---- the tile: an XCD takes a contiguous run of those in use, kRunRows row tiles by all columns ----
-    const int end = GROUPED ? min(p.ntp[0], p.P) : p.P;
-    const int mtiles = (end + BT - 1) / BT;
-    const int items = mtiles * ntiles, perx = (items + kTileXcds - 1) / kTileXcds;
-    const int jx = blockIdx.x / kTileXcds, item = (int)(blockIdx.x % kTileXcds) * perx + jx;
-    if (jx >= perx || item >= items) return;
-    const int run_items = kRunRows * ntiles;
-    const int m0 = item / run_items * kRunRows, rem = item % run_items;
-    const int rows_here = min(kRunRows, mtiles - m0);
-    const int row0 = (m0 + rem % rows_here) * BT, ct = rem / rows_here;
+    // ---- the tile. Dense: an XCD takes a contiguous run of them, run_rows row tiles by all columns.
+    // Grouped: XCDs take such runs in turn (how many row tiles are in use is known on the device only;
+    // a tile finds its rows before it knows, so that the loads below go out together). ----
+    const int xcd = blockIdx.x % kTileXcds, jx = blockIdx.x / kTileXcds;
+    const int mall = (p.P + BT - 1) / BT, run_items = run_rows * ntiles;
+    int m_tile, ct;
+    if constexpr (GROUPED) {
+        const int rem = jx % run_items;
+        m_tile = (jx / run_items * kTileXcds + xcd) * run_rows + rem % run_rows;
+        ct = rem / run_rows;
+        if (m_tile >= mall) return;
+    } else {
+        const int items = mall * ntiles, perx = (items + kTileXcds - 1) / kTileXcds, item = xcd * perx + jx;
+        if (jx >= perx || item >= items) return;
+        const int m0 = item / run_items * run_rows, rem = item % run_items;
+        const int rows_here = min(run_rows, mall - m0);
+        m_tile = m0 + rem % rows_here;
+        ct = rem / rows_here;
+    }
+    const int row0 = m_tile * BT;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int q = lane >> 4, c = lane & 15;
     const int K = p.K, G = p.G, N = p.N;
 
-    // the expert of fragment f's rows (-1: none)
-    auto expert_of = [&](int f) __attribute__((always_inline)) {
-        const int r = row0 + 16 * f;
-        if (r >= end) return -1;
-        if constexpr (!GROUPED) return 0;
-        const int e = __builtin_amdgcn_readfirstlane(p.expert_ids[r / p.block_m]);
-        return e >= 0 && e < p.E ? e : -1;
+    // the expert of fragment `lane`'s rows (-1: none)
+    int fe = 0;
+    if constexpr (GROUPED) fe = p.expert_ids[min(row0 + 16 * (lane % (BT / 16)), p.P - 1) / p.block_m];
+    // row r of the tile: the row of x it reads (a row that exists, for rows of no use)
+    auto xrow_of = [&](int r) __attribute__((always_inline)) {
+        const int row = min(row0 + r, p.P - 1);
+        if constexpr (!GROUPED) return (uint32_t)row;
+        if (!p.gather) return (uint32_t)min(row, p.x_rows - 1);
+        const int s = p.sorted_ids[row];
+        return (uint32_t)(s >= 0 && s < p.num_valid ? min(s / p.top_k, p.x_rows - 1) : 0);
     };
+    auto piece_k = [&](int r) __attribute__((always_inline)) {         // the piece's first k within a group
+        const int j = (tid & 7) ^ (r & 7);
+        return ((j >> 1) | (j & 1) << 2) * 16;
+    };
+    auto piece_row = [&](int i) __attribute__((always_inline)) {
+        const int pr = (tid + i * C::kThreads) >> 3;
+        return pr ^ ((pr >> 3) & 1);
+    };
+    // (entries of a table of row scales past the last one are the last one again)
+    auto entry = [&](int i) __attribute__((always_inline)) { return min(tid + i * C::kThreads, BT * C::kChunk - 1); };
+    uint32_t xoff[C::PX], toff[C::PT];
+#pragma unroll
+    for (int i = 0; i < C::PX; ++i) xoff[i] = xrow_of(piece_row(i));
+#pragma unroll
+    for (int i = 0; i < C::PT; ++i) toff[i] = xrow_of(entry(i) / C::kChunk);
+    const int end = GROUPED ? min(p.ntp[0], p.P) : p.P;
+    if (row0 >= end) return;
+#pragma unroll
+    for (int i = 0; i < C::PX; ++i) xoff[i] = xoff[i] * (uint32_t)p.ldx + (uint32_t)piece_k(piece_row(i));
+#pragma unroll
+    for (int i = 0; i < C::PT; ++i) toff[i] *= (uint32_t)G;
+    if (lane >= BT / 16 || row0 + 16 * lane >= end || fe >= p.E) fe = -1;
     const int wt = wave / C::WN, wn = wave % C::WN;
     // the weight row behind row r of the slot's BN: fragment r / 16 belongs to wave r / (16 FN); kSilu
     // takes FN / 2 fragments of the gate half and the same of the up half
@@ -100,40 +136,18 @@ __global__ void __launch_bounds__(C::kThreads, C::kWaves >= 8 || C::S == 2 ? 2 :
         }
     };
 
-    uint32_t todo = 0;                                           // row fragments not yet done
-#pragma unroll 1
-    for (int f = 0; f < BT / 16; ++f)
-        if (expert_of(f) >= 0) todo |= 1u << f;
+    uint32_t todo = (uint32_t)__ballot(fe >= 0);                 // row fragments not yet done
     while (todo != 0) {
-        const int e = expert_of(__builtin_ctz(todo));
-        uint32_t now = 0;
-#pragma unroll 1
-        for (int f = 0; f < BT / 16; ++f)
-            if ((todo >> f & 1) && expert_of(f) == e) now |= 1u << f;
+        const int e = __builtin_amdgcn_readlane(fe, __builtin_ctz(todo));
+        const uint32_t now = (uint32_t)__ballot(fe == e) & todo;
         todo &= ~now;
-        // row r of the tile: the row of x it reads (a row that exists, for rows of no use)
-        auto xrow_of = [&](int r) __attribute__((always_inline)) {
-            int xrow;
-            block_slot(p, row0 + r, (now >> (r >> 4) & 1) ? end : 0, xrow);
-            return (uint32_t)xrow;
-        };
 
         // ---- staging: piece i of a thread is row (tid + i kThreads) / 8 of the slot, slot piece tid % 8.
         // Row r lies at place r ^ ((r >> 3) & 1), its piece j at (2 (j % 4) + j / 4) ^ (r & 7): the sixteen
         // lanes that a 16-byte LDS read serves at once then read different banks.
         const uint8_t* xb = reinterpret_cast<const uint8_t*>(p.x);
         const uint8_t* wb = p.w + (int64_t)e * N * K;
-        uint32_t xoff[C::PX], woff[C::PW];
-        auto piece_k = [&](int r) __attribute__((always_inline)) {     // the piece's first k within a group
-            const int j = (tid & 7) ^ (r & 7);
-            return ((j >> 1) | (j & 1) << 2) * 16;
-        };
-        auto piece_row = [&](int i) __attribute__((always_inline)) {
-            const int pr = (tid + i * C::kThreads) >> 3;
-            return pr ^ ((pr >> 3) & 1);
-        };
-#pragma unroll
-        for (int i = 0; i < C::PX; ++i) xoff[i] = xrow_of(piece_row(i)) * (uint32_t)p.ldx + (uint32_t)piece_k(piece_row(i));
+        uint32_t woff[C::PW];
 #pragma unroll
         for (int i = 0; i < C::PW; ++i)
             woff[i] = (uint32_t)min(col_of(piece_row(i)), N - 1) * (uint32_t)K + (uint32_t)piece_k(piece_row(i));
@@ -164,11 +178,6 @@ __global__ void __launch_bounds__(C::kThreads, C::kWaves >= 8 || C::S == 2 ? 2 :
         auto issue = [&](uint8_t* slot, int g) __attribute__((always_inline)) { issue_part(slot, g, 0, 1); };
         // Row scales: kChunk groups at a time, through registers to a table (read group by group, each
         // row's scale is a request of its own: more of them than the rows and weights make together).
-        // (entries past the last one are the last one again)
-        auto entry = [&](int i) __attribute__((always_inline)) { return min(tid + i * C::kThreads, BT * C::kChunk - 1); };
-        uint32_t toff[C::PT];
-#pragma unroll
-        for (int i = 0; i < C::PT; ++i) toff[i] = xrow_of(entry(i) / C::kChunk) * (uint32_t)G;
         float tv[C::PT];
         auto load_scales = [&](int g0) __attribute__((always_inline)) {
 #pragma unroll
@@ -327,8 +336,10 @@ __global__ void __launch_bounds__(C::kThreads, C::kWaves >= 8 || C::S == 2 ? 2 :
         auto live = [&](int i, int& row) __attribute__((always_inline)) {
             const int f = wt * FT + i;
             row = row0 + f * 16 + c;
-            int xrow;
-            return (now >> f & 1) != 0 && block_slot(p, row, end, xrow) >= 0;
+            if (!(now >> f & 1) || row >= end) return false;
+            if (!GROUPED || p.all_rows) return true;
+            const int s = p.sorted_ids[row];
+            return s >= 0 && s < p.num_valid && (p.gather ? s / p.top_k : row) < p.x_rows;
         };
         if constexpr (kSilu) {
             // h of this wave's columns; a row's absmax over the 128 is joined over the waves in LDS
@@ -366,6 +377,29 @@ __global__ void __launch_bounds__(C::kThreads, C::kWaves >= 8 || C::S == 2 ? 2 :
                         pack4_e4m3(run[i][j][0] * inv, run[i][j][1] * inv, run[i][j][2] * inv, run[i][j][3] * inv);
                 if (wn == 0 && q == 0) p.out_scales[(int64_t)row * (half / kBlk) + ct] = sc;
             }
+        } else if constexpr (DST == Dst::kRowF16) {
+            // a row's largest value of this wave's columns to [2^14, 2^15): infinities, NaN and zeros as they are
+#pragma unroll
+            for (int i = 0; i < FT; ++i) {
+                float m = 0.f;
+#pragma unroll
+                for (int j = 0; j < FN; ++j)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) m = fmaxf(m, fabsf(run[i][j][r]));
+                const uint32_t eb = __float_as_uint(rows4_max(m)) >> 23;
+                const uint32_t sb = eb == 0 || eb == 255 ? 127u : eb > 15 ? eb - 14 : 1u;
+                const float inv = __uint_as_float((254u - sb) << 23);
+                int row;
+                if (!live(i, row)) continue;
+#pragma unroll
+                for (int j = 0; j < FN; ++j) {
+                    const int col = col_of((wn * FN + j) * 16) + 4 * q;      // (whole tiles: N % 128 == 0)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) run[i][j][r] *= inv;
+                    store16(p, row, col, N, run[i][j], false);
+                    if (q == 0 && j % 2 == 0) p.out_scales[(int64_t)row * (N / 32) + col / 32] = __uint_as_float(sb << 23);
+                }
+            }
         } else {
 #pragma unroll
             for (int i = 0; i < FT; ++i) {
@@ -386,18 +420,21 @@ template <typename C, Dst DST, bool GROUPED>
 int tiles_go(const BlockParams& p, hipStream_t s) {
     constexpr bool silu = DST == Dst::kSiluFp8;
     const int ntiles = silu ? p.N / 2 / kBlk : (p.N + C::BN - 1) / C::BN, mtiles = (p.P + C::BT - 1) / C::BT;
-    const int64_t items = (int64_t)mtiles * ntiles;
+    const int run_rows = GROUPED ? std::max(1, std::min(kRunRows, mtiles / kGroupedRuns)) : kRunRows;
+    const int64_t runs = (mtiles + run_rows - 1) / run_rows;
+    const int64_t items = GROUPED ? (runs + kTileXcds - 1) / kTileXcds * kTileXcds * run_rows * ntiles
+                                  : ((int64_t)mtiles * ntiles + kTileXcds - 1) / kTileXcds * kTileXcds;
     if (items >= (int64_t)1 << 30) {
         set_error("fp8 block product: too many tiles");
         return W4A8_ERR_INVALID;
     }
-    const dim3 grid((unsigned)((items + kTileXcds - 1) / kTileXcds * kTileXcds));
-    if constexpr (!silu)
+    const dim3 grid((unsigned)items);
+    if constexpr (DST == Dst::kF16)
         if (p.K % kBlk != 0) {
-            launch_kernel(&block_tiles_kernel<C, DST, silu, true, GROUPED>, grid, dim3(C::kThreads), 0, s, p, ntiles);
+            launch_kernel(&block_tiles_kernel<C, DST, silu, true, GROUPED>, grid, dim3(C::kThreads), 0, s, p, ntiles, run_rows);
             return check_launch("block_tiles_kernel");
         }
-    launch_kernel(&block_tiles_kernel<C, DST, silu, false, GROUPED>, grid, dim3(C::kThreads), 0, s, p, ntiles);
+    launch_kernel(&block_tiles_kernel<C, DST, silu, false, GROUPED>, grid, dim3(C::kThreads), 0, s, p, ntiles, run_rows);
     return check_launch("block_tiles_kernel");
 }
 
@@ -405,7 +442,10 @@ using Tile64x64 = TileCfg<1, 4, 4, 1, 3>;       // four waves, three work-groups
 using Tile64x128 = TileCfg<1, 4, 4, 2, 3>;      // four, two
 using Tile128x128 = TileCfg<2, 2, 4, 4, 2>;     // four, two
 using Tile256x128 = TileCfg<4, 2, 4, 4, 3>;     // eight, one
-using TileSilu = TileCfg<2, 4, 4, 4, 3>;        // 128 x 256: eight, one
+#ifndef ST
+#define ST 1, 8, 4, 2, 3
+#endif
+using TileSilu = TileCfg<ST>;        // 64 x 256: eight, one
 
 }  // namespace
 
@@ -414,6 +454,7 @@ bool block_tiles_supported(const BlockArgs& a) {
     const int64_t lim = (int64_t)1 << 32;
     return a.src == Src::kFp8 && a.x_rows * a.ldx < lim && a.x_rows * blk_groups(a.K) * 4 < lim && a.N * a.K < lim &&
            (a.dst == Dst::kF16 || a.dst == Dst::kBf16 ||
+            (a.dst == Dst::kRowF16 && a.sorted_ids != nullptr && a.K % kBlk == 0 && a.N % kBlk == 0) ||
             (a.dst == Dst::kSiluFp8 && a.sorted_ids != nullptr && a.K % kBlk == 0 && a.N % (2 * kBlk) == 0));
 }
 
@@ -425,6 +466,10 @@ int launch_block_tiles(const BlockArgs& a, hipStream_t s) {
         return W4A8_ERR_INVALID;
     }
     if (a.dst == Dst::kSiluFp8) return tiles_go<TileSilu, Dst::kSiluFp8, true>(p, s);
+#ifndef LT
+#define LT Tile64x128
+#endif
+    if (a.dst == Dst::kRowF16) return tiles_go<LT, Dst::kRowF16, true>(p, s);
     if (a.sorted_ids != nullptr) {
 #ifndef GT
 #define GT Tile128x128
