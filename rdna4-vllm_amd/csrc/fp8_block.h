@@ -25,7 +25,7 @@ enum class Src : int {
 };
 // What it writes.
 enum class Dst : int {
-    kF16 = 0,       // out[row, n] rounded to fp16 / bf16
+    kF16 = 0,       // out[row, n] rounded to fp16, or to bf16 (the kernels have one form for both)
     kBf16 = 1,
     kSiluF32 = 2,   // out[row, n] = silu(gate) * up in fp32, N = [gate | up] halves
     kSlotF32 = 3,   // out[slot, n] in fp32

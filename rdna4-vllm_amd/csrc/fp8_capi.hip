@@ -22,7 +22,7 @@ bool is16(int dt) { return dt == W4A8_DTYPE_F16 || dt == W4A8_DTYPE_BF16; }
 
 constexpr int64_t kMaxSide = (int64_t)1 << 24;    // rows of a weight, values of a row
 constexpr int64_t kMaxRows = ((int64_t)1 << 31) - 256;
-constexpr int64_t kStreamRows = 64;               // dense rows up to which the weights are streamed
+constexpr int64_t kStreamRows = 16;               // dense rows up to which the weights are streamed
 
 // Sizes and pointers that every product shares.
 int check_product(const void* x, int x_dtype, const float* xs, int64_t rows, int64_t K, int64_t ldx, const uint8_t* w,
@@ -57,7 +57,7 @@ struct LayerPlan {
 LayerPlan plan_layer(int64_t T, int64_t H, int64_t inter, int64_t E, int64_t top_k) {
     LayerPlan pl;
     const int64_t lim = (int64_t)1 << 32;
-    pl.tiles = T * top_k > 16 * E;
+    pl.tiles = T * top_k > 12 * E;
     pl.block_m = pl.tiles ? 64 : 16;
     pl.P = w4a8_moe_align_sorted_len(T * top_k, E, pl.block_m);
     if (pl.tiles && (T * H >= lim || pl.P * inter >= lim || 2 * inter * H >= lim)) {
@@ -65,6 +65,8 @@ LayerPlan plan_layer(int64_t T, int64_t H, int64_t inter, int64_t E, int64_t top
         pl.block_m = 16;
         pl.P = w4a8_moe_align_sorted_len(T * top_k, E, pl.block_m);
     }
+    // (every block in use holds a slot: few slots reach a small part of what the experts' padding allows)
+    pl.P = std::min(pl.P, T * top_k * pl.block_m);
     pl.nblk = pl.P / pl.block_m;
     return pl;
 }
@@ -201,7 +203,10 @@ int w4a8_moe_fp8_block_gemm(const void* x, const float* x_scales, int64_t x_rows
     a.sorted_ids = sorted_token_ids; a.expert_ids = expert_ids; a.ntp = num_tokens_post_padded;
     a.P = P; a.top_k = top_k; a.num_valid = num_slots; a.block_m = block_m; a.gather = gather != 0;
     a.src = Src::kFp8; a.dst = dst_of(out_dtype); a.out = out; a.ldo = N;
-    if (std::min(P, num_slots) > 16 * E && block_tiles_supported(a)) return launch_block_tiles(a, as_stream(stream));
+    // Blocks of 16: tiles pass over several experts (256 x 8 rows of 2048 -> 1024: 105 us, streamed 101;
+    // 16 rows an expert 137 / 135; 64 rows 110 / 222). Blocks of 64: streaming would find three of four row
+    // fragments empty (0.75 rows an expert: 170 us, tiles 58).
+    if ((block_m >= 64 || std::min(P, num_slots) > 32 * E) && block_tiles_supported(a)) return launch_block_tiles(a, as_stream(stream));
     return launch_block_stream(a, as_stream(stream));
 }
 

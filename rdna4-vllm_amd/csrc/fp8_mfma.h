@@ -5,22 +5,22 @@
 
 namespace w4a8 {
 
-using v8h = _Float16 __attribute__((ext_vector_type(8)));
+using v8bf = __bf16 __attribute__((ext_vector_type(8)));
 
-__device__ __forceinline__ v8h e4m3_to_half8(uint32_t lo, uint32_t hi) {
-    using v2h = _Float16 __attribute__((ext_vector_type(2)));
-    const v2h a = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)lo, 1.0f, false);
-    const v2h b = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)lo, 1.0f, true);
-    const v2h c = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)hi, 1.0f, false);
-    const v2h d = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)hi, 1.0f, true);
-    return v8h{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+__device__ __forceinline__ v8bf e4m3_to_bf16x8(uint32_t lo, uint32_t hi) {
+    using v2bf = __bf16 __attribute__((ext_vector_type(2)));
+    const v2bf a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)lo, 1.0f, false);
+    const v2bf b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)lo, 1.0f, true);
+    const v2bf c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)hi, 1.0f, false);
+    const v2bf d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)hi, 1.0f, true);
+    return v8bf{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
 // A lane's 32 e4m3 values of one row and group of 128 k (16-byte pieces q and q + 4) as an operand:
-// as they are, or (EXACT) as fp16.
+// as they are, or (EXACT) as bf16.
 //
 // The fp8 matrix core cuts products of eight neighbouring k to 2^-13 of their largest; EXACT feeds
-// the fp16 one (every e4m3 number is an fp16 number), which adds them as fp32 numbers, at a quarter
+// the bf16 one (every e4m3 number is a bf16 number), which adds them as fp32 numbers, at a quarter
 // of the rate and for sixteen conversions an operand. It is for sums that are quantised again: an
 // error of 1e-4 there moves values across a border between two e4m3 numbers, and the layer's output
 // by 1e-3 (one token by up to 6e-3), up to three times what the rounding to bf16 does.
@@ -30,16 +30,16 @@ struct GroupOp {
 };
 template <>
 struct GroupOp<true> {
-    v8h h[4];
+    v8bf h[4];
 };
 template <bool EXACT>
 __device__ __forceinline__ GroupOp<EXACT> group_op(const u32x4& lo, const u32x4& hi) {
     GroupOp<EXACT> o;
     if constexpr (EXACT) {
-        o.h[0] = e4m3_to_half8(lo[0], lo[1]);
-        o.h[1] = e4m3_to_half8(lo[2], lo[3]);
-        o.h[2] = e4m3_to_half8(hi[0], hi[1]);
-        o.h[3] = e4m3_to_half8(hi[2], hi[3]);
+        o.h[0] = e4m3_to_bf16x8(lo[0], lo[1]);
+        o.h[1] = e4m3_to_bf16x8(lo[2], lo[3]);
+        o.h[2] = e4m3_to_bf16x8(hi[0], hi[1]);
+        o.h[3] = e4m3_to_bf16x8(hi[2], hi[3]);
     } else {
         o.b = v8i{(int)lo[0], (int)lo[1], (int)lo[2], (int)lo[3], (int)hi[0], (int)hi[1], (int)hi[2], (int)hi[3]};
     }
@@ -50,10 +50,10 @@ template <bool EXACT>
 __device__ __forceinline__ v4f group_mfma(const GroupOp<EXACT>& w, const GroupOp<EXACT>& x) {
     const v4f zero{0.f, 0.f, 0.f, 0.f};
     if constexpr (EXACT) {
-        v4f t = __builtin_amdgcn_mfma_f32_16x16x32_f16(w.h[0], x.h[0], zero, 0, 0, 0);
-        t = __builtin_amdgcn_mfma_f32_16x16x32_f16(w.h[1], x.h[1], t, 0, 0, 0);
-        t = __builtin_amdgcn_mfma_f32_16x16x32_f16(w.h[2], x.h[2], t, 0, 0, 0);
-        return __builtin_amdgcn_mfma_f32_16x16x32_f16(w.h[3], x.h[3], t, 0, 0, 0);
+        v4f t = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w.h[0], x.h[0], zero, 0, 0, 0);
+        t = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w.h[1], x.h[1], t, 0, 0, 0);
+        t = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w.h[2], x.h[2], t, 0, 0, 0);
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(w.h[3], x.h[3], t, 0, 0, 0);
     } else {
         return mfma_16x16x128(w.b, x.b, zero);
     }
@@ -78,7 +78,7 @@ __device__ __forceinline__ void store4(const BlockParams& p, int64_t orow, int c
         // (whole layers: multiples of 128 columns)
         *reinterpret_cast<v4f*>(reinterpret_cast<float*>(p.out) + orow * p.ldo + col) = t;
     } else {
-        store16(p, orow, col, cols, t, DST == Dst::kBf16);
+        store16(p, orow, col, cols, t, p.out_bf16 != 0);
     }
 }
 

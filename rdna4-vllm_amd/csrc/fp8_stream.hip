@@ -1,12 +1,12 @@
 // Block-scaled fp8 products of few rows (gfx950): the weights are streamed once, dense or grouped.
 //
-// Bound: HBM, every weight once per 16 FT rows. Weights go from memory to the MFMA operands' registers
+// Bound: HBM, every weight once per 16 rows. Weights go from memory to the MFMA operands' registers
 // with no detour: of each group of 128 values, lane (q, c) = (lane / 16, lane % 16) holds the 16-byte
 // pieces q and q + 4 of row c, for rows and weights alike, so a load instruction touches 64 contiguous
 // bytes of sixteen rows. Weights are the first operand: a lane ends up with four adjacent columns of
 // one row, and the scale xs[row, g] * ws[block, g] is one number a lane and group.
 //
-// block_rows_kernel holds its rows in registers (16 FT rows by GPW groups a wave, quantised there
+// block_rows_kernel holds its rows in registers (16 rows by GPW groups a wave, quantised there
 // where they come in 16 or 32 bits) and walks over column fragments with D of them in flight; KS
 // waves share K and add their sums in LDS, one barrier per D fragments. block_stream_kernel takes any
 // K and reads the rows again for each column fragment.
@@ -78,37 +78,39 @@ __device__ __forceinline__ GroupOp<EXACT> row_operand(const RowRaw<SRC>& r, int 
     return group_op<EXACT>(u32x4{o[0], o[1], o[2], o[3]}, u32x4{o[4], o[5], o[6], o[7]});
 }
 
-// The expert and the end of the rows in use of the rows from row0; false: nothing to do.
-__device__ __forceinline__ bool block_expert(const BlockParams& p, int row0, int& e, int& end) {
+// The expert and the end of the rows in use of the 16 rows from row0, c of them this lane's; false:
+// nothing to do (blocks of more rows end in whole fragments of padding).
+__device__ __forceinline__ bool block_expert(const BlockParams& p, int row0, int c, int& e, int& end) {
     e = 0;
     end = p.P;
     if (p.sorted_ids != nullptr) {
-        end = min(p.ntp[0], p.P);
-        if (row0 >= end) return false;
+        const int s = p.sorted_ids[min(row0 + c, p.P - 1)];
         e = __builtin_amdgcn_readfirstlane(p.expert_ids[row0 / p.block_m]);
-        if (e < 0 || e >= p.E) return false;
+        end = min(p.ntp[0], p.P);
+        if (row0 >= end || e < 0 || e >= p.E) return false;
+        if (__ballot(row0 + c < end && s >= 0 && s < p.num_valid) == 0) return false;
     }
     return true;
 }
 
 // CG groups of KS waves; a group walks over its own `per` column fragments (kSiluF32: fragments of
-// the gate half, each with its up fragment), D in flight. part: [2][CG][D][FT][KS][64] v4f in LDS.
-template <int FT, int GPW, int KS, int CG, int D, Src SRC, Dst DST>
+// the gate half, each with its up fragment), D in flight. part: [2][CG][D][KS][64] v4f in LDS.
+template <int GPW, int KS, int CG, int D, Src SRC, Dst DST>
 __global__ void __launch_bounds__(64 * KS * CG) block_rows_kernel(BlockParams p, int slices, int per) {
     constexpr bool kSilu = DST == Dst::kSiluF32;
     constexpr bool EXACT = kSilu;
     constexpr int kPair = kSilu ? 2 : 1;                       // fragments of one output fragment
     static_assert(D % kPair == 0, "an output fragment's parts are in flight together");
-    constexpr int kUnits = D / kPair * FT;                     // output fragments of one round
-    __shared__ __attribute__((aligned(16))) v4f part[KS > 1 ? 2 : 1][KS > 1 ? CG : 1][KS > 1 ? D * FT : 1]
+    constexpr int kUnits = D / kPair;                     // output fragments of one round
+    __shared__ __attribute__((aligned(16))) v4f part[KS > 1 ? 2 : 1][KS > 1 ? CG : 1][KS > 1 ? D : 1]
                                                     [KS > 1 ? KS : 1][64];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int ks = wave % KS, cg = wave / KS;
     const int q = lane >> 4, c = lane & 15;
     const int tb = blockIdx.x / slices, sl = blockIdx.x % slices;
-    const int row0 = tb * (16 * FT);
+    const int row0 = tb * 16;
     int e, end;
-    if (!block_expert(p, row0, e, end)) return;
+    if (!block_expert(p, row0, c, e, end)) return;
     const int half = p.N / 2;
     const int cols = kSilu ? half : p.N;
     const int K = p.K, G = p.G;
@@ -124,7 +126,7 @@ __global__ void __launch_bounds__(64 * KS * CG) block_rows_kernel(BlockParams p,
         float ws[GPW];
     };
     auto load = [&](Stage& s, int i) __attribute__((always_inline)) {
-        const int f = min(f0 + i / kPair, frags - 1);
+        const int f = min(f0 + min(i / kPair, per - 1), frags - 1);
         const int up = kSilu && (i & 1) ? half : 0;
         // (columns past the end read the last one; never stored)
         const uint8_t* wr = we + (int64_t)(up + min(f * 16 + c, cols - 1)) * K;
@@ -144,81 +146,71 @@ __global__ void __launch_bounds__(64 * KS * CG) block_rows_kernel(BlockParams p,
     __builtin_amdgcn_sched_barrier(0);
 
     // ---- rows, held ----
-    int slot[FT];
-    GroupOp<EXACT> x[FT][GPW];
-    float xs[FT][GPW];
+    GroupOp<EXACT> x[GPW];
+    float xs[GPW];
+    int xrow;
+    const int slot = block_slot(p, row0 + c, end, xrow);
+    const uint8_t* xp = reinterpret_cast<const uint8_t*>(p.x) + (int64_t)xrow * p.ldx * kSrcBytes<SRC>;
+    // (some groups' raw bytes at a time: all of them beside the ring would not fit the registers)
+    constexpr int kAt = SRC == Src::kF32 ? (GPW < 2 ? GPW : 2) : GPW < 4 ? GPW : 4;
+    static_assert(GPW % kAt == 0, "groups divide");
 #pragma unroll
-    for (int i = 0; i < FT; ++i) {
-        int xrow;
-        slot[i] = block_slot(p, row0 + 16 * i + c, end, xrow);
-        const uint8_t* xp = reinterpret_cast<const uint8_t*>(p.x) + (int64_t)xrow * p.ldx * kSrcBytes<SRC>;
-        // (some groups' raw bytes at a time: all of them beside the ring would not fit the registers)
-        constexpr int kAt = SRC == Src::kF32 ? (GPW < 2 ? GPW : 2) : GPW < 4 ? GPW : 4;
-        static_assert(GPW % kAt == 0, "groups divide");
+    for (int j0 = 0; j0 < GPW; j0 += kAt) {
+        RowRaw<SRC> raw[kAt];
 #pragma unroll
-        for (int j0 = 0; j0 < GPW; j0 += kAt) {
-            RowRaw<SRC> raw[kAt];
-#pragma unroll
-            for (int j = 0; j < kAt; ++j) {
-                const int g = min(g0 + j0 + j, G - 1);
-                row_load(raw[j], xp, g, q, K);
-                xs[i][j0 + j] = 0.f;
-                if constexpr (SRC == Src::kFp8) xs[i][j0 + j] = p.xs[(int64_t)xrow * G + g];
-            }
-#pragma unroll
-            for (int j = 0; j < kAt; ++j) {
-                // groups past the end: zero rows and a zero scale (what the clamped addresses hold
-                // counts in its own group)
-                const int g = g0 + j0 + j;
-                x[i][j0 + j] = row_operand<SRC, EXACT>(raw[j], g, q, K, xs[i][j0 + j]);
-                if (g >= G) xs[i][j0 + j] = 0.f;
-            }
-            __builtin_amdgcn_sched_barrier(0);
+        for (int j = 0; j < kAt; ++j) {
+            const int g = min(g0 + j0 + j, G - 1);
+            row_load(raw[j], xp, g, q, K);
+            xs[j0 + j] = 0.f;
+            if constexpr (SRC == Src::kFp8) xs[j0 + j] = p.xs[(int64_t)xrow * G + g];
         }
+#pragma unroll
+        for (int j = 0; j < kAt; ++j) {
+            // groups past the end: zero rows and a zero scale (what the clamped addresses hold
+            // counts in its own group)
+            const int g = g0 + j0 + j;
+            x[j0 + j] = row_operand<SRC, EXACT>(raw[j], g, q, K, xs[j0 + j]);
+            if (g >= G) xs[j0 + j] = 0.f;
+        }
+        __builtin_amdgcn_sched_barrier(0);
     }
 
     const int mine = min(per, frags - f0);                     // output fragments of this group (may be <= 0)
     const int rounds = (per * kPair + D - 1) / D;              // of the work-group: the barriers agree
     for (int it = 0; it < rounds; ++it) {
-        v4f run[D][FT];
+        v4f run[D];
 #pragma unroll
         for (int d = 0; d < D; ++d) {
+            run[d] = v4f{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int i = 0; i < FT; ++i) {
-                run[d][i] = v4f{0.f, 0.f, 0.f, 0.f};
+            for (int j = 0; j < GPW; ++j) {
+                const v4f t = group_mfma<EXACT>(group_op<EXACT>(ring[d].w[j][0], ring[d].w[j][1]), x[j]);
+                const float s = xs[j] * ring[d].ws[j];
 #pragma unroll
-                for (int j = 0; j < GPW; ++j) {
-                    const v4f t = group_mfma<EXACT>(group_op<EXACT>(ring[d].w[j][0], ring[d].w[j][1]), x[i][j]);
-                    const float s = xs[i][j] * ring[d].ws[j];
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) run[d][i][r] = fmaf(t[r], s, run[d][i][r]);
-                }
+                for (int r = 0; r < 4; ++r) run[d][r] = fmaf(t[r], s, run[d][r]);
             }
             __builtin_amdgcn_sched_barrier(0);
             load(ring[d], (it + 1) * D + d);
             __builtin_amdgcn_sched_barrier(0);
         }
-        // unit u of the round: output fragment u / FT, row fragment u % FT
-        auto put = [&](int u, v4f t, const v4f& up, int sl_id) __attribute__((always_inline)) {
-            const int of = it * (D / kPair) + u / FT;
+        // unit u of the round: an output fragment
+        auto put = [&](int u, v4f t, const v4f& up) __attribute__((always_inline)) {
+            const int of = it * kUnits + u;
             const int col = (f0 + of) * 16 + 4 * q;
             if constexpr (kSilu) {
 #pragma unroll
                 for (int r = 0; r < 4; ++r) t[r] = silu_mul_f32(t[r], up[r]);
             }
-            if (of >= mine || sl_id < 0 || col >= cols) return;
-            store4<DST>(p, DST == Dst::kSlotF32 ? sl_id : row0 + 16 * (u % FT) + c, col, cols, t);
+            if (of >= mine || slot < 0 || col >= cols) return;
+            store4<DST>(p, DST == Dst::kSlotF32 ? slot : row0 + c, col, cols, t);
         };
         if constexpr (KS == 1) {
 #pragma unroll
-            for (int u = 0; u < kUnits; ++u)
-                put(u, run[u / FT * kPair][u % FT], run[u / FT * kPair + kPair - 1][u % FT], slot[u % FT]);
+            for (int u = 0; u < kUnits; ++u) put(u, run[u * kPair], run[u * kPair + kPair - 1]);
         } else {
             auto& buf = part[it & 1][cg];
 #pragma unroll
-            for (int d = 0; d < D; ++d)
-#pragma unroll
-                for (int i = 0; i < FT; ++i) buf[d * FT + i][ks][lane] = run[d][i];
+            for (int d = 0; d < D; ++d) buf[d][ks][lane] = run[d];
             lds_barrier();
             // (the next round writes the other buffer; this one is written again behind its barrier)
 #pragma unroll
@@ -226,18 +218,14 @@ __global__ void __launch_bounds__(64 * KS * CG) block_rows_kernel(BlockParams p,
                 const int u = u0 + ks;
                 if (kUnits % KS != 0 && u >= kUnits) break;
                 auto total = [&](int d) __attribute__((always_inline)) {
-                    v4f t = buf[d * FT + u % FT][0][lane];
+                    v4f t = buf[d][0][lane];
 #pragma unroll
-                    for (int w = 1; w < KS; ++w) t += buf[d * FT + u % FT][w][lane];
+                    for (int w = 1; w < KS; ++w) t += buf[d][w][lane];
                     return t;
                 };
-                const v4f t = total(u / FT * kPair);
-                int sl_id = slot[0];
-#pragma unroll
-                for (int i = 1; i < FT; ++i)
-                    if (u % FT == i) sl_id = slot[i];
-                if constexpr (kSilu) put(u, t, total(u / FT * kPair + 1), sl_id);
-                else put(u, t, t, sl_id);
+                const v4f t = total(u * kPair);
+                if constexpr (kSilu) put(u, t, total(u * kPair + 1));
+                else put(u, t, t);
             }
         }
     }
@@ -245,18 +233,18 @@ __global__ void __launch_bounds__(64 * KS * CG) block_rows_kernel(BlockParams p,
 
 // Any K: KS waves take the K groups in turn (what they read at one time is contiguous along K).
 constexpr int kRing = 3;          // groups of a wave in flight
-template <int FT, int FN, int KS, Src SRC, Dst DST>
+template <int FN, int KS, Src SRC, Dst DST>
 __global__ void __launch_bounds__(64 * KS) block_stream_kernel(BlockParams p, int slices) {
     constexpr bool kSilu = DST == Dst::kSiluF32;
     constexpr bool EXACT = kSilu;
     constexpr int kCols = kSilu ? FN / 2 : FN;                 // column fragments of the output
-    __shared__ __attribute__((aligned(16))) v4f part[KS][FT * FN][64];
+    __shared__ __attribute__((aligned(16))) v4f part[KS][FN][64];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int q = lane >> 4, c = lane & 15;
     const int tb = blockIdx.x / slices, sl = blockIdx.x % slices;
-    const int row0 = tb * (16 * FT);
+    const int row0 = tb * 16;
     int e, end;
-    if (!block_expert(p, row0, e, end)) return;
+    if (!block_expert(p, row0, c, e, end)) return;
     const int half = p.N / 2;
     const int cols = kSilu ? half : p.N;
     const int K = p.K, G = p.G;
@@ -269,20 +257,15 @@ __global__ void __launch_bounds__(64 * KS) block_stream_kernel(BlockParams p, in
         wp[j] = p.w + ((int64_t)e * p.N + up + min(f + c, cols - 1)) * K;
         wsp[j] = p.ws + ((int64_t)e * p.NB + (up + min(f, cols - 1)) / kBlk) * G;
     }
-    const uint8_t* xp[FT];
-    const float* xsp[FT];
-#pragma unroll
-    for (int i = 0; i < FT; ++i) {
-        int xrow;
-        block_slot(p, row0 + 16 * i + c, end, xrow);
-        xp[i] = reinterpret_cast<const uint8_t*>(p.x) + (int64_t)xrow * p.ldx * kSrcBytes<SRC>;
-        xsp[i] = p.xs + (SRC == Src::kFp8 ? (int64_t)xrow * G : 0);
-    }
+    int xrow;
+    const int slot = block_slot(p, row0 + c, end, xrow);
+    const uint8_t* xp = reinterpret_cast<const uint8_t*>(p.x) + (int64_t)xrow * p.ldx * kSrcBytes<SRC>;
+    const float* xsp = p.xs + (SRC == Src::kFp8 ? (int64_t)xrow * G : 0);
     struct Stage {
         u32x4 w[FN][2];
-        RowRaw<SRC> x[FT];
+        RowRaw<SRC> x;
         float ws[FN];
-        float xs[FT];
+        float xs;
     };
     auto load = [&](Stage& s, int step) __attribute__((always_inline)) {
         const int g = min(step * KS + wave, G - 1);
@@ -293,31 +276,23 @@ __global__ void __launch_bounds__(64 * KS) block_stream_kernel(BlockParams p, in
                 s.w[j][h] = *reinterpret_cast<const u32x4*>(wp[j] + min(g * kBlk + h * 64 + q * 16, K - 16));
             s.ws[j] = wsp[j][g];
         }
-#pragma unroll
-        for (int i = 0; i < FT; ++i) {
-            row_load(s.x[i], xp[i], g, q, K);
-            if constexpr (SRC == Src::kFp8) s.xs[i] = xsp[i][g];
-        }
+        row_load(s.x, xp, g, q, K);
+        if constexpr (SRC == Src::kFp8) s.xs = xsp[g];
     };
-    v4f run[FT][FN];
+    v4f run[FN];
 #pragma unroll
-    for (int i = 0; i < FT; ++i)
-#pragma unroll
-        for (int j = 0; j < FN; ++j) run[i][j] = v4f{0.f, 0.f, 0.f, 0.f};
+    for (int j = 0; j < FN; ++j) run[j] = v4f{0.f, 0.f, 0.f, 0.f};
     auto consume = [&](const Stage& s, int step) __attribute__((always_inline)) {
         const int g = step * KS + wave;
+        float xs = s.xs;
+        const GroupOp<EXACT> xv = row_operand<SRC, EXACT>(s.x, g, q, K, xs);   // zero past the end
+        if (g >= G) xs = 0.f;
 #pragma unroll
-        for (int i = 0; i < FT; ++i) {
-            float xs = s.xs[i];
-            const GroupOp<EXACT> xv = row_operand<SRC, EXACT>(s.x[i], g, q, K, xs);   // zero past the end
-            if (g >= G) xs = 0.f;
+        for (int j = 0; j < FN; ++j) {
+            const v4f t = group_mfma<EXACT>(group_op<EXACT>(s.w[j][0], s.w[j][1]), xv);
+            const float sc = xs * s.ws[j];
 #pragma unroll
-            for (int j = 0; j < FN; ++j) {
-                const v4f t = group_mfma<EXACT>(group_op<EXACT>(s.w[j][0], s.w[j][1]), xv);
-                const float sc = xs * s.ws[j];
-#pragma unroll
-                for (int r = 0; r < 4; ++r) run[i][j][r] = fmaf(t[r], sc, run[i][j][r]);
-            }
+            for (int r = 0; r < 4; ++r) run[j][r] = fmaf(t[r], sc, run[j][r]);
         }
     };
     const int steps = (G + KS - 1) / KS;
@@ -334,31 +309,25 @@ __global__ void __launch_bounds__(64 * KS) block_stream_kernel(BlockParams p, in
         }
     }
 #pragma unroll
-    for (int i = 0; i < FT; ++i)
-#pragma unroll
-        for (int j = 0; j < FN; ++j) part[wave][i * FN + j][lane] = run[i][j];
+    for (int j = 0; j < FN; ++j) part[wave][j][lane] = run[j];
     __syncthreads();
-    for (int u = tid; u < FT * kCols * 64; u += 64 * KS) {     // four adjacent columns of a row
-        const int ln = u & 63, f = u >> 6, i = f / kCols, j = f % kCols;
-        auto total = [&](int frag) __attribute__((always_inline)) {
-            v4f t = part[0][frag][ln];
+    // wave j joins column fragment j (four adjacent columns of a row a lane)
+    static_assert(kCols <= KS, "a wave a fragment");
+    if (wave >= kCols) return;
+    auto total = [&](int f) __attribute__((always_inline)) {
+        v4f t = part[0][f][lane];
 #pragma unroll
-            for (int w = 1; w < KS; ++w) t += part[w][frag][ln];
-            return t;
-        };
-        v4f t = total(i * FN + j);
-        if constexpr (kSilu) {
-            const v4f up = total(i * FN + kCols + j);
+        for (int w = 1; w < KS; ++w) t += part[w][f][lane];
+        return t;
+    };
+    v4f t = total(wave);
+    if constexpr (kSilu) {
+        const v4f up = total(kCols + wave);
 #pragma unroll
-            for (int r = 0; r < 4; ++r) t[r] = silu_mul_f32(t[r], up[r]);
-        }
-        int xrow;
-        const int row = row0 + 16 * i + (ln & 15);
-        const int sl_id = block_slot(p, row, end, xrow);
-        const int col = (sl * kCols + j) * 16 + 4 * (ln >> 4);
-        if (sl_id < 0 || col >= cols) continue;
-        store4<DST>(p, DST == Dst::kSlotF32 ? sl_id : row, col, cols, t);
+        for (int r = 0; r < 4; ++r) t[r] = silu_mul_f32(t[r], up[r]);
     }
+    const int col = (sl * kCols + wave) * 16 + 4 * q;
+    if (slot >= 0 && col < cols) store4<DST>(p, DST == Dst::kSlotF32 ? slot : row0 + c, col, cols, t);
 }
 
 int too_many() {
@@ -366,48 +335,59 @@ int too_many() {
     return W4A8_ERR_INVALID;
 }
 
-template <int FT, int FN, int KS, Src SRC, Dst DST>
+template <int FN, int KS, Src SRC, Dst DST>
 int go_any(const BlockParams& p, hipStream_t s) {
     constexpr bool silu = DST == Dst::kSiluF32;
     const int cols = silu ? p.N / 2 : p.N, per = 16 * (silu ? FN / 2 : FN);
     const int slices = (cols + per - 1) / per;
-    const int64_t grid = (int64_t)((p.P + 16 * FT - 1) / (16 * FT)) * slices;
+    const int64_t grid = (int64_t)((p.P + 15) / 16) * slices;
     if (grid >= (int64_t)1 << 31) return too_many();
-    launch_kernel(&block_stream_kernel<FT, FN, KS, SRC, DST>, dim3((unsigned)grid), dim3(64 * KS), 0, s, p, slices);
+    launch_kernel(&block_stream_kernel<FN, KS, SRC, DST>, dim3((unsigned)grid), dim3(64 * KS), 0, s, p, slices);
     return check_launch("block_stream_kernel");
 }
 
-// blocks: row blocks expected to hold rows
-template <int FT, int GPW, int KS, int CG, int D, Src SRC, Dst DST>
-int go_rows(const BlockParams& p, int64_t blocks, hipStream_t s) {
-    constexpr bool silu = DST == Dst::kSiluF32;
-    const int frags = ((silu ? p.N / 2 : p.N) + 15) / 16;
-    // a work-group a CU and round where there are fewer fragments than that, else some rounds' worth
-    // of groups, each with whole rounds of D
-    constexpr int unit = D / (silu ? 2 : 1);
-    const int64_t want = (int64_t)device_cu_count() * (8 / (KS * CG) > 0 ? 8 / (KS * CG) : 1) * 2;
-    int64_t per = (blocks * frags + want * CG - 1) / (want * CG);
-    per = std::max<int64_t>(unit, std::min<int64_t>((per + unit - 1) / unit * unit, 4 * unit));
+// per: output fragments a group of waves walks over. The kernel loads D fragments beforehand whatever
+// `per` is, so few of them take a variant with a smaller D.
+template <int GPW, int KS, int CG, int D, Src SRC, Dst DST>
+int launch_rows(const BlockParams& p, int frags, int64_t per, hipStream_t s) {
+    constexpr int pair = DST == Dst::kSiluF32 ? 2 : 1;
+    if constexpr (D > pair)
+        if (per * pair <= D / 2) return launch_rows<GPW, KS, CG, D / 2, SRC, DST>(p, frags, per, s);
     const int slices = (int)((frags + per * CG - 1) / (per * CG));
-    const int64_t grid = (int64_t)((p.P + 16 * FT - 1) / (16 * FT)) * slices;
+    const int64_t grid = (int64_t)((p.P + 15) / 16) * slices;
     if (grid >= (int64_t)1 << 31) return too_many();
-    launch_kernel(&block_rows_kernel<FT, GPW, KS, CG, D, SRC, DST>, dim3((unsigned)grid), dim3(64 * KS * CG), 0, s, p,
-                  slices, (int)per);
+    launch_kernel(&block_rows_kernel<GPW, KS, CG, D, SRC, DST>, dim3((unsigned)grid), dim3(64 * KS * CG), 0, s, p, slices,
+                  (int)per);
     return check_launch("block_rows_kernel");
 }
 
-// FT row fragments: the wave split by the number of K groups.
+// blocks: row blocks expected to hold rows
+template <int GPW, int KS, int CG, int D, Src SRC, Dst DST>
+int go_rows(const BlockParams& p, int64_t blocks, hipStream_t s) {
+    constexpr int unit = D / (DST == Dst::kSiluF32 ? 2 : 1);
+    const int frags = ((DST == Dst::kSiluF32 ? p.N / 2 : p.N) + 15) / 16;
+    // One round of work-groups (eight waves a CU), each walking over what that leaves it, up to eight
+    // rings' worth. us at most 8 / at most 4 / three rounds or more instead of one:
+    // 64 experts, 64 rows x 8, 4096 -> 2048: 110 / 118 / 126; layer of 256 experts, 128 tokens x 8: 187 / 208 / 211,
+    // 32 tokens: 142 / 140 / 150; 256 experts, 24 tokens x 8, 2048 -> 1024: 61 / 57 / 57.
+    const int64_t groups = (int64_t)device_cu_count() * std::max(1, 8 / (KS * CG)) * CG;
+    int64_t per = (blocks * frags + groups - 1) / groups;
+    if (per > unit) per = std::min<int64_t>((per + unit - 1) / unit, 8) * unit;
+    return launch_rows<GPW, KS, CG, D, SRC, DST>(p, frags, std::max<int64_t>(1, per), s);
+}
+
+// The wave split by the number of K groups: a wave holds the rows' values of up to four of them (four
+// weight fragments of four groups in flight are 128 registers), up to eight waves share K. Beyond 32
+// groups (4096 values) rows are read again: 4 x 4096 x 12288 in 15 us, 3.3 TB/s.
 template <Src SRC, Dst DST>
-int rows1(const BlockParams& p, int64_t blocks, hipStream_t s) {
-    if (p.G <= 1) return go_rows<1, 1, 1, 4, 4, SRC, DST>(p, blocks, s);
-    if (p.G <= 2) return go_rows<1, 2, 1, 4, 4, SRC, DST>(p, blocks, s);
-    if (p.G <= 4) return go_rows<1, 4, 1, 4, 2, SRC, DST>(p, blocks, s);
-    if (p.G <= 8) return go_rows<1, 2, 4, 1, 4, SRC, DST>(p, blocks, s);
-    if (p.G <= 16) return go_rows<1, 4, 4, 1, 2, SRC, DST>(p, blocks, s);
-    if (p.G <= 32) return go_rows<1, 4, 8, 1, 2, SRC, DST>(p, blocks, s);
-    if constexpr (DST != Dst::kSiluF32)
-        if (p.G <= 64) return go_rows<1, 8, 8, 1, 1, SRC, DST>(p, blocks, s);
-    return go_any<1, 2, 4, SRC, DST>(p, s);
+int rows16(const BlockParams& p, int64_t blocks, hipStream_t s) {
+    if (p.G <= 1) return go_rows<1, 1, 4, 4, SRC, DST>(p, blocks, s);
+    if (p.G <= 2) return go_rows<2, 1, 4, 4, SRC, DST>(p, blocks, s);
+    if (p.G <= 4) return go_rows<4, 1, 4, 2, SRC, DST>(p, blocks, s);
+    if (p.G <= 8) return go_rows<2, 4, 1, 4, SRC, DST>(p, blocks, s);
+    if (p.G <= 16) return go_rows<4, 4, 1, 2, SRC, DST>(p, blocks, s);
+    if (p.G <= 32) return go_rows<4, 8, 1, 2, SRC, DST>(p, blocks, s);
+    return go_any<DST == Dst::kSiluF32 ? 2 : 1, 8, SRC, DST>(p, s);
 }
 
 }  // namespace
@@ -419,9 +399,8 @@ int launch_block_stream(const BlockArgs& a, hipStream_t s) {
                                                    : (a.P + 15) / 16;
     auto out16 = [&](auto src) -> int {
         constexpr Src S = decltype(src)::value;
-        if (a.dst == Dst::kF16) return rows1<S, Dst::kF16>(p, blocks, s);
-        if (a.dst == Dst::kBf16) return rows1<S, Dst::kBf16>(p, blocks, s);
-        if (a.dst == Dst::kSiluF32) return rows1<S, Dst::kSiluF32>(p, blocks, s);
+        if (a.dst == Dst::kF16 || a.dst == Dst::kBf16) return rows16<S, Dst::kF16>(p, blocks, s);
+        if (a.dst == Dst::kSiluF32) return rows16<S, Dst::kSiluF32>(p, blocks, s);
         set_error("fp8 block product: output form not taken by the streaming kernel");
         return W4A8_ERR_INVALID;
     };
@@ -431,7 +410,7 @@ int launch_block_stream(const BlockArgs& a, hipStream_t s) {
         case Src::kBf16: return out16(std::integral_constant<Src, Src::kBf16>{});
         default: break;
     }
-    if (a.dst == Dst::kSlotF32) return rows1<Src::kF32, Dst::kSlotF32>(p, blocks, s);
+    if (a.dst == Dst::kSlotF32) return rows16<Src::kF32, Dst::kSlotF32>(p, blocks, s);
     set_error("fp8 block product: fp32 rows are the layer's second product's");
     return W4A8_ERR_INVALID;
 }

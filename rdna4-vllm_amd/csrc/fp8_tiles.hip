@@ -20,7 +20,6 @@ using global_cvoid_ptr = const __attribute__((address_space(1))) void*;
 
 constexpr int kTileXcds = 8;
 constexpr int kRunRows = 4;       // row tiles of an XCD's run
-constexpr int kGroupedRuns = 64;  // grouped: runs at least, where there are that many row tiles
 
 // What pieces past the end of K are read from.
 __device__ __attribute__((aligned(16))) uint32_t g_zero_piece[4];
@@ -37,11 +36,12 @@ __device__ __forceinline__ void group_barrier() {
     __builtin_amdgcn_sched_barrier(0);
 }
 
-// WT x WN waves of FT row fragments x FN column fragments of 16, S groups in LDS.
-template <int WT_, int WN_, int FT_, int FN_, int S_>
+// WT x WN waves of FT row fragments x FN column fragments of 16, S groups in LDS; KS such parts of a
+// work-group share K, each with slots of its own, and add their sums at the end.
+template <int WT_, int WN_, int FT_, int FN_, int S_, int KS_ = 1>
 struct TileCfg {
-    static constexpr int WT = WT_, WN = WN_, FT = FT_, FN = FN_, S = S_;
-    static constexpr int kWaves = WT * WN, kThreads = 64 * kWaves;
+    static constexpr int WT = WT_, WN = WN_, FT = FT_, FN = FN_, S = S_, KS = KS_;
+    static constexpr int kWaves = WT * WN, kThreads = 64 * kWaves;   // of a part
     static constexpr int BT = WT * FT * 16, BN = WN * FN * 16;
     static constexpr int kW = BT * kBlk;                         // weights behind the rows
     static constexpr int kSlot = kW + BN * kBlk;
@@ -56,15 +56,17 @@ struct TileCfg {
 };
 
 template <typename C, Dst DST, bool EXACT, bool TAIL, bool GROUPED>
-__global__ void __launch_bounds__(C::kThreads, 2) block_tiles_kernel(BlockParams p, int ntiles, int run_rows) {
+__global__ void __launch_bounds__(C::kThreads * C::KS, 2) block_tiles_kernel(BlockParams p, int ntiles, int run_rows) {
     constexpr int FT = C::FT, FN = C::FN, BT = C::BT, BN = C::BN, S = C::S;
     constexpr bool kSilu = DST == Dst::kSiluFp8;
+    constexpr int KS = C::KS;
     static_assert(!kSilu || BN == 256, "SiLU tiles hold 128 gate and 128 up columns");
+    static_assert(KS <= 2 && (KS == 1 || (DST == Dst::kF16 && !GROUPED)), "a divided K is for dense products");
     // arrays of their own: the compiler then sees that reads of one do not wait for loads into another
-    __shared__ __attribute__((aligned(1024))) uint8_t slot0[C::kSlot];
-    __shared__ __attribute__((aligned(1024))) uint8_t slot1[C::kSlot];
-    __shared__ __attribute__((aligned(1024))) uint8_t slot2[S > 2 ? C::kSlot : 16];
-    __shared__ float s_xs[2 * C::kChunk * BT];                   // row scales [group][row] of two chunks
+    __shared__ __attribute__((aligned(1024))) uint8_t slots0[KS * C::kSlot];
+    __shared__ __attribute__((aligned(1024))) uint8_t slots1[KS * C::kSlot];
+    __shared__ __attribute__((aligned(1024))) uint8_t slots2[S > 2 ? KS * C::kSlot : 16];
+    __shared__ float s_xs[KS * 2 * C::kChunk * BT];              // row scales [group][row] of two chunks
 
     // ---- the tile. Dense: an XCD takes a contiguous run of them, run_rows row tiles by all columns.
     // Grouped: XCDs take such runs in turn (how many row tiles are in use is known on the device only;
@@ -86,9 +88,14 @@ __global__ void __launch_bounds__(C::kThreads, 2) block_tiles_kernel(BlockParams
         ct = rem / rows_here;
     }
     const int row0 = m_tile * BT;
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int part = KS > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x / C::kThreads) : 0;
+    const int tid = KS > 1 ? threadIdx.x % C::kThreads : threadIdx.x;
+    const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int q = lane >> 4, c = lane & 15;
     const int K = p.K, G = p.G, N = p.N;
+    const int G1 = (G + KS - 1) / KS, g_first = part * G1;       // groups of a part, the first of them
+    uint8_t *const slot0 = slots0 + part * C::kSlot, *const slot1 = slots1 + part * C::kSlot;
+    uint8_t* const slot2 = slots2 + (S > 2 ? part * C::kSlot : 0);
 
     // the expert of fragment `lane`'s rows (-1: none)
     int fe = 0;
@@ -156,9 +163,9 @@ __global__ void __launch_bounds__(C::kThreads, 2) block_tiles_kernel(BlockParams
         };
         // Past the last group every lane reads one piece (nobody reads the slot). TAIL: absent pieces of
         // the last, partial group are zero in both operands.
-        auto issue_part = [&](uint8_t* slot, int g, int part, int parts) __attribute__((always_inline)) {
-            const uint32_t on = g < G ? ~0u : 0u;
-            const int gg = min(g, G - 1);
+        auto issue_some = [&](uint8_t* slot, int g, int some, int parts) __attribute__((always_inline)) {
+            const uint32_t on = g < G1 && g_first + g < G ? ~0u : 0u;
+            const int gg = min(g_first + g, G - 1);
             const uint8_t *xg = xb + (int64_t)gg * kBlk, *wg = wb + (int64_t)gg * kBlk;
             asm volatile("" : "+s"(xg), "+s"(wg));               // (scalar bases, 32-bit offsets)
             uint8_t *xd = slot + wave * 1024, *wd = slot + C::kW + wave * 1024;
@@ -170,23 +177,23 @@ __global__ void __launch_bounds__(C::kThreads, 2) block_tiles_kernel(BlockParams
             };
 #pragma unroll
             for (int i = 0; i < C::PX; ++i)
-                if (i * parts / C::kLoads == part) dma(src(xg, xoff[i], i), xd + i * C::kThreads * 16);
+                if (i * parts / C::kLoads == some) dma(src(xg, xoff[i], i), xd + i * C::kThreads * 16);
 #pragma unroll
             for (int i = 0; i < C::PW; ++i)
-                if ((C::PX + i) * parts / C::kLoads == part) dma(src(wg, woff[i], i), wd + i * C::kThreads * 16);
+                if ((C::PX + i) * parts / C::kLoads == some) dma(src(wg, woff[i], i), wd + i * C::kThreads * 16);
         };
-        auto issue = [&](uint8_t* slot, int g) __attribute__((always_inline)) { issue_part(slot, g, 0, 1); };
+        auto issue = [&](uint8_t* slot, int g) __attribute__((always_inline)) { issue_some(slot, g, 0, 1); };
         // Row scales: kChunk groups at a time, through registers to a table (read group by group, each
         // row's scale is a request of its own: more of them than the rows and weights make together).
         float tv[C::PT];
         auto load_scales = [&](int g0) __attribute__((always_inline)) {
 #pragma unroll
             for (int i = 0; i < C::PT; ++i)
-                tv[i] = p.xs[toff[i] + (uint32_t)min(g0 + entry(i) % C::kChunk, G - 1)];
+                tv[i] = p.xs[toff[i] + (uint32_t)min(g_first + g0 + entry(i) % C::kChunk, G - 1)];
         };
         auto store_scales = [&](int at) __attribute__((always_inline)) {
 #pragma unroll
-            for (int i = 0; i < C::PT; ++i) s_xs[at + entry(i) % C::kChunk * BT + entry(i) / C::kChunk] = tv[i];
+            for (int i = 0; i < C::PT; ++i) s_xs[part * 2 * C::kChunk * BT + at + entry(i) % C::kChunk * BT + entry(i) / C::kChunk] = tv[i];
         };
         const float* wsb = p.ws + (int64_t)e * p.NB * G;
         const float* wsg = wsb + (int64_t)(min(col_of(wn * FN * 16), N - 1) / kBlk) * G;
@@ -200,12 +207,12 @@ __global__ void __launch_bounds__(C::kThreads, 2) block_tiles_kernel(BlockParams
 
         const int cr = (c ^ (c >> 3)) * kBlk;
         const int p0 = cr + (((2 * q) ^ (c & 7)) << 4), p1 = cr + (((2 * q + 1) ^ (c & 7)) << 4);
-        const bool mine = !GROUPED || (now >> (wt * FT) & ((1u << FT) - 1)) != 0;   // this wave has rows in the pass
         // One group: the rows' fragments against the columns', of which the next is read while one is
         // multiplied and the one before is folded.
-        // next, gn: the slot and group whose loads are issued between the fragments, so that no wave waits
-        // for the address unit to take all of them (2048 x 4096 x 12288: 132 -> NN us)
-        auto compute = [&](const uint8_t* slot, uint8_t* next, int gn, int xs_at, float wg, float wu) __attribute__((always_inline)) {
+        // With three slots the loads of group g + 2 are issued between the fragments, into `next`, so that
+        // no wave waits for the address unit to take all of them (2048 x 4096 x 12288: 132 -> 102 us).
+        // A part's groups past the last one are read as anything and not folded.
+        auto compute = [&](const uint8_t* slot, uint8_t* next, int g, int xs_at, float wg, float wu) __attribute__((always_inline)) {
             auto frag = [&](int at, u32x4 (&f)[2]) __attribute__((always_inline)) {
                 f[0] = *reinterpret_cast<const u32x4*>(slot + at + p0);
                 f[1] = *reinterpret_cast<const u32x4*>(slot + at + p1);
@@ -214,6 +221,7 @@ __global__ void __launch_bounds__(C::kThreads, 2) block_tiles_kernel(BlockParams
             float xs[FT];
             GroupOp<EXACT> xf[FT];
             v4f pend[2][FT];
+            const bool on = KS == 1 || g_first + g < G;
             auto fold = [&](int j) __attribute__((always_inline)) {
 #pragma unroll
                 for (int i = 0; i < FT; ++i) {
@@ -222,30 +230,25 @@ __global__ void __launch_bounds__(C::kThreads, 2) block_tiles_kernel(BlockParams
                     for (int r = 0; r < 4; ++r) run[i][j][r] = fmaf(pend[j & 1][i][r], s, run[i][j][r]);
                 }
             };
-            if (mine) {
-                frag(C::kW + wn * FN * 16 * kBlk, wf[0]);
+            frag(C::kW + wn * FN * 16 * kBlk, wf[0]);
 #pragma unroll
-                for (int i = 0; i < FT; ++i) frag((wt * FT + i) * 16 * kBlk, xr[i]);
+            for (int i = 0; i < FT; ++i) frag((wt * FT + i) * 16 * kBlk, xr[i]);
 #pragma unroll
-                for (int i = 0; i < FT; ++i) xs[i] = s_xs[xs_at + i * 16];
+            for (int i = 0; i < FT; ++i) xs[i] = s_xs[xs_at + i * 16];
 #pragma unroll
-                for (int i = 0; i < FT; ++i) xf[i] = group_op<EXACT>(xr[i][0], xr[i][1]);
-            }
+            for (int i = 0; i < FT; ++i) xf[i] = group_op<EXACT>(xr[i][0], xr[i][1]);
 #pragma unroll
             for (int j = 0; j < FN; ++j) {
-                if (mine) {
-                    if (j + 1 < FN) frag(C::kW + (wn * FN + j + 1) * 16 * kBlk, wf[(j + 1) & 1]);
-                    __builtin_amdgcn_sched_barrier(0);
-                    const GroupOp<EXACT> w = group_op<EXACT>(wf[j & 1][0], wf[j & 1][1]);
+                if (j + 1 < FN) frag(C::kW + (wn * FN + j + 1) * 16 * kBlk, wf[(j + 1) & 1]);
+                __builtin_amdgcn_sched_barrier(0);
+                const GroupOp<EXACT> w = group_op<EXACT>(wf[j & 1][0], wf[j & 1][1]);
 #pragma unroll
-                    for (int i = 0; i < FT; ++i) pend[j & 1][i] = group_mfma<EXACT>(w, xf[i]);
-                }
-                // (outside the branch: the same loads in flight along every path)
-                if (S > 2) issue_part(next, gn, j, FN);
-                if (mine && j > 0) fold(j - 1);
+                for (int i = 0; i < FT; ++i) pend[j & 1][i] = group_mfma<EXACT>(w, xf[i]);
+                if (S > 2) issue_some(next, g + 2, j, FN);
+                if (j > 0 && on) fold(j - 1);
                 __builtin_amdgcn_sched_barrier(0);
             }
-            if (mine) fold(FN - 1);
+            if (on) fold(FN - 1);
         };
 
         // Group g. Its stage has landed for this wave when no more than the next one's loads are in
@@ -256,7 +259,7 @@ __global__ void __launch_bounds__(C::kThreads, 2) block_tiles_kernel(BlockParams
         auto step = [&](uint8_t* slot, uint8_t* next, int g, int xs_at, float wg, float wu) __attribute__((always_inline)) {
             __builtin_amdgcn_s_waitcnt(wait_vm(C::kLoads));
             group_barrier();
-            compute(slot, next, g + 2, xs_at, wg, wu);
+            compute(slot, next, g, xs_at, wg, wu);
             __builtin_amdgcn_sched_barrier(0);
             if constexpr (S == 2) {
                 group_barrier();
@@ -270,7 +273,7 @@ __global__ void __launch_bounds__(C::kThreads, 2) block_tiles_kernel(BlockParams
             base = g;
 #pragma unroll
             for (int t = 0; t < S; ++t) {
-                const int k = min(base + lane * S + t, G - 1);
+                const int k = min(g_first + base + lane * S + t, G - 1);
                 wgv[t] = wsg[k];
                 wuv[t] = kSilu ? wsu[k] : 0.f;
             }
@@ -278,7 +281,7 @@ __global__ void __launch_bounds__(C::kThreads, 2) block_tiles_kernel(BlockParams
 #pragma unroll
             for (int t = 0; t < S; ++t) asm volatile("" : "+v"(wgv[t]), "+v"(wuv[t]));
         };
-        const int xs_lane = wt * FT * 16 + c;
+        const int xs_lane = part * 2 * C::kChunk * BT + wt * FT * 16 + c;
         // A chunk's table is written behind the first round of the chunk before: its last readers are past
         // a barrier by then, and the chunk's own first barrier shows it to everybody.
         load_scales(0);
@@ -302,35 +305,47 @@ __global__ void __launch_bounds__(C::kThreads, 2) block_tiles_kernel(BlockParams
                 if constexpr (S > 2) step(slot2, slot1, g, xa + 2 * BT, pick(wgv[S > 2 ? 2 : 0]), pick(wuv[S > 2 ? 2 : 0]));
             };
             round0();
-            if (++g == G) goto summed;
+            if (++g == G1) goto summed;
             round1();
-            if (++g == G) goto summed;
+            if (++g == G1) goto summed;
             if constexpr (S > 2) {
                 round2();
-                if (++g == G) goto summed;
+                if (++g == G1) goto summed;
             }
             store_scales(at ^ (C::kChunk * BT));
             load_scales(g - S + 2 * C::kChunk);
             ++l;
             xa += S * BT;
             round0();
-            if (++g == G) goto summed;
+            if (++g == G1) goto summed;
             round1();
-            if (++g == G) goto summed;
+            if (++g == G1) goto summed;
             if constexpr (S > 2) {
                 round2();
-                if (++g == G) goto summed;
+                if (++g == G1) goto summed;
             } else {
                 ++l;
                 xa += S * BT;
                 round0();
-                if (++g == G) goto summed;
+                if (++g == G1) goto summed;
                 round1();
-                if (++g == G) goto summed;
+                if (++g == G1) goto summed;
             }
         }
     summed:
         __builtin_amdgcn_s_waitcnt(wait_vm(0));                  // (the loads past the last group)
+        if constexpr (KS > 1) {
+            v4f* sums = reinterpret_cast<v4f*>(slots0);          // [FT FN][kThreads]
+            static_assert(FT * FN * C::kThreads * sizeof(v4f) <= C::kSlot * KS, "sums fit");
+            group_barrier();                                     // nobody reads or loads a slot any more
+#pragma unroll
+            for (int i = 0; i < FT * FN; ++i)
+                if (part > 0) sums[i * C::kThreads + tid] = run[i / FN][i % FN];
+            lds_barrier();
+            if (part > 0) return;
+#pragma unroll
+            for (int i = 0; i < FT * FN; ++i) run[i / FN][i % FN] += sums[i * C::kThreads + tid];
+        }
 
         // ---- epilogue: lane (q, c) holds row 16 i + c, columns 4 q .. 4 q + 3 of each fragment ----
         auto live = [&](int i, int& row) __attribute__((always_inline)) {
@@ -412,7 +427,7 @@ __global__ void __launch_bounds__(C::kThreads, 2) block_tiles_kernel(BlockParams
                 }
             }
         }
-        group_barrier();                                         // the slots are free for the next pass
+        if (GROUPED) group_barrier();                            // the slots are free for the next pass
     }
 }
 
@@ -420,7 +435,7 @@ template <typename C, Dst DST, bool GROUPED>
 int tiles_go(const BlockParams& p, hipStream_t s) {
     constexpr bool silu = DST == Dst::kSiluFp8;
     const int ntiles = silu ? p.N / 2 / kBlk : (p.N + C::BN - 1) / C::BN, mtiles = (p.P + C::BT - 1) / C::BT;
-    const int run_rows = GROUPED ? std::max(1, std::min(kRunRows, mtiles / kGroupedRuns)) : kRunRows;
+    const int run_rows = std::min(kRunRows, mtiles);
     const int64_t runs = (mtiles + run_rows - 1) / run_rows;
     const int64_t items = GROUPED ? (runs + kTileXcds - 1) / kTileXcds * kTileXcds * run_rows * ntiles
                                   : ((int64_t)mtiles * ntiles + kTileXcds - 1) / kTileXcds * kTileXcds;
@@ -431,21 +446,39 @@ int tiles_go(const BlockParams& p, hipStream_t s) {
     const dim3 grid((unsigned)items);
     if constexpr (DST == Dst::kF16)
         if (p.K % kBlk != 0) {
-            launch_kernel(&block_tiles_kernel<C, DST, silu, true, GROUPED>, grid, dim3(C::kThreads), 0, s, p, ntiles, run_rows);
+            launch_kernel(&block_tiles_kernel<C, DST, silu, true, GROUPED>, grid, dim3(C::kThreads * C::KS), 0, s, p, ntiles, run_rows);
             return check_launch("block_tiles_kernel");
         }
-    launch_kernel(&block_tiles_kernel<C, DST, silu, false, GROUPED>, grid, dim3(C::kThreads), 0, s, p, ntiles, run_rows);
+    launch_kernel(&block_tiles_kernel<C, DST, silu, false, GROUPED>, grid, dim3(C::kThreads * C::KS), 0, s, p, ntiles, run_rows);
     return check_launch("block_tiles_kernel");
 }
 
-using Tile64x64 = TileCfg<1, 4, 4, 1, 3>;       // four waves, three work-groups a CU
+using Tile64x64K2 = TileCfg<1, 4, 4, 1, 3, 2>;  // eight waves, one work-group a CU
+using Tile64x64 = TileCfg<1, 4, 4, 1, 3>;       // four, three
 using Tile64x128 = TileCfg<1, 4, 4, 2, 3>;      // four, two
-using Tile128x128 = TileCfg<2, 2, 4, 4, 2>;     // four, two
 using Tile256x128 = TileCfg<4, 2, 4, 4, 3>;     // eight, one
-#ifndef ST
-#define ST 1, 8, 4, 2, 3
-#endif
-using TileSilu = TileCfg<ST>;        // 64 x 256: eight, one
+using TileSilu = TileCfg<1, 8, 4, 2, 3>;        // 64 x 256: eight, one
+
+// The dense tile of least cost, us at K = 4096 as measured (the cost of every tile is linear in K):
+//   work-groups a CU:    <= 1     2     3     4     8
+//   64 x 64, K in two     12    24
+//   64 x 64               14    19    29    36    64
+//   64 x 128              20    28    52    54
+//   256 x 128          34-42    84
+// 64 rows x 64 columns alone are bound by the latency of a group's loads (0.44 us of the 14 / 32), the
+// largest by what LDS gives the matrix cores (2048 x 4096 x 12288: 1.8 PFLOP/s).
+int dense_go(const BlockParams& p, hipStream_t s) {
+    const int64_t cus = device_cu_count();
+    auto tiles = [&](int bt, int bn) { return (int64_t)((p.P + bt - 1) / bt) * ((p.N + bn - 1) / bn); };
+    const int64_t n64 = tiles(64, 64), n128 = tiles(64, 128), n256 = tiles(256, 128);
+    if (n64 <= cus) return tiles_go<Tile64x64K2, Dst::kF16, false>(p, s);
+    const int64_t t64 = std::max<int64_t>(14 * cus, 9 * n64);
+    const int64_t t128 = n128 <= cus ? 20 * cus : (n128 + 2 * cus - 1) / (2 * cus) * 27 * cus;
+    const int64_t t256 = n256 <= cus ? 34 * cus + 8 * n256 : (n256 + cus - 1) / cus * 42 * cus;
+    if (t256 <= std::min(t64, t128)) return tiles_go<Tile256x128, Dst::kF16, false>(p, s);
+    if (t128 <= t64) return tiles_go<Tile64x128, Dst::kF16, false>(p, s);
+    return tiles_go<Tile64x64, Dst::kF16, false>(p, s);
+}
 
 }  // namespace
 
@@ -466,20 +499,9 @@ int launch_block_tiles(const BlockArgs& a, hipStream_t s) {
         return W4A8_ERR_INVALID;
     }
     if (a.dst == Dst::kSiluFp8) return tiles_go<TileSilu, Dst::kSiluFp8, true>(p, s);
-#ifndef LT
-#define LT Tile64x128
-#endif
-    if (a.dst == Dst::kRowF16) return tiles_go<LT, Dst::kRowF16, true>(p, s);
-    if (a.sorted_ids != nullptr) {
-#ifndef GT
-#define GT Tile128x128
-#endif
-        return tiles_go<GT, Dst::kF16, true>(p, s);
-    }
-#ifdef DT
-    return tiles_go<DT, Dst::kF16, false>(p, s);
-#endif
-    return tiles_go<Tile256x128, Dst::kF16, false>(p, s);
+    if (a.dst == Dst::kRowF16) return tiles_go<Tile64x128, Dst::kRowF16, true>(p, s);
+    if (a.sorted_ids != nullptr) return tiles_go<Tile64x128, Dst::kF16, true>(p, s);
+    return dense_go(p, s);
 }
 
 }  // namespace w4a8
