@@ -38,6 +38,11 @@ class NormQuant(NamedTuple):
     norm: Optional[torch.Tensor]          # the norm in x's dtype, where it was asked for
 
 
+# (torch.cuda.current_device / current_stream without their Python layers, which cost more than the
+# launch does; the tensors of a call have initialised torch.cuda)
+_current_device = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else torch.cuda.current_device
+
+
 class _on:
     """Makes a tensor's device the current one (a call on another device than the current one
     launches on the tensors' device)."""
@@ -48,8 +53,8 @@ class _on:
         self.back = None
 
     def __enter__(self):
-        now = torch.cuda.current_device()
-        if self.to is not None and self.to != now:
+        now = _current_device()
+        if self.to != now:
             self.back = now
             torch.cuda.set_device(self.to)
 
@@ -59,7 +64,7 @@ class _on:
 
 
 def _stream(t):
-    return torch.cuda.current_stream(t.device).cuda_stream
+    return torch._C._cuda_getCurrentRawStream(t.device.index)
 
 
 def _groups(n: int) -> int:
@@ -70,6 +75,8 @@ def _rows2d(x, name):
     """x with contiguous rows (row strides and padding between rows are kept)."""
     if x.dim() != 2:
         _fail(f"{name} must be 2D, got {tuple(x.shape)}")
+    if x.is_contiguous():
+        return x
     if x.shape[1] > 1 and x.stride(1) != 1 or x.shape[0] > 1 and x.stride(0) < x.shape[1]:
         return x.contiguous()
     return x
@@ -96,16 +103,16 @@ def _same_device(device, *tensors):
 
 
 def _check_scaled(q, s, rows, K, name):
-    if s.dtype != torch.float32 or tuple(s.shape) != (rows, _groups(K)):
+    if s.dtype != torch.float32 or s.shape != (rows, _groups(K)):
         _fail(f"{name} must be fp32 (rows, ceil(K/128))=({rows},{_groups(K)}); got {s.dtype} {tuple(s.shape)}")
     return s if s.is_contiguous() else s.contiguous()
 
 
 def _check_weight(w, s, lead, N, K, name):
     """e4m3 weights (*lead, N, K) and their block scales; contiguous (weights are never copied)."""
-    if w.dtype != FP8 or tuple(w.shape) != (*lead, N, K):
+    if w.dtype != FP8 or w.shape != (*lead, N, K):
         _fail(f"{name} must be float8_e4m3fn {(*lead, N, K)}; got {w.dtype} {tuple(w.shape)}")
-    if s.dtype != torch.float32 or tuple(s.shape) != (*lead, _groups(N), _groups(K)):
+    if s.dtype != torch.float32 or s.shape != (*lead, _groups(N), _groups(K)):
         _fail(f"{name} scales must be fp32 {(*lead, _groups(N), _groups(K))}; got {s.dtype} {tuple(s.shape)}")
     if not (w.is_contiguous() and s.is_contiguous()):
         _fail(f"{name} and its scales must be contiguous")
@@ -136,7 +143,7 @@ def rms_norm_quant_fp8(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6,
         _fail("x has no columns")
     if group_size not in (0, BLOCK):
         _fail(f"group_size must be 128 or 0 (one scale a row), got {group_size}")
-    if tuple(weight.shape) != (H,) or weight.dtype not in (x.dtype, torch.float32):
+    if weight.shape != (H,) or weight.dtype not in (x.dtype, torch.float32):
         _fail(f"weight must be ({H},) in x's dtype or fp32, got {weight.dtype} {tuple(weight.shape)}")
     if residual is not None:
         if residual.dtype != x.dtype or residual.shape != x.shape:
@@ -228,7 +235,7 @@ def fp8_block_gemm(x: torch.Tensor, x_scales: torch.Tensor | None, w: torch.Tens
     _same_device(dev, xs, w, w_scales)
     x = _mfma_rows(x, "x")
     out = torch.empty((M, N), dtype=dt, device=dev)
-    nbytes = lib.w4a8_fp8_block_gemm_workspace_size(_DT[x.dtype], M, K)
+    nbytes = 0 if xs is not None else lib.w4a8_fp8_block_gemm_workspace_size(_DT[x.dtype], M, K)
     ws = _workspace(nbytes, dev) if nbytes else None
     with _on(dev):
         check(lib.w4a8_fp8_block_gemm(
@@ -241,14 +248,17 @@ def moe_fp8_block_gemm(x: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor,
                        w_scales: torch.Tensor, sorted_token_ids: torch.Tensor,
                        expert_ids: torch.Tensor, num_tokens_post_padded: torch.Tensor, top_k: int,
                        block_m: int, out: torch.Tensor | None = None,
-                       out_dtype: torch.dtype | None = None, gather: bool = True) -> torch.Tensor:
+                       out_dtype: torch.dtype | None = None, gather: bool = True,
+                       num_slots: int | None = None) -> torch.Tensor:
     """Products grouped by expert, in the padded sorted layout of ``moe_align_block_size``.
 
     Row r < num_tokens_post_padded with slot s = sorted_token_ids[r] takes x[s // top_k] (or, with
-    ``gather=False``, x[r]: the rows of an earlier grouped product; slots then range over
-    x.shape[0]) times the weights of expert expert_ids[r // block_m] -> (P, N) in out_dtype (bf16 by
-    default) or in ``out``. Padding rows are not written. w (E, N, K) e4m3; block_m a multiple of 16
-    up to 128."""
+    ``gather=False``, x[r]: the rows of an earlier grouped product) times the weights of expert
+    expert_ids[r // block_m] -> (P, N) in out_dtype (bf16 by default) or in ``out``. Rows whose slot
+    is not in [0, num_slots) are padding and not written; num_slots is the number of routed slots,
+    tokens * top_k (default: x.shape[0] * top_k, which with ``gather=False`` counts padding rows of
+    x as slots too: pass it there to leave them as they are). w (E, N, K) e4m3; block_m a multiple
+    of 16 up to 128."""
     xs = _check_rows(x, x_scales)
     if xs is None:
         _fail("x must be float8_e4m3fn")
@@ -278,11 +288,14 @@ def moe_fp8_block_gemm(x: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor,
         _out_dtype(out.dtype)
     _same_device(dev, xs, w, w_scales, sorted_token_ids, expert_ids, num_tokens_post_padded, out)
     x = _mfma_rows(x, "x")
-    slots = rows * top_k if gather else max(rows * top_k, P)
+    if num_slots is None:
+        num_slots = rows * top_k if gather else max(rows * top_k, P)
+    elif num_slots < 0 or gather and num_slots > rows * top_k:
+        _fail(f"num_slots must be in 0 .. {rows * top_k}, got {num_slots}")
     with _on(dev):
         check(lib.w4a8_moe_fp8_block_gemm(
             _ptr(x), _ptr(xs), rows, K, _stride(x), _ptr(w), _ptr(w_scales), E, N,
-            _ptr(sorted_token_ids), P, _ptr(expert_ids), _ptr(num_tokens_post_padded), slots,
+            _ptr(sorted_token_ids), P, _ptr(expert_ids), _ptr(num_tokens_post_padded), int(num_slots),
             int(top_k), int(block_m), 1 if gather else 0, _ptr(out), _DT[out.dtype], _stream(x)),
             "moe_fp8_block_gemm")
     return out
@@ -356,7 +369,7 @@ _SCHEMAS = {
     "moe_fp8_block_gemm": "moe_fp8_block_gemm(Tensor x, Tensor x_scales, Tensor w, Tensor w_scales, "
                           "Tensor sorted_token_ids, Tensor expert_ids, "
                           "Tensor num_tokens_post_padded, int top_k, int block_m, "
-                          "ScalarType out_dtype, bool gather=True) -> Tensor",
+                          "ScalarType out_dtype, bool gather=True, int? num_slots=None) -> Tensor",
     "moe_fp8_block_apply": "moe_fp8_block_apply(Tensor x, Tensor w13, Tensor w2, Tensor w13_scales, "
                            "Tensor w2_scales, Tensor topk_weights, Tensor topk_ids, "
                            "Tensor? x_scales, Tensor? expert_map, ScalarType out_dtype) -> Tensor",
@@ -393,14 +406,14 @@ def _gemm_fake(x, x_scales, w, w_scales, out_dtype):
 
 
 def _moe_gemm_op(x, x_scales, w, w_scales, sorted_token_ids, expert_ids, num_tokens_post_padded,
-                 top_k, block_m, out_dtype, gather=True):
+                 top_k, block_m, out_dtype, gather=True, num_slots=None):
     return moe_fp8_block_gemm(x, x_scales, w, w_scales, sorted_token_ids, expert_ids,
                               num_tokens_post_padded, top_k, block_m, out_dtype=out_dtype,
-                              gather=gather)
+                              gather=gather, num_slots=num_slots)
 
 
 def _moe_gemm_fake(x, x_scales, w, w_scales, sorted_token_ids, expert_ids, num_tokens_post_padded,
-                   top_k, block_m, out_dtype, gather=True):
+                   top_k, block_m, out_dtype, gather=True, num_slots=None):
     return x.new_empty((sorted_token_ids.shape[0], w.shape[1]), dtype=out_dtype)
 
 
