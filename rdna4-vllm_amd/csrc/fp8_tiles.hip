@@ -56,7 +56,7 @@ struct TileCfg {
 };
 
 template <typename C, Dst DST, bool EXACT, bool TAIL, bool GROUPED>
-__global__ void __launch_bounds__(C::kThreads * C::KS, 2) block_tiles_kernel(BlockParams p, int ntiles, int run_rows) {
+__global__ void __launch_bounds__(C::kThreads * C::KS, 2) block_tiles_kernel(BlockParams p, int ntiles, int run_rows, int cts) {
     constexpr int FT = C::FT, FN = C::FN, BT = C::BT, BN = C::BN, S = C::S;
     constexpr bool kSilu = DST == Dst::kSiluFp8;
     constexpr int KS = C::KS;
@@ -67,26 +67,30 @@ __global__ void __launch_bounds__(C::kThreads * C::KS, 2) block_tiles_kernel(Blo
     __shared__ __attribute__((aligned(1024))) uint8_t slots1[KS * C::kSlot];
     __shared__ __attribute__((aligned(1024))) uint8_t slots2[S > 2 ? KS * C::kSlot : 16];
     __shared__ float s_xs[KS * 2 * C::kChunk * BT];              // row scales [group][row] of two chunks
+    __shared__ float s_max[kSilu ? C::WN * BT : 1];              // rows' absmax of a wave's columns
 
     // ---- the tile. Dense: an XCD takes a contiguous run of them, run_rows row tiles by all columns.
     // Grouped: XCDs take such runs in turn (how many row tiles are in use is known on the device only;
-    // a tile finds its rows before it knows, so that the loads below go out together). ----
+    // a tile finds its rows before it knows, so that the loads below go out together), and a work-group
+    // cts column tiles, one after the other: the next one's first loads are under way while it writes. ----
     const int xcd = blockIdx.x % kTileXcds, jx = blockIdx.x / kTileXcds;
-    const int mall = (p.P + BT - 1) / BT, run_items = run_rows * ntiles;
-    int m_tile, ct;
+    const int mall = (p.P + BT - 1) / BT;
+    int m_tile, ct_first;
     if constexpr (GROUPED) {
-        const int rem = jx % run_items;
+        const int run_items = run_rows * ((ntiles + cts - 1) / cts), rem = jx % run_items;
         m_tile = (jx / run_items * kTileXcds + xcd) * run_rows + rem % run_rows;
-        ct = rem / run_rows;
+        ct_first = rem / run_rows * cts;
         if (m_tile >= mall) return;
     } else {
+        const int run_items = run_rows * ntiles;
         const int items = mall * ntiles, perx = (items + kTileXcds - 1) / kTileXcds, item = xcd * perx + jx;
         if (jx >= perx || item >= items) return;
         const int m0 = item / run_items * run_rows, rem = item % run_items;
         const int rows_here = min(run_rows, mall - m0);
         m_tile = m0 + rem % rows_here;
-        ct = rem / rows_here;
+        ct_first = rem / rows_here;
     }
+    const int ct_end = GROUPED ? min(ct_first + cts, ntiles) : ct_first + 1;
     const int row0 = m_tile * BT;
     const int part = KS > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x / C::kThreads) : 0;
     const int tid = KS > 1 ? threadIdx.x % C::kThreads : threadIdx.x;
@@ -134,10 +138,13 @@ __global__ void __launch_bounds__(C::kThreads * C::KS, 2) block_tiles_kernel(Blo
     // the weight row behind row r of the slot's BN: fragment r / 16 belongs to wave r / (16 FN); kSilu
     // takes FN / 2 fragments of the gate half and the same of the up half
     const int half = N / 2;
-    auto col_of = [&](int r) __attribute__((always_inline)) {
+    auto col_of = [&](int ct, int r) __attribute__((always_inline)) {
         if constexpr (kSilu) {
             const int w = r / (FN * 16), j = r / 16 % FN;
             return ct * kBlk + (w * (FN / 2) + j % (FN / 2)) * 16 + r % 16 + (j >= FN / 2 ? half : 0);
+        } else if constexpr (FN % 2 == 0) {
+            // (a lane's four columns of two fragments are eight adjacent ones)
+            return ct * BN + (r & ~31) + (r % 16 / 4) * 8 + (r / 16 % 2) * 4 + r % 4;
         } else {
             return ct * BN + r;
         }
@@ -155,9 +162,6 @@ __global__ void __launch_bounds__(C::kThreads * C::KS, 2) block_tiles_kernel(Blo
         const uint8_t* xb = reinterpret_cast<const uint8_t*>(p.x);
         const uint8_t* wb = p.w + (int64_t)e * N * K;
         uint32_t woff[C::PW];
-#pragma unroll
-        for (int i = 0; i < C::PW; ++i)
-            woff[i] = (uint32_t)min(col_of(piece_row(i)), N - 1) * (uint32_t)K + (uint32_t)piece_k(piece_row(i));
         auto dma = [&](const uint8_t* src, uint8_t* dst) __attribute__((always_inline)) {
             __builtin_amdgcn_global_load_lds((global_cvoid_ptr)src, (lds_void_ptr)dst, 16, 0, 0);
         };
@@ -196,14 +200,16 @@ __global__ void __launch_bounds__(C::kThreads * C::KS, 2) block_tiles_kernel(Blo
             for (int i = 0; i < C::PT; ++i) s_xs[part * 2 * C::kChunk * BT + at + entry(i) % C::kChunk * BT + entry(i) / C::kChunk] = tv[i];
         };
         const float* wsb = p.ws + (int64_t)e * p.NB * G;
-        const float* wsg = wsb + (int64_t)(min(col_of(wn * FN * 16), N - 1) / kBlk) * G;
-        const float* wsu = kSilu ? wsb + (int64_t)(min(col_of((wn * FN + FN - 1) * 16), N - 1) / kBlk) * G : wsg;
-
+        const float *wsg = wsb, *wsu = wsb;
+        int ct = ct_first;
+        auto set_columns = [&]() __attribute__((always_inline)) {
+#pragma unroll
+            for (int i = 0; i < C::PW; ++i)
+                woff[i] = (uint32_t)min(col_of(ct, piece_row(i)), N - 1) * (uint32_t)K + (uint32_t)piece_k(piece_row(i));
+            wsg = wsb + (int64_t)(min(col_of(ct, wn * FN * 16), N - 1) / kBlk) * G;
+            if (kSilu) wsu = wsb + (int64_t)(min(col_of(ct, (wn * FN + FN - 1) * 16), N - 1) / kBlk) * G;
+        };
         v4f run[FT][FN];
-#pragma unroll
-        for (int i = 0; i < FT; ++i)
-#pragma unroll
-            for (int j = 0; j < FN; ++j) run[i][j] = v4f{0.f, 0.f, 0.f, 0.f};
 
         const int cr = (c ^ (c >> 3)) * kBlk;
         const int p0 = cr + (((2 * q) ^ (c & 7)) << 4), p1 = cr + (((2 * q + 1) ^ (c & 7)) << 4);
@@ -268,15 +274,15 @@ __global__ void __launch_bounds__(C::kThreads * C::KS, 2) block_tiles_kernel(Blo
         };
         constexpr int kSpan = 64 * S / C::kChunk * C::kChunk;     // groups of a table of weight scales
         float wgv[S], wuv[S];                                    // lane l: groups base + l S + t
-        int g = 0, base = 0;
-        auto ws_table = [&]() __attribute__((always_inline)) {
-            base = g;
+        auto load_ws = [&](int base) __attribute__((always_inline)) {
 #pragma unroll
             for (int t = 0; t < S; ++t) {
                 const int k = min(g_first + base + lane * S + t, G - 1);
                 wgv[t] = wsg[k];
                 wuv[t] = kSilu ? wsu[k] : 0.f;
             }
+        };
+        auto hold_ws = [&]() __attribute__((always_inline)) {
             // (waited for here: at their first use, in the loop, the wait would be every round's)
 #pragma unroll
             for (int t = 0; t < S; ++t) asm volatile("" : "+v"(wgv[t]), "+v"(wuv[t]));
@@ -284,16 +290,28 @@ __global__ void __launch_bounds__(C::kThreads * C::KS, 2) block_tiles_kernel(Blo
         const int xs_lane = part * 2 * C::kChunk * BT + wt * FT * 16 + c;
         // A chunk's table is written behind the first round of the chunk before: its last readers are past
         // a barrier by then, and the chunk's own first barrier shows it to everybody.
+        set_columns();
         load_scales(0);
-        ws_table();
-        store_scales(0);
+        load_ws(0);
         issue(slot0, 0);
         issue(slot1, 1);
+      for (;;) {                                                 // column tiles
+        hold_ws();
+        store_scales(0);
         load_scales(C::kChunk);
+#pragma unroll
+        for (int i = 0; i < FT; ++i)
+#pragma unroll
+            for (int j = 0; j < FN; ++j) run[i][j] = v4f{0.f, 0.f, 0.f, 0.f};
+        int g = 0, base = 0;
         // (the ways out of the loop are jumps: with a flag the compiler counts loads in flight along paths
         // from there back into the loop)
         for (int at = 0;; at ^= C::kChunk * BT) {
-            if (g - base >= kSpan) ws_table();
+            if (g - base >= kSpan) {
+                base = g;
+                load_ws(base);
+                hold_ws();
+            }
             int l = (g - base) / S, xa = at + xs_lane;
             auto pick = [&](float v) __attribute__((always_inline)) {
                 return __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(v), l));
@@ -347,7 +365,18 @@ __global__ void __launch_bounds__(C::kThreads * C::KS, 2) block_tiles_kernel(Blo
             for (int i = 0; i < FT * FN; ++i) run[i / FN][i % FN] += sums[i * C::kThreads + tid];
         }
 
-        // ---- epilogue: lane (q, c) holds row 16 i + c, columns 4 q .. 4 q + 3 of each fragment ----
+        // ---- the next column tile's first loads, and this one's epilogue: lane (q, c) holds row 16 i + c,
+        // columns 4 q .. 4 q + 3 of each fragment ----
+        const int at_ct = ct;
+        const bool more = GROUPED && ++ct < ct_end;
+        if (GROUPED) group_barrier();                            // nobody reads the slots or the tables any more
+        if (more) {
+            set_columns();
+            load_scales(0);
+            load_ws(0);
+            issue(slot0, 0);
+            issue(slot1, 1);
+        }
         auto live = [&](int i, int& row) __attribute__((always_inline)) {
             const int f = wt * FT + i;
             row = row0 + f * 16 + c;
@@ -358,7 +387,6 @@ __global__ void __launch_bounds__(C::kThreads * C::KS, 2) block_tiles_kernel(Blo
         };
         if constexpr (kSilu) {
             // h of this wave's columns; a row's absmax over the 128 is joined over the waves in LDS
-            float* s_max = reinterpret_cast<float*>(slot0);      // [WN][BT]
             float top[FT];
 #pragma unroll
             for (int i = 0; i < FT; ++i) {
@@ -372,7 +400,6 @@ __global__ void __launch_bounds__(C::kThreads * C::KS, 2) block_tiles_kernel(Blo
                     }
                 top[i] = rows4_max(m);
             }
-            group_barrier();                                     // (nobody reads slot 0 any more)
 #pragma unroll
             for (int i = 0; i < FT; ++i)
                 if (q == 0) s_max[wn * BT + (wt * FT + i) * 16 + c] = top[i];
@@ -388,9 +415,9 @@ __global__ void __launch_bounds__(C::kThreads * C::KS, 2) block_tiles_kernel(Blo
 #pragma unroll
                 for (int j = 0; j < FN / 2; ++j)
                     *reinterpret_cast<uint32_t*>(reinterpret_cast<uint8_t*>(p.out) + (int64_t)row * p.ldo +
-                                                 col_of((wn * FN + j) * 16) + 4 * q) =
+                                                 col_of(at_ct, (wn * FN + j) * 16 + 4 * q)) =
                         pack4_e4m3(run[i][j][0] * inv, run[i][j][1] * inv, run[i][j][2] * inv, run[i][j][3] * inv);
-                if (wn == 0 && q == 0) p.out_scales[(int64_t)row * (half / kBlk) + ct] = sc;
+                if (wn == 0 && q == 0) p.out_scales[(int64_t)row * (half / kBlk) + at_ct] = sc;
             }
         } else if constexpr (DST == Dst::kRowF16) {
             // a row's largest value of this wave's columns to [2^14, 2^15): infinities, NaN and zeros as they are
@@ -408,11 +435,12 @@ __global__ void __launch_bounds__(C::kThreads * C::KS, 2) block_tiles_kernel(Blo
                 if (!live(i, row)) continue;
 #pragma unroll
                 for (int j = 0; j < FN; ++j) {
-                    const int col = col_of((wn * FN + j) * 16) + 4 * q;      // (whole tiles: N % 128 == 0)
 #pragma unroll
                     for (int r = 0; r < 4; ++r) run[i][j][r] *= inv;
-                    store16(p, row, col, N, run[i][j], false);
-                    if (q == 0 && j % 2 == 0) p.out_scales[(int64_t)row * (N / 32) + col / 32] = __uint_as_float(sb << 23);
+                    if (j % 2 == 0) continue;
+                    const int col = col_of(at_ct, (wn * FN + j - 1) * 16 + 4 * q);  // (whole tiles: N % 128 == 0)
+                    store16x8(p, row, col, run[i][j - 1], run[i][j], false);
+                    if (q == 0) p.out_scales[(int64_t)row * (N / 32) + col / 32] = __uint_as_float(sb << 23);
                 }
             }
         } else {
@@ -422,12 +450,17 @@ __global__ void __launch_bounds__(C::kThreads * C::KS, 2) block_tiles_kernel(Blo
                 if (!live(i, row)) continue;
 #pragma unroll
                 for (int j = 0; j < FN; ++j) {
-                    const int col = col_of((wn * FN + j) * 16) + 4 * q;
-                    if (col < N) store16(p, row, col, N, run[i][j], p.out_bf16 != 0);
+                    const int col = col_of(at_ct, (wn * FN + j) * 16 + 4 * q);
+                    if (FN % 2 == 0 && p.out16 && p.ldo % 8 == 0) {
+                        if (j % 2 == 1 && col < N) store16x8(p, row, col - 4, run[i][j - 1], run[i][j], p.out_bf16 != 0);
+                    } else if (col < N) {
+                        store16(p, row, col, N, run[i][j], p.out_bf16 != 0);
+                    }
                 }
             }
         }
-        if (GROUPED) group_barrier();                            // the slots are free for the next pass
+        if (!more) break;
+      }
     }
 }
 
@@ -437,7 +470,13 @@ int tiles_go(const BlockParams& p, hipStream_t s) {
     const int ntiles = silu ? p.N / 2 / kBlk : (p.N + C::BN - 1) / C::BN, mtiles = (p.P + C::BT - 1) / C::BT;
     const int run_rows = std::min(kRunRows, mtiles);
     const int64_t runs = (mtiles + run_rows - 1) / run_rows;
-    const int64_t items = GROUPED ? (runs + kTileXcds - 1) / kTileXcds * kTileXcds * run_rows * ntiles
+    // Grouped: two column tiles a work-group where that leaves four rounds or more of them (a layer's
+    // products of 4096 tokens x 8, 256 experts: 260 -> 247 and 180 -> 162 us; four tiles: 279 and 167; 256 x 8
+    // slots of 8 experts, one round: 79 -> 83).
+    const int64_t passes = p.num_valid / C::BT + std::min(p.E, p.num_valid);
+    const int cts = GROUPED && ntiles > 1 && passes * ntiles >= 4 * (int64_t)device_cu_count() * (512 / C::kThreads) ? 2 : 1;
+    const int sets = (ntiles + cts - 1) / cts;
+    const int64_t items = GROUPED ? (runs + kTileXcds - 1) / kTileXcds * kTileXcds * run_rows * sets
                                   : ((int64_t)mtiles * ntiles + kTileXcds - 1) / kTileXcds * kTileXcds;
     if (items >= (int64_t)1 << 30) {
         set_error("fp8 block product: too many tiles");
@@ -446,10 +485,10 @@ int tiles_go(const BlockParams& p, hipStream_t s) {
     const dim3 grid((unsigned)items);
     if constexpr (DST == Dst::kF16)
         if (p.K % kBlk != 0) {
-            launch_kernel(&block_tiles_kernel<C, DST, silu, true, GROUPED>, grid, dim3(C::kThreads * C::KS), 0, s, p, ntiles, run_rows);
+            launch_kernel(&block_tiles_kernel<C, DST, silu, true, GROUPED>, grid, dim3(C::kThreads * C::KS), 0, s, p, ntiles, run_rows, cts);
             return check_launch("block_tiles_kernel");
         }
-    launch_kernel(&block_tiles_kernel<C, DST, silu, false, GROUPED>, grid, dim3(C::kThreads * C::KS), 0, s, p, ntiles, run_rows);
+    launch_kernel(&block_tiles_kernel<C, DST, silu, false, GROUPED>, grid, dim3(C::kThreads * C::KS), 0, s, p, ntiles, run_rows, cts);
     return check_launch("block_tiles_kernel");
 }
 
