@@ -22,7 +22,10 @@ bool is16(int dt) { return dt == W4A8_DTYPE_F16 || dt == W4A8_DTYPE_BF16; }
 
 constexpr int64_t kMaxSide = (int64_t)1 << 24;    // rows of a weight, values of a row
 constexpr int64_t kMaxRows = ((int64_t)1 << 31) - 256;
-constexpr int64_t kStreamRows = 16;               // dense rows up to which the weights are streamed
+constexpr int64_t kReduceRows = 65535;            // tokens of one slot reduce (its grid's second side)
+// Dense rows up to which the weights are streamed: one row block (us, streamed / 64 x 64 tiles with K in two:
+// 16 x 4096 x 4096 9.8 / 11.8, 16 x 2048 x 12288 18.7 / 25.9; two row blocks, 32 x 4096 x 4096, 15.2 / 12.0).
+constexpr int64_t kStreamRows = 16;
 
 // Sizes and pointers that every product shares.
 int check_product(const void* x, int x_dtype, const float* xs, int64_t rows, int64_t K, int64_t ldx, const uint8_t* w,
@@ -57,6 +60,8 @@ struct LayerPlan {
 LayerPlan plan_layer(int64_t T, int64_t H, int64_t inter, int64_t E, int64_t top_k) {
     LayerPlan pl;
     const int64_t lim = (int64_t)1 << 32;
+    // us streamed / tiles: 256 experts (2048 x 512), 8 rows each 227 / 252, 12.5 rows 231 / 233; 32 experts, 8 rows
+    // 52 / 48, 16 rows 62 / 48; 8 experts, 8 rows 23 / 43, 16 rows 37 / 43
     pl.tiles = T * top_k > 12 * E;
     pl.block_m = pl.tiles ? 64 : 16;
     pl.P = w4a8_moe_align_sorted_len(T * top_k, E, pl.block_m);
@@ -277,7 +282,12 @@ int w4a8_moe_fp8_block_apply(const void* x, int x_dtype, const float* x_scales, 
     }
     if (int rc = launch_block_stream(g1, s)) return rc;
     if (int rc = launch_block_stream(g2, s)) return rc;
-    return launch_slot_reduce(m.y32, topk_weights, topk_ids, expert_map, n_global, E, T, H, top_k, out, bf16, s);
+    for (int64_t t = 0; t < T; t += kReduceRows)
+        if (int rc = launch_slot_reduce(m.y32 + t * top_k * H, topk_weights + t * top_k, topk_ids + t * top_k, expert_map,
+                                        n_global, E, std::min(kReduceRows, T - t), H, top_k,
+                                        static_cast<uint16_t*>(out) + t * H, bf16, s))
+            return rc;
+    return W4A8_OK;
 }
 
 }  // extern "C"
