@@ -131,6 +131,9 @@ __device__ __forceinline__ uint32_t pack_out16(float a, float b, bool bf16) {
            ((uint32_t)__half_as_ushort(__float2half(as_f32(b))) << 16);
 }
 
+// A launch's work-items are counted in 32 bits.
+inline bool grid_fits(int64_t blocks, int64_t threads) { return blocks < ((int64_t)1 << 32) / threads; }
+
 // ---- launchers (all enqueue on the stream) ----
 struct NormArgs {
     const void* x;

@@ -364,6 +364,10 @@ int launch_rms_norm_quant(const NormArgs& a, hipStream_t s) {
     const bool whole = a.H % 8 == 0 && a.H <= 16384 && a.ldx % 8 == 0 && (a.residual == nullptr || a.ldr % 8 == 0) &&
                        aligned(a.x, 16) && aligned(a.residual, 16) && aligned(a.weight, 16) &&
                        aligned(a.residual_out, 16) && aligned(a.norm_out, 16) && aligned(a.q, 8);
+    if (!grid_fits(whole && a.H <= 512 ? (a.rows + 3) / 4 : a.rows, whole && a.H > 8192 ? 1024 : 256)) {
+        set_error("rms_norm_quant: too many rows");
+        return W4A8_ERR_INVALID;
+    }
     if (whole) {
         if (a.bf16) norm_sizes<true>(p, a.weight_f32, a.per_row, s);
         else norm_sizes<false>(p, a.weight_f32, a.per_row, s);
@@ -377,6 +381,10 @@ int launch_rms_norm_quant(const NormArgs& a, hipStream_t s) {
 int launch_block_reduce(const void* y, const float* ys, const int32_t* slot_to_row, const float* tw, int64_t T, int64_t N,
                         int64_t top_k, void* out, bool bf16, hipStream_t s) {
     if (T == 0) return W4A8_OK;
+    if (!grid_fits(T, 256)) {
+        set_error("block_reduce: too many rows");
+        return W4A8_ERR_INVALID;
+    }
     const dim3 grid((unsigned)T, (unsigned)((N / 8 + 255) / 256));
     if (bf16) block_reduce_kernel<true><<<grid, 256, 0, s>>>(y, ys, slot_to_row, tw, (int)N, (int)top_k, out);
     else block_reduce_kernel<false><<<grid, 256, 0, s>>>(y, ys, slot_to_row, tw, (int)N, (int)top_k, out);
@@ -389,7 +397,7 @@ int launch_act_quant_block(const void* x, bool bf16, int64_t rows, int64_t K, in
     const int64_t G = blk_groups(K);
     const bool whole = K % 8 == 0 && ldx % 8 == 0 && aligned(x, 16) && aligned(q, 8);
     const int64_t blocks = whole ? (rows * G * 16 + 255) / 256 : (rows * G + 3) / 4;
-    if (blocks >= (int64_t)1 << 31) {
+    if (!grid_fits(blocks, 256)) {
         set_error("act_quant_fp8_block: too many groups");
         return W4A8_ERR_INVALID;
     }

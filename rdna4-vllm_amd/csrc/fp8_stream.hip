@@ -341,7 +341,7 @@ int go_any(const BlockParams& p, hipStream_t s) {
     const int cols = silu ? p.N / 2 : p.N, per = 16 * (silu ? FN / 2 : FN);
     const int slices = (cols + per - 1) / per;
     const int64_t grid = (int64_t)((p.P + 15) / 16) * slices;
-    if (grid >= (int64_t)1 << 31) return too_many();
+    if (!grid_fits(grid, 64 * KS)) return too_many();
     launch_kernel(&block_stream_kernel<FN, KS, SRC, DST>, dim3((unsigned)grid), dim3(64 * KS), 0, s, p, slices);
     return check_launch("block_stream_kernel");
 }
@@ -355,7 +355,7 @@ int launch_rows(const BlockParams& p, int frags, int64_t per, hipStream_t s) {
         if (per * pair <= D / 2) return launch_rows<GPW, KS, CG, D / 2, SRC, DST>(p, frags, per, s);
     const int slices = (int)((frags + per * CG - 1) / (per * CG));
     const int64_t grid = (int64_t)((p.P + 15) / 16) * slices;
-    if (grid >= (int64_t)1 << 31) return too_many();
+    if (!grid_fits(grid, 64 * KS * CG)) return too_many();
     launch_kernel(&block_rows_kernel<GPW, KS, CG, D, SRC, DST>, dim3((unsigned)grid), dim3(64 * KS * CG), 0, s, p, slices,
                   (int)per);
     return check_launch("block_rows_kernel");

@@ -478,7 +478,7 @@ int tiles_go(const BlockParams& p, hipStream_t s) {
     const int sets = (ntiles + cts - 1) / cts;
     const int64_t items = GROUPED ? (runs + kTileXcds - 1) / kTileXcds * kTileXcds * run_rows * sets
                                   : ((int64_t)mtiles * ntiles + kTileXcds - 1) / kTileXcds * kTileXcds;
-    if (items >= (int64_t)1 << 30) {
+    if (!grid_fits(items, C::kThreads * C::KS)) {
         set_error("fp8 block product: too many tiles");
         return W4A8_ERR_INVALID;
     }

@@ -129,14 +129,16 @@ def norm(**k):
 @pytest.mark.parametrize("bad,says", [
     (dict(xd=E4M3), "fp16 or bf16"), (dict(rows=-1), "sizes"), (dict(H=0), "sizes"), (dict(x=None), "null"),
     (dict(w=None), "null"), (dict(q=None), "null"), (dict(s=None), "null"), (dict(r=P16, ldr=256), "go together"),
-    (dict(ro=P16), "go together"), (dict(ldx=255), "overlap"), (dict(r=P16, ro=P16, ldr=100), "overlap")])
+    (dict(ro=P16), "go together"), (dict(rows=1 << 24, H=7, ldx=7), "too many rows"),
+    (dict(rows=1 << 30), "too many rows"), (dict(ldx=255), "overlap"), (dict(r=P16, ro=P16, ldr=100), "overlap")])
 def test_norm_refusals(bad, says):
     assert norm(**bad) == INVALID and says in err()
 
 
 @pytest.mark.parametrize("bad,says", [
     (dict(xd=E4M3), "fp16 or bf16"), (dict(rows=-1), "sizes"), (dict(K=0), "sizes"), (dict(x=None), "null"),
-    (dict(q=None), "null"), (dict(s=None), "null"), (dict(ldx=255), "overlap"), (dict(silu=1, ldx=300), "overlap")])
+    (dict(q=None), "null"), (dict(s=None), "null"), (dict(ldx=255), "overlap"), (dict(silu=1, ldx=300), "overlap"),
+    (dict(rows=1 << 30), "too many groups"), (dict(rows=1 << 26, K=7, ldx=7), "too many groups")])
 def test_quant_refusals(bad, says):
     a = dict(x=P16, xd=BF16, rows=2, K=256, ldx=256, silu=0, q=P16, s=P16)
     a.update(bad)
