@@ -22,6 +22,7 @@ enum class Src : int {
     kF16 = 1,    // fp16 / bf16 rows, quantised in registers
     kBf16 = 2,
     kF32 = 3,    // fp32 rows, quantised in registers
+    kWide = 4,   // as kFp8, the e4m3 values as the bf16 numbers that they are (tiles of the layer's first product)
 };
 // What it writes.
 enum class Dst : int {
@@ -153,6 +154,10 @@ int launch_rms_norm_quant(const NormArgs& a, hipStream_t s);
 // slots / ntp (optional): only rows r < ntp whose slot is below num_valid.
 int launch_act_quant_block(const void* x, bool bf16, int64_t rows, int64_t K, int64_t ldx, bool silu,
                            uint8_t* q, float* scales, hipStream_t s);
+// The same rows for Src::kWide, from 16-bit rows (with their scales) or from e4m3 rows; K % 128 == 0,
+// rows contiguous and aligned to 16 bytes.
+int launch_act_quant_wide(const void* x, bool bf16, int64_t rows, int64_t K, uint16_t* q, float* scales, hipStream_t s);
+int launch_widen_rows(const void* x, int64_t rows, int64_t K, uint16_t* q, hipStream_t s);
 // Weight-streaming product (fp8_stream.hip): any sizes.
 int launch_block_stream(const BlockArgs& a, hipStream_t s);
 // Tiles (fp8_tiles.hip): e4m3 rows, sizes that 32-bit offsets reach.

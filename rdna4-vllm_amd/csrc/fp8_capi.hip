@@ -50,7 +50,7 @@ Dst dst_of(int dt) { return dt == W4A8_DTYPE_BF16 ? Dst::kBf16 : Dst::kF16; }
 
 // ---- the gated layer ----
 // Few rows an expert: blocks of 16 rows on the streaming kernels (rows quantised in registers, h and
-// the slots' rows in fp32). Else tiles: rows quantised beforehand, h by gemm1, the slots' rows in fp16
+// the slots' rows in fp32). Else tiles: rows quantised beforehand, as bf16 numbers, h by gemm1, the slots' rows in fp16
 // with scales (in the output's type they would add as much error as its own rounding: 1.5 times the
 // layer's in all), blocks of the 64 rows that a tile's wave takes.
 struct LayerPlan {
@@ -65,7 +65,7 @@ LayerPlan plan_layer(int64_t T, int64_t H, int64_t inter, int64_t E, int64_t top
     pl.tiles = T * top_k > 12 * E;
     pl.block_m = pl.tiles ? 64 : 16;
     pl.P = w4a8_moe_align_sorted_len(T * top_k, E, pl.block_m);
-    if (pl.tiles && (T * H >= lim || pl.P * inter >= lim || 2 * inter * H >= lim)) {
+    if (pl.tiles && (2 * T * H >= lim || pl.P * inter >= lim || 2 * inter * H >= lim)) {
         pl.tiles = false;
         pl.block_m = 16;
         pl.P = w4a8_moe_align_sorted_len(T * top_k, E, pl.block_m);
@@ -79,7 +79,8 @@ struct LayerScratch {
     int32_t *sti, *eid, *ntp, *s2r;
     void* align_ws;
     size_t align_bytes;
-    uint8_t *xq, *hq;
+    uint16_t* xq;
+    uint8_t* hq;
     float *xs, *hs, *h, *y32, *ys;
     uint16_t* y16;
 };
@@ -98,7 +99,7 @@ void carve_layer(WS& w, const LayerPlan& pl, int64_t T, int64_t H, int64_t inter
         return;
     }
     m.s2r = w.template take<int32_t>((size_t)(T * top_k));
-    m.xq = w.template take<uint8_t>(quantise ? (size_t)(T * H) : 0);
+    m.xq = w.template take<uint16_t>((size_t)(T * H));
     m.xs = w.template take<float>(quantise ? (size_t)(T * blk_groups(H)) : 0);
     m.hq = w.template take<uint8_t>((size_t)(pl.P * inter));
     m.hs = w.template take<float>((size_t)(pl.P * blk_groups(inter)));
@@ -257,16 +258,18 @@ int w4a8_moe_fp8_block_apply(const void* x, int x_dtype, const float* x_scales, 
     if (int rc = launch_align(topk_ids, T * top_k, E, pl.block_m, expert_map, n_global, m.sti, pl.P, m.eid, m.ntp,
                               m.align_ws, m.align_bytes, s, m.s2r))
         return rc;
-    if (pl.tiles && quantise)
-        if (int rc = launch_act_quant_block(x, x_dtype == W4A8_DTYPE_BF16, T, H, H, false, m.xq, m.xs, s)) return rc;
+    if (pl.tiles)
+        if (int rc = quantise ? launch_act_quant_wide(x, x_dtype == W4A8_DTYPE_BF16, T, H, m.xq, m.xs, s)
+                              : launch_widen_rows(x, T, H, m.xq, s))
+            return rc;
     BlockArgs g1{};
-    g1.x = pl.tiles && quantise ? m.xq : x;
+    g1.x = pl.tiles ? m.xq : x;
     g1.xs = pl.tiles && quantise ? m.xs : x_scales;
     g1.x_rows = T; g1.K = H; g1.ldx = H;
     g1.w = w13; g1.ws = w13_scales; g1.E = E; g1.N = 2 * inter;
     g1.sorted_ids = m.sti; g1.expert_ids = m.eid; g1.ntp = m.ntp; g1.P = pl.P;
     g1.top_k = top_k; g1.num_valid = T * top_k; g1.block_m = pl.block_m; g1.gather = true; g1.all_rows = true;
-    g1.src = pl.tiles ? Src::kFp8 : src_of(x_dtype);
+    g1.src = pl.tiles ? Src::kWide : src_of(x_dtype);
     g1.dst = pl.tiles ? Dst::kSiluFp8 : Dst::kSiluF32;
     g1.out = pl.tiles ? (void*)m.hq : (void*)m.h; g1.out_scales = m.hs; g1.ldo = inter;
     BlockArgs g2 = g1;

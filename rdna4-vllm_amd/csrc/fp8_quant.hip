@@ -6,7 +6,7 @@
 // sixteen neighbouring lanes, so its absmax is four DPP steps.
 #include <algorithm>
 
-#include "fp8_block.h"
+#include "fp8_mfma.h"
 
 namespace w4a8 {
 namespace {
@@ -226,8 +226,19 @@ __global__ void __launch_bounds__(256) rms_norm_quant_any_kernel(NormParams p, b
     }
 }
 
+// e4m3 values as bf16 numbers, eight of them.
+__device__ __forceinline__ u32x4 widen8(uint2 v) {
+    union {
+        v8bf h;
+        u32x4 u;
+    } o;
+    o.h = e4m3_to_bf16x8(v.x, v.y);
+    return o.u;
+}
+
 // Eight values a lane: sixteen lanes a group of 128, K8 = lanes that a row takes (ceil(K / 128) * 16).
-template <bool BF16, bool SILU>
+// WIDE: the e4m3 values as bf16 numbers.
+template <bool BF16, bool SILU, bool WIDE>
 __global__ void __launch_bounds__(256) act_quant_groups_kernel(const void* __restrict__ x, int64_t rows, int K, int G,
                                                                int64_t ldx, uint8_t* __restrict__ q,
                                                                float* __restrict__ scales) {
@@ -252,9 +263,16 @@ __global__ void __launch_bounds__(256) act_quant_groups_kernel(const void* __res
     }
     const float s = act_scale_from_absmax(lane_allreduce<4>(absmax8(f), MaxOp{}));
     if (k < K) {
-        *reinterpret_cast<uint2*>(q + row * K + k) = quant8(f, 1.0f / s);
+        const uint2 v = quant8(f, 1.0f / s);
+        if constexpr (WIDE) *reinterpret_cast<u32x4*>(reinterpret_cast<uint16_t*>(q) + row * K + k) = widen8(v);
+        else *reinterpret_cast<uint2*>(q + row * K + k) = v;
         if ((threadIdx.x & 15) == 0) scales[row * G + k / kBlk] = s;
     }
+}
+
+__global__ void __launch_bounds__(256) widen_rows_kernel(const uint2* __restrict__ x, int64_t n8, u32x4* __restrict__ q) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i < n8) q[i] = widen8(x[i]);
 }
 
 // Any sizes and alignments: a wave a group.
@@ -403,13 +421,38 @@ int launch_act_quant_block(const void* x, bool bf16, int64_t rows, int64_t K, in
     }
     auto go = [&](auto kernel) { kernel<<<(unsigned)blocks, 256, 0, s>>>(x, rows, (int)K, (int)G, ldx, q, scales); };
     if (whole) {
-        if (bf16) silu ? go(act_quant_groups_kernel<true, true>) : go(act_quant_groups_kernel<true, false>);
-        else silu ? go(act_quant_groups_kernel<false, true>) : go(act_quant_groups_kernel<false, false>);
+        if (bf16) silu ? go(act_quant_groups_kernel<true, true, false>) : go(act_quant_groups_kernel<true, false, false>);
+        else silu ? go(act_quant_groups_kernel<false, true, false>) : go(act_quant_groups_kernel<false, false, false>);
         return check_launch("act_quant_groups_kernel");
     }
     if (bf16) silu ? go(act_quant_groups_any_kernel<true, true>) : go(act_quant_groups_any_kernel<true, false>);
     else silu ? go(act_quant_groups_any_kernel<false, true>) : go(act_quant_groups_any_kernel<false, false>);
     return check_launch("act_quant_groups_any_kernel");
+}
+
+int launch_act_quant_wide(const void* x, bool bf16, int64_t rows, int64_t K, uint16_t* q, float* scales, hipStream_t s) {
+    if (rows == 0) return W4A8_OK;
+    const int64_t G = blk_groups(K), blocks = (rows * G * 16 + 255) / 256;
+    if (K % kBlk != 0 || !aligned(x, 16) || !aligned(q, 16) || !grid_fits(blocks, 256)) {
+        set_error("act_quant_fp8_block: sizes not taken by the wide form");
+        return W4A8_ERR_INVALID;
+    }
+    auto go = [&](auto kernel) {
+        kernel<<<(unsigned)blocks, 256, 0, s>>>(x, rows, (int)K, (int)G, K, reinterpret_cast<uint8_t*>(q), scales);
+    };
+    bf16 ? go(act_quant_groups_kernel<true, false, true>) : go(act_quant_groups_kernel<false, false, true>);
+    return check_launch("act_quant_groups_kernel");
+}
+
+int launch_widen_rows(const void* x, int64_t rows, int64_t K, uint16_t* q, hipStream_t s) {
+    if (rows == 0) return W4A8_OK;
+    const int64_t n8 = rows * (K / 8), blocks = (n8 + 255) / 256;
+    if (K % 8 != 0 || !aligned(x, 8) || !aligned(q, 16) || !grid_fits(blocks, 256)) {
+        set_error("widen_rows: sizes not taken");
+        return W4A8_ERR_INVALID;
+    }
+    widen_rows_kernel<<<(unsigned)blocks, 256, 0, s>>>(static_cast<const uint2*>(x), n8, reinterpret_cast<u32x4*>(q));
+    return check_launch("widen_rows_kernel");
 }
 
 }  // namespace w4a8

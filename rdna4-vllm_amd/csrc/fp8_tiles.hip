@@ -38,18 +38,19 @@ __device__ __forceinline__ void group_barrier() {
 
 // WT x WN waves of FT row fragments x FN column fragments of 16, S groups in LDS; KS such parts of a
 // work-group share K, each with slots of its own, and add their sums at the end.
-template <int WT_, int WN_, int FT_, int FN_, int S_, int KS_ = 1>
+// XB: bytes of a row's value (2: bf16 numbers that hold e4m3 values).
+template <int WT_, int WN_, int FT_, int FN_, int S_, int KS_ = 1, int XB_ = 1>
 struct TileCfg {
-    static constexpr int WT = WT_, WN = WN_, FT = FT_, FN = FN_, S = S_, KS = KS_;
+    static constexpr int WT = WT_, WN = WN_, FT = FT_, FN = FN_, S = S_, KS = KS_, XB = XB_;
     static constexpr int kWaves = WT * WN, kThreads = 64 * kWaves;   // of a part
     static constexpr int BT = WT * FT * 16, BN = WN * FN * 16;
-    static constexpr int kW = BT * kBlk;                         // weights behind the rows
+    static constexpr int kW = BT * kBlk * XB;                    // weights behind the rows
     static constexpr int kSlot = kW + BN * kBlk;
-    static constexpr int PX = BT * 8 / kThreads, PW = BN * 8 / kThreads;   // 16-byte pieces a thread
+    static constexpr int PX = BT * 8 * XB / kThreads, PW = BN * 8 / kThreads;   // 16-byte pieces a thread
     static constexpr int kLoads = PX + PW;                       // of a wave and group
     static constexpr int kChunk = 6;                             // groups whose row scales are loaded at once
     static constexpr int PT = (BT * kChunk + kThreads - 1) / kThreads;   // entries a thread
-    static_assert(PX * kThreads == BT * 8 && PW * kThreads == BN * 8, "pieces divide");
+    static_assert(PX * kThreads == BT * 8 * XB && PW * kThreads == BN * 8, "pieces divide");
     static_assert(FN * 16 <= kBlk && kBlk % (FN * 16) == 0, "a wave's columns lie in one block");
     static_assert(kChunk % S == 0, "rounds divide");
     static_assert((S == 2 || S == 3) && kLoads < 64, "slots; loads in flight can be counted");
@@ -61,6 +62,7 @@ __global__ void __launch_bounds__(C::kThreads * C::KS, 2) block_tiles_kernel(Blo
     constexpr bool kSilu = DST == Dst::kSiluFp8;
     constexpr int KS = C::KS;
     static_assert(!kSilu || BN == 256, "SiLU tiles hold 128 gate and 128 up columns");
+    static_assert(C::XB == 1 || (C::XB == 2 && EXACT && !TAIL), "wide rows are for the bf16 matrix cores");
     static_assert(KS <= 2 && (KS == 1 || (DST == Dst::kF16 && !GROUPED)), "a divided K is for dense products");
     // arrays of their own: the compiler then sees that reads of one do not wait for loads into another
     __shared__ __attribute__((aligned(1024))) uint8_t slots0[KS * C::kSlot];
@@ -122,15 +124,22 @@ __global__ void __launch_bounds__(C::kThreads * C::KS, 2) block_tiles_kernel(Blo
     };
     // (entries of a table of row scales past the last one are the last one again)
     auto entry = [&](int i) __attribute__((always_inline)) { return min(tid + i * C::kThreads, BT * C::kChunk - 1); };
+    // (rows of two bytes a value: sixteen pieces, piece j of row r at j ^ (r & 15))
+    auto xpiece_row = [&](int i) __attribute__((always_inline)) {
+        return C::XB == 2 ? (tid + i * C::kThreads) >> 4 : piece_row(i);
+    };
+    auto xpiece_at = [&](int i) __attribute__((always_inline)) {
+        return C::XB == 2 ? ((tid & 15) ^ (xpiece_row(i) & 15)) * 16 : piece_k(piece_row(i));
+    };
     uint32_t xoff[C::PX], toff[C::PT];
 #pragma unroll
-    for (int i = 0; i < C::PX; ++i) xoff[i] = xrow_of(piece_row(i));
+    for (int i = 0; i < C::PX; ++i) xoff[i] = xrow_of(xpiece_row(i));
 #pragma unroll
     for (int i = 0; i < C::PT; ++i) toff[i] = xrow_of(entry(i) / C::kChunk);
     const int end = GROUPED ? min(p.ntp[0], p.P) : p.P;
     if (row0 >= end) return;
 #pragma unroll
-    for (int i = 0; i < C::PX; ++i) xoff[i] = xoff[i] * (uint32_t)p.ldx + (uint32_t)piece_k(piece_row(i));
+    for (int i = 0; i < C::PX; ++i) xoff[i] = xoff[i] * (uint32_t)p.ldx * C::XB + (uint32_t)xpiece_at(i);
 #pragma unroll
     for (int i = 0; i < C::PT; ++i) toff[i] *= (uint32_t)G;
     if (lane >= BT / 16 || row0 + 16 * lane >= end || fe >= p.E) fe = -1;
@@ -170,7 +179,7 @@ __global__ void __launch_bounds__(C::kThreads * C::KS, 2) block_tiles_kernel(Blo
         auto issue_some = [&](uint8_t* slot, int g, int some, int parts) __attribute__((always_inline)) {
             const uint32_t on = g < G1 && g_first + g < G ? ~0u : 0u;
             const int gg = min(g_first + g, G - 1);
-            const uint8_t *xg = xb + (int64_t)gg * kBlk, *wg = wb + (int64_t)gg * kBlk;
+            const uint8_t *xg = xb + (int64_t)gg * kBlk * C::XB, *wg = wb + (int64_t)gg * kBlk;
             asm volatile("" : "+s"(xg), "+s"(wg));               // (scalar bases, 32-bit offsets)
             uint8_t *xd = slot + wave * 1024, *wd = slot + C::kW + wave * 1024;
             auto src = [&](const uint8_t* base, uint32_t off, int i) __attribute__((always_inline)) {
@@ -213,6 +222,7 @@ __global__ void __launch_bounds__(C::kThreads * C::KS, 2) block_tiles_kernel(Blo
 
         const int cr = (c ^ (c >> 3)) * kBlk;
         const int p0 = cr + (((2 * q) ^ (c & 7)) << 4), p1 = cr + (((2 * q + 1) ^ (c & 7)) << 4);
+        const int px = c * kBlk * 2 + (((2 * q) ^ c) << 4);      // (wide rows)
         // One group: the rows' fragments against the columns', of which the next is read while one is
         // multiplied and the one before is folded.
         // With three slots the loads of group g + 2 are issued between the fragments, into `next`, so that
@@ -223,7 +233,7 @@ __global__ void __launch_bounds__(C::kThreads * C::KS, 2) block_tiles_kernel(Blo
                 f[0] = *reinterpret_cast<const u32x4*>(slot + at + p0);
                 f[1] = *reinterpret_cast<const u32x4*>(slot + at + p1);
             };
-            u32x4 wf[2][2], xr[FT][2];
+            u32x4 wf[2][2];
             float xs[FT];
             GroupOp<EXACT> xf[FT];
             v4f pend[2][FT];
@@ -237,12 +247,24 @@ __global__ void __launch_bounds__(C::kThreads * C::KS, 2) block_tiles_kernel(Blo
                 }
             };
             frag(C::kW + wn * FN * 16 * kBlk, wf[0]);
+            if constexpr (C::XB == 2) {
 #pragma unroll
-            for (int i = 0; i < FT; ++i) frag((wt * FT + i) * 16 * kBlk, xr[i]);
+                for (int i = 0; i < FT; ++i)
 #pragma unroll
-            for (int i = 0; i < FT; ++i) xs[i] = s_xs[xs_at + i * 16];
+                    for (int h = 0; h < 4; ++h)              // pieces 2 q, 2 q + 1, 2 q + 8, 2 q + 9 of the row
+                        xf[i].h[h] = *reinterpret_cast<const v8bf*>(slot + (wt * FT + i) * 16 * kBlk * 2 +
+                                                                    (px ^ ((h & 1) * 16 + (h >> 1) * 128)));
 #pragma unroll
-            for (int i = 0; i < FT; ++i) xf[i] = group_op<EXACT>(xr[i][0], xr[i][1]);
+                for (int i = 0; i < FT; ++i) xs[i] = s_xs[xs_at + i * 16];
+            } else {
+                u32x4 xr[FT][2];
+#pragma unroll
+                for (int i = 0; i < FT; ++i) frag((wt * FT + i) * 16 * kBlk, xr[i]);
+#pragma unroll
+                for (int i = 0; i < FT; ++i) xs[i] = s_xs[xs_at + i * 16];
+#pragma unroll
+                for (int i = 0; i < FT; ++i) xf[i] = group_op<EXACT>(xr[i][0], xr[i][1]);
+            }
 #pragma unroll
             for (int j = 0; j < FN; ++j) {
                 if (j + 1 < FN) frag(C::kW + (wn * FN + j + 1) * 16 * kBlk, wf[(j + 1) & 1]);
@@ -496,7 +518,9 @@ using Tile64x64K2 = TileCfg<1, 4, 4, 1, 3, 2>;  // eight waves, one work-group a
 using Tile64x64 = TileCfg<1, 4, 4, 1, 3>;       // four, three
 using Tile64x128 = TileCfg<1, 4, 4, 2, 3>;      // four, two
 using Tile256x128 = TileCfg<4, 2, 4, 4, 3>;     // eight, one
-using TileSilu = TileCfg<1, 8, 4, 2, 3>;        // 64 x 256: eight, one
+// Rows in bf16: converting them in each of the eight waves takes two thirds of the conversions (layer of 4096
+// tokens, 256 experts: first product 247 -> 231 us; 1111 tokens x 6, 64 experts, the whole layer: 150 -> 142).
+using TileSilu = TileCfg<1, 8, 4, 2, 3, 1, 2>;        // 64 x 256: eight, one
 
 // The dense tile of least cost, us at K = 4096 as measured (the cost of every tile is linear in K):
 //   work-groups a CU:    <= 1     2     3     4     8
@@ -524,10 +548,11 @@ int dense_go(const BlockParams& p, hipStream_t s) {
 bool block_tiles_supported(const BlockArgs& a) {
     // rows, scales and an expert's weights are addressed in 32 bits
     const int64_t lim = (int64_t)1 << 32;
-    return a.src == Src::kFp8 && a.x_rows * a.ldx < lim && a.x_rows * blk_groups(a.K) * 4 < lim && a.N * a.K < lim &&
+    const bool silu = a.dst == Dst::kSiluFp8;
+    return a.src == (silu ? Src::kWide : Src::kFp8) && a.x_rows * a.ldx * (silu ? 2 : 1) < lim && a.x_rows * blk_groups(a.K) * 4 < lim && a.N * a.K < lim &&
            (a.dst == Dst::kF16 || a.dst == Dst::kBf16 ||
             (a.dst == Dst::kRowF16 && a.sorted_ids != nullptr && a.K % kBlk == 0 && a.N % kBlk == 0) ||
-            (a.dst == Dst::kSiluFp8 && a.sorted_ids != nullptr && a.K % kBlk == 0 && a.N % (2 * kBlk) == 0));
+            (silu && a.sorted_ids != nullptr && a.K % kBlk == 0 && a.N % (2 * kBlk) == 0));
 }
 
 int launch_block_tiles(const BlockArgs& a, hipStream_t s) {
