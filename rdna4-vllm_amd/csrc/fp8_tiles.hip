@@ -174,11 +174,22 @@ __global__ void __launch_bounds__(C::kThreads * C::KS, 2) block_tiles_kernel(Blo
         auto dma = [&](const uint8_t* src, uint8_t* dst) __attribute__((always_inline)) {
             __builtin_amdgcn_global_load_lds((global_cvoid_ptr)src, (lds_void_ptr)dst, 16, 0, 0);
         };
+        int ct = ct_first, turn = 0;
+        // The group of k of step g (one that exists, past the last step too). Grouped, rows of a multiple of 4096
+        // bytes: column tiles start at groups of their own. In step, work-groups would read the same few memory
+        // channels (64 experts, 32 slots each, 4096 -> 2048: 165 us, 3.3 TB/s of weights; 109 so; 2048 -> 1024: 112
+        // and 111; a layer of 2048 x 512, 4096 tokens: 471, 478 so). Dense weights are shared by more work-groups,
+        // which that would keep apart (2048 x 4096 x 12288: 110 us, 130 so).
+        auto group_at = [&](int g) __attribute__((always_inline)) {
+            if constexpr (!GROUPED) return min(g_first + g, G - 1);
+            const int at = min(g, G - 1) + turn;
+            return at < G ? at : at - G;
+        };
         // Past the last group every lane reads one piece (nobody reads the slot). TAIL: absent pieces of
         // the last, partial group are zero in both operands.
         auto issue_some = [&](uint8_t* slot, int g, int some, int parts) __attribute__((always_inline)) {
             const uint32_t on = g < G1 && g_first + g < G ? ~0u : 0u;
-            const int gg = min(g_first + g, G - 1);
+            const int gg = group_at(g);
             const uint8_t *xg = xb + (int64_t)gg * kBlk * C::XB, *wg = wb + (int64_t)gg * kBlk;
             asm volatile("" : "+s"(xg), "+s"(wg));               // (scalar bases, 32-bit offsets)
             uint8_t *xd = slot + wave * 1024, *wd = slot + C::kW + wave * 1024;
@@ -202,7 +213,7 @@ __global__ void __launch_bounds__(C::kThreads * C::KS, 2) block_tiles_kernel(Blo
         auto load_scales = [&](int g0) __attribute__((always_inline)) {
 #pragma unroll
             for (int i = 0; i < C::PT; ++i)
-                tv[i] = p.xs[toff[i] + (uint32_t)min(g_first + g0 + entry(i) % C::kChunk, G - 1)];
+                tv[i] = p.xs[toff[i] + (uint32_t)group_at(g0 + entry(i) % C::kChunk)];
         };
         auto store_scales = [&](int at) __attribute__((always_inline)) {
 #pragma unroll
@@ -210,8 +221,8 @@ __global__ void __launch_bounds__(C::kThreads * C::KS, 2) block_tiles_kernel(Blo
         };
         const float* wsb = p.ws + (int64_t)e * p.NB * G;
         const float *wsg = wsb, *wsu = wsb;
-        int ct = ct_first;
         auto set_columns = [&]() __attribute__((always_inline)) {
+            if (GROUPED && K % 4096 == 0) turn = ct * 5 % G;
 #pragma unroll
             for (int i = 0; i < C::PW; ++i)
                 woff[i] = (uint32_t)min(col_of(ct, piece_row(i)), N - 1) * (uint32_t)K + (uint32_t)piece_k(piece_row(i));
@@ -299,7 +310,7 @@ __global__ void __launch_bounds__(C::kThreads * C::KS, 2) block_tiles_kernel(Blo
         auto load_ws = [&](int base) __attribute__((always_inline)) {
 #pragma unroll
             for (int t = 0; t < S; ++t) {
-                const int k = min(g_first + base + lane * S + t, G - 1);
+                const int k = group_at(base + lane * S + t);
                 wgv[t] = wsg[k];
                 wuv[t] = kSilu ? wsu[k] : 0.f;
             }
