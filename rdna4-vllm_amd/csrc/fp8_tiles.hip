@@ -63,7 +63,7 @@ __global__ void __launch_bounds__(C::kThreads * C::KS, 2) block_tiles_kernel(Blo
     constexpr int KS = C::KS;
     static_assert(!kSilu || BN == 256, "SiLU tiles hold 128 gate and 128 up columns");
     static_assert(C::XB == 1 || (C::XB == 2 && EXACT && !TAIL), "wide rows are for the bf16 matrix cores");
-    static_assert(KS <= 2 && (KS == 1 || (DST == Dst::kF16 && !GROUPED)), "a divided K is for dense products");
+    static_assert(KS == 1 || (DST == Dst::kF16 && !GROUPED), "a divided K is for dense products");
     // arrays of their own: the compiler then sees that reads of one do not wait for loads into another
     __shared__ __attribute__((aligned(1024))) uint8_t slots0[KS * C::kSlot];
     __shared__ __attribute__((aligned(1024))) uint8_t slots1[KS * C::kSlot];
@@ -386,16 +386,18 @@ __global__ void __launch_bounds__(C::kThreads * C::KS, 2) block_tiles_kernel(Blo
     summed:
         __builtin_amdgcn_s_waitcnt(wait_vm(0));                  // (the loads past the last group)
         if constexpr (KS > 1) {
-            v4f* sums = reinterpret_cast<v4f*>(slots0);          // [FT FN][kThreads]
-            static_assert(FT * FN * C::kThreads * sizeof(v4f) <= C::kSlot * KS, "sums fit");
+            v4f* sums = reinterpret_cast<v4f*>(slots0);          // [KS - 1][FT FN][kThreads]
+            static_assert((KS - 1) * FT * FN * C::kThreads * sizeof(v4f) <= C::kSlot * KS, "sums fit");
             group_barrier();                                     // nobody reads or loads a slot any more
 #pragma unroll
             for (int i = 0; i < FT * FN; ++i)
-                if (part > 0) sums[i * C::kThreads + tid] = run[i / FN][i % FN];
+                if (part > 0) sums[((part - 1) * FT * FN + i) * C::kThreads + tid] = run[i / FN][i % FN];
             lds_barrier();
             if (part > 0) return;
 #pragma unroll
-            for (int i = 0; i < FT * FN; ++i) run[i / FN][i % FN] += sums[i * C::kThreads + tid];
+            for (int w = 0; w < KS - 1; ++w)
+#pragma unroll
+                for (int i = 0; i < FT * FN; ++i) run[i / FN][i % FN] += sums[(w * FT * FN + i) * C::kThreads + tid];
         }
 
         // ---- the next column tile's first loads, and this one's epilogue: lane (q, c) holds row 16 i + c,
@@ -525,6 +527,8 @@ int tiles_go(const BlockParams& p, hipStream_t s) {
     return check_launch("block_tiles_kernel");
 }
 
+using Tile64x32K4 = TileCfg<2, 2, 2, 1, 3, 4>;  // sixteen waves, one work-group a CU
+using Tile64x32K2 = TileCfg<2, 2, 2, 1, 3, 2>;  // eight waves, two work-groups a CU
 using Tile64x64K2 = TileCfg<1, 4, 4, 1, 3, 2>;  // eight waves, one work-group a CU
 using Tile64x64 = TileCfg<1, 4, 4, 1, 3>;       // four, three
 using Tile64x128 = TileCfg<1, 4, 4, 2, 3>;      // four, two
@@ -533,18 +537,22 @@ using Tile256x128 = TileCfg<4, 2, 4, 4, 3>;     // eight, one
 // tokens, 256 experts: first product 247 -> 231 us; 1111 tokens x 6, 64 experts, the whole layer: 150 -> 142).
 using TileSilu = TileCfg<1, 8, 4, 2, 3, 1, 2>;        // 64 x 256: eight, one
 
-// The dense tile of least cost, us at K = 4096 as measured (the cost of every tile is linear in K):
+// The dense tile of least cost. us at K = 4096 as measured (the cost of every tile is linear in K):
 //   work-groups a CU:    <= 1     2     3     4     8
 //   64 x 64, K in two     12    24
 //   64 x 64               14    19    29    36    64
 //   64 x 128              20    28    52    54
 //   256 x 128          34-42    84
-// 64 rows x 64 columns alone are bound by the latency of a group's loads (0.44 us of the 14 / 32), the
-// largest by what LDS gives the matrix cores (2048 x 4096 x 12288: 1.8 PFLOP/s).
+// 64 rows x 64 columns alone are bound by what one CU has under way (45 GB/s), so where they leave CUs idle half
+// the columns and K in two or four parts: 64 x 4096 x 4096 64 x 64 14.7, K in two 12.2, 64 x 32 in two 10.8, in four
+// 9.6; 17 x 2048 x 12288 35 / 26 / 23 / 16; 48 x 1024 x 1024 (8 groups) 5.3 / 5.3 / 4.6 / 5.3. The largest tile is
+// bound by what LDS gives the matrix cores (2048 x 4096 x 12288: 2.0 PFLOP/s).
 int dense_go(const BlockParams& p, hipStream_t s) {
     const int64_t cus = device_cu_count();
     auto tiles = [&](int bt, int bn) { return (int64_t)((p.P + bt - 1) / bt) * ((p.N + bn - 1) / bn); };
     const int64_t n64 = tiles(64, 64), n128 = tiles(64, 128), n256 = tiles(256, 128);
+    if (tiles(64, 32) <= cus)
+        return p.G > 16 ? tiles_go<Tile64x32K4, Dst::kF16, false>(p, s) : tiles_go<Tile64x32K2, Dst::kF16, false>(p, s);
     if (n64 <= cus) return tiles_go<Tile64x64K2, Dst::kF16, false>(p, s);
     const int64_t t64 = std::max<int64_t>(14 * cus, 9 * n64);
     const int64_t t128 = n128 <= cus ? 20 * cus : (n128 + 2 * cus - 1) / (2 * cus) * 27 * cus;
