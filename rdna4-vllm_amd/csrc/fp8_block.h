@@ -151,7 +151,6 @@ struct NormArgs {
 };
 int launch_rms_norm_quant(const NormArgs& a, hipStream_t s);
 // e4m3 rows and scales of x (rows, K), or of silu(gate) * up of x = [gate | up] (rows, 2 K).
-// slots / ntp (optional): only rows r < ntp whose slot is below num_valid.
 int launch_act_quant_block(const void* x, bool bf16, int64_t rows, int64_t K, int64_t ldx, bool silu,
                            uint8_t* q, float* scales, hipStream_t s);
 // The same rows for Src::kWide, from 16-bit rows (with their scales) or from e4m3 rows; K % 128 == 0,

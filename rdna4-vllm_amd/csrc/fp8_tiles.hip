@@ -1,7 +1,7 @@
 // Block-scaled fp8 products of many rows (gfx950 MFMA), dense or grouped.
 //
 // A work-group owns BT rows by BN weight rows (columns); per group of 128 k both come straight from
-// memory to LDS (16 bytes a lane, no registers), S groups deep. Weights are the first MFMA operand: a
+// memory to LDS (16 bytes a lane, no registers), three groups deep. Weights are the first MFMA operand: a
 // lane ends up with four adjacent columns of one row, so the scale xs[row, g] * ws[block, g] is one
 // number a row fragment, lane and group (a wave's columns lie in one 128-block of the weights).
 //
@@ -36,12 +36,14 @@ __device__ __forceinline__ void group_barrier() {
     __builtin_amdgcn_sched_barrier(0);
 }
 
-// WT x WN waves of FT row fragments x FN column fragments of 16, S groups in LDS; KS such parts of a
-// work-group share K, each with slots of its own, and add their sums at the end.
+constexpr int kSlots = 3;         // groups of k in LDS
+
+// WT x WN waves of FT row fragments x FN column fragments of 16, three groups in LDS; KS such parts of
+// a work-group share K, each with slots of its own, and add their sums at the end.
 // XB: bytes of a row's value (2: bf16 numbers that hold e4m3 values).
-template <int WT_, int WN_, int FT_, int FN_, int S_, int KS_ = 1, int XB_ = 1>
+template <int WT_, int WN_, int FT_, int FN_, int KS_ = 1, int XB_ = 1>
 struct TileCfg {
-    static constexpr int WT = WT_, WN = WN_, FT = FT_, FN = FN_, S = S_, KS = KS_, XB = XB_;
+    static constexpr int WT = WT_, WN = WN_, FT = FT_, FN = FN_, KS = KS_, XB = XB_;
     static constexpr int kWaves = WT * WN, kThreads = 64 * kWaves;   // of a part
     static constexpr int BT = WT * FT * 16, BN = WN * FN * 16;
     static constexpr int kW = BT * kBlk * XB;                    // weights behind the rows
@@ -52,13 +54,13 @@ struct TileCfg {
     static constexpr int PT = (BT * kChunk + kThreads - 1) / kThreads;   // entries a thread
     static_assert(PX * kThreads == BT * 8 * XB && PW * kThreads == BN * 8, "pieces divide");
     static_assert(FN * 16 <= kBlk && kBlk % (FN * 16) == 0, "a wave's columns lie in one block");
-    static_assert(kChunk % S == 0, "rounds divide");
-    static_assert((S == 2 || S == 3) && kLoads < 64, "slots; loads in flight can be counted");
+    static_assert(kChunk == 2 * kSlots, "two rounds a chunk");
+    static_assert(kLoads < 64, "loads in flight can be counted");
 };
 
 template <typename C, Dst DST, bool EXACT, bool TAIL, bool GROUPED>
 __global__ void __launch_bounds__(C::kThreads * C::KS, 2) block_tiles_kernel(BlockParams p, int ntiles, int run_rows, int cts) {
-    constexpr int FT = C::FT, FN = C::FN, BT = C::BT, BN = C::BN, S = C::S;
+    constexpr int FT = C::FT, FN = C::FN, BT = C::BT, BN = C::BN;
     constexpr bool kSilu = DST == Dst::kSiluFp8;
     constexpr int KS = C::KS;
     static_assert(!kSilu || BN == 256, "SiLU tiles hold 128 gate and 128 up columns");
@@ -67,7 +69,7 @@ __global__ void __launch_bounds__(C::kThreads * C::KS, 2) block_tiles_kernel(Blo
     // arrays of their own: the compiler then sees that reads of one do not wait for loads into another
     __shared__ __attribute__((aligned(1024))) uint8_t slots0[KS * C::kSlot];
     __shared__ __attribute__((aligned(1024))) uint8_t slots1[KS * C::kSlot];
-    __shared__ __attribute__((aligned(1024))) uint8_t slots2[S > 2 ? KS * C::kSlot : 16];
+    __shared__ __attribute__((aligned(1024))) uint8_t slots2[KS * C::kSlot];
     __shared__ float s_xs[KS * 2 * C::kChunk * BT];              // row scales [group][row] of two chunks
     __shared__ float s_max[kSilu ? C::WN * BT : 1];              // rows' absmax of a wave's columns
 
@@ -101,7 +103,7 @@ __global__ void __launch_bounds__(C::kThreads * C::KS, 2) block_tiles_kernel(Blo
     const int K = p.K, G = p.G, N = p.N;
     const int G1 = (G + KS - 1) / KS, g_first = part * G1;       // groups of a part, the first of them
     uint8_t *const slot0 = slots0 + part * C::kSlot, *const slot1 = slots1 + part * C::kSlot;
-    uint8_t* const slot2 = slots2 + (S > 2 ? part * C::kSlot : 0);
+    uint8_t* const slot2 = slots2 + part * C::kSlot;
 
     // the expert of fragment `lane`'s rows (-1: none)
     int fe = 0;
@@ -235,9 +237,8 @@ __global__ void __launch_bounds__(C::kThreads * C::KS, 2) block_tiles_kernel(Blo
         const int p0 = cr + (((2 * q) ^ (c & 7)) << 4), p1 = cr + (((2 * q + 1) ^ (c & 7)) << 4);
         const int px = c * kBlk * 2 + (((2 * q) ^ c) << 4);      // (wide rows)
         // One group: the rows' fragments against the columns', of which the next is read while one is
-        // multiplied and the one before is folded.
-        // With three slots the loads of group g + 2 are issued between the fragments, into `next`, so that
-        // no wave waits for the address unit to take all of them (2048 x 4096 x 12288: 132 -> 102 us).
+        // multiplied and the one before is folded. The loads of group g + 2 are issued between the fragments, into
+        // `next`, so that no wave waits for the address unit to take all of them (2048 x 4096 x 12288: 132 -> 102 us).
         // A part's groups past the last one are read as anything and not folded.
         auto compute = [&](const uint8_t* slot, uint8_t* next, int g, int xs_at, float wg, float wu) __attribute__((always_inline)) {
             auto frag = [&](int at, u32x4 (&f)[2]) __attribute__((always_inline)) {
@@ -283,34 +284,29 @@ __global__ void __launch_bounds__(C::kThreads * C::KS, 2) block_tiles_kernel(Blo
                 const GroupOp<EXACT> w = group_op<EXACT>(wf[j & 1][0], wf[j & 1][1]);
 #pragma unroll
                 for (int i = 0; i < FT; ++i) pend[j & 1][i] = group_mfma<EXACT>(w, xf[i]);
-                if (S > 2) issue_some(next, g + 2, j, FN);
+                issue_some(next, g + 2, j, FN);
                 if (j > 0 && on) fold(j - 1);
                 __builtin_amdgcn_sched_barrier(0);
             }
             if (on) fold(FN - 1);
         };
 
-        // Group g. Its stage has landed for this wave when no more than the next one's loads are in
-        // flight, and for all waves behind the barrier. With three slots the barrier also says that
-        // nobody reads group g - 1's slot, which the next loads go to; with two a second one does. Loads
-        // are issued in every step, past the last group too: the compiler counts those in flight along
-        // every path, and would wait for all of them where some path issues none.
+        // Group g. Its stage has landed for this wave when no more than the next one's loads are in flight, and
+        // for all waves behind the barrier, which also says that nobody reads group g - 1's slot any more, where
+        // the next loads go. Loads are issued in every step, past the last group too: the compiler counts those
+        // in flight along every path, and would wait for all of them where some path issues none.
         auto step = [&](uint8_t* slot, uint8_t* next, int g, int xs_at, float wg, float wu) __attribute__((always_inline)) {
             __builtin_amdgcn_s_waitcnt(wait_vm(C::kLoads));
             group_barrier();
             compute(slot, next, g, xs_at, wg, wu);
             __builtin_amdgcn_sched_barrier(0);
-            if constexpr (S == 2) {
-                group_barrier();
-                issue(slot, g + 2);
-            }
         };
-        constexpr int kSpan = 64 * S / C::kChunk * C::kChunk;     // groups of a table of weight scales
-        float wgv[S], wuv[S];                                    // lane l: groups base + l S + t
+        constexpr int kSpan = 64 * kSlots;                       // groups of a table of weight scales
+        float wgv[kSlots], wuv[kSlots];                          // lane l: groups base + l kSlots + t
         auto load_ws = [&](int base) __attribute__((always_inline)) {
 #pragma unroll
-            for (int t = 0; t < S; ++t) {
-                const int k = group_at(base + lane * S + t);
+            for (int t = 0; t < kSlots; ++t) {
+                const int k = group_at(base + lane * kSlots + t);
                 wgv[t] = wsg[k];
                 wuv[t] = kSilu ? wsu[k] : 0.f;
             }
@@ -318,7 +314,7 @@ __global__ void __launch_bounds__(C::kThreads * C::KS, 2) block_tiles_kernel(Blo
         auto hold_ws = [&]() __attribute__((always_inline)) {
             // (waited for here: at their first use, in the loop, the wait would be every round's)
 #pragma unroll
-            for (int t = 0; t < S; ++t) asm volatile("" : "+v"(wgv[t]), "+v"(wuv[t]));
+            for (int t = 0; t < kSlots; ++t) asm volatile("" : "+v"(wgv[t]), "+v"(wuv[t]));
         };
         const int xs_lane = part * 2 * C::kChunk * BT + wt * FT * 16 + c;
         // A chunk's table is written behind the first round of the chunk before: its last readers are past
@@ -345,43 +341,30 @@ __global__ void __launch_bounds__(C::kThreads * C::KS, 2) block_tiles_kernel(Blo
                 load_ws(base);
                 hold_ws();
             }
-            int l = (g - base) / S, xa = at + xs_lane;
+            int l = (g - base) / kSlots, xa = at + xs_lane;
             auto pick = [&](float v) __attribute__((always_inline)) {
                 return __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(v), l));
             };
-            // S groups
-            auto round0 = [&]() __attribute__((always_inline)) { step(slot0, S > 2 ? slot2 : slot0, g, xa, pick(wgv[0]), pick(wuv[0])); };
+            // three groups
+            auto round0 = [&]() __attribute__((always_inline)) { step(slot0, slot2, g, xa, pick(wgv[0]), pick(wuv[0])); };
             auto round1 = [&]() __attribute__((always_inline)) { step(slot1, slot0, g, xa + BT, pick(wgv[1]), pick(wuv[1])); };
-            auto round2 = [&]() __attribute__((always_inline)) {
-                if constexpr (S > 2) step(slot2, slot1, g, xa + 2 * BT, pick(wgv[S > 2 ? 2 : 0]), pick(wuv[S > 2 ? 2 : 0]));
-            };
+            auto round2 = [&]() __attribute__((always_inline)) { step(slot2, slot1, g, xa + 2 * BT, pick(wgv[2]), pick(wuv[2])); };
             round0();
             if (++g == G1) goto summed;
             round1();
             if (++g == G1) goto summed;
-            if constexpr (S > 2) {
-                round2();
-                if (++g == G1) goto summed;
-            }
+            round2();
+            if (++g == G1) goto summed;
             store_scales(at ^ (C::kChunk * BT));
-            load_scales(g - S + 2 * C::kChunk);
+            load_scales(g - kSlots + 2 * C::kChunk);
             ++l;
-            xa += S * BT;
+            xa += kSlots * BT;
             round0();
             if (++g == G1) goto summed;
             round1();
             if (++g == G1) goto summed;
-            if constexpr (S > 2) {
-                round2();
-                if (++g == G1) goto summed;
-            } else {
-                ++l;
-                xa += S * BT;
-                round0();
-                if (++g == G1) goto summed;
-                round1();
-                if (++g == G1) goto summed;
-            }
+            round2();
+            if (++g == G1) goto summed;
         }
     summed:
         __builtin_amdgcn_s_waitcnt(wait_vm(0));                  // (the loads past the last group)
@@ -527,15 +510,15 @@ int tiles_go(const BlockParams& p, hipStream_t s) {
     return check_launch("block_tiles_kernel");
 }
 
-using Tile64x32K4 = TileCfg<2, 2, 2, 1, 3, 4>;  // sixteen waves, one work-group a CU
-using Tile64x32K2 = TileCfg<2, 2, 2, 1, 3, 2>;  // eight waves, two work-groups a CU
-using Tile64x64K2 = TileCfg<1, 4, 4, 1, 3, 2>;  // eight waves, one work-group a CU
-using Tile64x64 = TileCfg<1, 4, 4, 1, 3>;       // four, three
-using Tile64x128 = TileCfg<1, 4, 4, 2, 3>;      // four, two
-using Tile256x128 = TileCfg<4, 2, 4, 4, 3>;     // eight, one
+using Tile64x32K4 = TileCfg<2, 2, 2, 1, 4>;  // sixteen waves, one work-group a CU
+using Tile64x32K2 = TileCfg<2, 2, 2, 1, 2>;  // eight waves, two work-groups a CU
+using Tile64x64K2 = TileCfg<1, 4, 4, 1, 2>;  // eight waves, one work-group a CU
+using Tile64x64 = TileCfg<1, 4, 4, 1>;       // four, three
+using Tile64x128 = TileCfg<1, 4, 4, 2>;      // four, two
+using Tile256x128 = TileCfg<4, 2, 4, 4>;     // eight, one
 // Rows in bf16: converting them in each of the eight waves takes two thirds of the conversions (layer of 4096
 // tokens, 256 experts: first product 247 -> 231 us; 1111 tokens x 6, 64 experts, the whole layer: 150 -> 142).
-using TileSilu = TileCfg<1, 8, 4, 2, 3, 1, 2>;        // 64 x 256: eight, one
+using TileSilu = TileCfg<1, 8, 4, 2, 1, 2>;  // 64 x 256: eight, one
 
 // The dense tile of least cost. us at K = 4096 as measured (the cost of every tile is linear in K):
 //   work-groups a CU:    <= 1     2     3     4     8
