@@ -11,8 +11,8 @@
 // waves share K and add their sums in LDS, one barrier per D fragments. block_stream_kernel takes any
 // K and reads the rows again for each column fragment. Measured: 1 x 4096 x 4096 7.4 us (2.3 TB/s: one
 // work-group a CU, a load's and a join's latency), 24 tokens x 8 of 256 experts, 2048 -> 1024, 65 us (4.4 TB/s);
-// a layer's products of 32 tokens x 8, 2048 x 512: 79 us (4.4 TB/s) and 54 us (3.2 TB/s: 64 KB of weights a
-// group of four waves, behind the ids, the rows and their quantisation).
+// a layer's products of 32 tokens x 8, 2048 x 512: 79 us (4.4 TB/s) and 54 us (3.2 TB/s: 128 KB of weights a
+// wave, behind the ids, the rows and their quantisation).
 #include <algorithm>
 #include <type_traits>
 
