@@ -140,3 +140,83 @@ def layer(xq, xs, w13, s13, w2, s2, tw, ids, y_half=0.0):
         np.add.at(tol, t, dy * w)
         np.add.at(mag, t, np.abs(y) * w)
     return out, tol + mag * (ids.shape[1] + 1) * U32
+
+
+# ------------------------------------------------------------------ layers whose h is known
+# Where the first product's sums are exact in fp32 in any order (whole numbers that stay below 2^24 units),
+# h is off by its own evaluation only, and a token none of whose h lies that near to a border between two
+# e4m3 numbers has e4m3 rows that are known. What is left, the second product and the output's rounding, can
+# be held to far less than `layer` allows, where any sum may move any value by a step.
+
+def sums_are_exact(x, xs, w, ws):
+    """Whole numbers x (M, K), w (N, K) with powers of two as scales: every sum of `product`'s terms, in any
+    order, is an fp32 number."""
+    whole = lambda v: np.array_equal(v, np.rint(v))                          # noqa: E731
+    power = lambda v: bool((np.frexp(v)[0] == 0.5).all())                    # noqa: E731
+    if not (whole(x) and whole(w) and power(xs) and power(ws)):
+        return False
+    scale = xs.astype(np.float64)[:, None, :] * np.repeat(ws.astype(np.float64), BLOCK, axis=0)[None, : w.shape[0]]
+    total = np.zeros(scale.shape[:2])
+    for g in range(scale.shape[2]):
+        k = slice(g * BLOCK, (g + 1) * BLOCK)
+        total += np.abs(x[:, k]) @ np.abs(w[:, k]).T * scale[:, :, g]
+    return bool((total < 2 ** 24 * scale.min(2)).all())
+
+
+def cut_variance(x, xs, w, ws):
+    """(M, N) variance of what the fp8 matrix core cuts (see `product`) where signs are random: seven products
+    of eight lose up to 2^(E - 13), evenly spread."""
+    K, N = x.shape[1], w.shape[0]
+    up = lambda v: np.where(v != 0, np.maximum(np.abs(v), 2.0 ** -6), 0.0)   # noqa: E731
+    power = lambda v: np.where(v > 0, np.exp2(np.frexp(v)[1] - 1.0), 0.0).astype(np.float32)   # noqa: E731
+    a, b = power(up(x)), power(up(w))
+    scale = xs.astype(np.float64)[:, None, :] * np.repeat(ws.astype(np.float64), BLOCK, axis=0)[None, :N]
+    out = np.zeros((x.shape[0], N))
+    for k in range(0, K, 8):
+        top = np.zeros(out.shape, np.float32)
+        for j in range(k, min(k + 8, K)):
+            np.maximum(top, np.multiply.outer(a[:, j], b[:, j]), out=top)
+        out += 7 / 3 * (top * scale[:, :, k // BLOCK] * 2.0 ** -13) ** 2
+    return out
+
+
+def known_rows(xq, xs, w13, s13, inter):
+    """As `gated_rows` for exact sums: (e4m3 values, fp32 scales, the scales' relative errors, rows some of
+    whose values the evaluation of h may move)."""
+    gu = (xq * spread(xs.astype(np.float64), xq.shape[1])) @ (
+        w13 * spread(np.repeat(s13.astype(np.float64), BLOCK, axis=0), xq.shape[1])).T
+    g, h = gu[:, :inter], silu_mul(gu[:, :inter], gu[:, inter:])
+    dh = np.abs(h) * (2 * np.abs(g) + 8) * U32
+    q, s = quantise(h)
+    rel = dh.reshape(len(h), -1, BLOCK).max(-1) / E4M3_MAX / s + 2 * U32
+    each = spread(s.astype(np.float64), inter)
+    du = dh / each + np.abs(h / each) * (spread(rel, inter) + 3 * U32)
+    moved = (round_e4m3(h / each + du) != q) | (round_e4m3(h / each - du) != q)
+    return q, s, rel, moved.any(1)
+
+
+def known_layer(xq, xs, w13, s13, w2, s2, tw, ids, row_half=0.0):
+    """The gated layer: (values, how far they may be off before they are rounded to the output's type, the
+    variance of what the fp8 matrix core cuts and of slots' rows rounded by row_half (half a step, relative)
+    in between, which tokens this holds for). The first product's sums are exact (`sums_are_exact`)."""
+    T, H = xq.shape
+    out, tol, var = np.zeros((T, H)), np.zeros((T, H)), np.zeros((T, H))
+    mag, clear = np.zeros((T, H)), np.ones(T, bool)
+    for e in np.unique(ids):
+        if not 0 <= e < w13.shape[0]:
+            continue
+        t, j = np.nonzero(ids == e)
+        q, s, rel, moved = known_rows(xq[t], xs[t], w13[e], s13[e], w13.shape[1] // 2)
+        clear[t[moved]] = False
+        y, dy = product(q, s, w2[e], s2[e])
+        b = np.abs(w2[e]) * spread(np.repeat(s2[e].astype(np.float64), BLOCK, axis=0)[:H], w2.shape[2])
+        dy = dy * 1.001 + (np.abs(q) * spread(s * rel, q.shape[1])) @ b.T
+        # (a slot's row keeps its relative step down to 2^-29 of the largest of 32 columns, then an absolute one)
+        top = np.abs(y).reshape(len(t), -1, 32).max(-1).repeat(32, axis=1)
+        dy += row_half * (np.abs(y) * 1.001 + top * 2.0 ** -27)
+        w = tw[t, j].astype(np.float64)[:, None]
+        np.add.at(out, t, y * w)
+        np.add.at(tol, t, dy * np.abs(w))
+        np.add.at(mag, t, np.abs(y * w))
+        np.add.at(var, t, (cut_variance(q, s, w2[e], s2[e]) + (row_half * y) ** 2 / 3) * w * w)
+    return out, tol + mag * (ids.shape[1] + 1) * U32, var, clear

@@ -1,0 +1,73 @@
+"""The gated fp8 layer's accuracy on the GPU, held to what its design says (fp8_layer_check.py): rows that are
+streamed and rows in tiles, from 16-bit rows and from e4m3 rows with their scales, in both output types."""
+import numpy as np
+import pytest
+import torch
+
+import fp8_layer_check as C
+import w4a8_fp8_wmma as W
+from oracle import fp8_block as O
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+FP8 = torch.float8_e4m3fn
+
+
+def dev8(v):
+    return torch.from_numpy(np.asarray(v, np.float32)).to(DEV).to(FP8)
+
+
+def dev(v):
+    return torch.from_numpy(np.ascontiguousarray(v)).to(DEV)
+
+
+def args_of(case):
+    x, xs, w13, s13, w2, s2, tw, ids = case
+    return dev8(w13), dev8(w2), dev(s13), dev(s2), dev(tw), dev(ids)
+
+
+def rows_of(case, dtype, e4m3):
+    return (dev8(case[0]), dev(case[1])) if e4m3 else (C.rows16(case[0], case[1], dtype).to(DEV), None)
+
+
+def check(case, dtype, e4m3, tiles):
+    for e in range(len(case[2])):
+        assert O.sums_are_exact(case[0][:8], case[1][:8], case[2][e], case[3][e])
+    x, xs = rows_of(case, dtype, e4m3)
+    out = W.moe_fp8_block_apply(x, *args_of(case), x_scales=xs, out_dtype=dtype)
+    half = C.ROW_HALF if tiles and dtype == torch.bfloat16 else 0.0
+    assert C.complaints(out.double().cpu().numpy(), dtype, O.known_layer(*case, half)) == []
+
+
+# up to 12 slots an expert are streamed; K groups: 2 and 1, 5 and 3, 40 and 1
+@pytest.mark.parametrize("e4m3", [False, True])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("T,k,E,H,I", [(24, 2, 8, 256, 128), (21, 4, 8, 640, 384), (20, 2, 4, 5120, 128)])
+def test_streamed(T, k, E, H, I, dtype, e4m3):
+    assert T * k <= 12 * E
+    check(C.exact_case(T, k, E, H, I), dtype, e4m3, False)
+
+
+@pytest.mark.parametrize("e4m3", [False, True])
+@pytest.mark.parametrize("T,k,E,H,I", [(96, 2, 4, 256, 256), (61, 4, 8, 640, 384), (70, 2, 4, 5120, 128)])
+def test_tiles_bf16(T, k, E, H, I, e4m3):
+    assert T * k > 12 * E
+    check(C.exact_case(T, k, E, H, I), torch.bfloat16, e4m3, True)
+
+
+def test_decoder_half_in_tiles():
+    """Norm with the residual, router and expert layer from the norm's e4m3 rows, more than 12 slots an expert:
+    against the oracle, element by element."""
+    from test_gpu_fp8_block import check_layer, check_norm, gen, hidden, layer_case, on
+    g = gen(78)
+    T, H, I, E, k = 90, 256, 128, 8, 2
+    x, r = hidden(g, T, H, torch.bfloat16), hidden(g, T, H, torch.bfloat16)
+    nw = (torch.randn((H,), generator=g) * 0.2 + 1).to(torch.bfloat16)
+    _, w13, s13, w2, s2, _, _ = layer_case(T, k, E, H, I, torch.bfloat16)
+    rw = torch.randn((H, E), generator=g)
+    dx, dr, dnw, dw13, ds13, dw2, ds2, drw = on(x, r, nw, w13, s13, w2, s2, rw)
+    n = W.rms_norm_quant_fp8(dx, dnw, residual=dr, return_norm=True)
+    tw, ids = W.fused_topk(None, n.norm.float() @ drw, k)
+    y = W.moe_fp8_block_apply(n.q, dw13, dw2, ds13, ds2, tw, ids, x_scales=n.scales)
+    check_norm(x, r, nw, 1e-6, False, True, n)
+    check_layer(y, x, w13, s13, w2, s2, tw.cpu(), ids.cpu(), torch.bfloat16, q=(n.q, n.scales))
