@@ -29,7 +29,7 @@ enum class Dst : int {
     kF16 = 0,       // out[row, n] rounded to fp16, or to bf16 (the kernels have one form for both)
     kBf16 = 1,
     kSiluF32 = 2,   // out[row, n] = silu(gate) * up in fp32, N = [gate | up] halves
-    kSlotF32 = 3,   // out[slot, n] in fp32
+    kSlotF32 = 3,   // out[slot, n] in fp32 (the layer's second product)
     kSiluFp8 = 4,   // silu(gate) * up quantised: e4m3 rows (out) and their scales (out_scales)
     kRowF16 = 5,    // out[row, n] in fp16 with a power of two per row and 32 columns (out_scales), so that
                     // no value overflows and none loses bits to a fixed range
@@ -163,8 +163,8 @@ int launch_block_stream(const BlockArgs& a, hipStream_t s);
 bool block_tiles_supported(const BlockArgs& a);
 int launch_block_tiles(const BlockArgs& a, hipStream_t s);
 // out[t, n] = sum over the slots j in order of tw[t, j] * y[slot_to_row[t, j], n] in fp32, rounded to
-// 16 bits; y as kRowF16 leaves it, rows < 0 contribute nothing. N % 32 == 0.
+// bf16; y as kRowF16 leaves it, rows < 0 contribute nothing. N % 32 == 0.
 int launch_block_reduce(const void* y, const float* ys, const int32_t* slot_to_row, const float* tw, int64_t T, int64_t N,
-                        int64_t top_k, void* out, bool bf16, hipStream_t s);
+                        int64_t top_k, void* out, hipStream_t s);
 
 }  // namespace w4a8

@@ -50,9 +50,11 @@ Dst dst_of(int dt) { return dt == W4A8_DTYPE_BF16 ? Dst::kBf16 : Dst::kF16; }
 
 // ---- the gated layer ----
 // Few rows an expert: blocks of 16 rows on the streaming kernels (rows quantised in registers, h and
-// the slots' rows in fp32). Else tiles: rows quantised beforehand, as bf16 numbers, h by gemm1, the slots' rows in fp16
-// with scales (in the output's type they would add as much error as its own rounding: 1.5 times the
-// layer's in all), blocks of the 64 rows that a tile's wave takes.
+// the slots' rows in fp32). Else tiles: rows quantised beforehand, as bf16 numbers, h by gemm1, blocks of the 64
+// rows that a tile's wave takes. The slots' rows are rounded before the sum only where that is lost in the output's
+// own rounding: for bf16 output they are fp16 with scales (an eighth of its step: layer error 1.66e-3 -> 1.67e-3), for
+// fp16 output fp32 (fp16 there adds as much error as the output's rounding does: 2.1e-4 -> 2.9e-4), which a layer of
+// 4096 tokens x 8 (256 experts, 2048 x 512) pays with 466 us for 424.
 struct LayerPlan {
     bool tiles;
     int64_t block_m, P, nblk;
@@ -84,9 +86,10 @@ struct LayerScratch {
     float *xs, *hs, *h, *y32, *ys;
     uint16_t* y16;
 };
+// bf16: of the output
 template <typename WS>
 void carve_layer(WS& w, const LayerPlan& pl, int64_t T, int64_t H, int64_t inter, int64_t E, int64_t top_k,
-                 bool quantise, LayerScratch& m) {
+                 bool quantise, bool bf16, LayerScratch& m) {
     m = LayerScratch{};
     m.sti = w.template take<int32_t>((size_t)pl.P);
     m.eid = w.template take<int32_t>((size_t)pl.nblk);
@@ -98,11 +101,15 @@ void carve_layer(WS& w, const LayerPlan& pl, int64_t T, int64_t H, int64_t inter
         m.y32 = w.template take<float>((size_t)(T * top_k * H));
         return;
     }
-    m.s2r = w.template take<int32_t>((size_t)(T * top_k));
     m.xq = w.template take<uint16_t>((size_t)(T * H));
     m.xs = w.template take<float>(quantise ? (size_t)(T * blk_groups(H)) : 0);
     m.hq = w.template take<uint8_t>((size_t)(pl.P * inter));
     m.hs = w.template take<float>((size_t)(pl.P * blk_groups(inter)));
+    if (!bf16) {
+        m.y32 = w.template take<float>((size_t)(T * top_k * H));
+        return;
+    }
+    m.s2r = w.template take<int32_t>((size_t)(T * top_k));
     m.y16 = w.template take<uint16_t>((size_t)(pl.P * H));
     m.ys = w.template take<float>((size_t)(pl.P * (H / 32)));
 }
@@ -111,6 +118,17 @@ struct SizeProbe {
     template <typename T>
     T* take(size_t n) { s.take<T>(n); return nullptr; }
 };
+// Bytes for either output type (the size that callers ask for does not name it).
+size_t layer_bytes(const LayerPlan& pl, int64_t T, int64_t H, int64_t inter, int64_t E, int64_t top_k, bool quantise) {
+    size_t most = 0;
+    for (const bool bf16 : {false, true}) {
+        SizeProbe p;
+        LayerScratch m;
+        carve_layer(p, pl, T, H, inter, E, top_k, quantise, bf16, m);
+        most = std::max(most, p.s.used);
+    }
+    return most;
+}
 
 }  // namespace
 }  // namespace w4a8
@@ -218,10 +236,7 @@ int w4a8_moe_fp8_block_gemm(const void* x, const float* x_scales, int64_t x_rows
 
 size_t w4a8_moe_fp8_block_workspace_size(int64_t T, int64_t H, int64_t inter, int64_t E, int64_t top_k) {
     if (T <= 0 || H <= 0 || inter <= 0 || E <= 0 || top_k <= 0) return 0;
-    SizeProbe p;
-    LayerScratch m;
-    carve_layer(p, plan_layer(T, H, inter, E, top_k), T, H, inter, E, top_k, true, m);
-    return p.s.used;
+    return layer_bytes(plan_layer(T, H, inter, E, top_k), T, H, inter, E, top_k, true);
 }
 
 int w4a8_moe_fp8_block_apply(const void* x, int x_dtype, const float* x_scales, int64_t T, int64_t H, int64_t inter,
@@ -245,16 +260,15 @@ int w4a8_moe_fp8_block_apply(const void* x, int x_dtype, const float* x_scales, 
     W4A8_REQUIRE(aligned16(w2) && aligned16(out), "moe_fp8_block_apply: w2 and out must be aligned to 16 bytes");
     const LayerPlan pl = plan_layer(T, H, inter, E, top_k);
     W4A8_REQUIRE(pl.P <= kMaxRows, "moe_fp8_block_apply: too many slots");
-    const bool quantise = x_dtype != W4A8_DTYPE_E4M3;
+    const bool quantise = x_dtype != W4A8_DTYPE_E4M3, bf16 = out_dtype == W4A8_DTYPE_BF16;
     Workspace w(workspace, workspace_bytes);
     LayerScratch m;
-    carve_layer(w, pl, T, H, inter, E, top_k, quantise, m);
-    if (workspace == nullptr || !w.ok()) {
+    carve_layer(w, pl, T, H, inter, E, top_k, quantise, bf16, m);
+    if (workspace == nullptr || !w.ok() || workspace_bytes < layer_bytes(pl, T, H, inter, E, top_k, quantise)) {
         set_error("moe_fp8_block_apply: workspace smaller than w4a8_moe_fp8_block_workspace_size()");
         return W4A8_ERR_WORKSPACE;
     }
     hipStream_t s = as_stream(stream);
-    const bool bf16 = out_dtype == W4A8_DTYPE_BF16;
     if (int rc = launch_align(topk_ids, T * top_k, E, pl.block_m, expert_map, n_global, m.sti, pl.P, m.eid, m.ntp,
                               m.align_ws, m.align_bytes, s, m.s2r))
         return rc;
@@ -275,16 +289,18 @@ int w4a8_moe_fp8_block_apply(const void* x, int x_dtype, const float* x_scales, 
     BlockArgs g2 = g1;
     g2.x = pl.tiles ? (const void*)m.hq : (const void*)m.h; g2.xs = m.hs; g2.x_rows = pl.P; g2.K = inter; g2.ldx = inter;
     g2.w = w2; g2.ws = w2_scales; g2.N = H; g2.gather = false;
+    const bool row16 = pl.tiles && bf16;
     g2.src = pl.tiles ? Src::kFp8 : Src::kF32;
-    g2.dst = pl.tiles ? Dst::kRowF16 : Dst::kSlotF32;
-    g2.out = pl.tiles ? (void*)m.y16 : (void*)m.y32; g2.out_scales = m.ys; g2.ldo = H;
+    g2.dst = row16 ? Dst::kRowF16 : Dst::kSlotF32;
+    g2.out = row16 ? (void*)m.y16 : (void*)m.y32; g2.out_scales = m.ys; g2.ldo = H; g2.all_rows = row16;
     if (pl.tiles) {
         if (int rc = launch_block_tiles(g1, s)) return rc;
         if (int rc = launch_block_tiles(g2, s)) return rc;
-        return launch_block_reduce(m.y16, m.ys, m.s2r, topk_weights, T, H, top_k, out, bf16, s);
+        if (row16) return launch_block_reduce(m.y16, m.ys, m.s2r, topk_weights, T, H, top_k, out, s);
+    } else {
+        if (int rc = launch_block_stream(g1, s)) return rc;
+        if (int rc = launch_block_stream(g2, s)) return rc;
     }
-    if (int rc = launch_block_stream(g1, s)) return rc;
-    if (int rc = launch_block_stream(g2, s)) return rc;
     for (int64_t t = 0; t < T; t += kReduceRows)
         if (int rc = launch_slot_reduce(m.y32 + t * top_k * H, topk_weights + t * top_k, topk_ids + t * top_k, expert_map,
                                         n_global, E, std::min(kReduceRows, T - t), H, top_k,

@@ -307,7 +307,6 @@ __global__ void __launch_bounds__(256) act_quant_groups_any_kernel(const void* _
 
 // Eight columns a lane; a token's rows are requested together, eight at a time (4096 tokens x 8 rows of 2048:
 // 26 us, 5.8 TB/s).
-template <bool BF16>
 __global__ void __launch_bounds__(256) block_reduce_kernel(const void* __restrict__ y, const float* __restrict__ ys,
                                                            const int32_t* __restrict__ s2r,
                                                            const float* __restrict__ tw, int N, int top_k,
@@ -342,7 +341,7 @@ __global__ void __launch_bounds__(256) block_reduce_kernel(const void* __restric
             for (int i = 0; i < 8; ++i) acc[i] = fmaf(w[j], f[i], acc[i]);
         }
     }
-    *reinterpret_cast<u32x4*>(reinterpret_cast<uint16_t*>(out) + t * N + n) = pack8<BF16>(acc);
+    *reinterpret_cast<u32x4*>(reinterpret_cast<uint16_t*>(out) + t * N + n) = pack8<true>(acc);
 }
 
 template <int W, int NV, bool BF16, bool RES, bool KEEP, bool WF32>
@@ -399,15 +398,14 @@ int launch_rms_norm_quant(const NormArgs& a, hipStream_t s) {
 }
 
 int launch_block_reduce(const void* y, const float* ys, const int32_t* slot_to_row, const float* tw, int64_t T, int64_t N,
-                        int64_t top_k, void* out, bool bf16, hipStream_t s) {
+                        int64_t top_k, void* out, hipStream_t s) {
     if (T == 0) return W4A8_OK;
     if (!grid_fits(T, 256)) {
         set_error("block_reduce: too many rows");
         return W4A8_ERR_INVALID;
     }
     const dim3 grid((unsigned)T, (unsigned)((N / 8 + 255) / 256));
-    if (bf16) block_reduce_kernel<true><<<grid, 256, 0, s>>>(y, ys, slot_to_row, tw, (int)N, (int)top_k, out);
-    else block_reduce_kernel<false><<<grid, 256, 0, s>>>(y, ys, slot_to_row, tw, (int)N, (int)top_k, out);
+    block_reduce_kernel<<<grid, 256, 0, s>>>(y, ys, slot_to_row, tw, (int)N, (int)top_k, out);
     return check_launch("block_reduce_kernel");
 }
 

@@ -461,6 +461,16 @@ __global__ void __launch_bounds__(C::kThreads * C::KS, 2) block_tiles_kernel(Blo
                     if (q == 0) p.out_scales[(int64_t)row * (N / 32) + col / 32] = __uint_as_float(sb << 23);
                 }
             }
+        } else if constexpr (DST == Dst::kSlotF32) {
+#pragma unroll
+            for (int i = 0; i < FT; ++i) {
+                int row;
+                if (!live(i, row)) continue;                     // (padding has no slot)
+                const int slot = p.sorted_ids[row];
+#pragma unroll
+                for (int j = 0; j < FN; ++j)                     // (whole tiles: N % 128 == 0)
+                    store4<DST>(p, slot, col_of(at_ct, (wn * FN + j) * 16 + 4 * q), N, run[i][j]);
+            }
         } else {
 #pragma unroll
             for (int i = 0; i < FT; ++i) {
@@ -553,7 +563,7 @@ bool block_tiles_supported(const BlockArgs& a) {
     const bool silu = a.dst == Dst::kSiluFp8;
     return a.src == (silu ? Src::kWide : Src::kFp8) && a.x_rows * a.ldx * (silu ? 2 : 1) < lim && a.x_rows * blk_groups(a.K) * 4 < lim && a.N * a.K < lim &&
            (a.dst == Dst::kF16 || a.dst == Dst::kBf16 ||
-            (a.dst == Dst::kRowF16 && a.sorted_ids != nullptr && a.K % kBlk == 0 && a.N % kBlk == 0) ||
+            ((a.dst == Dst::kRowF16 || (a.dst == Dst::kSlotF32 && !a.all_rows)) && a.sorted_ids != nullptr && a.K % kBlk == 0 && a.N % kBlk == 0) ||
             (silu && a.sorted_ids != nullptr && a.K % kBlk == 0 && a.N % (2 * kBlk) == 0));
 }
 
@@ -566,6 +576,7 @@ int launch_block_tiles(const BlockArgs& a, hipStream_t s) {
     }
     if (a.dst == Dst::kSiluFp8) return tiles_go<TileSilu, Dst::kSiluFp8, true>(p, s);
     if (a.dst == Dst::kRowF16) return tiles_go<Tile64x128, Dst::kRowF16, true>(p, s);
+    if (a.dst == Dst::kSlotF32) return tiles_go<Tile64x128, Dst::kSlotF32, true>(p, s);
     if (a.sorted_ids != nullptr) return tiles_go<Tile64x128, Dst::kF16, true>(p, s);
     return dense_go(p, s);
 }

@@ -55,6 +55,30 @@ def test_tiles_bf16(T, k, E, H, I, e4m3):
     check(C.exact_case(T, k, E, H, I), torch.bfloat16, e4m3, True)
 
 
+@pytest.mark.parametrize("e4m3", [False, True])
+@pytest.mark.parametrize("T,k,E,H,I", [(96, 2, 4, 256, 256), (61, 4, 8, 640, 384), (70, 2, 4, 5120, 128)])
+def test_tiles_fp16(T, k, E, H, I, e4m3):
+    """Slots' rows in fp32: in fp16 they would add as much error as the output's own rounding."""
+    assert T * k > 12 * E
+    check(C.exact_case(T, k, E, H, I), torch.float16, e4m3, True)
+
+
+@pytest.mark.parametrize("T", [3, 80])
+def test_expert_map_fp16(T):
+    """Slots of experts that live elsewhere have no rows: what their place in the workspace holds does not count."""
+    case = C.exact_case(T, 3, 12, 256, 128)
+    x, xs, w13, s13, w2, s2, tw, ids = case
+    emap = np.full(12, -1, np.int32)
+    emap[[1, 4, 5, 9]] = [2, 0, 3, 1]
+    local = emap[ids]
+    small = (x, xs, w13[:4], s13[:4], w2[:4], s2[:4], tw, local)
+    if T * 3 > 48:
+        torch.full((1 << 24,), float("nan"), device=DEV)            # (freed: the workspace's memory)
+    out = W.moe_fp8_block_apply(rows_of(case, torch.float16, False)[0], *args_of(small)[:4], dev(tw), dev(ids),
+                                expert_map=dev(emap))
+    assert C.complaints(out.double().cpu().numpy(), torch.float16, O.known_layer(*small)) == []
+
+
 def test_decoder_half_in_tiles():
     """Norm with the residual, router and expert layer from the norm's e4m3 rows, more than 12 slots an expert:
     against the oracle, element by element."""
