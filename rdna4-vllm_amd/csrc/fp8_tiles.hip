@@ -438,16 +438,19 @@ __global__ void __launch_bounds__(C::kThreads * C::KS, 2) block_tiles_kernel(Blo
                 if (wn == 0 && q == 0) p.out_scales[(int64_t)row * (half / kBlk) + at_ct] = sc;
             }
         } else if constexpr (DST == Dst::kRowF16) {
-            // a row's largest value of this wave's columns to [2^14, 2^15): infinities, NaN and zeros as they are
+            // a row's largest finite value of this wave's columns to [2^14, 2^15): infinities, NaN and zeros as they are
 #pragma unroll
             for (int i = 0; i < FT; ++i) {
                 float m = 0.f;
 #pragma unroll
                 for (int j = 0; j < FN; ++j)
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) m = fmaxf(m, fabsf(run[i][j][r]));
+                    for (int r = 0; r < 4; ++r) {
+                        const float v = fabsf(run[i][j][r]);
+                        m = fmaxf(m, v < INFINITY ? v : 0.f);
+                    }
                 const uint32_t eb = __float_as_uint(rows4_max(m)) >> 23;
-                const uint32_t sb = eb == 0 || eb == 255 ? 127u : eb > 15 ? eb - 14 : 1u;
+                const uint32_t sb = eb == 0 ? 127u : eb > 15 ? eb - 14 : 1u;
                 const float inv = __uint_as_float((254u - sb) << 23);
                 int row;
                 if (!live(i, row)) continue;

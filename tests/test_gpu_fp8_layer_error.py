@@ -95,3 +95,31 @@ def test_decoder_half_in_tiles():
     y = W.moe_fp8_block_apply(n.q, dw13, dw2, ds13, ds2, tw, ids, x_scales=n.scales)
     check_norm(x, r, nw, 1e-6, False, True, n)
     check_layer(y, x, w13, s13, w2, s2, tw.cpu(), ids.cpu(), torch.bfloat16, q=(n.q, n.scales))
+
+
+def far_case(T, power, weight):
+    """Column 5 of the second product is some 2^17 times as large as the others, column 9 is zero."""
+    x, xs, w13, s13, w2, s2, tw, ids = C.exact_case(T, 1, 4, 256, 128)
+    w2 = np.sign(w2) * 2.0 ** -9
+    w2[:, 5], w2[:, 9] = 448 * np.sign(w2[:, 5]), 0
+    s2 = np.exp2(np.full(s2.shape, power)).astype(np.float32)
+    tw = np.exp2(np.full(tw.shape, weight)).astype(np.float32)
+    return x, xs, w13, s13, w2, s2, tw, ids
+
+
+def check_far(T, power, weight):
+    case = far_case(T, power, weight)
+    out = W.moe_fp8_block_apply(rows_of(case, torch.bfloat16, False)[0], *args_of(case)).double().cpu().numpy()
+    ref, tol, _, clear = O.known_layer(*case, C.ROW_HALF)
+    tol = tol + (np.abs(ref) + tol) * C.HALF[torch.bfloat16]
+    over, inside = (np.abs(ref) > 4e38) & clear[:, None], (np.abs(ref) < 3e38) & clear[:, None]
+    assert np.array_equal(out[over], np.sign(ref[over]) * np.inf)
+    assert (np.abs(out - ref)[inside] <= tol[inside]).all()
+    return over
+
+
+@pytest.mark.parametrize("T", [20, 96])
+def test_an_infinite_column_leaves_the_others(T):
+    """A sum past fp32's range is infinite; the columns beside it, finite in bf16, stay as they are."""
+    assert check_far(T, 118, 0)[:, 5].any()
+    check_far(T, 0, 0)
