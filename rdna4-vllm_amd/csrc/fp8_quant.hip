@@ -306,7 +306,8 @@ __global__ void __launch_bounds__(256) act_quant_groups_any_kernel(const void* _
 }
 
 // Eight columns a lane; a token's rows are requested together, eight at a time (4096 tokens x 8 rows of 2048:
-// 26 us, 5.8 TB/s).
+// 26 us, 5.8 TB/s). A value is scaled back (exactly) before its weight: their scale times the weight can
+// leave fp32's range where the product of all three does not.
 __global__ void __launch_bounds__(256) block_reduce_kernel(const void* __restrict__ y, const float* __restrict__ ys,
                                                            const int32_t* __restrict__ s2r,
                                                            const float* __restrict__ tw, int N, int top_k,
@@ -318,7 +319,7 @@ __global__ void __launch_bounds__(256) block_reduce_kernel(const void* __restric
     for (int j0 = 0; j0 < top_k; j0 += 8) {
         int32_t r[8];
         u32x4 v[8];
-        float w[8];
+        float w[8], sc[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             r[j] = j0 + j < top_k ? s2r[t * top_k + j0 + j] : -1;
@@ -327,9 +328,10 @@ __global__ void __launch_bounds__(256) block_reduce_kernel(const void* __restric
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             v[j] = u32x4{0, 0, 0, 0};
+            sc[j] = 0.f;
             if (r[j] >= 0) {
                 v[j] = *reinterpret_cast<const u32x4*>(reinterpret_cast<const uint16_t*>(y) + (int64_t)r[j] * N + n);
-                w[j] *= ys[(int64_t)r[j] * (N / 32) + n / 32];
+                sc[j] = ys[(int64_t)r[j] * (N / 32) + n / 32];
             }
         }
 #pragma unroll
@@ -338,7 +340,7 @@ __global__ void __launch_bounds__(256) block_reduce_kernel(const void* __restric
             float f[8];
             unpack8<false>(v[j], f);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) acc[i] = fmaf(w[j], f[i], acc[i]);
+            for (int i = 0; i < 8; ++i) acc[i] = fmaf(w[j], f[i] * sc[j], acc[i]);
         }
     }
     *reinterpret_cast<u32x4*>(reinterpret_cast<uint16_t*>(out) + t * N + n) = pack8<true>(acc);

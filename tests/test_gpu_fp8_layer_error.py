@@ -111,7 +111,8 @@ def check_far(T, power, weight):
     case = far_case(T, power, weight)
     out = W.moe_fp8_block_apply(rows_of(case, torch.bfloat16, False)[0], *args_of(case)).double().cpu().numpy()
     ref, tol, _, clear = O.known_layer(*case, C.ROW_HALF)
-    tol = tol + (np.abs(ref) + tol) * C.HALF[torch.bfloat16]
+    # (bf16's subnormal numbers lie 2^-126 / 2^7 = 2^-133 apart: a rounding among them is off by up to 2^-134)
+    tol = tol + (np.abs(ref) + tol) * C.HALF[torch.bfloat16] + 2.0 ** -134
     over, inside = (np.abs(ref) > 4e38) & clear[:, None], (np.abs(ref) < 3e38) & clear[:, None]
     assert np.array_equal(out[over], np.sign(ref[over]) * np.inf)
     assert (np.abs(out - ref)[inside] <= tol[inside]).all()
@@ -123,3 +124,10 @@ def test_an_infinite_column_leaves_the_others(T):
     """A sum past fp32's range is infinite; the columns beside it, finite in bf16, stay as they are."""
     assert check_far(T, 118, 0)[:, 5].any()
     check_far(T, 0, 0)
+
+
+@pytest.mark.parametrize("T", [20, 96])
+def test_weights_far_from_one(T):
+    """Sums of 2^124 in one column, a router's weight of 2^20: zeros stay zeros, small columns finite."""
+    assert check_far(T, 110, 20)[:, 5].all()
+    check_far(T, -110, -20)
