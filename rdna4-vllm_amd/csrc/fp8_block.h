@@ -117,11 +117,34 @@ __device__ __forceinline__ float rows4_max(float v) {
     return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
 
-// SiLU(g) * u in fp32: 2^(-g log2 e) and the reciprocal from the hardware (each within an ulp), so
-// about |g| * 2^-24 relative: far below the e4m3 step (2^-4) that every result is rounded to.
-__device__ __forceinline__ float silu_mul_f32(float g, float u) {
-    const float d = 1.0f + __builtin_amdgcn_exp2f(g * -1.44269504088896340736f);
-    return g * __builtin_amdgcn_rcpf(d) * u;
+// SiLU(g) * u in fp32, N of them: 2^(-g log2 e) and the reciprocal from the hardware (each within an ulp),
+// so about |g| * 2^-24 relative: far below the e4m3 step (2^-4) that every result is rounded to.
+// FAR: u may be as large as fp32 numbers are. The reciprocal of 1 + e^-g is no normal number below -87.3 (the
+// hardware gives 0), which a u of 1e30 shows; below -80 SiLU(g) = g e^g to 35 digits, as two factors e^(g / 2) of
+// which u takes one. Asked for all N at once: with a choice for each value silu(gate) * up of 4111 x 12288
+// bf16 takes 44.3 us for 42.8, and a layer of 4096 tokens 427 for 421. An fp16 u needs none (65504 e^-87 rounds to 0).
+template <bool FAR, int N>
+__device__ __forceinline__ void silu_mul_f32(const float (&g)[N], const float (&u)[N], float (&h)[N]) {
+    float least = 0.f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        h[i] = g[i] * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(g[i] * -1.44269504088896340736f)) * u[i];
+        least = fminf(least, g[i]);
+    }
+    if constexpr (FAR)
+        if (least < -80.f) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const float t = __builtin_amdgcn_exp2f(g[i] * 0.72134752044448170368f);
+                if (g[i] < -80.f) h[i] = (g[i] * t) * (t * u[i]);
+            }
+        }
+}
+__device__ __forceinline__ v4f silu_mul_f32(const v4f& g, const v4f& u) {
+    const float a[4] = {g[0], g[1], g[2], g[3]}, b[4] = {u[0], u[1], u[2], u[3]};
+    float h[4];
+    silu_mul_f32<true>(a, b, h);
+    return v4f{h[0], h[1], h[2], h[3]};
 }
 
 __device__ __forceinline__ uint32_t pack_out16(float a, float b, bool bf16) {

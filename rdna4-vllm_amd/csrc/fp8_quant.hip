@@ -253,11 +253,10 @@ __global__ void __launch_bounds__(256) act_quant_groups_kernel(const void* __res
         const u32x4 a = *reinterpret_cast<const u32x4*>(xr);
         if constexpr (SILU) {
             const u32x4 b = *reinterpret_cast<const u32x4*>(xr + K);
-            float u[8];
-            unpack8<BF16>(a, f);
+            float g[8], u[8];
+            unpack8<BF16>(a, g);
             unpack8<BF16>(b, u);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) f[j] = silu_mul_f32(f[j], u[j]);
+            silu_mul_f32<BF16>(g, u, f);
         } else {
             unpack8<BF16>(a, f);
         }
@@ -292,7 +291,12 @@ __global__ void __launch_bounds__(256) act_quant_groups_any_kernel(const void* _
         v[h] = 0.f;
         if (k < K) {
             v[h] = load16<BF16>(x, row * ldx + k);
-            if constexpr (SILU) v[h] = silu_mul_f32(v[h], load16<BF16>(x, row * ldx + K + k));
+            if constexpr (SILU) {
+                const float g[1] = {v[h]}, u[1] = {load16<BF16>(x, row * ldx + K + k)};
+                float o[1];
+                silu_mul_f32<BF16>(g, u, o);
+                v[h] = o[0];
+            }
         }
     }
     const float s = act_scale_from_absmax(wave_max(fmaxf(fabsf(v[0]), fabsf(v[1]))));

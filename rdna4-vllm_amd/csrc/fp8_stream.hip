@@ -200,10 +200,7 @@ __global__ void __launch_bounds__(64 * KS * CG) block_rows_kernel(BlockParams p,
         auto put = [&](int u, v4f t, const v4f& up) __attribute__((always_inline)) {
             const int of = it * kUnits + u;
             const int col = (f0 + of) * 16 + 4 * q;
-            if constexpr (kSilu) {
-#pragma unroll
-                for (int r = 0; r < 4; ++r) t[r] = silu_mul_f32(t[r], up[r]);
-            }
+            if constexpr (kSilu) t = silu_mul_f32(t, up);
             if (of >= mine || slot < 0 || col >= cols) return;
             store4<DST>(p, DST == Dst::kSlotF32 ? slot : row0 + c, col, cols, t);
         };
@@ -324,11 +321,7 @@ __global__ void __launch_bounds__(64 * KS) block_stream_kernel(BlockParams p, in
         return t;
     };
     v4f t = total(wave);
-    if constexpr (kSilu) {
-        const v4f up = total(kCols + wave);
-#pragma unroll
-        for (int r = 0; r < 4; ++r) t[r] = silu_mul_f32(t[r], up[r]);
-    }
+    if constexpr (kSilu) t = silu_mul_f32(t, total(kCols + wave));
     const int col = (sl * kCols + wave) * 16 + 4 * q;
     if (slot >= 0 && col < cols) store4<DST>(p, DST == Dst::kSlotF32 ? slot : row0 + c, col, cols, t);
 }

@@ -410,12 +410,11 @@ __global__ void __launch_bounds__(C::kThreads * C::KS, 2) block_tiles_kernel(Blo
             for (int i = 0; i < FT; ++i) {
                 float m = 0.f;
 #pragma unroll
-                for (int j = 0; j < FN / 2; ++j)
+                for (int j = 0; j < FN / 2; ++j) {
+                    run[i][j] = silu_mul_f32(run[i][j], run[i][j + FN / 2]);
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        run[i][j][r] = silu_mul_f32(run[i][j][r], run[i][j + FN / 2][r]);
-                        m = fmaxf(m, fabsf(run[i][j][r]));
-                    }
+                    for (int r = 0; r < 4; ++r) m = fmaxf(m, fabsf(run[i][j][r]));
+                }
                 top[i] = rows4_max(m);
             }
 #pragma unroll
