@@ -392,7 +392,8 @@ W4A8_API int w4a8_moe_fp8_block_gemm(const void* x, const float* x_scales, int64
  * SiLU * mul and quantisation of h (fp32 in between), gemm2, reduce over the slots in order with
  * topk_weights. x (T, H) contiguous -> out (T, H). w13 (E, 2 inter, H) = [gate | up], w2
  * (E, H, inter); H and inter multiples of 128. topk_ids, expert_map and num_global_experts as in
- * w4a8_moe_apply. */
+ * w4a8_moe_apply. The workspace's size is that of the larger of both output types and is asked for
+ * with either. */
 W4A8_API size_t w4a8_moe_fp8_block_workspace_size(int64_t T, int64_t H, int64_t inter, int64_t E,
                                                   int64_t top_k);
 W4A8_API int w4a8_moe_fp8_block_apply(const void* x, int x_dtype, const float* x_scales,

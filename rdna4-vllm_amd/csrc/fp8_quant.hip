@@ -237,7 +237,7 @@ __device__ __forceinline__ u32x4 widen8(uint2 v) {
     return o.u;
 }
 
-// Eight values a lane: sixteen lanes a group of 128, K8 = lanes that a row takes (ceil(K / 128) * 16).
+// Eight values a lane, sixteen lanes a group of 128, so G * 16 lanes a row.
 // WIDE: the e4m3 values as bf16 numbers.
 template <bool BF16, bool SILU, bool WIDE>
 __global__ void __launch_bounds__(256) act_quant_groups_kernel(const void* __restrict__ x, int64_t rows, int K, int G,

@@ -532,7 +532,8 @@ using Tile256x128 = TileCfg<4, 2, 4, 4>;     // eight, one
 // tokens, 256 experts: first product 247 -> 231 us; 1111 tokens x 6, 64 experts, the whole layer: 150 -> 142).
 using TileSilu = TileCfg<1, 8, 4, 2, 1, 2>;  // 64 x 256: eight, one
 
-// The dense tile of least cost. us at K = 4096 as measured (the cost of every tile is linear in K):
+// The dense tile of least cost. us as measured at K = 4096 (the rule compares tiles at one K, as if all their
+// costs grew with it alike; other K were timed for the chosen tiles only):
 //   work-groups a CU:    <= 1     2     3     4     8
 //   64 x 64, K in two     12    24
 //   64 x 64               14    19    29    36    64
