@@ -9,7 +9,7 @@
 // block_rows_kernel holds its rows in registers (16 rows by GPW groups a wave, quantised there
 // where they come in 16 or 32 bits) and walks over column fragments with D of them in flight; KS
 // waves share K and add their sums in LDS, one barrier per D fragments. block_stream_kernel takes any
-// K and reads the rows again for each column fragment. Measured: 1 x 4096 x 4096 7.4 us (2.3 TB/s: one
+// K and reads the rows again for each column fragment. Measured: 1 x 4096 x 4096 8.0 us (2.1 TB/s: one
 // work-group a CU, a load's and a join's latency), 24 tokens x 8 of 256 experts, 2048 -> 1024, 65 us (4.4 TB/s);
 // a layer's products of 32 tokens x 8, 2048 x 512: 79 us (4.4 TB/s) and 54 us (3.2 TB/s: 128 KB of weights a
 // wave, behind the ids, the rows and their quantisation).
