@@ -4,8 +4,9 @@
 // scale per 128 x 128 block (n / 128, k / 128):
 //   out[m, n] = sum_g xs[m, g] * ws[n / 128, g] * sum_{k in group g} x[m, k] w[n, k].
 // The inner sum is one fp8 MFMA of 128 k with a zero accumulator (fp32), in the layer's first product four
-// chained bf16 MFMAs (fp8_mfma.h says why); the outer one is an fp32 FMA chain over g in each wave. Quantisation: s = max(absmax / 448, 1e-8), q = e4m3(x * (1 / s)) in
-// fp32, to nearest even; NaN counts for no absmax and stays NaN.
+// chained bf16 MFMAs (fp8_mfma.h says why); the outer one is an fp32 FMA chain over g in each wave.
+// Quantisation: s = max(absmax / 448, 1e-8), q = e4m3(x * (1 / s)) in fp32, to nearest even; NaN counts for
+// no absmax and stays NaN.
 #pragma once
 
 #include "grouped_params.h"

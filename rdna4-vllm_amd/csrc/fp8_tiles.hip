@@ -566,7 +566,8 @@ bool block_tiles_supported(const BlockArgs& a) {
     const bool silu = a.dst == Dst::kSiluFp8;
     return a.src == (silu ? Src::kWide : Src::kFp8) && a.x_rows * a.ldx * (silu ? 2 : 1) < lim && a.x_rows * blk_groups(a.K) * 4 < lim && a.N * a.K < lim &&
            (a.dst == Dst::kF16 || a.dst == Dst::kBf16 ||
-            ((a.dst == Dst::kRowF16 || (a.dst == Dst::kSlotF32 && !a.all_rows)) && a.sorted_ids != nullptr && a.K % kBlk == 0 && a.N % kBlk == 0) ||
+            ((a.dst == Dst::kRowF16 || (a.dst == Dst::kSlotF32 && !a.all_rows)) && a.sorted_ids != nullptr &&
+             a.K % kBlk == 0 && a.N % kBlk == 0) ||
             (silu && a.sorted_ids != nullptr && a.K % kBlk == 0 && a.N % (2 * kBlk) == 0));
 }
 
