@@ -256,9 +256,9 @@ def moe_fp8_block_gemm(x: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor,
     ``gather=False``, x[r]: the rows of an earlier grouped product) times the weights of expert
     expert_ids[r // block_m] -> (P, N) in out_dtype (bf16 by default) or in ``out``. Rows whose slot
     is not in [0, num_slots) are padding and not written (without ``out``, and from the torch op, they
-    hold anything); num_slots is the number of routed slots, tokens * top_k (default: x.shape[0] * top_k, which with ``gather=False`` counts padding rows of
-    x as slots too: pass it there to leave them as they are). w (E, N, K) e4m3; block_m a multiple
-    of 16 up to 128."""
+    hold anything); num_slots is the number of routed slots, tokens * top_k (default: x.shape[0] *
+    top_k, which with ``gather=False`` counts padding rows of x as slots too: pass it there to leave
+    them as they are). w (E, N, K) e4m3; block_m a multiple of 16 up to 128."""
     xs = _check_rows(x, x_scales)
     if xs is None:
         _fail("x must be float8_e4m3fn")
