@@ -52,6 +52,7 @@ extern "C" {
 #define W4A8_DTYPE_F16 0
 #define W4A8_DTYPE_BF16 1
 #define W4A8_DTYPE_E4M3 2   /* block-scaled fp8 operators only */
+#define W4A8_DTYPE_F32 4    /* router logits only (3: int8, w4a8_int8.h) */
 
 /* Version of this ABI (bumped on any signature change). */
 W4A8_API int w4a8_abi_version(void);
@@ -86,6 +87,19 @@ W4A8_API int w4a8_dequant_fp8(const int32_t* w_packed, const int32_t* w_zeros, i
  */
 W4A8_API int w4a8_topk_softmax(const float* logits, int64_t T, int64_t E, int64_t top_k,
                       int renormalize, float* topk_weights, int32_t* topk_ids, void* stream);
+
+/* Choice of experts with softmax (scoring 0) or sigmoid (1) scores p, a bias for balance and groups of experts. c = p +
+ * bias; the E experts are num_groups equal runs, a group's score is the sum of its two largest c with a bias and its
+ * largest c without, the top_groups best groups stay, and of those the top_k largest c are picked, in descending order,
+ * ties to the lower expert (and group), as the true numbers compare. Weights: p of the picks, divided by their sum with
+ * renormalize, times scale. logits (T, E) fp32, fp16 or bf16, rows logits_stride elements apart; bias (E,) or NULL.
+ * A logit of -inf or NaN (and a bias of -inf or NaN) masks its expert: never picked; picks that find no expert are -1
+ * with weight 0. +inf counts as the largest finite number. E <= 1024; top_k and num_groups <= 64. No reference
+ * counterpart. */
+W4A8_API int w4a8_route_topk(const void* logits, int dtype, int64_t T, int64_t E, int64_t logits_stride,
+                             int64_t top_k, int scoring, const float* bias, int64_t num_groups,
+                             int64_t top_groups, int renormalize, float scale, float* topk_weights,
+                             int32_t* topk_ids, void* stream);
 
 /* ---------------------------------------------------------------------------------
  * moe_align_block_size (vLLM op called at moe_experts.py:587-589, contract mirrored

@@ -1,8 +1,9 @@
-"""Build the gfx950 C-ABI library ``w4a8_fp8_wmma/libw4a8moe.so`` in-tree.
+"""Build the gfx950 C-ABI libraries in-tree: ``w4a8_fp8_wmma/libw4a8moe.so`` and ``libw4a8int8.so``.
 
-Every ``csrc/*.hip`` file is compiled with hipcc for gfx950 only, then linked into one
-shared library whose exported symbols are exactly the ``extern "C"`` entry points of
-``include/w4a8_moe.h``. Usage: ``python rdna4-vllm_amd/build.py [-j N]``.
+Every ``csrc/*.hip`` file is compiled with hipcc for gfx950 only. The files ``int8_*.hip`` (the operators
+of the integer matrix cores) and the ``SHARED`` ones make the second library, the others the first. The
+exported symbols of each are exactly the ``extern "C"`` entry points of its header
+(``include/w4a8_moe.h``, ``include/w4a8_int8.h``). Usage: ``python rdna4-vllm_amd/build.py [-j N]``.
 """
 from __future__ import annotations
 
@@ -18,6 +19,9 @@ HERE = Path(__file__).resolve().parent
 CSRC = HERE / "csrc"
 OUT_DIR = HERE / "w4a8_fp8_wmma"
 LIB_NAME = "libw4a8moe.so"
+INT8_LIB_NAME = "libw4a8int8.so"
+# in both libraries: errors and launch facts, and the slots' alignment
+SHARED = ("host.hip", "routing.hip")
 BUILD_DIR = HERE / "_build"
 ARCH = "gfx950"
 
@@ -64,12 +68,17 @@ def _compile(src: Path, obj: Path) -> None:
 def build(jobs: int | None = None, verbose: bool = True) -> Path:
     BUILD_DIR.mkdir(exist_ok=True)
     srcs = sorted(CSRC.glob("*.hip"))
-    objs = [BUILD_DIR / (s.stem + ".o") for s in srcs]
+    objs = {src.name: BUILD_DIR / (src.stem + ".o") for src in srcs}
     jobs = jobs or min(8, os.cpu_count() or 1, len(srcs))
     with cf.ThreadPoolExecutor(max_workers=jobs) as ex:
-        list(ex.map(lambda so: _compile(*so), zip(srcs, objs)))
-    lib = OUT_DIR / LIB_NAME
-    tmp = OUT_DIR / (LIB_NAME + ".tmp")
+        list(ex.map(lambda src: _compile(src, objs[src.name]), srcs))
+    int8 = [o for n, o in objs.items() if n.startswith("int8_") or n in SHARED]
+    _link(OUT_DIR / INT8_LIB_NAME, int8, verbose)
+    return _link(OUT_DIR / LIB_NAME, [o for n, o in objs.items() if not n.startswith("int8_")], verbose)
+
+
+def _link(lib: Path, objs: list[Path], verbose: bool) -> Path:
+    tmp = lib.with_name(lib.name + ".tmp")
     cmd = [hipcc(), f"--offload-arch={ARCH}", "-shared", "-fPIC", "-o", str(tmp), *map(str, objs)]
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:

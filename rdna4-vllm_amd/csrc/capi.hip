@@ -14,8 +14,6 @@
 namespace w4a8 {
 
 namespace {
-thread_local std::string g_error;
-
 hipStream_t as_stream(void* s) { return reinterpret_cast<hipStream_t>(s); }
 
 #define W4A8_REQUIRE(cond, msg)            \
@@ -155,75 +153,6 @@ int dense_impl(const void* x, bool x_bf16, int64_t M, int64_t K, const int32_t* 
 }
 
 }  // namespace
-
-void set_error(const std::string& msg) { g_error = msg; }
-
-KernelStamp& next_kernel_stamp() {
-    thread_local KernelStamp stamp;
-    return stamp;
-}
-void clear_error() { g_error.clear(); }
-
-int check_launch(const char* what) {
-    const hipError_t e = hipGetLastError();
-    if (e != hipSuccess) {
-        set_error(std::string(what) + ": " + hipGetErrorString(e));
-        return W4A8_ERR_HIP;
-    }
-    return W4A8_OK;
-}
-
-namespace {
-std::mutex g_dev_mu;
-// (device, kind, kernel, threads, lds) -> cached value; kind 0: LDS reserved, 1: blocks
-// per CU, 2: CU count
-std::map<std::tuple<int, int, const void*, int, size_t>, int> g_dev_facts;
-int current_device() {
-    int dev = 0;
-    return hipGetDevice(&dev) == hipSuccess ? dev : 0;
-}
-}  // namespace
-
-int reserve_dyn_lds(const void* kernel, int bytes, const char* what) {
-    const auto key = std::make_tuple(current_device(), 0, kernel, 0, (size_t)bytes);
-    std::lock_guard<std::mutex> lock(g_dev_mu);
-    if (g_dev_facts.count(key)) return W4A8_OK;
-    const hipError_t e =
-        hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
-    if (e != hipSuccess) {
-        set_error(std::string(what) + ": cannot reserve dynamic LDS: " + hipGetErrorString(e));
-        return W4A8_ERR_HIP;
-    }
-    g_dev_facts[key] = 1;
-    return W4A8_OK;
-}
-
-int device_cu_count() {
-    const int dev = current_device();
-    const auto key = std::make_tuple(dev, 2, (const void*)nullptr, 0, (size_t)0);
-    std::lock_guard<std::mutex> lock(g_dev_mu);
-    auto it = g_dev_facts.find(key);
-    if (it != g_dev_facts.end()) return it->second;
-    int ncu = 0;
-    if (hipDeviceGetAttribute(&ncu, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess ||
-        ncu <= 0)
-        ncu = 256;
-    g_dev_facts[key] = ncu;
-    return ncu;
-}
-
-int blocks_per_cu(const void* kernel, int threads, size_t lds) {
-    const auto key = std::make_tuple(current_device(), 1, kernel, threads, lds);
-    std::lock_guard<std::mutex> lock(g_dev_mu);
-    auto it = g_dev_facts.find(key);
-    if (it != g_dev_facts.end()) return it->second;
-    int occ = 0;
-    if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&occ, kernel, threads, lds) != hipSuccess ||
-        occ < 0)
-        occ = 0;
-    g_dev_facts[key] = occ;
-    return occ;
-}
 
 }  // namespace w4a8
 
@@ -693,7 +622,7 @@ extern "C" {
 
 int w4a8_abi_version(void) { return 3; }
 
-const char* w4a8_last_error(void) { return g_error.c_str(); }
+const char* w4a8_last_error(void) { return last_error().c_str(); }
 
 int w4a8_act_quant_fp8(const void* x_f16, int64_t rows, int64_t K, uint8_t* x_fp8,
                        float* act_scales, int k8_interleave, void* stream) {
@@ -725,6 +654,27 @@ int w4a8_topk_softmax(const float* logits, int64_t T, int64_t E, int64_t top_k,
     W4A8_REQUIRE(T == 0 || (logits && topk_weights && topk_ids), "topk_softmax: null pointer");
     return launch_topk_softmax(logits, T, E, top_k, renormalize != 0, topk_weights, topk_ids,
                                as_stream(stream));
+}
+
+int w4a8_route_topk(const void* logits, int dtype, int64_t T, int64_t E, int64_t logits_stride, int64_t top_k, int scoring,
+                    const float* bias, int64_t num_groups, int64_t top_groups, int renormalize, float scale,
+                    float* topk_weights, int32_t* topk_ids, void* stream) {
+    clear_error();
+    W4A8_REQUIRE(dtype == W4A8_DTYPE_F32 || dtype == W4A8_DTYPE_F16 || dtype == W4A8_DTYPE_BF16,
+                 "route_topk: logits must be fp32, fp16 or bf16");
+    W4A8_REQUIRE(scoring == 0 || scoring == 1, "route_topk: scoring must be 0 (softmax) or 1 (sigmoid)");
+    W4A8_REQUIRE(T >= 0 && T < ((int64_t)1 << 25) && E > 0 && E <= 1024 && top_k > 0 && top_k <= 64,
+                 "route_topk: need T < 2^25, E <= 1024 and top_k in 1 .. 64");
+    W4A8_REQUIRE(num_groups > 0 && num_groups <= 64 && E % num_groups == 0,
+                 "route_topk: num_groups must divide E and be at most 64");
+    W4A8_REQUIRE(top_groups > 0 && top_groups <= num_groups && top_k <= E / num_groups * top_groups,
+                 "route_topk: top_groups must be in 1 .. num_groups and hold top_k experts");
+    if (T == 0) return W4A8_OK;
+    W4A8_REQUIRE(logits && topk_weights && topk_ids, "route_topk: null pointer");
+    W4A8_REQUIRE(logits_stride >= E || T == 1, "route_topk: rows overlap");
+    RouteArgs a{logits, dtype, T, E, logits_stride, top_k, scoring == 1, bias, num_groups, top_groups, renormalize != 0,
+                scale, topk_weights, topk_ids};
+    return launch_route_topk(a, as_stream(stream));
 }
 
 int64_t w4a8_moe_align_sorted_len(int64_t numel, int64_t num_experts, int64_t block_m) {

@@ -1,0 +1,205 @@
+// C ABI entry points of the int8 operators (include/w4a8_int8.h): argument checks, workspace carving, the choice of
+// kernel and the whole-layer composition.
+#include <algorithm>
+#include <string>
+
+#include "../../include/w4a8_int8.h"
+#include "int8.h"
+
+namespace w4a8 {
+namespace {
+
+#define W4A8_REQUIRE(cond, msg)            \
+    do {                                   \
+        if (!(cond)) {                     \
+            ::w4a8::set_error(msg);        \
+            return W4A8_ERR_INVALID;       \
+        }                                  \
+    } while (0)
+
+hipStream_t as_stream(void* s) { return reinterpret_cast<hipStream_t>(s); }
+bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+bool is16(int dt) { return dt == W4A8_DTYPE_F16 || dt == W4A8_DTYPE_BF16; }
+Rows rows_of(int dt) { return dt == W4A8_DTYPE_BF16 ? Rows::kBf16 : Rows::kF16; }
+
+constexpr int64_t kMaxSide = (int64_t)1 << 24;    // rows of a weight
+constexpr int64_t kMaxRows = ((int64_t)1 << 31) - 256;
+
+// Sizes and pointers that every product shares.
+int check_product(const void* x, int x_dtype, const float* xs, int64_t rows, int64_t K, int64_t ldx, const int8_t* w,
+                  const float* ws, int64_t E, int64_t N) {
+    W4A8_REQUIRE(rows >= 0 && rows <= kMaxRows && K > 0 && N > 0 && E > 0, "int8 product: invalid sizes");
+    W4A8_REQUIRE(K <= kMaxInt8K, "int8 product: K is over 131071, where sums may pass 32 bits");
+    W4A8_REQUIRE(N <= kMaxSide && E <= kMaxSide, "int8 product: a size is over 2^24");
+    W4A8_REQUIRE(K % 16 == 0, "int8 product: K must be a multiple of 16");
+    W4A8_REQUIRE(x_dtype == W4A8_DTYPE_INT8 || is16(x_dtype), "int8 product: x must be int8, fp16 or bf16");
+    if (rows == 0) return W4A8_OK;
+    W4A8_REQUIRE(x && w && ws, "int8 product: null pointer");
+    W4A8_REQUIRE(x_dtype != W4A8_DTYPE_INT8 || xs, "int8 product: int8 rows need their scales");
+    W4A8_REQUIRE(ldx >= K && ldx * (x_dtype == W4A8_DTYPE_INT8 ? 1 : 2) % 16 == 0,
+                 "int8 product: rows of x must start at multiples of 16 bytes");
+    W4A8_REQUIRE(aligned16(x) && aligned16(w), "int8 product: x and w must be aligned to 16 bytes");
+    return W4A8_OK;
+}
+
+// ---- the gated layer ----
+struct LayerPlan {
+    int64_t block_m, P, nblk;
+};
+LayerPlan plan_layer(int64_t T, int64_t E, int64_t top_k) {
+    LayerPlan pl;
+    pl.block_m = 16;
+    // every block in use holds a slot
+    pl.P = std::min((T * top_k + E * (pl.block_m - 1) + pl.block_m - 1) / pl.block_m * pl.block_m, T * top_k * pl.block_m);
+    pl.nblk = pl.P / pl.block_m;
+    return pl;
+}
+struct LayerScratch {
+    int32_t *sti, *eid, *ntp;
+    void* align_ws;
+    size_t align_bytes;
+    int8_t *xq, *hq;
+    float *xs, *hs, *h, *y;
+};
+template <typename WS>
+void carve_layer(WS& w, const LayerPlan& pl, int64_t T, int64_t H, int64_t inter, int64_t E, int64_t top_k, LayerScratch& m) {
+    m = LayerScratch{};
+    m.sti = w.template take<int32_t>((size_t)pl.P);
+    m.eid = w.template take<int32_t>((size_t)pl.nblk);
+    m.ntp = w.template take<int32_t>(1);
+    m.align_bytes = align_workspace_bytes(T * top_k, E);
+    m.align_ws = w.template take<uint8_t>(m.align_bytes);
+    m.xq = w.template take<int8_t>((size_t)(T * H));
+    m.xs = w.template take<float>((size_t)T);
+    m.h = w.template take<float>((size_t)(pl.P * inter));
+    m.hq = w.template take<int8_t>((size_t)(pl.P * inter));
+    m.hs = w.template take<float>((size_t)pl.P);
+    m.y = w.template take<float>((size_t)(T * top_k * H));
+}
+struct SizeProbe {
+    WorkspaceSize s;
+    template <typename T>
+    T* take(size_t n) { s.take<T>(n); return nullptr; }
+};
+
+}  // namespace
+}  // namespace w4a8
+
+using namespace w4a8;
+
+extern "C" {
+
+int w4a8_int8_abi_version(void) { return 1; }
+const char* w4a8_int8_last_error(void) { return last_error().c_str(); }
+
+int w4a8_act_quant_int8(const void* x, int x_dtype, int64_t rows, int64_t K, int64_t x_stride, int silu_gate_up, int8_t* q,
+                        float* scales, void* stream) {
+    clear_error();
+    W4A8_REQUIRE(is16(x_dtype), "act_quant_int8: x must be fp16 or bf16");
+    W4A8_REQUIRE(rows >= 0 && rows <= kMaxRows && K > 0 && K <= kMaxSide, "act_quant_int8: invalid sizes");
+    if (rows == 0) return W4A8_OK;
+    W4A8_REQUIRE(x && q && scales, "act_quant_int8: null pointer");
+    W4A8_REQUIRE(x_stride >= (silu_gate_up ? 2 * K : K) || rows == 1, "act_quant_int8: rows overlap");
+    return launch_act_quant_int8(x, rows_of(x_dtype), rows, K, x_stride, silu_gate_up != 0, q, scales, nullptr, nullptr, 0,
+                                 as_stream(stream));
+}
+
+size_t w4a8_int8_gemm_workspace_size(int x_dtype, int64_t M, int64_t K) {
+    if (x_dtype == W4A8_DTYPE_INT8 || M <= 0 || K <= 0) return 0;
+    WorkspaceSize s;
+    s.take<int8_t>((size_t)(M * K));
+    s.take<float>((size_t)M);
+    return s.used;
+}
+
+int w4a8_int8_gemm(const void* x, int x_dtype, const float* x_scales, int64_t M, int64_t K, int64_t x_stride, const int8_t* w,
+                   const float* w_scales, int64_t N, const void* bias, int bias_is_f32, void* out, int out_dtype,
+                   void* workspace, size_t workspace_bytes, void* stream) {
+    clear_error();
+    if (int rc = check_product(x, x_dtype, x_scales, M, K, x_stride, w, w_scales, 1, N)) return rc;
+    W4A8_REQUIRE(is16(out_dtype), "int8_gemm: out must be fp16 or bf16");
+    if (M == 0) return W4A8_OK;
+    W4A8_REQUIRE(out, "int8_gemm: null pointer");
+    hipStream_t s = as_stream(stream);
+    Int8Args a{};
+    a.x = static_cast<const int8_t*>(x); a.xs = x_scales; a.x_rows = M; a.K = K; a.ldx = x_stride;
+    a.w = w; a.ws = w_scales; a.E = 1; a.N = N; a.bias = bias; a.bias_f32 = bias_is_f32 != 0;
+    a.P = M; a.top_k = 1; a.num_valid = M; a.block_m = 16;
+    a.dst = Out8::k16; a.bf16 = out_dtype == W4A8_DTYPE_BF16; a.out = out; a.ldo = N;
+    if (x_dtype != W4A8_DTYPE_INT8) {
+        Workspace ws(workspace, workspace_bytes);
+        int8_t* xq = ws.take<int8_t>((size_t)(M * K));
+        float* xs = ws.take<float>((size_t)M);
+        if (workspace == nullptr || !ws.ok()) {
+            set_error("int8_gemm: workspace smaller than w4a8_int8_gemm_workspace_size()");
+            return W4A8_ERR_WORKSPACE;
+        }
+        if (int rc = launch_act_quant_int8(x, rows_of(x_dtype), M, K, x_stride, false, xq, xs, nullptr, nullptr, 0, s)) return rc;
+        a.x = xq; a.xs = xs; a.ldx = K;
+    }
+    return launch_int8_stream(a, s);
+}
+
+size_t w4a8_moe_int8_workspace_size(int64_t T, int64_t H, int64_t inter, int64_t E, int64_t top_k) {
+    if (T <= 0 || H <= 0 || inter <= 0 || E <= 0 || top_k <= 0) return 0;
+    SizeProbe p;
+    LayerScratch m;
+    carve_layer(p, plan_layer(T, E, top_k), T, H, inter, E, top_k, m);
+    return p.s.used;
+}
+
+int w4a8_moe_int8_apply(const void* x, int x_dtype, const float* x_scales, int64_t T, int64_t H, int64_t inter, int64_t E,
+                        int64_t top_k, const int8_t* w13, const float* w13_scales, const int8_t* w2, const float* w2_scales,
+                        const float* topk_weights, const int32_t* topk_ids, const int32_t* expert_map,
+                        int64_t num_global_experts, void* out, int out_dtype, void* workspace, size_t workspace_bytes,
+                        void* stream) {
+    clear_error();
+    W4A8_REQUIRE(inter > 0 && inter % 64 == 0 && H > 0 && H % 64 == 0 && inter <= kMaxInt8K,
+                 "moe_int8_apply: hidden and intermediate sizes must be multiples of 64");
+    W4A8_REQUIRE(top_k > 0 && top_k <= 1024, "moe_int8_apply: invalid top_k");
+    W4A8_REQUIRE(T >= 0 && T <= kMaxRows / top_k, "moe_int8_apply: invalid sizes");
+    if (int rc = check_product(x, x_dtype, x_scales, T, H, H, w13, w13_scales, E, 2 * inter)) return rc;
+    W4A8_REQUIRE(is16(out_dtype), "moe_int8_apply: out must be fp16 or bf16");
+    const int64_t n_global = num_global_experts > 0 ? num_global_experts : E;
+    W4A8_REQUIRE(expert_map != nullptr || n_global == E,
+                 "moe_int8_apply: global expert count differs from the local one; pass expert_map");
+    W4A8_REQUIRE(E <= 1024 && n_global <= (int64_t)1 << 20, "moe_int8_apply: too many experts");
+    if (T == 0) return W4A8_OK;
+    W4A8_REQUIRE(w2 && w2_scales && topk_weights && topk_ids && out, "moe_int8_apply: null pointer");
+    W4A8_REQUIRE(aligned16(w2) && aligned16(out), "moe_int8_apply: w2 and out must be aligned to 16 bytes");
+    const LayerPlan pl = plan_layer(T, E, top_k);
+    W4A8_REQUIRE(pl.P <= kMaxRows, "moe_int8_apply: too many slots");
+    Workspace w(workspace, workspace_bytes);
+    LayerScratch m;
+    carve_layer(w, pl, T, H, inter, E, top_k, m);
+    if (workspace == nullptr || !w.ok()) {
+        set_error("moe_int8_apply: workspace smaller than w4a8_moe_int8_workspace_size()");
+        return W4A8_ERR_WORKSPACE;
+    }
+    hipStream_t s = as_stream(stream);
+    if (int rc = launch_align(topk_ids, T * top_k, E, pl.block_m, expert_map, n_global, m.sti, pl.P, m.eid, m.ntp, m.align_ws,
+                              m.align_bytes, s))
+        return rc;
+    Int8Args g1{};
+    g1.x = static_cast<const int8_t*>(x); g1.xs = x_scales;
+    if (x_dtype != W4A8_DTYPE_INT8) {
+        if (int rc = launch_act_quant_int8(x, rows_of(x_dtype), T, H, H, false, m.xq, m.xs, nullptr, nullptr, 0, s)) return rc;
+        g1.x = m.xq; g1.xs = m.xs;
+    }
+    g1.x_rows = T; g1.K = H; g1.ldx = H;
+    g1.w = w13; g1.ws = w13_scales; g1.E = E; g1.N = 2 * inter;
+    g1.sorted_ids = m.sti; g1.expert_ids = m.eid; g1.ntp = m.ntp; g1.P = pl.P;
+    g1.top_k = top_k; g1.num_valid = T * top_k; g1.block_m = pl.block_m; g1.gather = true;
+    g1.dst = Out8::kSiluF32; g1.out = m.h; g1.ldo = inter;
+    if (int rc = launch_int8_stream(g1, s)) return rc;
+    if (int rc = launch_act_quant_int8(m.h, Rows::kF32, pl.P, inter, inter, false, m.hq, m.hs, m.sti, m.ntp, T * top_k, s)) return rc;
+    Int8Args g2 = g1;
+    g2.x = m.hq; g2.xs = m.hs; g2.x_rows = pl.P; g2.K = inter; g2.ldx = inter;
+    g2.w = w2; g2.ws = w2_scales; g2.N = H; g2.gather = false;
+    g2.dst = Out8::kSlotF32; g2.out = m.y; g2.ldo = H;
+    if (int rc = launch_int8_stream(g2, s)) return rc;
+    return launch_int8_reduce(m.y, topk_weights, topk_ids, expert_map, n_global, E, T, H, top_k, out,
+                              out_dtype == W4A8_DTYPE_BF16, s);
+}
+
+}  // extern "C"

@@ -11,7 +11,8 @@
 
 namespace w4a8 {
 
-// Thread-local error slot behind w4a8_last_error().
+// The calling thread's error text (one per library).
+const std::string& last_error();
 void set_error(const std::string& msg);
 void clear_error();
 
@@ -94,6 +95,19 @@ int launch_topk_softmax(const float* logits, int64_t T, int64_t E, int64_t top_k
                         bool renorm, float* w, int32_t* ids, hipStream_t stream,
                         const void* x = nullptr, bool x_bf16 = false, int64_t K = 0,
                         uint8_t* xq = nullptr, float* xs = nullptr, float* gsum = nullptr);
+struct RouteArgs {
+    const void* logits;          // rows ldl elements apart
+    int dtype;                   // W4A8_DTYPE_F32, _F16 or _BF16
+    int64_t T, E, ldl, top_k;
+    bool sigmoid;
+    const float* bias;           // (E,) or null
+    int64_t groups, top_groups;
+    bool renorm;
+    float scale;
+    float* tw;
+    int32_t* ids;
+};
+int launch_route_topk(const RouteArgs& a, hipStream_t stream);
 size_t align_workspace_bytes(int64_t numel, int64_t num_experts);
 // Decode prologue in one launch (numel <= 1024): the single-work-group align plus per-row
 // act-quant of x (k8: k8-interleaved, else natural order) with optional group sums.

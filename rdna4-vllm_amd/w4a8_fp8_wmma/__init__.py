@@ -35,6 +35,14 @@ from .fp8_block import (  # noqa: E402,F401  block-scaled fp8 (W8A8) layers
     rms_norm_quant_fp8,
 )
 
+from .int8 import (  # noqa: E402,F401  int8 (W8A8) layers
+    act_quant_int8,
+    int8_gemm,
+    moe_int8_apply,
+)
+
+from .routing import route_topk  # noqa: E402,F401
+
 _MOE_KERNELS = {"scalar": 0, "wmma": 6, "gemv": 7}
 
 _DENSE_KERNELS = {
@@ -136,4 +144,5 @@ __all__ = [
     "set_prefill_pair", "silu_and_mul",
     "act_quant_fp8_block", "fp8_block_gemm", "moe_fp8_block_apply", "moe_fp8_block_gemm",
     "rms_norm_quant_fp8",
+    "act_quant_int8", "int8_gemm", "moe_int8_apply", "route_topk",
 ]

@@ -24,6 +24,8 @@ SIGNATURES = {
                                 _c_void_p]),
     "w4a8_topk_softmax": (_int, [_c_void_p, _i64, _i64, _i64, _int, _c_void_p, _c_void_p,
                                  _c_void_p]),
+    "w4a8_route_topk": (_int, [_c_void_p, _int, _i64, _i64, _i64, _i64, _int, _c_void_p, _i64, _i64,
+                               _int, ctypes.c_float, _c_void_p, _c_void_p, _c_void_p]),
     "w4a8_moe_align_sorted_len": (_i64, [_i64, _i64, _i64]),
     "w4a8_moe_align_workspace_size": (_size, [_i64, _i64]),
     "w4a8_moe_align_block_size": (_int, [_c_void_p, _i64, _i64, _i64, _c_void_p, _c_void_p, _i64,
