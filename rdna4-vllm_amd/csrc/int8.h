@@ -163,6 +163,19 @@ __device__ __forceinline__ void store16(const Int8Params& p, int64_t row, int co
     }
 }
 
+// Eight adjacent columns of one row.
+__device__ __forceinline__ void store16x8(const Int8Params& p, int64_t row, int col, const float (&t)[8]) {
+    if (p.out16 && col + 8 <= p.N) {
+        const bool bf16 = p.bf16 != 0;
+        *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(p.out) + row * p.ldo + col) =
+            make_uint4(pack_out16(t[0], t[1], bf16), pack_out16(t[2], t[3], bf16), pack_out16(t[4], t[5], bf16),
+                       pack_out16(t[6], t[7], bf16));
+    } else {
+        if (col < p.N) store16(p, row, col, v4f{t[0], t[1], t[2], t[3]});
+        if (col + 4 < p.N) store16(p, row, col + 4, v4f{t[4], t[5], t[6], t[7]});
+    }
+}
+
 // ---- launchers (all enqueue on the stream) ----
 enum class Rows : int { kF16 = 0, kBf16 = 1, kF32 = 2 };   // what rows are quantised from
 // int8 rows and scales of x (rows, K), or of silu(gate) * up of x = [gate | up] (rows, 2 K). With sorted_ids, padded
@@ -171,6 +184,10 @@ int launch_act_quant_int8(const void* x, Rows src, int64_t rows, int64_t K, int6
                           const int32_t* sorted_ids, const int32_t* ntp, int64_t num_valid, hipStream_t s);
 // Weight-streaming product (int8_stream.hip): any sizes.
 int launch_int8_stream(const Int8Args& a, hipStream_t s);
+// Tiles (int8_tiles.hip): sizes that 32-bit offsets reach; grouped, blocks of as many rows as a tile has.
+constexpr int64_t kTileRows = 64;
+bool int8_tiles_supported(const Int8Args& a);
+int launch_int8_tiles(const Int8Args& a, hipStream_t s);
 // out[t, n] = sum over the slots j in order of tw[t, j] * y[t top_k + j, n] (fp32), rounded to 16 bits; slots whose
 // (mapped) expert is not in [0, E) contribute nothing. N % 4 == 0.
 int launch_int8_reduce(const float* y, const float* tw, const int32_t* ids, const int32_t* emap, int64_t emap_len, int64_t E,

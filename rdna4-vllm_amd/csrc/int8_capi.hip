@@ -23,6 +23,7 @@ bool is16(int dt) { return dt == W4A8_DTYPE_F16 || dt == W4A8_DTYPE_BF16; }
 Rows rows_of(int dt) { return dt == W4A8_DTYPE_BF16 ? Rows::kBf16 : Rows::kF16; }
 
 constexpr int64_t kMaxSide = (int64_t)1 << 24;    // rows of a weight
+constexpr int64_t kStreamRows = 16;               // dense rows up to which the weights are streamed
 constexpr int64_t kMaxRows = ((int64_t)1 << 31) - 256;
 
 // Sizes and pointers that every product shares.
@@ -44,11 +45,15 @@ int check_product(const void* x, int x_dtype, const float* xs, int64_t rows, int
 
 // ---- the gated layer ----
 struct LayerPlan {
+    bool tiles;
     int64_t block_m, P, nblk;
 };
-LayerPlan plan_layer(int64_t T, int64_t E, int64_t top_k) {
+LayerPlan plan_layer(int64_t T, int64_t H, int64_t inter, int64_t E, int64_t top_k) {
     LayerPlan pl;
-    pl.block_m = 16;
+    // (the tiles address rows and an expert's weights in 32 bits)
+    const int64_t lim = (int64_t)1 << 32, most = (T * top_k + E * (kTileRows - 1) + kTileRows - 1) / kTileRows * kTileRows;
+    pl.tiles = T * top_k > 12 * E && T * H < lim && most * inter < lim && 2 * inter * H < lim;
+    pl.block_m = pl.tiles ? kTileRows : 16;
     // every block in use holds a slot
     pl.P = std::min((T * top_k + E * (pl.block_m - 1) + pl.block_m - 1) / pl.block_m * pl.block_m, T * top_k * pl.block_m);
     pl.nblk = pl.P / pl.block_m;
@@ -137,6 +142,7 @@ int w4a8_int8_gemm(const void* x, int x_dtype, const float* x_scales, int64_t M,
         if (int rc = launch_act_quant_int8(x, rows_of(x_dtype), M, K, x_stride, false, xq, xs, nullptr, nullptr, 0, s)) return rc;
         a.x = xq; a.xs = xs; a.ldx = K;
     }
+    if (M > kStreamRows && int8_tiles_supported(a)) return launch_int8_tiles(a, s);
     return launch_int8_stream(a, s);
 }
 
@@ -144,7 +150,7 @@ size_t w4a8_moe_int8_workspace_size(int64_t T, int64_t H, int64_t inter, int64_t
     if (T <= 0 || H <= 0 || inter <= 0 || E <= 0 || top_k <= 0) return 0;
     SizeProbe p;
     LayerScratch m;
-    carve_layer(p, plan_layer(T, E, top_k), T, H, inter, E, top_k, m);
+    carve_layer(p, plan_layer(T, H, inter, E, top_k), T, H, inter, E, top_k, m);
     return p.s.used;
 }
 
@@ -167,7 +173,7 @@ int w4a8_moe_int8_apply(const void* x, int x_dtype, const float* x_scales, int64
     if (T == 0) return W4A8_OK;
     W4A8_REQUIRE(w2 && w2_scales && topk_weights && topk_ids && out, "moe_int8_apply: null pointer");
     W4A8_REQUIRE(aligned16(w2) && aligned16(out), "moe_int8_apply: w2 and out must be aligned to 16 bytes");
-    const LayerPlan pl = plan_layer(T, E, top_k);
+    const LayerPlan pl = plan_layer(T, H, inter, E, top_k);
     W4A8_REQUIRE(pl.P <= kMaxRows, "moe_int8_apply: too many slots");
     Workspace w(workspace, workspace_bytes);
     LayerScratch m;
@@ -191,13 +197,13 @@ int w4a8_moe_int8_apply(const void* x, int x_dtype, const float* x_scales, int64
     g1.sorted_ids = m.sti; g1.expert_ids = m.eid; g1.ntp = m.ntp; g1.P = pl.P;
     g1.top_k = top_k; g1.num_valid = T * top_k; g1.block_m = pl.block_m; g1.gather = true;
     g1.dst = Out8::kSiluF32; g1.out = m.h; g1.ldo = inter;
-    if (int rc = launch_int8_stream(g1, s)) return rc;
+    if (int rc = pl.tiles ? launch_int8_tiles(g1, s) : launch_int8_stream(g1, s)) return rc;
     if (int rc = launch_act_quant_int8(m.h, Rows::kF32, pl.P, inter, inter, false, m.hq, m.hs, m.sti, m.ntp, T * top_k, s)) return rc;
     Int8Args g2 = g1;
     g2.x = m.hq; g2.xs = m.hs; g2.x_rows = pl.P; g2.K = inter; g2.ldx = inter;
     g2.w = w2; g2.ws = w2_scales; g2.N = H; g2.gather = false;
     g2.dst = Out8::kSlotF32; g2.out = m.y; g2.ldo = H;
-    if (int rc = launch_int8_stream(g2, s)) return rc;
+    if (int rc = pl.tiles ? launch_int8_tiles(g2, s) : launch_int8_stream(g2, s)) return rc;
     return launch_int8_reduce(m.y, topk_weights, topk_ids, expert_map, n_global, E, T, H, top_k, out,
                               out_dtype == W4A8_DTYPE_BF16, s);
 }

@@ -1,0 +1,425 @@
+// int8 products of many rows (gfx950 MFMA), dense or grouped.
+//
+// A work-group owns BT rows by BN weight rows (columns); per step of 128 k both come straight from memory to LDS
+// (16 bytes a lane, no registers), S steps deep. Weights are the first MFMA operand (32 x 32 x 32, whole numbers): a lane
+// ends up with sixteen values of one row, which are sixteen adjacent columns, as the weight rows of 32 lie in LDS in an
+// order that makes them so.
+//
+// Work-groups are persistent: a tile's ids are read under the one before, its first steps are loaded under the one
+// before's epilogue.
+#include <algorithm>
+#include <type_traits>
+
+#include "int8.h"
+
+namespace w4a8 {
+namespace {
+
+using lds_void_ptr = __attribute__((address_space(3))) void*;
+using global_cvoid_ptr = const __attribute__((address_space(1))) void*;
+
+constexpr int kTileXcds = 8;
+constexpr int kRunRows = 4;       // row tiles of a run: they share its columns' weights
+
+// What pieces past the end of K are read from.
+__device__ __attribute__((aligned(16))) uint32_t g_zero_piece[4];
+
+// s_waitcnt operand: at most n vector-memory loads and no LDS operation in flight.
+constexpr int wait_vm(int n) { return 0x0070 | (n & 0xF) | ((n >> 4) << 14); }
+
+// Work-group barrier that no load or store may be moved across and that waits for none of them.
+__device__ __forceinline__ void group_barrier() {
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+}
+
+__device__ __forceinline__ v16i mfma_i8_32(const u32x4& a, const u32x4& b, const v16i& c) {
+    const v4i x{(int)a[0], (int)a[1], (int)a[2], (int)a[3]}, y{(int)b[0], (int)b[1], (int)b[2], (int)b[3]};
+    return __builtin_amdgcn_mfma_i32_32x32x32_i8(x, y, c, 0, 0, 0);
+}
+
+// WT x WN waves of FT row fragments x FN column fragments of 32, S steps in LDS; KS such parts of a work-group share
+// K, each with slots of its own, and add their sums at the end. EU: waves a SIMD.
+template <int WT_, int WN_, int FT_, int FN_, int S_, int KS_, int EU_>
+struct Tile {
+    static constexpr int WT = WT_, WN = WN_, FT = FT_, FN = FN_, S = S_, KS = KS_, EU = EU_;
+    static constexpr int kWaves = WT * WN, kThreads = 64 * kWaves;   // of a part
+    static constexpr int BT = WT * FT * 32, BN = WN * FN * 32;
+    static constexpr int kW = BT * kStep;                        // weights behind the rows
+    static constexpr int kSlot = kW + BN * kStep;
+    static constexpr int PX = BT * 8 / kThreads, PW = BN * 8 / kThreads;   // 16-byte pieces a thread
+    static constexpr int kLoads = PX + PW;                       // of a wave and step
+    static_assert(PX * kThreads == BT * 8 && PW * kThreads == BN * 8, "pieces divide");
+    static_assert(kThreads % 128 == 0, "a thread's pieces are the same one of their rows");
+    static_assert(S == 2 || S == 3, "two or three slots");
+    static_assert(kLoads * (S - 1) < 64, "loads in flight can be counted");
+};
+
+template <typename C, Out8 DST, bool TAIL, bool GROUPED>
+__global__ void __launch_bounds__(C::kThreads * C::KS, C::EU) int8_tiles_kernel(Int8Params p, int ntiles) {
+    constexpr int FT = C::FT, FN = C::FN, BT = C::BT, BN = C::BN, KS = C::KS, S = C::S;
+    constexpr bool kSilu = DST == Out8::kSiluF32;
+    static_assert(!kSilu || FN % 2 == 0, "gate and up fragments of a wave go together");
+    // arrays of their own: the compiler then sees that reads of one do not wait for loads into another
+    __shared__ __attribute__((aligned(1024))) int8_t slots0[KS * C::kSlot];
+    __shared__ __attribute__((aligned(1024))) int8_t slots1[KS * C::kSlot];
+    __shared__ __attribute__((aligned(1024))) int8_t slots2[S == 3 ? KS * C::kSlot : 16];
+    // Tables for the epilogue, in slot 1 between a tile's last step and the next one's second.
+    float *const s_xs = reinterpret_cast<float*>(slots1), *const s_ws = s_xs + BT, *const s_bias = s_ws + BN;
+    int* const s_slot = reinterpret_cast<int*>(s_bias + BN);
+    static_assert(KS * C::kSlot >= 4 * (2 * BT + 2 * BN), "tables fit");
+
+    // ---- the tiles of this work-group: an XCD takes a contiguous run of them, kRunRows row tiles by all columns
+    // each; its work-groups take its tiles in turn ----
+    const int xcd = blockIdx.x % kTileXcds, jx = blockIdx.x / kTileXcds, step_items = gridDim.x / kTileXcds;
+    const int end = GROUPED ? min(p.ntp[0], p.P) : p.P;
+    const int mall = (end + BT - 1) / BT;
+    const int items = mall * ntiles, perx = (items + kTileXcds - 1) / kTileXcds;
+    const int last = min((xcd + 1) * perx, items);
+    int item = xcd * perx + jx;
+    if (item >= last) return;
+
+    const int part = KS > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x / C::kThreads) : 0;
+    const int tid = KS > 1 ? threadIdx.x % C::kThreads : threadIdx.x;
+    const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int h = lane >> 5, c = lane & 31;
+    const int wt = wave / C::WN, wn = wave % C::WN;
+    const int K = p.K, N = p.N, G = (K + kStep - 1) / kStep;
+    const int G1 = (G + KS - 1) / KS, g_first = part * G1;       // steps of a part, the first of them
+    int8_t *const slot0 = slots0 + part * C::kSlot, *const slot1 = slots1 + part * C::kSlot;
+    int8_t* const slot2 = S == 3 ? slots2 + part * C::kSlot : slots0;
+
+    // Piece i of a thread is the slot's piece tid + i kThreads: place / 8 and piece % 8. Row r lies at place
+    // r ^ ((r >> 3) & 1), its piece j at j ^ (r & 7): the sixteen lanes that a 16-byte LDS read serves at once then read
+    // different banks.
+    auto piece_row = [&](int i) __attribute__((always_inline)) {
+        const int pl = (tid + i * C::kThreads) >> 3;
+        return pl ^ ((pl >> 3) & 1);
+    };
+    const int piece_k = ((tid & 7) ^ (piece_row(0) & 7)) * 16;
+    // The column behind row r of the slot's BN: of each 32, MFMA row 8 a + 4 b + d is column 16 b + 4 a + d. kSilu takes
+    // FN / 2 fragments of the gate half and the same of the up half.
+    const int half = N / 2;
+    auto col_of = [&](int ct, int r) __attribute__((always_inline)) {
+        const int f = r >> 5, in = (r & 4) * 4 + (r >> 3 & 3) * 4 + (r & 3);
+        if constexpr (kSilu) {
+            const int w = f / FN, j = f % FN;
+            return min(ct * (BN / 2) + (w * (FN / 2) + j % (FN / 2)) * 32 + in, half - 1) + (j >= FN / 2 ? half : 0);
+        } else {
+            return min(ct * BN + f * 32 + in, N - 1);
+        }
+    };
+    auto place_of = [&](int it, int& row0, int& ct) __attribute__((always_inline)) {
+        const int run_items = kRunRows * ntiles, m0 = it / run_items * kRunRows, rem = it % run_items;
+        const int rows_here = min(kRunRows, mall - m0);
+        row0 = (m0 + rem % rows_here) * BT;
+        ct = rem / rows_here;
+    };
+
+    // ---- a tile's addresses ----
+    int row0, ct, e = 0;
+    const int8_t* we = p.w;                                      // the expert's weights
+    uint32_t xoff[C::PX], woff[C::PW];
+    constexpr int NX = (BT + C::kThreads - 1) / C::kThreads, NW = (BN + C::kThreads - 1) / C::kThreads;
+    int ids[C::PX], eid = 0, tids[NX];                           // tids: of the tables' rows
+    auto read_ids = [&](int r0) __attribute__((always_inline)) {
+        if constexpr (GROUPED) {
+            eid = p.expert_ids[r0 / p.block_m];
+#pragma unroll
+            for (int i = 0; i < C::PX; ++i) ids[i] = p.sorted_ids[min(r0 + piece_row(i), p.P - 1)];
+#pragma unroll
+            for (int i = 0; i < NX; ++i) tids[i] = p.sorted_ids[min(r0 + tid + i * C::kThreads, p.P - 1)];
+        }
+    };
+    // row r of the tile: the row of x it reads (a row that exists, for rows of no use)
+    auto xrow_of = [&](int r, int s) __attribute__((always_inline)) {
+        if constexpr (!GROUPED) return (uint32_t)min(r, p.P - 1);
+        if (!p.gather) return (uint32_t)min(r, p.x_rows - 1);
+        return (uint32_t)(s >= 0 && s < p.num_valid ? s / p.top_k : 0);
+    };
+    float xs_v[NX], ws_v[NW], bias_v[NW];
+    int slot_v[NX];
+    auto set_tile = [&]() __attribute__((always_inline)) {
+        e = GROUPED ? min(max(__builtin_amdgcn_readfirstlane(eid), 0), p.E - 1) : 0;
+        we = p.w + (int64_t)e * N * K;
+#pragma unroll
+        for (int i = 0; i < C::PX; ++i)
+            xoff[i] = xrow_of(row0 + piece_row(i), GROUPED ? ids[i] : 0) * (uint32_t)p.ldx + (uint32_t)piece_k;
+#pragma unroll
+        for (int i = 0; i < C::PW; ++i) woff[i] = (uint32_t)col_of(ct, piece_row(i)) * (uint32_t)K + (uint32_t)piece_k;
+        // the tile's scales, for its epilogue
+#pragma unroll
+        for (int i = 0; i < NX; ++i) {
+            const int row = row0 + tid + i * C::kThreads, s = GROUPED ? tids[i] : row;
+            xs_v[i] = p.xs[xrow_of(row, s)];
+            slot_v[i] = row < end && s >= 0 && s < p.num_valid ? s : -1;
+        }
+#pragma unroll
+        for (int i = 0; i < NW; ++i) {
+            const int r = (tid + i * C::kThreads) % BN;
+            // (column 32 f + n of the tile, not the MFMA row)
+            const int n = kSilu ? (r >> 5) % FN : 0;
+            const int col = kSilu ? min(ct * (BN / 2) + ((r >> 5) / FN * (FN / 2) + n % (FN / 2)) * 32 + (r & 31), half - 1) +
+                                        (n >= FN / 2 ? half : 0)
+                                  : min(ct * BN + r, N - 1);
+            ws_v[i] = p.ws[(int64_t)e * N + col];
+            bias_v[i] = DST == Out8::k16 ? bias_at(p, col) : 0.f;
+        }
+    };
+
+    auto dma = [&](const int8_t* src, int8_t* dst) __attribute__((always_inline)) {
+        __builtin_amdgcn_global_load_lds((global_cvoid_ptr)src, (lds_void_ptr)dst, 16, 0, 0);
+    };
+    // Past the last step every lane reads zeros. TAIL: absent pieces of the last, partial step are zero in both
+    // operands. Loads some of parts.
+    const int8_t* const zeros = reinterpret_cast<const int8_t*>(g_zero_piece);
+    auto issue = [&](int8_t* slot, int g, int some, int parts) __attribute__((always_inline)) {
+        const bool is = g < G1 && g_first + g < G;
+        const uint32_t on = is ? ~0u : 0u;
+        const int gg = g_first + g;
+        const uint64_t at = (uint64_t)(uint32_t)gg * kStep;
+        const uint64_t far = is ? ~0ull : 0ull, z = reinterpret_cast<uint64_t>(zeros) & ~far;
+        const int8_t* xg = reinterpret_cast<const int8_t*>(((reinterpret_cast<uint64_t>(p.x) + at) & far) | z);
+        const int8_t* wg = reinterpret_cast<const int8_t*>(((reinterpret_cast<uint64_t>(we) + at) & far) | z);
+        asm volatile("" : "+s"(xg), "+s"(wg));                   // (scalar bases, 32-bit offsets)
+        int8_t *xd = slot + wave * 1024, *wd = slot + C::kW + wave * 1024;
+        auto src = [&](const int8_t* base, uint32_t off) __attribute__((always_inline)) {
+            const int8_t* at = base + opaque_u32(off & on);
+            if constexpr (TAIL)
+                if (gg * kStep + piece_k >= K) at = zeros;
+            return at;
+        };
+#pragma unroll
+        for (int i = 0; i < C::PX; ++i)
+            if (i * parts / C::kLoads == some) dma(src(xg, xoff[i]), xd + i * C::kThreads * 16);
+#pragma unroll
+        for (int i = 0; i < C::PW; ++i)
+            if ((C::PX + i) * parts / C::kLoads == some) dma(src(wg, woff[i]), wd + i * C::kThreads * 16);
+    };
+
+    // ---- fragments: lane (h, c) reads piece 2 s + h of row c of each 32, sub-step s of four ----
+    const int at0 = (c ^ ((c >> 3) & 1)) * kStep + ((h ^ (c & 7)) << 4);
+    u32x4 xf[2][FT], wf[2][FN];
+    auto frags = [&](const int8_t* slot, int s) __attribute__((always_inline)) {
+        const int8_t* b = slot + (at0 ^ (s << 5));
+#pragma unroll
+        for (int j = 0; j < FN; ++j) wf[s & 1][j] = *reinterpret_cast<const u32x4*>(b + C::kW + (wn * FN + j) * 32 * kStep);
+#pragma unroll
+        for (int i = 0; i < FT; ++i) xf[s & 1][i] = *reinterpret_cast<const u32x4*>(b + (wt * FT + i) * 32 * kStep);
+    };
+    v16i run[FT][FN];
+    auto multiply = [&](int s, int i0, int i1) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = i0; i < i1; ++i)
+#pragma unroll
+            for (int j = 0; j < FN; ++j) run[i][j] = mfma_i8_32(wf[s & 1][j], xf[s & 1][i], run[i][j]);
+    };
+    // Step g from `slot`, whose first fragments are in registers. Before its last quarter the next step's stage has to
+    // have landed for all waves, and none reads `slot` any more: there the loads of step g + S go, among the last
+    // quarter's MFMAs, and the next step's first fragments are read. Loads are issued in every step, past the last one
+    // too, so that those in flight can be counted.
+    auto step = [&](int8_t* slot, const int8_t* next, int g) __attribute__((always_inline)) {
+#pragma unroll
+        for (int s = 0; s < 3; ++s) {
+            frags(slot, s + 1);
+            __builtin_amdgcn_sched_barrier(0);
+            multiply(s, 0, FT);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        __builtin_amdgcn_s_waitcnt(wait_vm(C::kLoads * (S - 2)));
+        group_barrier();
+        frags(next, 0);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int i = 0; i < FT; ++i) {
+            issue(slot, g + S, i, FT);
+            multiply(3, i, i + 1);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+
+    place_of(item, row0, ct);
+    read_ids(row0);
+    set_tile();
+    issue(slot0, 0, 0, 1);
+    issue(slot1, 1, 0, 1);
+    if (S == 3) issue(slot2, 2, 0, 1);
+    for (;;) {
+        const int r0_now = row0, ct_now = ct, next_item = item + step_items;
+        const bool more = next_item < last;
+        int row0_next = 0, ct_next = 0;
+        if (more) {
+            place_of(next_item, row0_next, ct_next);
+            read_ids(row0_next);
+        }
+#pragma unroll
+        for (int i = 0; i < FT; ++i)
+#pragma unroll
+            for (int j = 0; j < FN; ++j)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) run[i][j][r] = 0;
+        __builtin_amdgcn_s_waitcnt(wait_vm(0));
+        group_barrier();
+        frags(slot0, 0);
+        // (whole rounds of S steps: those past the last one multiply zeros)
+        for (int g = 0; g < G1; g += S) {
+            step(slot0, slot1, g);
+            step(slot1, S == 3 ? slot2 : slot0, g + 1);
+            if constexpr (S == 3) step(slot2, slot0, g + 2);
+        }
+        __builtin_amdgcn_s_waitcnt(wait_vm(0));                  // (the loads past the last step)
+        group_barrier();                                         // nobody reads or loads a slot any more
+        if constexpr (KS > 1) {
+            v4i* sums = reinterpret_cast<v4i*>(slots0);          // [KS - 1][FT FN 4][kThreads]
+            static_assert(KS == 1 || (KS - 1) * FT * FN * 4 * C::kThreads * sizeof(v4i) <= C::kSlot * KS, "sums fit");
+            if (part > 0)
+#pragma unroll
+                for (int i = 0; i < FT * FN * 4; ++i) {
+                    const v16i& v = run[i / 4 / FN][i / 4 % FN];
+                    sums[((part - 1) * FT * FN * 4 + i) * C::kThreads + tid] =
+                        v4i{v[i % 4 * 4], v[i % 4 * 4 + 1], v[i % 4 * 4 + 2], v[i % 4 * 4 + 3]};
+                }
+            lds_barrier();
+            if (part == 0)
+#pragma unroll
+                for (int w = 0; w < KS - 1; ++w)
+#pragma unroll
+                    for (int i = 0; i < FT * FN * 4; ++i) {
+                        const v4i v = sums[(w * FT * FN * 4 + i) * C::kThreads + tid];
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) run[i / 4 / FN][i / 4 % FN][i % 4 * 4 + r] += v[r];
+                    }
+            lds_barrier();
+        }
+
+        // ---- the next tile's first loads, and this one's epilogue: lane (h, c) holds row 32 i + c, columns 16 h .. 16 h +
+        // 15 of each fragment ----
+        if (part == 0) {
+#pragma unroll
+            for (int i = 0; i < NX; ++i) {
+                const int r = tid + i * C::kThreads;
+                if (r < BT) {
+                    s_xs[r] = xs_v[i];
+                    s_slot[r] = slot_v[i];
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < NW; ++i) {
+                const int r = tid + i * C::kThreads;
+                if (r < BN) {
+                    s_ws[r] = ws_v[i];
+                    if (DST == Out8::k16) s_bias[r] = bias_v[i];
+                }
+            }
+        }
+        if (more) {
+            row0 = row0_next;
+            ct = ct_next;
+            set_tile();
+            issue(slot0, 0, 0, 1);
+            if (S == 3) issue(slot2, 2, 0, 1);
+        }
+        lds_barrier();
+        float xs[FT];
+        int slot_of[FT];
+#pragma unroll
+        for (int i = 0; i < FT; ++i) {
+            xs[i] = s_xs[(wt * FT + i) * 32 + c];
+            slot_of[i] = s_slot[(wt * FT + i) * 32 + c];
+        }
+        if (KS == 1 || part == 0) {
+#pragma unroll
+            for (int j = 0; j < (kSilu ? FN / 2 : FN); ++j) {
+                const int f = wn * FN + j;                       // fragment of the tile
+                const int col = (kSilu ? ct_now * (BN / 2) + (wn * (FN / 2) + j) * 32 : ct_now * BN + f * 32) + 16 * h;
+                const int cols = kSilu ? half : N;
+                if (col >= cols) continue;
+#pragma unroll
+                for (int q = 0; q < 2; ++q) {                    // eight columns
+                    float ws[8], wu[8], b[8];
+#pragma unroll
+                    for (int r = 0; r < 8; ++r) {
+                        ws[r] = s_ws[f * 32 + 16 * h + 8 * q + r];
+                        wu[r] = kSilu ? s_ws[(f + FN / 2) * 32 + 16 * h + 8 * q + r] : 0.f;
+                        b[r] = DST == Out8::k16 ? s_bias[f * 32 + 16 * h + 8 * q + r] : 0.f;
+                    }
+#pragma unroll
+                    for (int i = 0; i < FT; ++i) {
+                        const int row = r0_now + (wt * FT + i) * 32 + c;
+                        if (slot_of[i] < 0) continue;
+                        float t[8];
+#pragma unroll
+                        for (int r = 0; r < 8; ++r) {
+                            t[r] = (float)run[i][j][8 * q + r] * (xs[i] * ws[r]);
+                            if constexpr (kSilu) t[r] = silu_mul(t[r], (float)run[i][j + FN / 2][8 * q + r] * (xs[i] * wu[r]));
+                            if constexpr (DST == Out8::k16) t[r] += b[r];
+                        }
+                        if constexpr (DST == Out8::k16) {
+                            store16x8(p, row, col + 8 * q, t);
+                        } else {
+                            float* o = reinterpret_cast<float*>(p.out) + (int64_t)(DST == Out8::kSlotF32 ? slot_of[i] : row) * p.ldo +
+                                       col + 8 * q;
+                            *reinterpret_cast<v4f*>(o) = v4f{t[0], t[1], t[2], t[3]};
+                            *reinterpret_cast<v4f*>(o + 4) = v4f{t[4], t[5], t[6], t[7]};
+                        }
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            }
+        }
+        if (!more) break;
+        item = next_item;
+        lds_barrier();                                           // nobody reads the tables any more
+        issue(slot1, 1, 0, 1);
+    }
+}
+
+template <typename C, Out8 DST, bool GROUPED>
+int tiles_go(const Int8Params& p, hipStream_t s) {
+    constexpr bool silu = DST == Out8::kSiluF32;
+    const int cols = silu ? p.N / 2 : p.N, per = silu ? C::BN / 2 : C::BN;
+    const int ntiles = (cols + per - 1) / per;
+    const int64_t mtiles = (p.P + C::BT - 1) / C::BT;
+    if (mtiles * ntiles >= ((int64_t)1 << 30)) {
+        set_error("int8 product: too many tiles");
+        return W4A8_ERR_INVALID;
+    }
+    const auto whole = &int8_tiles_kernel<C, DST, false, GROUPED>;
+    const auto tail = &int8_tiles_kernel<C, DST, true, GROUPED>;
+    const auto kernel = p.K % kStep != 0 ? tail : whole;
+    const int threads = C::kThreads * C::KS;
+    const int64_t each = std::max(1, blocks_per_cu(reinterpret_cast<const void*>(kernel), threads, 0));
+    const int64_t perx = (mtiles * ntiles + kTileXcds - 1) / kTileXcds;
+    const int64_t grid = kTileXcds * std::min<int64_t>(perx, std::max<int64_t>(1, each * device_cu_count() / kTileXcds));
+    launch_kernel(kernel, dim3((unsigned)grid), dim3(threads), 0, s, p, ntiles);
+    return check_launch("int8_tiles_kernel");
+}
+
+//                  WT WN FT FN S KS EU
+using Tile256x256 = Tile<2, 2, 4, 4, 2, 1, 1>;
+using Tile128x256 = Tile<2, 2, 2, 4, 3, 1, 1>;
+using Tile128x128 = Tile<2, 2, 2, 2, 2, 1, 2>;
+using Tile64x256 = Tile<1, 4, 2, 2, 2, 1, 2>;
+
+}  // namespace
+
+bool int8_tiles_supported(const Int8Args& a) {
+    // rows and an expert's weights are addressed in 32 bits
+    const int64_t lim = (int64_t)1 << 32;
+    return a.x_rows * a.ldx < lim && a.N * a.K < lim;
+}
+
+int launch_int8_tiles(const Int8Args& a, hipStream_t s) {
+    const Int8Params p = int8_params(a);
+    if (p.P == 0) return W4A8_OK;
+    if (a.dst == Out8::kSiluF32) return tiles_go<Tile64x256, Out8::kSiluF32, true>(p, s);
+    if (a.dst == Out8::kSlotF32) return tiles_go<Tile64x256, Out8::kSlotF32, true>(p, s);
+    if (a.P > 1024) return tiles_go<Tile256x256, Out8::k16, false>(p, s);
+    if (a.P > 128) return tiles_go<Tile128x256, Out8::k16, false>(p, s);
+    return tiles_go<Tile128x128, Out8::k16, false>(p, s);
+}
+
+}  // namespace w4a8
