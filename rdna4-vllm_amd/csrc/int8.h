@@ -112,14 +112,25 @@ __device__ __forceinline__ uint32_t quant4(float a, float b, float c, float d, c
     return lo | hi;
 }
 
-// silu(g) u in fp32 with the library's exponential and division: rows are quantised by it, where an error
-// moves a value across a border between two whole numbers. Below -80 e^-g may be no normal number, and u
-// as large as fp32 numbers are: silu(g) = g e^g to 35 digits there, as two factors e^(g / 2).
+// silu(g) u in fp32, to about three roundings: rows are quantised by it, where an error moves a value across a
+// border between two whole numbers (in the layer each such move costs up to a step). e^-g is the hardware's
+// 2^t, t = -g log2(e) with its rounding error put back, and 1 / (1 + e^-g) the hardware's reciprocal corrected
+// once. Below -80 e^-g may be no normal number, and u as large as fp32 numbers are: silu(g) = g e^g to 35 digits
+// there, as two factors e^(g / 2).
 __device__ __forceinline__ float silu_mul(float g, float u) {
-    const float h = g / (1.0f + expf(-g)) * u;
-    if (g >= -80.f || g != g) return h;
-    const float t = expf(0.5f * g);
-    return (g * t) * (t * u);
+    constexpr float l2e = 1.44269504088896340736f, l2e_lo = 1.92596299112661746887e-8f;
+    const float t = -g * l2e;
+    const float lo = fmaf(-g, l2e, -t) - g * l2e_lo;
+    const float p2 = __builtin_amdgcn_exp2f(t);
+    const float d = 1.0f + fmaf(p2 * 0.69314718055994530942f, lo, p2);
+    float r = __builtin_amdgcn_rcpf(d);
+    r = fmaf(fmaf(-d, r, 1.0f), r, r);
+    float h = g * r * u;
+    if (g < -80.f) {
+        const float m = __builtin_amdgcn_exp2f(g * 0.72134752044448170368f);
+        h = (g * m) * (m * u);
+    }
+    return h;
 }
 
 // ---- products ----
@@ -149,31 +160,39 @@ __device__ __forceinline__ float bias_at(const Int8Params& p, int n) {
     return p.bf16 ? __uint_as_float((uint32_t)v << 16) : __half2float(__ushort_as_half(v));
 }
 
-// Four adjacent columns of one row, rounded to 16 bits.
-__device__ __forceinline__ void store16(const Int8Params& p, int64_t row, int col, const v4f& t) {
-    uint16_t* o = reinterpret_cast<uint16_t*>(p.out) + row * p.ldo + col;
-    const uint32_t a = pack_out16(t[0], t[1], p.bf16 != 0), b = pack_out16(t[2], t[3], p.bf16 != 0);
-    if (p.out8 && col + 4 <= p.N) {
-        *reinterpret_cast<uint2*>(o) = make_uint2(a, b);
+// Two values rounded to 16 bits.
+template <bool BF16>
+__device__ __forceinline__ uint32_t pack16(float a, float b) {
+    if constexpr (BF16) {
+        using v2bf = __bf16 __attribute__((ext_vector_type(2)));
+        return __builtin_bit_cast(uint32_t, v2bf{(__bf16)a, (__bf16)b});
     } else {
-        const uint32_t v[4] = {a & 0xFFFF, a >> 16, b & 0xFFFF, b >> 16};
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-            if (col + r < p.N) o[r] = (uint16_t)v[r];
+        using v2h = _Float16 __attribute__((ext_vector_type(2)));
+        return __builtin_bit_cast(uint32_t, v2h{(_Float16)a, (_Float16)b});
     }
 }
-
-// Eight adjacent columns of one row.
-__device__ __forceinline__ void store16x8(const Int8Params& p, int64_t row, int col, const float (&t)[8]) {
-    if (p.out16 && col + 8 <= p.N) {
-        const bool bf16 = p.bf16 != 0;
-        *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(p.out) + row * p.ldo + col) =
-            make_uint4(pack_out16(t[0], t[1], bf16), pack_out16(t[2], t[3], bf16), pack_out16(t[4], t[5], bf16),
-                       pack_out16(t[6], t[7], bf16));
+// Some of N adjacent 16-bit values (words w) from column col on.
+template <int N>
+__device__ __forceinline__ void store16_some(const Int8Params& p, int64_t row, int col, const uint32_t (&w)[N / 2]) {
+    uint16_t* o = reinterpret_cast<uint16_t*>(p.out) + row * p.ldo + col;
+#pragma unroll
+    for (int r = 0; r < N; ++r)
+        if (col + r < p.N) o[r] = (uint16_t)(w[r / 2] >> (r % 2 * 16));
+}
+// Four adjacent columns of one row.
+__device__ __forceinline__ void store16(const Int8Params& p, int64_t row, int col, const v4f& t) {
+    uint32_t w[2];
+    if (p.bf16) {
+        w[0] = pack16<true>(t[0], t[1]);
+        w[1] = pack16<true>(t[2], t[3]);
     } else {
-        if (col < p.N) store16(p, row, col, v4f{t[0], t[1], t[2], t[3]});
-        if (col + 4 < p.N) store16(p, row, col + 4, v4f{t[4], t[5], t[6], t[7]});
+        w[0] = pack16<false>(t[0], t[1]);
+        w[1] = pack16<false>(t[2], t[3]);
     }
+    if (p.out8 && col + 4 <= p.N)
+        *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(p.out) + row * p.ldo + col) = make_uint2(w[0], w[1]);
+    else
+        store16_some<4>(p, row, col, w);
 }
 
 // ---- launchers (all enqueue on the stream) ----

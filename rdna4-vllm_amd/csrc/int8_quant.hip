@@ -190,7 +190,7 @@ __global__ void __launch_bounds__(128) int8_reduce_kernel(const float* __restric
             for (int r = 0; r < 4; ++r) sum[r] = fmaf(w[i], v[i][r], sum[r]);
         }
     }
-    *reinterpret_cast<uint2*>(out + t * N + n) = make_uint2(pack_out16(sum[0], sum[1], BF16), pack_out16(sum[2], sum[3], BF16));
+    *reinterpret_cast<uint2*>(out + t * N + n) = make_uint2(pack16<BF16>(sum[0], sum[1]), pack16<BF16>(sum[2], sum[3]));
 }
 
 }  // namespace

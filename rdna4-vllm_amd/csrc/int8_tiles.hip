@@ -70,7 +70,6 @@ __global__ void __launch_bounds__(C::kThreads * C::KS, C::EU) int8_tiles_kernel(
     // Tables for the epilogue, in slot 1 between a tile's last step and the next one's second.
     float *const s_xs = reinterpret_cast<float*>(slots1), *const s_ws = s_xs + BT, *const s_bias = s_ws + BN;
     int* const s_slot = reinterpret_cast<int*>(s_bias + BN);
-    static_assert(KS * C::kSlot >= 4 * (2 * BT + 2 * BN), "tables fit");
 
     // ---- the tiles of this work-group: an XCD takes a contiguous run of them, kRunRows row tiles by all columns
     // each; its work-groups take its tiles in turn ----
@@ -323,51 +322,79 @@ __global__ void __launch_bounds__(C::kThreads * C::KS, C::EU) int8_tiles_kernel(
             if (S == 3) issue(slot2, 2, 0, 1);
         }
         lds_barrier();
-        float xs[FT];
-        int slot_of[FT];
+        // A wave turns 32 rows at a time through LDS, so that its stores are whole lines: a row's values lie in
+        // chunks of 16 bytes, chunk i of row r at i ^ (r & 15) (rows of 256 bytes or more) or i ^ (r / 2 & 7) (of 128).
+        constexpr int kOutCols = (kSilu ? FN / 2 : FN) * 32, kSize = DST == Out8::k16 ? 2 : 4;
+        constexpr int kRowBytes = kOutCols * kSize, kChunks = kRowBytes / 16;
+        static_assert(kChunks >= 8, "a row is 128 bytes or more");
+        static_assert(KS * C::kSlot >= 4 * (2 * BT + 2 * BN) + C::kWaves * 32 * kRowBytes, "tables and rows fit");
+        int8_t* const strip = slots1 + 4 * (2 * BT + 2 * BN) + wave * 32 * kRowBytes;
+        auto chunk_at = [&](int row, int i) __attribute__((always_inline)) {
+            return row * kRowBytes + ((i ^ (kChunks >= 16 ? row & 15 : row >> 1 & 7)) << 4);
+        };
+        const int col0 = kSilu ? ct_now * (BN / 2) + wn * kOutCols : ct_now * BN + wn * kOutCols;
+        auto turn = [&](int i, auto bf16) __attribute__((always_inline)) {
+            const float xs = s_xs[(wt * FT + i) * 32 + c];
 #pragma unroll
-        for (int i = 0; i < FT; ++i) {
-            xs[i] = s_xs[(wt * FT + i) * 32 + c];
-            slot_of[i] = s_slot[(wt * FT + i) * 32 + c];
-        }
-        if (KS == 1 || part == 0) {
-#pragma unroll
-            for (int j = 0; j < (kSilu ? FN / 2 : FN); ++j) {
-                const int f = wn * FN + j;                       // fragment of the tile
-                const int col = (kSilu ? ct_now * (BN / 2) + (wn * (FN / 2) + j) * 32 : ct_now * BN + f * 32) + 16 * h;
-                const int cols = kSilu ? half : N;
-                if (col >= cols) continue;
+            for (int j = 0; j < kOutCols / 32; ++j) {
 #pragma unroll
                 for (int q = 0; q < 2; ++q) {                    // eight columns
-                    float ws[8], wu[8], b[8];
+                    const int at = (wn * FN + j) * 32 + 16 * h + 8 * q;
+                    float t[8];
 #pragma unroll
                     for (int r = 0; r < 8; ++r) {
-                        ws[r] = s_ws[f * 32 + 16 * h + 8 * q + r];
-                        wu[r] = kSilu ? s_ws[(f + FN / 2) * 32 + 16 * h + 8 * q + r] : 0.f;
-                        b[r] = DST == Out8::k16 ? s_bias[f * 32 + 16 * h + 8 * q + r] : 0.f;
+                        const float v = (float)run[i][j][8 * q + r], f = xs * s_ws[at + r];
+                        if constexpr (kSilu)
+                            t[r] = silu_mul(v * f, (float)run[i][j + FN / 2][8 * q + r] * (xs * s_ws[at + FN / 2 * 32 + r]));
+                        else if constexpr (DST == Out8::k16) t[r] = fmaf(v, f, s_bias[at + r]);
+                        else t[r] = v * f;
                     }
-#pragma unroll
-                    for (int i = 0; i < FT; ++i) {
-                        const int row = r0_now + (wt * FT + i) * 32 + c;
-                        if (slot_of[i] < 0) continue;
-                        float t[8];
-#pragma unroll
-                        for (int r = 0; r < 8; ++r) {
-                            t[r] = (float)run[i][j][8 * q + r] * (xs[i] * ws[r]);
-                            if constexpr (kSilu) t[r] = silu_mul(t[r], (float)run[i][j + FN / 2][8 * q + r] * (xs[i] * wu[r]));
-                            if constexpr (DST == Out8::k16) t[r] += b[r];
-                        }
-                        if constexpr (DST == Out8::k16) {
-                            store16x8(p, row, col + 8 * q, t);
-                        } else {
-                            float* o = reinterpret_cast<float*>(p.out) + (int64_t)(DST == Out8::kSlotF32 ? slot_of[i] : row) * p.ldo +
-                                       col + 8 * q;
-                            *reinterpret_cast<v4f*>(o) = v4f{t[0], t[1], t[2], t[3]};
-                            *reinterpret_cast<v4f*>(o + 4) = v4f{t[4], t[5], t[6], t[7]};
-                        }
+                    const int chunk = (j * 32 + 16 * h + 8 * q) * kSize / 16;
+                    if constexpr (DST == Out8::k16) {
+                        constexpr bool b = decltype(bf16)::value;
+                        *reinterpret_cast<u32x4*>(strip + chunk_at(c, chunk)) =
+                            u32x4{pack16<b>(t[0], t[1]), pack16<b>(t[2], t[3]), pack16<b>(t[4], t[5]), pack16<b>(t[6], t[7])};
+                    } else {
+                        *reinterpret_cast<v4f*>(strip + chunk_at(c, chunk)) = v4f{t[0], t[1], t[2], t[3]};
+                        *reinterpret_cast<v4f*>(strip + chunk_at(c, chunk + 1)) = v4f{t[4], t[5], t[6], t[7]};
                     }
-                    __builtin_amdgcn_sched_barrier(0);
                 }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        };
+        auto put = [&](int i) __attribute__((always_inline)) {
+            constexpr int kRows = 64 / kChunks > 0 ? 64 / kChunks : 1;   // rows of one store
+            static_assert(kChunks <= 64 && 32 % kRows == 0, "a store takes whole rows");
+            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront", "local");
+            __builtin_amdgcn_wave_barrier();
+#pragma unroll
+            for (int r0 = 0; r0 < 32; r0 += kRows) {
+                const int r = r0 + lane / kChunks, chunk = lane % kChunks;
+                const u32x4 v = *reinterpret_cast<const u32x4*>(strip + chunk_at(r, chunk));
+                const int slot = s_slot[(wt * FT + i) * 32 + r];
+                const int64_t row = DST == Out8::kSlotF32 ? slot : r0_now + (wt * FT + i) * 32 + r;
+                const int col = col0 + chunk * 16 / kSize;
+                if (slot < 0 || col >= (kSilu ? half : N)) continue;
+                if constexpr (DST == Out8::k16) {
+                    if (p.out16 && col + 8 <= N) {
+                        *reinterpret_cast<u32x4*>(reinterpret_cast<uint16_t*>(p.out) + row * p.ldo + col) = v;
+                    } else {
+                        const uint32_t w[4] = {v[0], v[1], v[2], v[3]};
+                        store16_some<8>(p, row, col, w);
+                    }
+                } else {                                         // (whole layers: multiples of 64 columns)
+                    *reinterpret_cast<u32x4*>(reinterpret_cast<float*>(p.out) + row * p.ldo + col) = v;
+                }
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront", "local");
+            __builtin_amdgcn_wave_barrier();
+        };
+        if (KS == 1 || part == 0) {
+#pragma unroll
+            for (int i = 0; i < FT; ++i) {
+                if (DST == Out8::k16 && p.bf16) turn(i, std::true_type{});
+                else turn(i, std::false_type{});
+                put(i);
             }
         }
         if (!more) break;
