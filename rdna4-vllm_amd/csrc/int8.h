@@ -27,6 +27,16 @@ enum class Out8 : int {
     kSlotF32 = 2,   // out[slot, n] in fp32
 };
 
+// What the streaming kernels read their rows from.
+enum class Src8 : int {
+    kI8 = 0,        // int8 rows with their scales
+    kF16 = 1,       // fp16 / bf16 / fp32 rows, quantised in registers
+    kBf16 = 2,
+    kF32 = 3,
+};
+constexpr int kScanSlots = 4096;              // routed slots that a streaming kernel looks through
+
+// Tiles (int8_tiles.hip).
 struct Int8Args {
     const int8_t* x;             // (x_rows, K)
     const float* xs;             // (x_rows,)
@@ -48,36 +58,76 @@ struct Int8Args {
     int64_t ldo;
 };
 
-// The same on the device.
-struct Int8Params {
-    const int8_t* x;
-    const float* xs;
+// Streaming kernels (int8_rows.hip).
+struct RowsArgs {
+    const void* x;               // rows, see Src8
+    Src8 src;
+    const float* xs;             // int8 rows: their scales
+    int64_t rows, K, ldx;        // rows: of x
     const int8_t* w;
     const float* ws;
     const void* bias;
-    const int32_t* sorted_ids;
-    const int32_t* expert_ids;
-    const int32_t* ntp;
+    bool bias_f32;
+    int64_t E, N;
+    const int32_t* ids;          // (slots,) routed experts; null: one expert, all rows (dense)
+    const int32_t* emap;         // global -> local expert, or null
+    int64_t emap_len, slots, top_k;
+    bool gather;                 // slot s reads x[s / top_k], else x[s]
+    bool single;                 // a work-group takes one slot, not an expert's
+    Out8 dst;                    // out rows are slots (dense: rows)
+    bool bf16;
+    void* out;
+    int64_t ldo;
+};
+
+// What both have on the device.
+struct OutParams {
+    const int8_t* w;
+    const float* ws;
+    const void* bias;
     void* out;
     int64_t ldx, ldo;
-    int P, K, N, E;
-    int x_rows, top_k, num_valid, block_m, gather;
+    int K, N, E, top_k, gather;
     int bf16, bias_f32;
     int out8, out16;             // rows of out are aligned to 8, to 16 bytes
 };
+struct Int8Params : OutParams {
+    const int8_t* x;
+    const float* xs;
+    const int32_t* sorted_ids;
+    const int32_t* expert_ids;
+    const int32_t* ntp;
+    int P, x_rows, num_valid, block_m;
+};
+struct RowsParams : OutParams {
+    const void* x;
+    const float* xs;
+    const int32_t* ids;
+    const int32_t* emap;
+    int rows, slots, emap_len, single;
+};
 
-inline Int8Params int8_params(const Int8Args& a) {
-    Int8Params p;
-    p.x = a.x; p.xs = a.xs; p.w = a.w; p.ws = a.ws; p.bias = a.bias;
-    p.sorted_ids = a.sorted_ids; p.expert_ids = a.expert_ids; p.ntp = a.ntp;
-    p.out = a.out; p.ldx = a.ldx; p.ldo = a.ldo;
-    p.P = (int)a.P; p.K = (int)a.K; p.N = (int)a.N; p.E = (int)a.E;
-    p.x_rows = (int)a.x_rows; p.top_k = (int)a.top_k; p.num_valid = (int)a.num_valid;
-    p.block_m = (int)a.block_m; p.gather = a.gather ? 1 : 0;
+template <typename A>
+inline void out_params(const A& a, OutParams& p) {
+    p.w = a.w; p.ws = a.ws; p.bias = a.bias; p.out = a.out; p.ldx = a.ldx; p.ldo = a.ldo;
+    p.K = (int)a.K; p.N = (int)a.N; p.E = (int)a.E; p.top_k = (int)a.top_k; p.gather = a.gather ? 1 : 0;
     p.bf16 = a.bf16 ? 1 : 0; p.bias_f32 = a.bias_f32 ? 1 : 0;
     const uintptr_t at = reinterpret_cast<uintptr_t>(a.out);
     p.out8 = at % 8 == 0 && a.ldo % 4 == 0 ? 1 : 0;
     p.out16 = at % 16 == 0 && a.ldo % 8 == 0 ? 1 : 0;
+}
+inline Int8Params int8_params(const Int8Args& a) {
+    Int8Params p;
+    out_params(a, p);
+    p.x = a.x; p.xs = a.xs; p.sorted_ids = a.sorted_ids; p.expert_ids = a.expert_ids; p.ntp = a.ntp;
+    p.P = (int)a.P; p.x_rows = (int)a.x_rows; p.num_valid = (int)a.num_valid; p.block_m = (int)a.block_m;
+    return p;
+}
+inline RowsParams rows_params(const RowsArgs& a) {
+    RowsParams p;
+    out_params(a, p);
+    p.x = a.x; p.xs = a.xs; p.ids = a.ids; p.emap = a.emap;
+    p.rows = (int)a.rows; p.slots = (int)a.slots; p.emap_len = (int)a.emap_len; p.single = a.single ? 1 : 0;
     return p;
 }
 
@@ -139,21 +189,7 @@ __device__ __forceinline__ v4i mfma_i8(const u32x4& a, const u32x4& b, const v4i
     return __builtin_amdgcn_mfma_i32_16x16x64_i8(x, y, c, 0, 0, 0);
 }
 
-// Padded row r: its slot (dense: r), or -1 for padding, and the row of x it reads (0 for padding).
-__device__ __forceinline__ int int8_slot(const Int8Params& p, int r, int end, int& xrow) {
-    xrow = 0;
-    if (r >= end) return -1;
-    if (p.sorted_ids == nullptr) {
-        xrow = r;
-        return r;
-    }
-    const int s = p.sorted_ids[r];
-    if (s < 0 || s >= p.num_valid) return -1;
-    xrow = p.gather ? s / p.top_k : r;
-    return s;
-}
-
-__device__ __forceinline__ float bias_at(const Int8Params& p, int n) {
+__device__ __forceinline__ float bias_at(const OutParams& p, int n) {
     if (p.bias == nullptr) return 0.f;
     if (p.bias_f32) return reinterpret_cast<const float*>(p.bias)[n];
     const uint16_t v = reinterpret_cast<const uint16_t*>(p.bias)[n];
@@ -173,14 +209,14 @@ __device__ __forceinline__ uint32_t pack16(float a, float b) {
 }
 // Some of N adjacent 16-bit values (words w) from column col on.
 template <int N>
-__device__ __forceinline__ void store16_some(const Int8Params& p, int64_t row, int col, const uint32_t (&w)[N / 2]) {
+__device__ __forceinline__ void store16_some(const OutParams& p, int64_t row, int col, const uint32_t (&w)[N / 2]) {
     uint16_t* o = reinterpret_cast<uint16_t*>(p.out) + row * p.ldo + col;
 #pragma unroll
     for (int r = 0; r < N; ++r)
         if (col + r < p.N) o[r] = (uint16_t)(w[r / 2] >> (r % 2 * 16));
 }
 // Four adjacent columns of one row.
-__device__ __forceinline__ void store16(const Int8Params& p, int64_t row, int col, const v4f& t) {
+__device__ __forceinline__ void store16(const OutParams& p, int64_t row, int col, const v4f& t) {
     uint32_t w[2];
     if (p.bf16) {
         w[0] = pack16<true>(t[0], t[1]);
@@ -201,8 +237,10 @@ enum class Rows : int { kF16 = 0, kBf16 = 1, kF32 = 2 };   // what rows are quan
 // rows r < ntp without a slot in [0, num_valid) are left out.
 int launch_act_quant_int8(const void* x, Rows src, int64_t rows, int64_t K, int64_t ldx, bool silu, int8_t* q, float* scales,
                           const int32_t* sorted_ids, const int32_t* ntp, int64_t num_valid, hipStream_t s);
-// Weight-streaming product (int8_stream.hip): any sizes.
-int launch_int8_stream(const Int8Args& a, hipStream_t s);
+// Weight-streaming product (int8_rows.hip): any sizes, up to kScanSlots slots; rows that are not int8 up to
+// int8_rows_quantised_in_kernel().
+bool int8_rows_quantised_in_kernel(int64_t K);
+int launch_int8_rows(const RowsArgs& a, hipStream_t s);
 // Tiles (int8_tiles.hip): sizes that 32-bit offsets reach; grouped, blocks of as many rows as a tile has.
 constexpr int64_t kTileRows = 64;
 bool int8_tiles_supported(const Int8Args& a);

@@ -20,6 +20,7 @@ namespace {
 hipStream_t as_stream(void* s) { return reinterpret_cast<hipStream_t>(s); }
 bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 bool is16(int dt) { return dt == W4A8_DTYPE_F16 || dt == W4A8_DTYPE_BF16; }
+Src8 src_of(int dt) { return dt == W4A8_DTYPE_INT8 ? Src8::kI8 : dt == W4A8_DTYPE_BF16 ? Src8::kBf16 : Src8::kF16; }
 Rows rows_of(int dt) { return dt == W4A8_DTYPE_BF16 ? Rows::kBf16 : Rows::kF16; }
 
 constexpr int64_t kMaxSide = (int64_t)1 << 24;    // rows of a weight
@@ -44,19 +45,29 @@ int check_product(const void* x, int x_dtype, const float* xs, int64_t rows, int
 }
 
 // ---- the gated layer ----
+// Few rows an expert: the streaming kernels, which find their rows in the routed ids (h and the slots' rows in fp32, by
+// slot). Else tiles: rows quantised beforehand, slots aligned to blocks of the 64 rows that a tile has. Tokens are taken in
+// parts of as many as either can address.
 struct LayerPlan {
-    bool tiles;
-    int64_t block_m, P, nblk;
+    bool tiles, single;
+    int64_t part;                // tokens of a part
+    int64_t P, nblk;             // of a part: padded rows and blocks
+    bool quant_x, quant_h;       // rows quantised by a launch of their own
 };
-LayerPlan plan_layer(int64_t T, int64_t H, int64_t inter, int64_t E, int64_t top_k) {
-    LayerPlan pl;
-    // (the tiles address rows and an expert's weights in 32 bits)
-    const int64_t lim = (int64_t)1 << 32, most = (T * top_k + E * (kTileRows - 1) + kTileRows - 1) / kTileRows * kTileRows;
-    pl.tiles = T * top_k > 12 * E && T * H < lim && most * inter < lim && 2 * inter * H < lim;
-    pl.block_m = pl.tiles ? kTileRows : 16;
+LayerPlan plan_layer(int64_t T, int64_t H, int64_t inter, int64_t E, int64_t top_k, int x_dtype) {
+    LayerPlan pl{};
+    const int64_t lim = ((int64_t)1 << 32) - 1, pad = E * (kTileRows - 1) + kTileRows;
+    pl.tiles = T * top_k > std::min<int64_t>(12 * E, kScanSlots) && 2 * inter * H <= lim;
+    const int64_t most = pl.tiles ? std::min(lim / H, (lim / inter - pad) / top_k) : kScanSlots / top_k;
+    pl.part = std::min(T, std::max<int64_t>(1, most));
     // every block in use holds a slot
-    pl.P = std::min((T * top_k + E * (pl.block_m - 1) + pl.block_m - 1) / pl.block_m * pl.block_m, T * top_k * pl.block_m);
-    pl.nblk = pl.P / pl.block_m;
+    const int64_t n = pl.part * top_k;
+    pl.P = pl.tiles ? std::min((n + E * (kTileRows - 1) + kTileRows - 1) / kTileRows * kTileRows, n * kTileRows) : n;
+    pl.nblk = pl.P / kTileRows;
+    // few slots: hardly two of one expert
+    pl.single = n * 8 <= E;
+    pl.quant_x = x_dtype != W4A8_DTYPE_INT8 && (pl.tiles || !int8_rows_quantised_in_kernel(H));
+    pl.quant_h = pl.tiles || !int8_rows_quantised_in_kernel(inter);
     return pl;
 }
 struct LayerScratch {
@@ -67,19 +78,87 @@ struct LayerScratch {
     float *xs, *hs, *h, *y;
 };
 template <typename WS>
-void carve_layer(WS& w, const LayerPlan& pl, int64_t T, int64_t H, int64_t inter, int64_t E, int64_t top_k, LayerScratch& m) {
+void carve_layer(WS& w, const LayerPlan& pl, int64_t H, int64_t inter, int64_t E, int64_t top_k, LayerScratch& m) {
     m = LayerScratch{};
-    m.sti = w.template take<int32_t>((size_t)pl.P);
-    m.eid = w.template take<int32_t>((size_t)pl.nblk);
-    m.ntp = w.template take<int32_t>(1);
-    m.align_bytes = align_workspace_bytes(T * top_k, E);
-    m.align_ws = w.template take<uint8_t>(m.align_bytes);
-    m.xq = w.template take<int8_t>((size_t)(T * H));
-    m.xs = w.template take<float>((size_t)T);
+    const int64_t n = pl.part * top_k;
+    if (pl.tiles) {
+        m.sti = w.template take<int32_t>((size_t)pl.P);
+        m.eid = w.template take<int32_t>((size_t)pl.nblk);
+        m.ntp = w.template take<int32_t>(1);
+        m.align_bytes = align_workspace_bytes(n, E);
+        m.align_ws = w.template take<uint8_t>(m.align_bytes);
+    }
+    if (pl.quant_x) {
+        m.xq = w.template take<int8_t>((size_t)(pl.part * H));
+        m.xs = w.template take<float>((size_t)pl.part);
+    }
     m.h = w.template take<float>((size_t)(pl.P * inter));
-    m.hq = w.template take<int8_t>((size_t)(pl.P * inter));
-    m.hs = w.template take<float>((size_t)pl.P);
-    m.y = w.template take<float>((size_t)(T * top_k * H));
+    if (pl.quant_h) {
+        m.hq = w.template take<int8_t>((size_t)(pl.P * inter));
+        m.hs = w.template take<float>((size_t)pl.P);
+    }
+    m.y = w.template take<float>((size_t)(n * H));
+}
+struct Layer {
+    const void* x;
+    int x_dtype;
+    const float* xs;
+    int64_t T, H, inter, E, top_k;
+    const int8_t* w13;
+    const float* s13;
+    const int8_t* w2;
+    const float* s2;
+    const float* tw;
+    const int32_t* ids;
+    const int32_t* emap;
+    int64_t n_global;
+    void* out;
+    bool bf16;
+};
+int run_layer(const Layer& l, const LayerPlan& pl, const LayerScratch& m, hipStream_t s) {
+    const int64_t n = l.T * l.top_k;
+    const void* x = l.x;
+    const float* xs = l.xs;
+    if (pl.quant_x) {
+        if (int rc = launch_act_quant_int8(x, rows_of(l.x_dtype), l.T, l.H, l.H, false, m.xq, m.xs, nullptr, nullptr, 0, s)) return rc;
+        x = m.xq;
+        xs = m.xs;
+    }
+    if (pl.tiles) {
+        if (int rc = launch_align(l.ids, n, l.E, kTileRows, l.emap, l.n_global, m.sti, pl.P, m.eid, m.ntp, m.align_ws,
+                                  m.align_bytes, s))
+            return rc;
+        Int8Args g1{};
+        g1.x = static_cast<const int8_t*>(x); g1.xs = xs; g1.x_rows = l.T; g1.K = l.H; g1.ldx = l.H;
+        g1.w = l.w13; g1.ws = l.s13; g1.E = l.E; g1.N = 2 * l.inter;
+        g1.sorted_ids = m.sti; g1.expert_ids = m.eid; g1.ntp = m.ntp; g1.P = pl.P;
+        g1.top_k = l.top_k; g1.num_valid = n; g1.block_m = kTileRows; g1.gather = true;
+        g1.dst = Out8::kSiluF32; g1.out = m.h; g1.ldo = l.inter;
+        if (int rc = launch_int8_tiles(g1, s)) return rc;
+        if (int rc = launch_act_quant_int8(m.h, Rows::kF32, pl.P, l.inter, l.inter, false, m.hq, m.hs, m.sti, m.ntp, n, s)) return rc;
+        Int8Args g2 = g1;
+        g2.x = m.hq; g2.xs = m.hs; g2.x_rows = pl.P; g2.K = l.inter; g2.ldx = l.inter;
+        g2.w = l.w2; g2.ws = l.s2; g2.N = l.H; g2.gather = false;
+        g2.dst = Out8::kSlotF32; g2.out = m.y; g2.ldo = l.H;
+        if (int rc = launch_int8_tiles(g2, s)) return rc;
+    } else {
+        RowsArgs g1{};
+        g1.x = x; g1.src = pl.quant_x ? Src8::kI8 : src_of(l.x_dtype); g1.xs = xs; g1.rows = l.T; g1.K = l.H; g1.ldx = l.H;
+        g1.w = l.w13; g1.ws = l.s13; g1.E = l.E; g1.N = 2 * l.inter;
+        g1.ids = l.ids; g1.emap = l.emap; g1.emap_len = l.n_global; g1.slots = n; g1.top_k = l.top_k;
+        g1.gather = true; g1.single = pl.single; g1.dst = Out8::kSiluF32; g1.out = m.h; g1.ldo = l.inter;
+        if (int rc = launch_int8_rows(g1, s)) return rc;
+        RowsArgs g2 = g1;
+        g2.x = m.h; g2.src = Src8::kF32; g2.rows = n; g2.K = l.inter; g2.ldx = l.inter;
+        if (pl.quant_h) {
+            if (int rc = launch_act_quant_int8(m.h, Rows::kF32, n, l.inter, l.inter, false, m.hq, m.hs, nullptr, nullptr, 0, s)) return rc;
+            g2.x = m.hq; g2.src = Src8::kI8; g2.xs = m.hs;
+        }
+        g2.w = l.w2; g2.ws = l.s2; g2.N = l.H; g2.gather = false;
+        g2.dst = Out8::kSlotF32; g2.out = m.y; g2.ldo = l.H;
+        if (int rc = launch_int8_rows(g2, s)) return rc;
+    }
+    return launch_int8_reduce(m.y, l.tw, l.ids, l.emap, l.n_global, l.E, l.T, l.H, l.top_k, l.out, l.bf16, s);
 }
 struct SizeProbe {
     WorkspaceSize s;
@@ -110,7 +189,7 @@ int w4a8_act_quant_int8(const void* x, int x_dtype, int64_t rows, int64_t K, int
 }
 
 size_t w4a8_int8_gemm_workspace_size(int x_dtype, int64_t M, int64_t K) {
-    if (x_dtype == W4A8_DTYPE_INT8 || M <= 0 || K <= 0) return 0;
+    if (x_dtype == W4A8_DTYPE_INT8 || M <= 0 || K <= 0 || (M <= kStreamRows && int8_rows_quantised_in_kernel(K))) return 0;
     WorkspaceSize s;
     s.take<int8_t>((size_t)(M * K));
     s.take<float>((size_t)M);
@@ -126,12 +205,9 @@ int w4a8_int8_gemm(const void* x, int x_dtype, const float* x_scales, int64_t M,
     if (M == 0) return W4A8_OK;
     W4A8_REQUIRE(out, "int8_gemm: null pointer");
     hipStream_t s = as_stream(stream);
-    Int8Args a{};
-    a.x = static_cast<const int8_t*>(x); a.xs = x_scales; a.x_rows = M; a.K = K; a.ldx = x_stride;
-    a.w = w; a.ws = w_scales; a.E = 1; a.N = N; a.bias = bias; a.bias_f32 = bias_is_f32 != 0;
-    a.P = M; a.top_k = 1; a.num_valid = M; a.block_m = 16;
-    a.dst = Out8::k16; a.bf16 = out_dtype == W4A8_DTYPE_BF16; a.out = out; a.ldo = N;
-    if (x_dtype != W4A8_DTYPE_INT8) {
+    const bool in_kernel = M <= kStreamRows && int8_rows_quantised_in_kernel(K);
+    Src8 src = src_of(x_dtype);
+    if (src != Src8::kI8 && !in_kernel) {
         Workspace ws(workspace, workspace_bytes);
         int8_t* xq = ws.take<int8_t>((size_t)(M * K));
         float* xs = ws.take<float>((size_t)M);
@@ -140,17 +216,26 @@ int w4a8_int8_gemm(const void* x, int x_dtype, const float* x_scales, int64_t M,
             return W4A8_ERR_WORKSPACE;
         }
         if (int rc = launch_act_quant_int8(x, rows_of(x_dtype), M, K, x_stride, false, xq, xs, nullptr, nullptr, 0, s)) return rc;
-        a.x = xq; a.xs = xs; a.ldx = K;
+        x = xq; x_scales = xs; x_stride = K; src = Src8::kI8;
     }
+    Int8Args a{};
+    a.x = static_cast<const int8_t*>(x); a.xs = x_scales; a.x_rows = M; a.K = K; a.ldx = x_stride;
+    a.w = w; a.ws = w_scales; a.E = 1; a.N = N; a.bias = bias; a.bias_f32 = bias_is_f32 != 0;
+    a.P = M; a.top_k = 1; a.num_valid = M; a.block_m = 16;
+    a.dst = Out8::k16; a.bf16 = out_dtype == W4A8_DTYPE_BF16; a.out = out; a.ldo = N;
     if (M > kStreamRows && int8_tiles_supported(a)) return launch_int8_tiles(a, s);
-    return launch_int8_stream(a, s);
+    RowsArgs r{};
+    r.x = x; r.src = src; r.xs = x_scales; r.rows = M; r.K = K; r.ldx = x_stride;
+    r.w = w; r.ws = w_scales; r.E = 1; r.N = N; r.bias = bias; r.bias_f32 = a.bias_f32; r.top_k = 1;
+    r.dst = Out8::k16; r.bf16 = a.bf16; r.out = out; r.ldo = N;
+    return launch_int8_rows(r, s);
 }
 
 size_t w4a8_moe_int8_workspace_size(int64_t T, int64_t H, int64_t inter, int64_t E, int64_t top_k) {
     if (T <= 0 || H <= 0 || inter <= 0 || E <= 0 || top_k <= 0) return 0;
     SizeProbe p;
     LayerScratch m;
-    carve_layer(p, plan_layer(T, H, inter, E, top_k), T, H, inter, E, top_k, m);
+    carve_layer(p, plan_layer(T, H, inter, E, top_k, W4A8_DTYPE_F16), H, inter, E, top_k, m);
     return p.s.used;
 }
 
@@ -173,39 +258,23 @@ int w4a8_moe_int8_apply(const void* x, int x_dtype, const float* x_scales, int64
     if (T == 0) return W4A8_OK;
     W4A8_REQUIRE(w2 && w2_scales && topk_weights && topk_ids && out, "moe_int8_apply: null pointer");
     W4A8_REQUIRE(aligned16(w2) && aligned16(out), "moe_int8_apply: w2 and out must be aligned to 16 bytes");
-    const LayerPlan pl = plan_layer(T, H, inter, E, top_k);
-    W4A8_REQUIRE(pl.P <= kMaxRows, "moe_int8_apply: too many slots");
+    const LayerPlan pl = plan_layer(T, H, inter, E, top_k, x_dtype);
     Workspace w(workspace, workspace_bytes);
     LayerScratch m;
-    carve_layer(w, pl, T, H, inter, E, top_k, m);
-    if (workspace == nullptr || !w.ok()) {
+    carve_layer(w, pl, H, inter, E, top_k, m);
+    if (workspace == nullptr || workspace_bytes < w4a8_moe_int8_workspace_size(T, H, inter, E, top_k)) {
         set_error("moe_int8_apply: workspace smaller than w4a8_moe_int8_workspace_size()");
         return W4A8_ERR_WORKSPACE;
     }
-    hipStream_t s = as_stream(stream);
-    if (int rc = launch_align(topk_ids, T * top_k, E, pl.block_m, expert_map, n_global, m.sti, pl.P, m.eid, m.ntp, m.align_ws,
-                              m.align_bytes, s))
-        return rc;
-    Int8Args g1{};
-    g1.x = static_cast<const int8_t*>(x); g1.xs = x_scales;
-    if (x_dtype != W4A8_DTYPE_INT8) {
-        if (int rc = launch_act_quant_int8(x, rows_of(x_dtype), T, H, H, false, m.xq, m.xs, nullptr, nullptr, 0, s)) return rc;
-        g1.x = m.xq; g1.xs = m.xs;
+    const int64_t xbytes = x_dtype == W4A8_DTYPE_INT8 ? 1 : 2;
+    for (int64_t t = 0; t < T; t += pl.part) {
+        const Layer l{static_cast<const char*>(x) + t * H * xbytes, x_dtype, x_scales == nullptr ? nullptr : x_scales + t,
+                      std::min(pl.part, T - t), H, inter, E, top_k, w13, w13_scales, w2, w2_scales,
+                      topk_weights + t * top_k, topk_ids + t * top_k, expert_map, n_global,
+                      static_cast<uint16_t*>(out) + t * H, out_dtype == W4A8_DTYPE_BF16};
+        if (int rc = run_layer(l, pl, m, as_stream(stream))) return rc;
     }
-    g1.x_rows = T; g1.K = H; g1.ldx = H;
-    g1.w = w13; g1.ws = w13_scales; g1.E = E; g1.N = 2 * inter;
-    g1.sorted_ids = m.sti; g1.expert_ids = m.eid; g1.ntp = m.ntp; g1.P = pl.P;
-    g1.top_k = top_k; g1.num_valid = T * top_k; g1.block_m = pl.block_m; g1.gather = true;
-    g1.dst = Out8::kSiluF32; g1.out = m.h; g1.ldo = inter;
-    if (int rc = pl.tiles ? launch_int8_tiles(g1, s) : launch_int8_stream(g1, s)) return rc;
-    if (int rc = launch_act_quant_int8(m.h, Rows::kF32, pl.P, inter, inter, false, m.hq, m.hs, m.sti, m.ntp, T * top_k, s)) return rc;
-    Int8Args g2 = g1;
-    g2.x = m.hq; g2.xs = m.hs; g2.x_rows = pl.P; g2.K = inter; g2.ldx = inter;
-    g2.w = w2; g2.ws = w2_scales; g2.N = H; g2.gather = false;
-    g2.dst = Out8::kSlotF32; g2.out = m.y; g2.ldo = H;
-    if (int rc = pl.tiles ? launch_int8_tiles(g2, s) : launch_int8_stream(g2, s)) return rc;
-    return launch_int8_reduce(m.y, topk_weights, topk_ids, expert_map, n_global, E, T, H, top_k, out,
-                              out_dtype == W4A8_DTYPE_BF16, s);
+    return W4A8_OK;
 }
 
 }  // extern "C"

@@ -1,0 +1,459 @@
+// int8 products of few rows (gfx950): the weights are streamed once, dense or grouped by expert.
+//
+// Bound: HBM, every weight once per 16 rows. Weights go from memory to the MFMA operands' registers with no
+// detour: of each step of 128 values, lane (q, c) = (lane / 16, lane % 16) holds the 16-byte pieces q and q + 4 of
+// row c, for rows and weights alike (a sum of whole numbers may take its k in any order). Weights are the first
+// operand: a lane ends up with four adjacent columns of one row.
+//
+// Grouped, a work-group finds its rows itself: it scans the routed ids for the slots of its expert (or, of few slots,
+// takes one slot), so that no launch has to sort them first.
+//
+// int8_rows_kernel holds its rows in registers (16 rows by GPW steps a wave, quantised there where they come in 16 or 32
+// bits) and walks over column fragments with D of them in flight; KS waves share K and add their sums in LDS.
+// int8_stream_kernel takes any K and reads int8 rows again for each column fragment.
+#include <algorithm>
+#include <type_traits>
+
+#include "int8.h"
+
+namespace w4a8 {
+namespace {
+
+// ---- a work-group's rows ----
+struct Routed {
+    int e;            // expert
+    int n;            // its rows
+};
+// The expert of slot i (an id of no local expert: -1).
+__device__ __forceinline__ int expert_of(const RowsParams& p, int i) {
+    int e = p.ids[i];
+    if (p.emap != nullptr) e = e >= 0 && e < p.emap_len ? p.emap[e] : -1;
+    return e >= 0 && e < p.E ? e : -1;
+}
+// Group g of rows: dense, all of them; with `single`, slot g; else the slots of expert g, in order, in `list`.
+// WAVES: of the work-group, all of which call this.
+template <int WAVES>
+__device__ __forceinline__ Routed find_rows(const RowsParams& p, int g, uint16_t* list, int* counts) {
+    if (p.ids == nullptr) return {0, p.rows};
+    if (p.single) {
+        const int e = expert_of(p, g);
+        return {e, e >= 0 ? 1 : 0};
+    }
+    constexpr int kMost = kScanSlots / (64 * WAVES);             // slots a lane
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int per = (p.slots + 64 * WAVES - 1) / (64 * WAVES);   // steps of 64 slots a wave
+    const int first = wave * per * 64 + lane;
+    uint32_t mine = 0;                                           // bit i: slot first + 64 i
+#pragma unroll 4
+    for (int i = 0; i < kMost; ++i) {
+        if (i >= per) break;
+        const int s = first + 64 * i;
+        if (s < p.slots && expert_of(p, s) == g) mine |= 1u << i;
+    }
+    int before = 0;
+    for (int i = 0; i < per; ++i) before += __popcll(__ballot(mine >> i & 1));
+    if (lane == 0) counts[wave] = before;
+    __syncthreads();
+    int at = 0, n = 0;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) {
+        if (w < wave) at += counts[w];
+        n += counts[w];
+    }
+    if (n == 0) return {g, 0};
+    for (int i = 0; i < per; ++i) {
+        const uint64_t m = __ballot(mine >> i & 1);
+        if (mine >> i & 1) list[at + __popcll(m & ((1ull << lane) - 1))] = (uint16_t)(first + 64 * i);
+        at += __popcll(m);
+    }
+    __syncthreads();
+    return {g, n};
+}
+// Row r of the group: its slot (dense: r), -1 past the end.
+__device__ __forceinline__ int slot_at(const RowsParams& p, const Routed& d, int g, int r, const uint16_t* list) {
+    if (r >= d.n) return -1;
+    return p.ids == nullptr ? r : p.single ? g : list[r];
+}
+
+// ---- rows' values ----
+template <Src8 SRC>
+constexpr int kSrcBytes = SRC == Src8::kI8 ? 1 : SRC == Src8::kF32 ? 4 : 2;
+template <Src8 SRC>
+struct RawStep {                                                 // a lane's 32 values of one step
+    u32x4 v[2 * kSrcBytes<SRC>];
+    __device__ __forceinline__ void load(const uint8_t* row, int g, int q, int K) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int k = min(g * kStep + h * 64 + q * 16, K - 16);
+#pragma unroll
+            for (int b = 0; b < kSrcBytes<SRC>; ++b)
+                v[h * kSrcBytes<SRC> + b] = *reinterpret_cast<const u32x4*>(row + (int64_t)k * kSrcBytes<SRC> + 16 * b);
+        }
+    }
+    __device__ __forceinline__ float value(int h, int t) const {
+        if constexpr (SRC == Src8::kF32) return __uint_as_float(v[h * 4 + t / 4][t % 4]);
+        const uint32_t u = v[h * 2 + t / 8][(t / 2) % 4];
+        if constexpr (SRC == Src8::kBf16) return __uint_as_float((t & 1) ? u & 0xFFFF0000u : u << 16);
+        return __half2float(__ushort_as_half((uint16_t)((t & 1) ? u >> 16 : u & 0xFFFF)));
+    }
+    // (what the clamped addresses past the end hold counts for no maximum, and its quotients are cleared)
+    __device__ __forceinline__ uint32_t top() const {
+        uint32_t m = 0;
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int t = 0; t < 16; ++t) m = max(m, abs_bits(value(h, t)));
+        return m;
+    }
+};
+
+__device__ __forceinline__ uint32_t rows4_umax(uint32_t v) {    // over the four lanes that hold a row's values
+    const auto a = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    v = max(a[0], a[1]);
+    const auto b = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    return max(b[0], b[1]);
+}
+
+// CG groups of KS waves; a group walks over its own `per` column fragments (kSiluF32: fragments of the gate half, each
+// with its up fragment), D in flight.
+template <int GPW, int KS, int CG, int D, Src8 SRC, Out8 DST>
+__global__ void __launch_bounds__(64 * KS * CG, KS * CG <= 4 ? 2 : 1) int8_rows_kernel(RowsParams p, int slices, int per) {
+    constexpr bool kSilu = DST == Out8::kSiluF32;
+    constexpr int kPair = kSilu ? 2 : 1;                         // fragments of one output fragment
+    static_assert(D % kPair == 0, "an output fragment's parts are in flight together");
+    constexpr int kUnits = D / kPair;                            // output fragments of one round
+    constexpr int kWaves = KS * CG;
+    __shared__ __attribute__((aligned(16))) v4i part[KS > 1 ? 2 : 1][KS > 1 ? CG : 1][KS > 1 ? D : 1][KS > 1 ? KS : 1][64];
+    __shared__ uint16_t list[kScanSlots];
+    __shared__ int counts[kWaves];
+    __shared__ uint32_t s_top[KS > 1 ? kWaves : 1][16];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int ks = wave % KS, cg = wave / KS;
+    const int q = lane >> 4, c = lane & 15;
+    const int group = blockIdx.x / slices, sl = blockIdx.x % slices;
+    const Routed rt = find_rows<kWaves>(p, group, list, counts);
+    if (rt.n == 0) return;
+    const int half = p.N / 2;
+    const int cols = kSilu ? half : p.N;
+    const int K = p.K, G = (K + kStep - 1) / kStep;
+    const int frags = (cols + 15) / 16;
+    const int f0 = (sl * CG + cg) * per;                         // first output fragment of this group
+    const int g0 = ks * GPW;                                     // first step of this wave
+    const int8_t* we = p.w + (int64_t)rt.e * p.N * K;
+    const float* wse = p.ws + (int64_t)rt.e * p.N;
+
+    // ---- weights: step i is fragment f0 + i / kPair of the gate (i even) or the up half ----
+    struct Stage {
+        u32x4 w[GPW][2];
+    };
+    auto load = [&](Stage& s, int i) __attribute__((always_inline)) {
+        const int f = min(f0 + min(i / kPair, per - 1), frags - 1);
+        const int up = kSilu && (i & 1) ? half : 0;
+        // (columns past the end read the last one; never stored)
+        const int8_t* wr = we + (int64_t)(up + min(f * 16 + c, cols - 1)) * K;
+#pragma unroll
+        for (int j = 0; j < GPW; ++j)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int k = min(min(g0 + j, G - 1) * kStep + h * 64 + q * 16, K - 16);
+                s.w[j][h] = *reinterpret_cast<const u32x4*>(wr + k);
+            }
+    };
+    Stage ring[D];
+#pragma unroll
+    for (int d = 0; d < D; ++d) load(ring[d], d);
+    __builtin_amdgcn_sched_barrier(0);
+
+    const int mine = min(per, frags - f0);                       // output fragments of this group (may be <= 0)
+    const int rounds = (per * kPair + D - 1) / D;                // of the work-group: the barriers agree
+    for (int r0 = 0; r0 < rt.n; r0 += 16) {
+        // ---- sixteen rows, held ----
+        const int slot = slot_at(p, rt, group, r0 + c, list);
+        const int row = slot < 0 ? slot_at(p, rt, group, r0, list) : slot;   // (a row that exists; never stored)
+        const int xrow = p.gather ? row / p.top_k : row;
+        const uint8_t* xp = reinterpret_cast<const uint8_t*>(p.x) + (int64_t)xrow * p.ldx * kSrcBytes<SRC>;
+        u32x4 x[GPW][2];
+        float xs;
+        if constexpr (SRC == Src8::kI8) {
+            xs = p.xs[xrow];
+#pragma unroll
+            for (int j = 0; j < GPW; ++j) {
+                RawStep<SRC> raw;
+                raw.load(xp, min(g0 + j, G - 1), q, K);
+                x[j][0] = raw.v[0];
+                x[j][1] = raw.v[1];
+            }
+        } else {
+            RawStep<SRC> raw[GPW];
+#pragma unroll
+            for (int j = 0; j < GPW; ++j) raw[j].load(xp, min(g0 + j, G - 1), q, K);
+            uint32_t top = 0;
+#pragma unroll
+            for (int j = 0; j < GPW; ++j) top = max(top, raw[j].top());
+            top = rows4_umax(top);
+            if constexpr (KS > 1) {
+                if (r0 > 0) __syncthreads();                     // (the last rows' maxima have been read)
+                if (q == 0) s_top[wave][c] = top;
+                lds_barrier();
+#pragma unroll
+                for (int w = 0; w < KS; ++w) top = max(top, s_top[cg * KS + w][c]);
+            }
+            const RowScale r = row_scale(top);
+            xs = r.s;
+#pragma unroll
+            for (int j = 0; j < GPW; ++j)
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int d = 0; d < 4; ++d)
+                        x[j][h][d] = quant4(raw[j].value(h, 4 * d), raw[j].value(h, 4 * d + 1), raw[j].value(h, 4 * d + 2),
+                                            raw[j].value(h, 4 * d + 3), r);
+        }
+        // (what the clamped addresses hold counts in its own place)
+#pragma unroll
+        for (int j = 0; j < GPW; ++j)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+                if ((g0 + j) * kStep + h * 64 + q * 16 >= K) x[j][h] = u32x4{0, 0, 0, 0};
+        __builtin_amdgcn_sched_barrier(0);
+
+        for (int it = 0; it < rounds; ++it) {
+            v4i run[D];
+#pragma unroll
+            for (int d = 0; d < D; ++d) {
+                run[d] = v4i{0, 0, 0, 0};
+#pragma unroll
+                for (int j = 0; j < GPW; ++j)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) run[d] = mfma_i8(ring[d].w[j][h], x[j][h], run[d]);
+                __builtin_amdgcn_sched_barrier(0);
+                // (behind the last round: the first fragments again, for the next sixteen rows)
+                const int next = (it + 1) * D + d;
+                load(ring[d], it + 1 < rounds ? next : d);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            // unit u of the round: an output fragment
+            auto put = [&](int u, const v4i& a, const v4i& b) __attribute__((always_inline)) {
+                const int of = it * kUnits + u;
+                const int col = (f0 + of) * 16 + 4 * q;
+                if (of >= mine || slot < 0 || col >= cols) return;
+                v4f t;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int n = min(col + r, cols - 1);
+                    const float f = xs * wse[n];
+                    if constexpr (kSilu) t[r] = silu_mul((float)a[r] * f, (float)b[r] * (xs * wse[half + n]));
+                    else if constexpr (DST == Out8::k16) t[r] = fmaf((float)a[r], f, bias_at(p, n));
+                    else t[r] = (float)a[r] * f;
+                }
+                if constexpr (DST == Out8::k16) store16(p, slot, col, t);
+                else *reinterpret_cast<v4f*>(reinterpret_cast<float*>(p.out) + (int64_t)slot * p.ldo + col) = t;
+            };
+            if constexpr (KS == 1) {
+#pragma unroll
+                for (int u = 0; u < kUnits; ++u) put(u, run[u * kPair], run[u * kPair + kPair - 1]);
+            } else {
+                auto& buf = part[it & 1][cg];
+#pragma unroll
+                for (int d = 0; d < D; ++d) buf[d][ks][lane] = run[d];
+                lds_barrier();
+                // (the next round writes the other buffer; this one is written again behind its barrier)
+#pragma unroll
+                for (int u0 = 0; u0 < kUnits; u0 += KS) {
+                    const int u = u0 + ks;
+                    if (kUnits % KS != 0 && u >= kUnits) break;
+                    auto total = [&](int d) __attribute__((always_inline)) {
+                        v4i t = buf[d][0][lane];
+#pragma unroll
+                        for (int w = 1; w < KS; ++w) t += buf[d][w][lane];
+                        return t;
+                    };
+                    const v4i t = total(u * kPair);
+                    if constexpr (kSilu) put(u, t, total(u * kPair + 1));
+                    else put(u, t, t);
+                }
+            }
+        }
+        if (KS > 1) lds_barrier();                               // (an odd number of rounds: the first buffer is read)
+    }
+}
+
+// Any K, int8 rows: KS waves take the steps of K in turn (what they read at one time is contiguous along K).
+constexpr int kRing = 3;          // steps of a wave in flight
+template <int FN, int KS, Out8 DST>
+__global__ void __launch_bounds__(64 * KS) int8_stream_kernel(RowsParams p, int slices) {
+    constexpr bool kSilu = DST == Out8::kSiluF32;
+    constexpr int kCols = kSilu ? FN / 2 : FN;                   // column fragments of the output
+    __shared__ __attribute__((aligned(16))) v4i part[KS][FN][64];
+    __shared__ uint16_t list[kScanSlots];
+    __shared__ int counts[KS];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int q = lane >> 4, c = lane & 15;
+    const int group = blockIdx.x / slices, sl = blockIdx.x % slices;
+    const Routed rt = find_rows<KS>(p, group, list, counts);
+    if (rt.n == 0) return;
+    const int half = p.N / 2;
+    const int cols = kSilu ? half : p.N;
+    const int K = p.K;
+    const int8_t* wp[FN];
+#pragma unroll
+    for (int j = 0; j < FN; ++j) {
+        const int f = (sl * kCols + j % kCols) * 16, up = kSilu && j >= kCols ? half : 0;
+        wp[j] = p.w + ((int64_t)rt.e * p.N + up + min(f + c, cols - 1)) * K;
+    }
+    const float* ws = p.ws + (int64_t)rt.e * p.N;
+    const int G = (K + kStep - 1) / kStep, steps = (G + KS - 1) / KS;
+    for (int r0 = 0; r0 < rt.n; r0 += 16) {
+        const int slot = slot_at(p, rt, group, r0 + c, list);
+        const int row = slot < 0 ? slot_at(p, rt, group, r0, list) : slot;
+        const int xrow = p.gather ? row / p.top_k : row;
+        const int8_t* xp = reinterpret_cast<const int8_t*>(p.x) + (int64_t)xrow * p.ldx;
+        struct Stage {
+            u32x4 w[FN][2], x[2];
+        };
+        auto load = [&](Stage& s, int step) __attribute__((always_inline)) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                // (pieces past the end: the last one, and zeros for the rows')
+                const int k = (step * KS + wave) * kStep + h * 64 + q * 16, at = min(k, K - 16);
+#pragma unroll
+                for (int j = 0; j < FN; ++j) s.w[j][h] = *reinterpret_cast<const u32x4*>(wp[j] + at);
+                s.x[h] = *reinterpret_cast<const u32x4*>(xp + at);
+                if (k >= K) s.x[h] = u32x4{0, 0, 0, 0};
+            }
+        };
+        v4i run[FN];
+#pragma unroll
+        for (int j = 0; j < FN; ++j) run[j] = v4i{0, 0, 0, 0};
+        Stage ring[kRing];
+#pragma unroll
+        for (int d = 0; d < kRing; ++d) load(ring[d], d);
+        for (int s0 = 0; s0 < steps; s0 += kRing) {
+#pragma unroll
+            for (int d = 0; d < kRing; ++d) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int j = 0; j < FN; ++j) run[j] = mfma_i8(ring[d].w[j][h], ring[d].x[h], run[j]);
+                __builtin_amdgcn_sched_barrier(0);
+                load(ring[d], s0 + d + kRing);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+        if (r0 > 0) __syncthreads();                             // (the last rows' sums have been read)
+#pragma unroll
+        for (int j = 0; j < FN; ++j) part[wave][j][lane] = run[j];
+        __syncthreads();
+        // wave j joins column fragment j (four adjacent columns of a row a lane)
+        static_assert(kCols <= KS, "a wave a fragment");
+        const int col = (sl * kCols + wave) * 16 + 4 * q;
+        if (wave >= kCols || slot < 0 || col >= cols) continue;
+        auto total = [&](int f) __attribute__((always_inline)) {
+            v4i t = part[0][f][lane];
+#pragma unroll
+            for (int w = 1; w < KS; ++w) t += part[w][f][lane];
+            return t;
+        };
+        const v4i a = total(wave), b = kSilu ? total(kCols + wave) : a;
+        const float xs = p.xs[xrow];
+        v4f t;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int n = min(col + r, cols - 1);
+            const float f = xs * ws[n];
+            if constexpr (kSilu) t[r] = silu_mul((float)a[r] * f, (float)b[r] * (xs * ws[half + n]));
+            else if constexpr (DST == Out8::k16) t[r] = fmaf((float)a[r], f, bias_at(p, n));
+            else t[r] = (float)a[r] * f;
+        }
+        if constexpr (DST == Out8::k16) store16(p, slot, col, t);
+        else *reinterpret_cast<v4f*>(reinterpret_cast<float*>(p.out) + (int64_t)slot * p.ldo + col) = t;
+    }
+}
+
+int too_many() {
+    set_error("int8 product: too many tiles");
+    return W4A8_ERR_INVALID;
+}
+// Groups of rows that work-groups take, and how many of them hold rows.
+int64_t groups_of(const RowsParams& p) { return p.ids == nullptr ? 1 : p.single ? p.slots : p.E; }
+int64_t busy_of(const RowsParams& p) { return p.ids == nullptr ? 1 : std::min(p.slots, p.E); }
+
+template <int FN, int KS, Out8 DST>
+int stream_go(const RowsParams& p, hipStream_t s) {
+    constexpr bool silu = DST == Out8::kSiluF32;
+    const int cols = silu ? p.N / 2 : p.N, per = 16 * (silu ? FN / 2 : FN);
+    const int slices = (cols + per - 1) / per;
+    const int64_t grid = groups_of(p) * slices;
+    if (!grid_fits(grid, 64 * KS)) return too_many();
+    launch_kernel(&int8_stream_kernel<FN, KS, DST>, dim3((unsigned)grid), dim3(64 * KS), 0, s, p, slices);
+    return check_launch("int8_stream_kernel");
+}
+
+// per: output fragments a group of waves walks over. The kernel loads D fragments beforehand whatever `per` is, so few of
+// them take a variant with a smaller D.
+template <int GPW, int KS, int CG, int D, Src8 SRC, Out8 DST>
+int rows_launch(const RowsParams& p, int frags, int64_t per, hipStream_t s) {
+    constexpr int pair = DST == Out8::kSiluF32 ? 2 : 1;
+    if constexpr (D > pair)
+        if (per * pair <= D / 2) return rows_launch<GPW, KS, CG, D / 2, SRC, DST>(p, frags, per, s);
+    const int slices = (int)((frags + per * CG - 1) / (per * CG));
+    const int64_t grid = groups_of(p) * slices;
+    if (!grid_fits(grid, 64 * KS * CG)) return too_many();
+    launch_kernel(&int8_rows_kernel<GPW, KS, CG, D, SRC, DST>, dim3((unsigned)grid), dim3(64 * KS * CG), 0, s, p, slices, (int)per);
+    return check_launch("int8_rows_kernel");
+}
+
+template <int GPW, int KS, int CG, int D, Src8 SRC, Out8 DST>
+int rows_go(const RowsParams& p, hipStream_t s) {
+    constexpr int unit = D / (DST == Out8::kSiluF32 ? 2 : 1);
+    const int frags = ((DST == Out8::kSiluF32 ? p.N / 2 : p.N) + 15) / 16;
+    // One round of work-groups (eight waves a CU), each walking over what that leaves it, up to eight rings' worth.
+    const int64_t groups = (int64_t)device_cu_count() * std::max(1, 8 / (KS * CG)) * CG;
+    int64_t per = (busy_of(p) * frags + groups - 1) / groups;
+    if (per > unit) per = std::min<int64_t>((per + unit - 1) / unit, 8) * unit;
+    return rows_launch<GPW, KS, CG, D, SRC, DST>(p, frags, std::max<int64_t>(1, per), s);
+}
+
+// The wave split by the number of steps: a wave holds the rows' values of up to four of them, up to eight waves share K.
+template <Src8 SRC, Out8 DST>
+int rows_any(const RowsParams& p, hipStream_t s) {
+    const int G = (p.K + kStep - 1) / kStep;
+    if (G <= 1) return rows_go<1, 1, 4, 4, SRC, DST>(p, s);
+    if (G <= 2) return rows_go<2, 1, 4, 4, SRC, DST>(p, s);
+    if (G <= 4) return rows_go<4, 1, 4, 2, SRC, DST>(p, s);
+    if (G <= 8) return rows_go<2, 4, 1, 4, SRC, DST>(p, s);
+    if (G <= 16) return rows_go<4, 4, 1, 2, SRC, DST>(p, s);
+    if (G <= 32) return rows_go<4, 8, 1, 2, SRC, DST>(p, s);
+    if constexpr (SRC == Src8::kI8) return stream_go<DST == Out8::kSiluF32 ? 2 : 1, 8, DST>(p, s);
+    set_error("int8 product: rows too long to be quantised in the kernel");
+    return W4A8_ERR_INVALID;
+}
+
+}  // namespace
+
+bool int8_rows_quantised_in_kernel(int64_t K) { return K <= 32 * kStep; }
+
+int launch_int8_rows(const RowsArgs& a, hipStream_t s) {
+    const RowsParams p = rows_params(a);
+    if (p.rows == 0 || (p.ids != nullptr && p.slots == 0)) return W4A8_OK;
+    if (p.ids != nullptr && p.slots > kScanSlots) {
+        set_error("int8 product: too many slots for the streaming kernels");
+        return W4A8_ERR_INVALID;
+    }
+    if (a.dst == Out8::kSlotF32) return a.src == Src8::kI8 ? rows_any<Src8::kI8, Out8::kSlotF32>(p, s) : rows_any<Src8::kF32, Out8::kSlotF32>(p, s);
+    auto from = [&](auto dst) -> int {
+        constexpr Out8 DST = decltype(dst)::value;
+        switch (a.src) {
+            case Src8::kI8: return rows_any<Src8::kI8, DST>(p, s);
+            case Src8::kF16: return rows_any<Src8::kF16, DST>(p, s);
+            case Src8::kBf16: return rows_any<Src8::kBf16, DST>(p, s);
+            default: break;
+        }
+        set_error("int8 product: fp32 rows are the layer's second product's");
+        return W4A8_ERR_INVALID;
+    };
+    if (a.dst == Out8::kSiluF32) return from(std::integral_constant<Out8, Out8::kSiluF32>{});
+    return from(std::integral_constant<Out8, Out8::k16>{});
+}
+
+}  // namespace w4a8
