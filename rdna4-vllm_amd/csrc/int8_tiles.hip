@@ -8,6 +8,7 @@
 // Work-groups are persistent: a tile's ids are read under the one before, its first steps are loaded under the one
 // before's epilogue.
 #include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 #include "int8.h"
@@ -42,9 +43,11 @@ __device__ __forceinline__ v16i mfma_i8_32(const u32x4& a, const u32x4& b, const
 }
 
 // WT x WN waves of FT row fragments x FN column fragments of 32, S steps in LDS; KS such parts of a work-group share
-// K, each with slots of its own, and add their sums at the end. EU: waves a SIMD.
-template <int WT_, int WN_, int FT_, int FN_, int S_, int KS_, int EU_>
+// K, each with slots of its own, and add their sums at the end. EU: waves a SIMD. DEEP: a step's fragments are read
+// during the step before (small wave tiles, whose MFMAs of a quarter step take less than an LDS read).
+template <int WT_, int WN_, int FT_, int FN_, int S_, int KS_, int EU_, bool DEEP_ = false>
 struct Tile {
+    static constexpr bool DEEP = DEEP_;
     static constexpr int WT = WT_, WN = WN_, FT = FT_, FN = FN_, S = S_, KS = KS_, EU = EU_;
     static constexpr int kWaves = WT * WN, kThreads = 64 * kWaves;   // of a part
     static constexpr int BT = WT * FT * 32, BN = WN * FN * 32;
@@ -54,7 +57,7 @@ struct Tile {
     static constexpr int kLoads = PX + PW;                       // of a wave and step
     static_assert(PX * kThreads == BT * 8 && PW * kThreads == BN * 8, "pieces divide");
     static_assert(kThreads % 128 == 0, "a thread's pieces are the same one of their rows");
-    static_assert(S == 2 || S == 3, "two or three slots");
+    static_assert(S >= 2 && S <= 6 && (!DEEP || S % 2 == 0), "two to six slots, for two sets of fragments in turn");
     static_assert(kLoads * (S - 1) < 64, "loads in flight can be counted");
 };
 
@@ -66,7 +69,10 @@ __global__ void __launch_bounds__(C::kThreads * C::KS, C::EU) int8_tiles_kernel(
     // arrays of their own: the compiler then sees that reads of one do not wait for loads into another
     __shared__ __attribute__((aligned(1024))) int8_t slots0[KS * C::kSlot];
     __shared__ __attribute__((aligned(1024))) int8_t slots1[KS * C::kSlot];
-    __shared__ __attribute__((aligned(1024))) int8_t slots2[S == 3 ? KS * C::kSlot : 16];
+    __shared__ __attribute__((aligned(1024))) int8_t slots2[S > 2 ? KS * C::kSlot : 16];
+    __shared__ __attribute__((aligned(1024))) int8_t slots3[S > 3 ? KS * C::kSlot : 16];
+    __shared__ __attribute__((aligned(1024))) int8_t slots4[S > 4 ? KS * C::kSlot : 16];
+    __shared__ __attribute__((aligned(1024))) int8_t slots5[S > 5 ? KS * C::kSlot : 16];
     // Tables for the epilogue, in slot 1 between a tile's last step and the next one's second.
     float *const s_xs = reinterpret_cast<float*>(slots1), *const s_ws = s_xs + BT, *const s_bias = s_ws + BN;
     int* const s_slot = reinterpret_cast<int*>(s_bias + BN);
@@ -88,8 +94,11 @@ __global__ void __launch_bounds__(C::kThreads * C::KS, C::EU) int8_tiles_kernel(
     const int wt = wave / C::WN, wn = wave % C::WN;
     const int K = p.K, N = p.N, G = (K + kStep - 1) / kStep;
     const int G1 = (G + KS - 1) / KS, g_first = part * G1;       // steps of a part, the first of them
-    int8_t *const slot0 = slots0 + part * C::kSlot, *const slot1 = slots1 + part * C::kSlot;
-    int8_t* const slot2 = S == 3 ? slots2 + part * C::kSlot : slots0;
+    auto slot_of = [&](auto i) __attribute__((always_inline)) {      // slot i % S
+        constexpr int n = decltype(i)::value % S;
+        int8_t* const all = n == 0 ? slots0 : n == 1 ? slots1 : n == 2 ? slots2 : n == 3 ? slots3 : n == 4 ? slots4 : slots5;
+        return all + part * C::kSlot;
+    };
 
     // Piece i of a thread is the slot's piece tid + i kThreads: place / 8 and piece % 8. Row r lies at place
     // r ^ ((r >> 3) & 1), its piece j at j ^ (r & 7): the sixteen lanes that a 16-byte LDS read serves at once then read
@@ -201,51 +210,75 @@ __global__ void __launch_bounds__(C::kThreads * C::KS, C::EU) int8_tiles_kernel(
 
     // ---- fragments: lane (h, c) reads piece 2 s + h of row c of each 32, sub-step s of four ----
     const int at0 = (c ^ ((c >> 3) & 1)) * kStep + ((h ^ (c & 7)) << 4);
-    u32x4 xf[2][FT], wf[2][FN];
-    auto frags = [&](const int8_t* slot, int s) __attribute__((always_inline)) {
+    constexpr bool DEEP = C::DEEP;
+    constexpr int kSets = DEEP ? 8 : 2;                          // sub-steps in registers
+    u32x4 xf[kSets][FT], wf[kSets][FN];
+    auto frags = [&](const int8_t* slot, int s, int set) __attribute__((always_inline)) {
         const int8_t* b = slot + (at0 ^ (s << 5));
 #pragma unroll
-        for (int j = 0; j < FN; ++j) wf[s & 1][j] = *reinterpret_cast<const u32x4*>(b + C::kW + (wn * FN + j) * 32 * kStep);
+        for (int j = 0; j < FN; ++j) wf[set][j] = *reinterpret_cast<const u32x4*>(b + C::kW + (wn * FN + j) * 32 * kStep);
 #pragma unroll
-        for (int i = 0; i < FT; ++i) xf[s & 1][i] = *reinterpret_cast<const u32x4*>(b + (wt * FT + i) * 32 * kStep);
+        for (int i = 0; i < FT; ++i) xf[set][i] = *reinterpret_cast<const u32x4*>(b + (wt * FT + i) * 32 * kStep);
     };
     v16i run[FT][FN];
-    auto multiply = [&](int s, int i0, int i1) __attribute__((always_inline)) {
+    auto multiply = [&](int set, int i0, int i1) __attribute__((always_inline)) {
 #pragma unroll
         for (int i = i0; i < i1; ++i)
 #pragma unroll
-            for (int j = 0; j < FN; ++j) run[i][j] = mfma_i8_32(wf[s & 1][j], xf[s & 1][i], run[i][j]);
+            for (int j = 0; j < FN; ++j) run[i][j] = mfma_i8_32(wf[set][j], xf[set][i], run[i][j]);
     };
-    // Step g from `slot`, whose first fragments are in registers. Before its last quarter the next step's stage has to
-    // have landed for all waves, and none reads `slot` any more: there the loads of step g + S go, among the last
-    // quarter's MFMAs, and the next step's first fragments are read. Loads are issued in every step, past the last one
-    // too, so that those in flight can be counted.
-    auto step = [&](int8_t* slot, const int8_t* next, int g) __attribute__((always_inline)) {
+    // Step g from `slot`. Loads are issued in every step, past the last one too, so that those in flight can be
+    // counted: the next step's stage has landed for this wave when those of S - 2 later ones are in flight, and for all
+    // waves behind the barrier, which also says that none reads `slot` any more. There the loads of step g + S go.
+    auto step = [&](int8_t* slot, const int8_t* next, int g, auto odd) __attribute__((always_inline)) {
+        if constexpr (DEEP) {
+            // its fragments are in registers
+            constexpr int now = decltype(odd)::value % 2 * 4, then = 4 - now;
+            __builtin_amdgcn_s_waitcnt(wait_vm(C::kLoads * (S - 2)));
+            group_barrier();
 #pragma unroll
-        for (int s = 0; s < 3; ++s) {
-            frags(slot, s + 1);
+            for (int s = 0; s < 4; ++s) frags(next, s, then + s);
             __builtin_amdgcn_sched_barrier(0);
-            multiply(s, 0, FT);
-            __builtin_amdgcn_sched_barrier(0);
-        }
-        __builtin_amdgcn_s_waitcnt(wait_vm(C::kLoads * (S - 2)));
-        group_barrier();
-        frags(next, 0);
-        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int i = 0; i < FT; ++i) {
-            issue(slot, g + S, i, FT);
-            multiply(3, i, i + 1);
+            for (int s = 0; s < 4; ++s) {
+                issue(slot, g + S, s, 4);
+                multiply(now + s, 0, FT);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        } else {
+            // its first quarter's fragments are in registers
+#pragma unroll
+            for (int s = 0; s < 3; ++s) {
+                frags(slot, s + 1, (s + 1) & 1);
+                __builtin_amdgcn_sched_barrier(0);
+                multiply(s & 1, 0, FT);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            __builtin_amdgcn_s_waitcnt(wait_vm(C::kLoads * (S - 2)));
+            group_barrier();
+            frags(next, 0, 0);
             __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int i = 0; i < FT; ++i) {
+                issue(slot, g + S, i, FT);
+                multiply(1, i, i + 1);
+                __builtin_amdgcn_sched_barrier(0);
+            }
         }
     };
 
     place_of(item, row0, ct);
     read_ids(row0);
     set_tile();
-    issue(slot0, 0, 0, 1);
-    issue(slot1, 1, 0, 1);
-    if (S == 3) issue(slot2, 2, 0, 1);
+    auto each_slot = [&](auto&& f) __attribute__((always_inline)) {
+        f(std::integral_constant<int, 0>{});
+        f(std::integral_constant<int, 1>{});
+        if constexpr (S > 2) f(std::integral_constant<int, 2>{});
+        if constexpr (S > 3) f(std::integral_constant<int, 3>{});
+        if constexpr (S > 4) f(std::integral_constant<int, 4>{});
+        if constexpr (S > 5) f(std::integral_constant<int, 5>{});
+    };
+    each_slot([&](auto i) __attribute__((always_inline)) { issue(slot_of(i), decltype(i)::value, 0, 1); });
     for (;;) {
         const int r0_now = row0, ct_now = ct, next_item = item + step_items;
         const bool more = next_item < last;
@@ -262,13 +295,14 @@ __global__ void __launch_bounds__(C::kThreads * C::KS, C::EU) int8_tiles_kernel(
                 for (int r = 0; r < 16; ++r) run[i][j][r] = 0;
         __builtin_amdgcn_s_waitcnt(wait_vm(0));
         group_barrier();
-        frags(slot0, 0);
+#pragma unroll
+        for (int s = 0; s < (DEEP ? 4 : 1); ++s) frags(slot_of(std::integral_constant<int, 0>{}), s, s);
         // (whole rounds of S steps: those past the last one multiply zeros)
-        for (int g = 0; g < G1; g += S) {
-            step(slot0, slot1, g);
-            step(slot1, S == 3 ? slot2 : slot0, g + 1);
-            if constexpr (S == 3) step(slot2, slot0, g + 2);
-        }
+        for (int g = 0; g < G1; g += S)
+            each_slot([&](auto i) __attribute__((always_inline)) {
+                constexpr int n = decltype(i)::value;
+                step(slot_of(i), slot_of(std::integral_constant<int, n + 1>{}), g + n, i);
+            });
         __builtin_amdgcn_s_waitcnt(wait_vm(0));                  // (the loads past the last step)
         group_barrier();                                         // nobody reads or loads a slot any more
         if constexpr (KS > 1) {
@@ -318,19 +352,21 @@ __global__ void __launch_bounds__(C::kThreads * C::KS, C::EU) int8_tiles_kernel(
             row0 = row0_next;
             ct = ct_next;
             set_tile();
-            issue(slot0, 0, 0, 1);
-            if (S == 3) issue(slot2, 2, 0, 1);
+            each_slot([&](auto i) __attribute__((always_inline)) {
+                if (decltype(i)::value != 1) issue(slot_of(i), decltype(i)::value, 0, 1);
+            });
         }
         lds_barrier();
         // A wave turns 32 rows at a time through LDS, so that its stores are whole lines: a row's values lie in
-        // chunks of 16 bytes, chunk i of row r at i ^ (r & 15) (rows of 256 bytes or more) or i ^ (r / 2 & 7) (of 128).
+        // chunks of 16 bytes, chunk i of row r at i ^ (r & 15) (rows of 256 bytes or more), i ^ (r / 2 & 7) (of 128) or
+        // i ^ (r / 4 & 3) (of 64): sixteen lanes then write to different banks.
         constexpr int kOutCols = (kSilu ? FN / 2 : FN) * 32, kSize = DST == Out8::k16 ? 2 : 4;
         constexpr int kRowBytes = kOutCols * kSize, kChunks = kRowBytes / 16;
-        static_assert(kChunks >= 8, "a row is 128 bytes or more");
+        static_assert(kChunks >= 4, "a row is 64 bytes or more");
         static_assert(KS * C::kSlot >= 4 * (2 * BT + 2 * BN) + C::kWaves * 32 * kRowBytes, "tables and rows fit");
         int8_t* const strip = slots1 + 4 * (2 * BT + 2 * BN) + wave * 32 * kRowBytes;
         auto chunk_at = [&](int row, int i) __attribute__((always_inline)) {
-            return row * kRowBytes + ((i ^ (kChunks >= 16 ? row & 15 : row >> 1 & 7)) << 4);
+            return row * kRowBytes + ((i ^ (kChunks >= 16 ? row & 15 : kChunks == 8 ? row >> 1 & 7 : row >> 2 & 3)) << 4);
         };
         const int col0 = kSilu ? ct_now * (BN / 2) + wn * kOutCols : ct_now * BN + wn * kOutCols;
         auto turn = [&](int i, auto bf16) __attribute__((always_inline)) {
@@ -400,7 +436,7 @@ __global__ void __launch_bounds__(C::kThreads * C::KS, C::EU) int8_tiles_kernel(
         if (!more) break;
         item = next_item;
         lds_barrier();                                           // nobody reads the tables any more
-        issue(slot1, 1, 0, 1);
+        issue(slot_of(std::integral_constant<int, 1>{}), 1, 0, 1);
     }
 }
 
@@ -425,11 +461,48 @@ int tiles_go(const Int8Params& p, hipStream_t s) {
     return check_launch("int8_tiles_kernel");
 }
 
-//                  WT WN FT FN S KS EU
-using Tile256x256 = Tile<2, 2, 4, 4, 2, 1, 1>;
-using Tile128x256 = Tile<2, 2, 2, 4, 3, 1, 1>;
-using Tile128x128 = Tile<2, 2, 2, 2, 2, 1, 2>;
-using Tile64x256 = Tile<1, 4, 2, 2, 2, 1, 2>;
+//                      WT WN FT FN S KS EU
+using Tile64x32K2 = Tile<2, 1, 1, 1, 4, 2, 1, true>;
+using Tile64x64 = Tile<2, 2, 1, 1, 4, 1, 2, true>;       // two work-groups a CU, the others one
+using Tile128x64 = Tile<4, 2, 1, 1, 4, 1, 2, true>;
+using Tile128x128 = Tile<2, 4, 2, 1, 4, 1, 2, true>;
+using Tile256x128 = Tile<4, 2, 2, 2, 3, 1, 2>;
+using Tile256x256 = Tile<2, 4, 4, 2, 2, 1, 2>;
+using Tile64x256 = Tile<1, 4, 2, 2, 2, 1, 2>;            // grouped; two a CU
+
+// The dense tile of least cost. us as measured at N = K = 4096 (the rule compares tiles at one K, as if all their costs
+// grew with it alike), by the tiles a CU has to take:
+//                            1/4   1/2   3/4     1   1.5     2     3     4
+//   64 x 32, K in two        8.3   8.4         14.7*
+//   64 x 64                  9.3   9.4  ...    10.0  14.8  15.6  21.8  28.5
+//   128 x 64                10.2  11.5  12.1   13.7  23.4  25.5  36.8  49.8
+//   128 x 128               15.0  15.8  18.1   21.2  35.3  40.7        79.2
+//   256 x 128               25.5  27.3  30.4   35.9        71.7       218 (6)
+//   256 x 256               42.9  44.5         59.0       190.7 (3)
+// (* two a CU do not run beside each other.) What a CU loads into LDS bounds the small ones: about 95 bytes a
+// nanosecond with all CUs at it, 120 with few. The largest does 2.3 PFLOP/s (4096^3), where MFMAs alone on such data, by
+// the card's power, do 3.4.
+int dense_go(const Int8Params& p, hipStream_t s) {
+    const float cus = (float)device_cu_count();
+    auto share = [&](int bt, int bn) { return (float)((int64_t)((p.P + bt - 1) / bt) * ((p.N + bn - 1) / bn)) / cus; };
+    auto cost = [](float f, float base, float slope, float least, float each) {   // f: tiles a CU
+        return f <= 1.f ? std::max(least, base + slope * f) : each * std::ceil(f);
+    };
+    const float f32 = share(64, 32), f64 = share(64, 64);
+    const float c32 = f32 <= 1.f ? 8.4f : 1e9f;
+    const float c64 = f64 <= 1.f ? 9.7f : 2.2f + 6.7f * std::ceil(f64);
+    const float c128x64 = cost(share(128, 64), 10.4f, 3.2f, 0.f, 12.5f);
+    const float c128 = cost(share(128, 128), 10.4f, 10.8f, 15.2f, 20.f);
+    const float c256x128 = cost(share(256, 128), 18.f, 18.f, 26.5f, 36.f);
+    const float c256 = cost(share(256, 256), 30.f, 29.f, 43.f, 62.f);
+    const float best = std::min({c32, c64, c128x64, c128, c256x128, c256});
+    if (c256 == best) return tiles_go<Tile256x256, Out8::k16, false>(p, s);
+    if (c256x128 == best) return tiles_go<Tile256x128, Out8::k16, false>(p, s);
+    if (c128 == best) return tiles_go<Tile128x128, Out8::k16, false>(p, s);
+    if (c128x64 == best) return tiles_go<Tile128x64, Out8::k16, false>(p, s);
+    if (c64 == best) return tiles_go<Tile64x64, Out8::k16, false>(p, s);
+    return tiles_go<Tile64x32K2, Out8::k16, false>(p, s);
+}
 
 }  // namespace
 
@@ -444,9 +517,7 @@ int launch_int8_tiles(const Int8Args& a, hipStream_t s) {
     if (p.P == 0) return W4A8_OK;
     if (a.dst == Out8::kSiluF32) return tiles_go<Tile64x256, Out8::kSiluF32, true>(p, s);
     if (a.dst == Out8::kSlotF32) return tiles_go<Tile64x256, Out8::kSlotF32, true>(p, s);
-    if (a.P > 1024) return tiles_go<Tile256x256, Out8::k16, false>(p, s);
-    if (a.P > 128) return tiles_go<Tile128x256, Out8::k16, false>(p, s);
-    return tiles_go<Tile128x128, Out8::k16, false>(p, s);
+    return dense_go(p, s);
 }
 
 }  // namespace w4a8

@@ -129,6 +129,23 @@ def test_dense_int8_rows(M, N, K, dtype):
     assert_close(y, *O.product(f64(x), xs.numpy(), f64(w), ws.numpy()), dtype)
 
 
+# a size for each dense tile, by the rule's costs on 256 CUs, with ragged sides and K in odd steps and a partial one
+REACH = [(64, 4096, 272), (250, 4090, 208), (500, 4100, 144), (1000, 4090, 400), (1500, 4090, 272), (4000, 4100, 208)]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("M,N,K", REACH)
+def test_dense_tiles(M, N, K, dtype):
+    g = gen(M, N, K, 20)
+    (x, xs), (w, ws) = rows8(g, M, K), weight(g, N, K)
+    y = W.int8_gemm(*on(x, xs, w, ws), out_dtype=dtype)
+    # (on the GPU in fp64: the sums of whole numbers below 2^53 are exact in any order)
+    X, XS, V, VS = on(x.double(), xs.double(), w.double(), ws.double())
+    ref = (X @ V.t()) * XS * VS
+    tol = ref.abs() * (4 * O.U32 + HALF[dtype] * (1 + 4 * O.U32)) + (2.0 ** -25 if dtype == torch.float16 else 0)
+    assert bool(((y.double() - ref).abs() <= tol).all())
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("M,N,K", SIZES)
 def test_dense_16bit_rows_with_bias(M, N, K, dtype):
