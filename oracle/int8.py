@@ -57,8 +57,10 @@ def expert(q, xs, w13, s13, w2, s2):
     return y, tol
 
 
-def layer(q, xs, w13, s13, w2, s2, tw, ids, expert_map=None):
-    """(out, how far fp32 arithmetic may be off); ids without a local expert contribute nothing."""
+def layer(q, xs, w13, s13, w2, s2, tw, ids, expert_map=None, rows16=False):
+    """(out, how far fp32 arithmetic may be off); ids without a local expert contribute nothing. rows16: each slot's
+    row is rounded to fp16 before the sum, times a power of two that puts the largest of 32 columns into [2^14, 2^15):
+    off by 2^-11 of a value, and by 2^-25 (half of fp16's least step) of 2^-14 of that largest one."""
     T, k = ids.shape
     out, tol = np.zeros((T, w2.shape[1])), np.zeros((T, w2.shape[1]))
     size = np.zeros_like(out)
@@ -69,6 +71,9 @@ def layer(q, xs, w13, s13, w2, s2, tw, ids, expert_map=None):
         if len(t) == 0:
             continue
         y, d = expert(q[t], xs[t], w13[e], s13[e], w2[e], s2[e])
+        if rows16:
+            block = np.abs(y).reshape(len(t), -1, 32).max(-1).repeat(32, axis=1)
+            d = d + (np.abs(y) + d) * 2.0 ** -11 + block * 2.0 ** -39
         w = tw[t, j].astype(np.float64)[:, None]
         np.add.at(out, t, y * w)
         np.add.at(tol, t, d * np.abs(w))

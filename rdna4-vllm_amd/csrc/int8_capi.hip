@@ -46,24 +46,30 @@ int check_product(const void* x, int x_dtype, const float* xs, int64_t rows, int
 
 // ---- the gated layer ----
 // Few rows an expert: the streaming kernels, which find their rows in the routed ids (h and the slots' rows in fp32, by
-// slot). Else tiles: rows quantised beforehand, slots aligned to blocks of the 64 rows that a tile has. Tokens are taken in
-// parts of as many as either can address.
+// slot). Else tiles: rows quantised beforehand, slots aligned to blocks of the rows that a tile has. The slots' rows
+// are rounded before the sum only where that is lost in the output's own rounding: for bf16 output they are fp16 with
+// a power of two for 32 columns (an eighth of its step), for fp16 output fp32. Tokens are taken in parts of as many as
+// either can address.
+// Slots an expert from which tiles have 128 rows.
+constexpr int64_t kWideRows = 192;
 struct LayerPlan {
     bool tiles, single;
     int64_t part;                // tokens of a part
+    int64_t block_m;             // tiles: rows of a block
     int64_t P, nblk;             // of a part: padded rows and blocks
     bool quant_x, quant_h;       // rows quantised by a launch of their own
 };
 LayerPlan plan_layer(int64_t T, int64_t H, int64_t inter, int64_t E, int64_t top_k, int x_dtype) {
     LayerPlan pl{};
-    const int64_t lim = ((int64_t)1 << 32) - 1, pad = E * (kTileRows - 1) + kTileRows;
+    const int64_t lim = ((int64_t)1 << 32) - 1, pad = E * 127 + 128;
     pl.tiles = T * top_k > std::min<int64_t>(12 * E, kScanSlots) && 2 * inter * H <= lim;
     const int64_t most = pl.tiles ? std::min(lim / H, (lim / inter - pad) / top_k) : kScanSlots / top_k;
     pl.part = std::min(T, std::max<int64_t>(1, most));
-    // every block in use holds a slot
     const int64_t n = pl.part * top_k;
-    pl.P = pl.tiles ? std::min((n + E * (kTileRows - 1) + kTileRows - 1) / kTileRows * kTileRows, n * kTileRows) : n;
-    pl.nblk = pl.P / kTileRows;
+    pl.block_m = n >= kWideRows * E ? 128 : 64;
+    // every block in use holds a slot
+    pl.P = pl.tiles ? std::min((n + E * (pl.block_m - 1) + pl.block_m - 1) / pl.block_m * pl.block_m, n * pl.block_m) : n;
+    pl.nblk = pl.P / pl.block_m;
     // few slots: hardly two of one expert
     pl.single = n * 8 <= E;
     pl.quant_x = x_dtype != W4A8_DTYPE_INT8 && (pl.tiles || !int8_rows_quantised_in_kernel(H));
@@ -76,6 +82,7 @@ struct LayerScratch {
     size_t align_bytes;
     int8_t *xq, *hq;
     float *xs, *hs, *h, *y;
+    uint8_t* ye;                 // y in fp16: its exponents, behind it
 };
 template <typename WS>
 void carve_layer(WS& w, const LayerPlan& pl, int64_t H, int64_t inter, int64_t E, int64_t top_k, LayerScratch& m) {
@@ -98,6 +105,7 @@ void carve_layer(WS& w, const LayerPlan& pl, int64_t H, int64_t inter, int64_t E
         m.hs = w.template take<float>((size_t)pl.P);
     }
     m.y = w.template take<float>((size_t)(n * H));
+    m.ye = reinterpret_cast<uint8_t*>(m.y) + n * H * 2;
 }
 struct Layer {
     const void* x;
@@ -125,21 +133,21 @@ int run_layer(const Layer& l, const LayerPlan& pl, const LayerScratch& m, hipStr
         xs = m.xs;
     }
     if (pl.tiles) {
-        if (int rc = launch_align(l.ids, n, l.E, kTileRows, l.emap, l.n_global, m.sti, pl.P, m.eid, m.ntp, m.align_ws,
+        if (int rc = launch_align(l.ids, n, l.E, pl.block_m, l.emap, l.n_global, m.sti, pl.P, m.eid, m.ntp, m.align_ws,
                                   m.align_bytes, s))
             return rc;
         Int8Args g1{};
         g1.x = static_cast<const int8_t*>(x); g1.xs = xs; g1.x_rows = l.T; g1.K = l.H; g1.ldx = l.H;
         g1.w = l.w13; g1.ws = l.s13; g1.E = l.E; g1.N = 2 * l.inter;
         g1.sorted_ids = m.sti; g1.expert_ids = m.eid; g1.ntp = m.ntp; g1.P = pl.P;
-        g1.top_k = l.top_k; g1.num_valid = n; g1.block_m = kTileRows; g1.gather = true;
+        g1.top_k = l.top_k; g1.num_valid = n; g1.block_m = pl.block_m; g1.gather = true;
         g1.dst = Out8::kSiluF32; g1.out = m.h; g1.ldo = l.inter;
         if (int rc = launch_int8_tiles(g1, s)) return rc;
         if (int rc = launch_act_quant_int8(m.h, Rows::kF32, pl.P, l.inter, l.inter, false, m.hq, m.hs, m.sti, m.ntp, n, s)) return rc;
         Int8Args g2 = g1;
         g2.x = m.hq; g2.xs = m.hs; g2.x_rows = pl.P; g2.K = l.inter; g2.ldx = l.inter;
         g2.w = l.w2; g2.ws = l.s2; g2.N = l.H; g2.gather = false;
-        g2.dst = Out8::kSlotF32; g2.out = m.y; g2.ldo = l.H;
+        g2.dst = l.bf16 ? Out8::kSlot16 : Out8::kSlotF32; g2.out = m.y; g2.out_exp = m.ye; g2.ldo = l.H;
         if (int rc = launch_int8_tiles(g2, s)) return rc;
     } else {
         RowsArgs g1{};
@@ -158,7 +166,7 @@ int run_layer(const Layer& l, const LayerPlan& pl, const LayerScratch& m, hipStr
         g2.dst = Out8::kSlotF32; g2.out = m.y; g2.ldo = l.H;
         if (int rc = launch_int8_rows(g2, s)) return rc;
     }
-    return launch_int8_reduce(m.y, l.tw, l.ids, l.emap, l.n_global, l.E, l.T, l.H, l.top_k, l.out, l.bf16, s);
+    return launch_int8_reduce(m.y, pl.tiles && l.bf16 ? m.ye : nullptr, l.tw, l.ids, l.emap, l.n_global, l.E, l.T, l.H, l.top_k, l.out, l.bf16, s);
 }
 struct SizeProbe {
     WorkspaceSize s;

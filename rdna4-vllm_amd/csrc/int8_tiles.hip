@@ -360,19 +360,36 @@ __global__ void __launch_bounds__(C::kThreads * C::KS, C::EU) int8_tiles_kernel(
         // A wave turns 32 rows at a time through LDS, so that its stores are whole lines: a row's values lie in
         // chunks of 16 bytes, chunk i of row r at i ^ (r & 15) (rows of 256 bytes or more), i ^ (r / 2 & 7) (of 128) or
         // i ^ (r / 4 & 3) (of 64): sixteen lanes then write to different banks.
-        constexpr int kOutCols = (kSilu ? FN / 2 : FN) * 32, kSize = DST == Out8::k16 ? 2 : 4;
-        constexpr int kRowBytes = kOutCols * kSize, kChunks = kRowBytes / 16;
+        // 16-bit rows of all the wave's columns, fp32 rows of a fragment's.
+        constexpr bool k2 = DST == Out8::k16 || DST == Out8::kSlot16;
+        constexpr int kFrags = kSilu ? FN / 2 : FN, kAt = k2 ? kFrags : 1, kSize = k2 ? 2 : 4;
+        constexpr int kRowBytes = kAt * 32 * kSize, kChunks = kRowBytes / 16;
         static_assert(kChunks >= 4, "a row is 64 bytes or more");
         static_assert(KS * C::kSlot >= 4 * (2 * BT + 2 * BN) + C::kWaves * 32 * kRowBytes, "tables and rows fit");
         int8_t* const strip = slots1 + 4 * (2 * BT + 2 * BN) + wave * 32 * kRowBytes;
         auto chunk_at = [&](int row, int i) __attribute__((always_inline)) {
             return row * kRowBytes + ((i ^ (kChunks >= 16 ? row & 15 : kChunks == 8 ? row >> 1 & 7 : row >> 2 & 3)) << 4);
         };
-        const int col0 = kSilu ? ct_now * (BN / 2) + wn * kOutCols : ct_now * BN + wn * kOutCols;
-        auto turn = [&](int i, auto bf16) __attribute__((always_inline)) {
+        const int col0 = (ct_now * C::WN + wn) * kFrags * 32;
+        auto turn_rows = [&](int i, int j0, auto bf16) __attribute__((always_inline)) {
             const float xs = s_xs[(wt * FT + i) * 32 + c];
 #pragma unroll
-            for (int j = 0; j < kOutCols / 32; ++j) {
+            for (int j = j0; j < j0 + kAt; ++j) {
+                float to = 1.f;                                  // kSlot16: a power of two
+                if constexpr (DST == Out8::kSlot16) {
+                    // the row's largest finite value of these 32 columns to [2^14, 2^15): infinities, NaN and zeros as they are
+                    float m = 0.f;
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        const float v = fabsf((float)run[i][j][r] * (xs * s_ws[(wn * FN + j) * 32 + 16 * h + r]));
+                        m = fmaxf(m, v < INFINITY ? v : 0.f);
+                    }
+                    const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(m), __float_as_uint(m), false, false);
+                    const uint32_t eb = max(both[0], both[1]) >> 23, sb = eb == 0 ? 127u : eb > 15 ? eb - 14 : 1u;
+                    to = __uint_as_float((254u - sb) << 23);
+                    const int slot = s_slot[(wt * FT + i) * 32 + c], col = col0 + j * 32;
+                    if (h == 0 && slot >= 0 && col < N) p.out_exp[(int64_t)slot * (p.ldo / 32) + col / 32] = (uint8_t)sb;
+                }
 #pragma unroll
                 for (int q = 0; q < 2; ++q) {                    // eight columns
                     const int at = (wn * FN + j) * 32 + 16 * h + 8 * q;
@@ -383,10 +400,10 @@ __global__ void __launch_bounds__(C::kThreads * C::KS, C::EU) int8_tiles_kernel(
                         if constexpr (kSilu)
                             t[r] = silu_mul(v * f, (float)run[i][j + FN / 2][8 * q + r] * (xs * s_ws[at + FN / 2 * 32 + r]));
                         else if constexpr (DST == Out8::k16) t[r] = fmaf(v, f, s_bias[at + r]);
-                        else t[r] = v * f;
+                        else t[r] = v * f * to;
                     }
-                    const int chunk = (j * 32 + 16 * h + 8 * q) * kSize / 16;
-                    if constexpr (DST == Out8::k16) {
+                    const int chunk = ((j - j0) * 32 + 16 * h + 8 * q) * kSize / 16;
+                    if constexpr (k2) {
                         constexpr bool b = decltype(bf16)::value;
                         *reinterpret_cast<u32x4*>(strip + chunk_at(c, chunk)) =
                             u32x4{pack16<b>(t[0], t[1]), pack16<b>(t[2], t[3]), pack16<b>(t[4], t[5]), pack16<b>(t[6], t[7])};
@@ -398,8 +415,8 @@ __global__ void __launch_bounds__(C::kThreads * C::KS, C::EU) int8_tiles_kernel(
                 __builtin_amdgcn_sched_barrier(0);
             }
         };
-        auto put = [&](int i) __attribute__((always_inline)) {
-            constexpr int kRows = 64 / kChunks > 0 ? 64 / kChunks : 1;   // rows of one store
+        auto put = [&](int i, int j0) __attribute__((always_inline)) {
+            constexpr int kRows = 64 / kChunks;                  // rows of one store
             static_assert(kChunks <= 64 && 32 % kRows == 0, "a store takes whole rows");
             __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront", "local");
             __builtin_amdgcn_wave_barrier();
@@ -408,11 +425,11 @@ __global__ void __launch_bounds__(C::kThreads * C::KS, C::EU) int8_tiles_kernel(
                 const int r = r0 + lane / kChunks, chunk = lane % kChunks;
                 const u32x4 v = *reinterpret_cast<const u32x4*>(strip + chunk_at(r, chunk));
                 const int slot = s_slot[(wt * FT + i) * 32 + r];
-                const int64_t row = DST == Out8::kSlotF32 ? slot : r0_now + (wt * FT + i) * 32 + r;
-                const int col = col0 + chunk * 16 / kSize;
+                const int64_t row = DST == Out8::kSlotF32 || DST == Out8::kSlot16 ? slot : r0_now + (wt * FT + i) * 32 + r;
+                const int col = col0 + j0 * 32 + chunk * 16 / kSize;
                 if (slot < 0 || col >= (kSilu ? half : N)) continue;
-                if constexpr (DST == Out8::k16) {
-                    if (p.out16 && col + 8 <= N) {
+                if constexpr (k2) {
+                    if (DST == Out8::kSlot16 || (p.out16 && col + 8 <= N)) {
                         *reinterpret_cast<u32x4*>(reinterpret_cast<uint16_t*>(p.out) + row * p.ldo + col) = v;
                     } else {
                         const uint32_t w[4] = {v[0], v[1], v[2], v[3]};
@@ -427,11 +444,13 @@ __global__ void __launch_bounds__(C::kThreads * C::KS, C::EU) int8_tiles_kernel(
         };
         if (KS == 1 || part == 0) {
 #pragma unroll
-            for (int i = 0; i < FT; ++i) {
-                if (DST == Out8::k16 && p.bf16) turn(i, std::true_type{});
-                else turn(i, std::false_type{});
-                put(i);
-            }
+            for (int i = 0; i < FT; ++i)
+#pragma unroll
+                for (int j = 0; j < kFrags; j += kAt) {
+                    if (DST == Out8::k16 && p.bf16) turn_rows(i, j, std::true_type{});
+                    else turn_rows(i, j, std::false_type{});
+                    put(i, j);
+                }
         }
         if (!more) break;
         item = next_item;
@@ -469,6 +488,7 @@ using Tile128x128 = Tile<2, 4, 2, 1, 4, 1, 2, true>;
 using Tile256x128 = Tile<4, 2, 2, 2, 3, 1, 2>;
 using Tile256x256 = Tile<2, 4, 4, 2, 2, 1, 2>;
 using Tile64x256 = Tile<1, 4, 2, 2, 2, 1, 2>;            // grouped; two a CU
+using Tile128x256 = Tile<2, 4, 2, 2, 3, 1, 2>;           // grouped
 
 // The dense tile of least cost. us as measured at N = K = 4096 (the rule compares tiles at one K, as if all their costs
 // grew with it alike), by the tiles a CU has to take:
@@ -515,8 +535,13 @@ bool int8_tiles_supported(const Int8Args& a) {
 int launch_int8_tiles(const Int8Args& a, hipStream_t s) {
     const Int8Params p = int8_params(a);
     if (p.P == 0) return W4A8_OK;
-    if (a.dst == Out8::kSiluF32) return tiles_go<Tile64x256, Out8::kSiluF32, true>(p, s);
-    if (a.dst == Out8::kSlotF32) return tiles_go<Tile64x256, Out8::kSlotF32, true>(p, s);
+    auto grouped = [&](auto tile) -> int {
+        using C = decltype(tile);
+        if (a.dst == Out8::kSiluF32) return tiles_go<C, Out8::kSiluF32, true>(p, s);
+        if (a.dst == Out8::kSlot16) return tiles_go<C, Out8::kSlot16, true>(p, s);
+        return tiles_go<C, Out8::kSlotF32, true>(p, s);
+    };
+    if (a.sorted_ids != nullptr) return a.block_m == 128 ? grouped(Tile128x256{}) : grouped(Tile64x256{});
     return dense_go(p, s);
 }
 

@@ -214,6 +214,11 @@ def make_routing(g, T, E, k, skew=0.0):
     return top / top.sum(1, keepdim=True), ids.to(torch.int32)
 
 
+def rows16(T, E, k, dtype):
+    """Whether the layer rounds its slots' rows to 16 bits: many tokens, bf16 output."""
+    return T * k > min(12 * E, 4096) and dtype == torch.bfloat16
+
+
 LAYERS = [(1, 8, 2, 64, 64), (1, 256, 8, 512, 128), (3, 16, 4, 192, 320), (5, 4, 4, 256, 64), (17, 8, 2, 64, 192), (32, 32, 4, 512, 256),
           (40, 2, 1, 128, 128), (65, 16, 2, 320, 704), (130, 8, 3, 256, 384), (200, 64, 6, 448, 128), (333, 4, 2, 512, 512),
           (700, 8, 8, 128, 192)]
@@ -227,7 +232,8 @@ def test_layer(T, E, k, H, I, dtype):
     tw, ids = make_routing(g, T, E, k, 0.5)
     x = hidden(g, T, H, dtype)
     y = W.moe_int8_apply(*on(x, w13, w2, s13, s2, tw, ids))
-    ref, tol = O.layer(*O.quantise(f64(x)), f64(w13), s13.numpy(), f64(w2), s2.numpy(), tw.numpy(), ids.numpy())
+    ref, tol = O.layer(*O.quantise(f64(x)), f64(w13), s13.numpy(), f64(w2), s2.numpy(), tw.numpy(), ids.numpy(),
+                       rows16=rows16(T, E, k, dtype))
     assert_close(y, ref, tol, dtype)
     q, s = W.act_quant_int8(x.to(DEV))
     assert torch.equal(W.moe_int8_apply(q, *on(w13, w2, s13, s2, tw, ids), x_scales=s, out_dtype=dtype), y)
@@ -246,7 +252,8 @@ def test_layer_expert_map_and_absent_slots(T):
     ids[1, 1], ids[2, 0] = -1, glob + 5
     x = hidden(g, T, H, torch.bfloat16)
     y = W.moe_int8_apply(*on(x, w13, w2, s13, s2, tw, ids), expert_map=emap.to(DEV), global_num_experts=glob)
-    ref, tol = O.layer(*O.quantise(f64(x)), f64(w13), s13.numpy(), f64(w2), s2.numpy(), tw.numpy(), ids.numpy(), emap.numpy())
+    ref, tol = O.layer(*O.quantise(f64(x)), f64(w13), s13.numpy(), f64(w2), s2.numpy(), tw.numpy(), ids.numpy(), emap.numpy(),
+                       rows16=rows16(T, E, k, torch.bfloat16))
     assert_close(y, ref, tol, torch.bfloat16)
     assert not y[0].any()
     none = W.moe_int8_apply(*on(x, w13, w2, s13, s2, tw, torch.full_like(ids, -1)))
@@ -262,7 +269,8 @@ def test_layer_repeats_and_twice_the_same_expert(T):
     x = hidden(g, T, 128, torch.bfloat16)
     args = on(x, w13, w2, s13, s2, tw, ids)
     y = W.moe_int8_apply(*args)
-    ref, tol = O.layer(*O.quantise(f64(x)), f64(w13), s13.numpy(), f64(w2), s2.numpy(), tw.numpy(), ids.numpy())
+    ref, tol = O.layer(*O.quantise(f64(x)), f64(w13), s13.numpy(), f64(w2), s2.numpy(), tw.numpy(), ids.numpy(),
+                       rows16=rows16(T, 4, 2, torch.bfloat16))
     assert_close(y, ref, tol, torch.bfloat16)
     for _ in range(3):
         assert torch.equal(W.moe_int8_apply(*args), y)
@@ -279,6 +287,23 @@ def test_layer_rows_that_are_not_finite_leave_the_others(T):
     y = W.moe_int8_apply(*on(x, w13, w2, s13, s2, tw, ids))
     keep = torch.arange(T) != 3
     assert y[3].isnan().all() and torch.equal(y[keep.to(DEV)], clean[keep.to(DEV)])
+
+
+@pytest.mark.parametrize("T", [6, 500])
+def test_layer_channels_of_other_sizes(T):
+    """A channel scale that is infinite, or 2^20 times its neighbours', leaves the columns beside it."""
+    g = gen(T, 14)
+    w13, w2, s13, s2 = make_layer(g, 4, 128, 128)
+    tw, ids = make_routing(g, T, 4, 2)
+    x = hidden(g, T, 128, torch.bfloat16)
+    s2[:, 40] *= 2.0 ** 20
+    args = (O.quantise(f64(x)), f64(w13), s13.numpy(), f64(w2))
+    ref, tol = O.layer(*args[0], *args[1:], s2.numpy(), tw.numpy(), ids.numpy(), rows16=rows16(T, 4, 2, torch.bfloat16))
+    s2[:, 7] = float("inf")
+    y = W.moe_int8_apply(*on(x, w13, w2, s13, s2, tw, ids))
+    keep = [n for n in range(128) if n != 7]
+    assert_close(y[:, keep], ref[:, keep], tol[:, keep], torch.bfloat16)
+    assert not y[:, 7].isfinite().any()
 
 
 def test_layer_no_tokens():
