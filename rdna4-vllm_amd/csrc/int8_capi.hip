@@ -82,7 +82,7 @@ struct LayerScratch {
     size_t align_bytes;
     int8_t *xq, *hq;
     float *xs, *hs, *h, *y;
-    uint8_t* ye;                 // y in fp16: its exponents, behind it
+    float* ys;                   // y in fp16: its scales, behind it
 };
 template <typename WS>
 void carve_layer(WS& w, const LayerPlan& pl, int64_t H, int64_t inter, int64_t E, int64_t top_k, LayerScratch& m) {
@@ -105,7 +105,7 @@ void carve_layer(WS& w, const LayerPlan& pl, int64_t H, int64_t inter, int64_t E
         m.hs = w.template take<float>((size_t)pl.P);
     }
     m.y = w.template take<float>((size_t)(n * H));
-    m.ye = reinterpret_cast<uint8_t*>(m.y) + n * H * 2;
+    m.ys = m.y + n * H / 2;
 }
 struct Layer {
     const void* x;
@@ -147,7 +147,7 @@ int run_layer(const Layer& l, const LayerPlan& pl, const LayerScratch& m, hipStr
         Int8Args g2 = g1;
         g2.x = m.hq; g2.xs = m.hs; g2.x_rows = pl.P; g2.K = l.inter; g2.ldx = l.inter;
         g2.w = l.w2; g2.ws = l.s2; g2.N = l.H; g2.gather = false;
-        g2.dst = l.bf16 ? Out8::kSlot16 : Out8::kSlotF32; g2.out = m.y; g2.out_exp = m.ye; g2.ldo = l.H;
+        g2.dst = l.bf16 ? Out8::kSlot16 : Out8::kSlotF32; g2.out = m.y; g2.out_scales = m.ys; g2.ldo = l.H;
         if (int rc = launch_int8_tiles(g2, s)) return rc;
     } else {
         RowsArgs g1{};
@@ -166,7 +166,7 @@ int run_layer(const Layer& l, const LayerPlan& pl, const LayerScratch& m, hipStr
         g2.dst = Out8::kSlotF32; g2.out = m.y; g2.ldo = l.H;
         if (int rc = launch_int8_rows(g2, s)) return rc;
     }
-    return launch_int8_reduce(m.y, pl.tiles && l.bf16 ? m.ye : nullptr, l.tw, l.ids, l.emap, l.n_global, l.E, l.T, l.H, l.top_k, l.out, l.bf16, s);
+    return launch_int8_reduce(m.y, pl.tiles && l.bf16 ? m.ys : nullptr, l.tw, l.ids, l.emap, l.n_global, l.E, l.T, l.H, l.top_k, l.out, l.bf16, s);
 }
 struct SizeProbe {
     WorkspaceSize s;

@@ -161,11 +161,11 @@ int quant_go(const QuantParams& p, bool wide, hipStream_t s) {
     return go(&quant_rows_kernel<SRC, SILU, 16, 4>, 1, 1024);
 }
 
-// Eight columns a lane; a token's slots in order, their rows requested together. SCALED: fp16 rows with an exponent
-// for 32 columns; a value is scaled back (exactly) before its weight, as their scale times the weight can leave fp32's
-// range where the product of all three does not.
+// Eight columns a lane; a token's slots in order, their rows requested together. SCALED: fp16 rows with a scale
+// for 32 columns; a value is scaled back before its weight, as their scale times the weight can leave fp32's range where
+// the product of all three does not.
 template <bool BF16, bool SCALED>
-__global__ void __launch_bounds__(256) int8_reduce_kernel(const void* __restrict__ y, const uint8_t* __restrict__ ye,
+__global__ void __launch_bounds__(256) int8_reduce_kernel(const void* __restrict__ y, const float* __restrict__ ys,
                                                          const float* __restrict__ tw, const int32_t* __restrict__ ids,
                                                          const int32_t* __restrict__ emap, int emap_len, int E, int N, int top_k,
                                                          int64_t pieces, uint16_t* __restrict__ out) {
@@ -187,7 +187,7 @@ __global__ void __launch_bounds__(256) int8_reduce_kernel(const void* __restrict
             w[i] = tw[slot];
             if constexpr (SCALED) {
                 v[i][0] = *reinterpret_cast<const u32x4*>(reinterpret_cast<const uint16_t*>(y) + slot * N + n);
-                sc[i] = __uint_as_float((uint32_t)ye[slot * (N / 32) + n / 32] << 23);
+                sc[i] = ys[slot * (N / 32) + n / 32];
             } else {
                 v[i][0] = *reinterpret_cast<const u32x4*>(reinterpret_cast<const float*>(y) + slot * N + n);
                 v[i][1] = *reinterpret_cast<const u32x4*>(reinterpret_cast<const float*>(y) + slot * N + n + 4);
@@ -230,7 +230,7 @@ int launch_act_quant_int8(const void* x, Rows src, int64_t rows, int64_t K, int6
     return silu ? quant_go<Rows::kF16, true>(p, wide, s) : quant_go<Rows::kF16, false>(p, wide, s);
 }
 
-int launch_int8_reduce(const void* y, const uint8_t* y_exp, const float* tw, const int32_t* ids, const int32_t* emap,
+int launch_int8_reduce(const void* y, const float* y_scales, const float* tw, const int32_t* ids, const int32_t* emap,
                        int64_t emap_len, int64_t E, int64_t T, int64_t N, int64_t top_k, void* out, bool bf16, hipStream_t s) {
     if (T == 0) return W4A8_OK;
     const int64_t pieces = T * (N / 8), blocks = (pieces + 255) / 256;
@@ -239,11 +239,11 @@ int launch_int8_reduce(const void* y, const uint8_t* y_exp, const float* tw, con
         return W4A8_ERR_INVALID;
     }
     auto go = [&](auto kernel) {
-        launch_kernel(kernel, dim3((unsigned)blocks), dim3(256), 0, s, y, y_exp, tw, ids, emap, (int)emap_len, (int)E, (int)N,
+        launch_kernel(kernel, dim3((unsigned)blocks), dim3(256), 0, s, y, y_scales, tw, ids, emap, (int)emap_len, (int)E, (int)N,
                       (int)top_k, pieces, static_cast<uint16_t*>(out));
         return check_launch("int8_reduce_kernel");
     };
-    if (y_exp != nullptr) return bf16 ? go(&int8_reduce_kernel<true, true>) : go(&int8_reduce_kernel<false, true>);
+    if (y_scales != nullptr) return bf16 ? go(&int8_reduce_kernel<true, true>) : go(&int8_reduce_kernel<false, true>);
     return bf16 ? go(&int8_reduce_kernel<true, false>) : go(&int8_reduce_kernel<false, false>);
 }
 

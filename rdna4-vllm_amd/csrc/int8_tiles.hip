@@ -73,8 +73,9 @@ __global__ void __launch_bounds__(C::kThreads * C::KS, C::EU) int8_tiles_kernel(
     __shared__ __attribute__((aligned(1024))) int8_t slots3[S > 3 ? KS * C::kSlot : 16];
     __shared__ __attribute__((aligned(1024))) int8_t slots4[S > 4 ? KS * C::kSlot : 16];
     __shared__ __attribute__((aligned(1024))) int8_t slots5[S > 5 ? KS * C::kSlot : 16];
-    // Tables for the epilogue, in slot 1 between a tile's last step and the next one's second.
-    float *const s_xs = reinterpret_cast<float*>(slots1), *const s_ws = s_xs + BT, *const s_bias = s_ws + BN;
+    // Tables for the epilogue, in the last slot between a tile's last step and the next one's loads into it.
+    int8_t* const aside = S == 2 ? slots1 : S == 3 ? slots2 : S == 4 ? slots3 : S == 5 ? slots4 : slots5;
+    float *const s_xs = reinterpret_cast<float*>(aside), *const s_ws = s_xs + BT, *const s_bias = s_ws + BN;
     int* const s_slot = reinterpret_cast<int*>(s_bias + BN);
 
     // ---- the tiles of this work-group: an XCD takes a contiguous run of them, kRunRows row tiles by all columns
@@ -174,7 +175,7 @@ __global__ void __launch_bounds__(C::kThreads * C::KS, C::EU) int8_tiles_kernel(
                                         (n >= FN / 2 ? half : 0)
                                   : min(ct * BN + r, N - 1);
             ws_v[i] = p.ws[(int64_t)e * N + col];
-            bias_v[i] = DST == Out8::k16 ? bias_at(p, col) : 0.f;
+            bias_v[i] = DST == Out8::k16 ? w4a8::bias_at(p, col) : 0.f;
         }
     };
 
@@ -293,7 +294,7 @@ __global__ void __launch_bounds__(C::kThreads * C::KS, C::EU) int8_tiles_kernel(
             for (int j = 0; j < FN; ++j)
 #pragma unroll
                 for (int r = 0; r < 16; ++r) run[i][j][r] = 0;
-        __builtin_amdgcn_s_waitcnt(wait_vm(0));
+        __builtin_amdgcn_s_waitcnt(wait_vm(C::kLoads * (S - 1)));
         group_barrier();
 #pragma unroll
         for (int s = 0; s < (DEEP ? 4 : 1); ++s) frags(slot_of(std::integral_constant<int, 0>{}), s, s);
@@ -353,7 +354,7 @@ __global__ void __launch_bounds__(C::kThreads * C::KS, C::EU) int8_tiles_kernel(
             ct = ct_next;
             set_tile();
             each_slot([&](auto i) __attribute__((always_inline)) {
-                if (decltype(i)::value != 1) issue(slot_of(i), decltype(i)::value, 0, 1);
+                if (decltype(i)::value != S - 1) issue(slot_of(i), decltype(i)::value, 0, 1);
             });
         }
         lds_barrier();
@@ -366,51 +367,75 @@ __global__ void __launch_bounds__(C::kThreads * C::KS, C::EU) int8_tiles_kernel(
         constexpr int kRowBytes = kAt * 32 * kSize, kChunks = kRowBytes / 16;
         static_assert(kChunks >= 4, "a row is 64 bytes or more");
         static_assert(KS * C::kSlot >= 4 * (2 * BT + 2 * BN) + C::kWaves * 32 * kRowBytes, "tables and rows fit");
-        int8_t* const strip = slots1 + 4 * (2 * BT + 2 * BN) + wave * 32 * kRowBytes;
+        int8_t* const strip = aside + 4 * (2 * BT + 2 * BN) + wave * 32 * kRowBytes;
         auto chunk_at = [&](int row, int i) __attribute__((always_inline)) {
             return row * kRowBytes + ((i ^ (kChunks >= 16 ? row & 15 : kChunks == 8 ? row >> 1 & 7 : row >> 2 & 3)) << 4);
         };
         const int col0 = (ct_now * C::WN + wn) * kFrags * 32;
+        // (scales and bias of the lane's columns: held where registers allow, else read again for each 32 rows)
+        constexpr bool kHeld = FT <= 2;
+        float ws[kHeld ? FN : 1][16], bias[kHeld && DST == Out8::k16 ? FN : 1][16];
+        if constexpr (kHeld)
+#pragma unroll
+            for (int j = 0; j < FN; ++j)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    ws[j][r] = s_ws[(wn * FN + j) * 32 + 16 * h + r];
+                    if constexpr (DST == Out8::k16) bias[j][r] = s_bias[(wn * FN + j) * 32 + 16 * h + r];
+                }
+        auto ws_at = [&](int j, int r) __attribute__((always_inline)) {
+            return kHeld ? ws[kHeld ? j : 0][r] : s_ws[(wn * FN + j) * 32 + 16 * h + r];
+        };
+        auto bias_at = [&](int j, int r) __attribute__((always_inline)) {
+            return kHeld ? bias[kHeld && DST == Out8::k16 ? j : 0][r] : s_bias[(wn * FN + j) * 32 + 16 * h + r];
+        };
         auto turn_rows = [&](int i, int j0, auto bf16) __attribute__((always_inline)) {
             const float xs = s_xs[(wt * FT + i) * 32 + c];
 #pragma unroll
             for (int j = j0; j < j0 + kAt; ++j) {
-                float to = 1.f;                                  // kSlot16: a power of two
-                if constexpr (DST == Out8::kSlot16) {
-                    // the row's largest finite value of these 32 columns to [2^14, 2^15): infinities, NaN and zeros as they are
-                    float m = 0.f;
+                float t[16];
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) {
-                        const float v = fabsf((float)run[i][j][r] * (xs * s_ws[(wn * FN + j) * 32 + 16 * h + r]));
-                        m = fmaxf(m, v < INFINITY ? v : 0.f);
-                    }
-                    const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(m), __float_as_uint(m), false, false);
-                    const uint32_t eb = max(both[0], both[1]) >> 23, sb = eb == 0 ? 127u : eb > 15 ? eb - 14 : 1u;
-                    to = __uint_as_float((254u - sb) << 23);
-                    const int slot = s_slot[(wt * FT + i) * 32 + c], col = col0 + j * 32;
-                    if (h == 0 && slot >= 0 && col < N) p.out_exp[(int64_t)slot * (p.ldo / 32) + col / 32] = (uint8_t)sb;
+                for (int r = 0; r < 16; ++r) {
+                    const float v = (float)run[i][j][r];
+                    if constexpr (kSilu)
+                        t[r] = silu_mul(v * (xs * ws_at(j, r)), (float)run[i][j + FN / 2][r] * (xs * ws_at(j + FN / 2, r)));
+                    else if constexpr (DST == Out8::k16) t[r] = fmaf(v, xs * ws_at(j, r), bias_at(j, r));
+                    else if constexpr (DST == Out8::kSlot16) t[r] = v * ws_at(j, r);
+                    else t[r] = v * (xs * ws_at(j, r));
                 }
+                if constexpr (DST == Out8::kSlot16) {
+                    // the largest finite value of these 32 columns to [2^14, 2^15): infinities, NaN and zeros as they are
+                    auto largest = [&](auto real) __attribute__((always_inline)) {
+                        float m = 0.f;
 #pragma unroll
-                for (int q = 0; q < 2; ++q) {                    // eight columns
-                    const int at = (wn * FN + j) * 32 + 16 * h + 8 * q;
-                    float t[8];
+                        for (int r = 0; r < 16; ++r)
+                            m = fmaxf(m, !decltype(real)::value || fabsf(t[r]) < INFINITY ? fabsf(t[r]) : 0.f);
+                        const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(m), __float_as_uint(m), false, false);
+                        return max(both[0], both[1]) >> 23;
+                    };
+                    uint32_t eb = largest(std::false_type{});
+                    if (__ballot(eb == 255) != 0) eb = largest(std::true_type{});
+                    const uint32_t sb = eb == 0 ? 127u : eb > 15 ? eb - 14 : 1u;
+                    const float to = __uint_as_float((254u - sb) << 23);
 #pragma unroll
-                    for (int r = 0; r < 8; ++r) {
-                        const float v = (float)run[i][j][8 * q + r], f = xs * s_ws[at + r];
-                        if constexpr (kSilu)
-                            t[r] = silu_mul(v * f, (float)run[i][j + FN / 2][8 * q + r] * (xs * s_ws[at + FN / 2 * 32 + r]));
-                        else if constexpr (DST == Out8::k16) t[r] = fmaf(v, f, s_bias[at + r]);
-                        else t[r] = v * f * to;
-                    }
-                    const int chunk = ((j - j0) * 32 + 16 * h + 8 * q) * kSize / 16;
-                    if constexpr (k2) {
-                        constexpr bool b = decltype(bf16)::value;
-                        *reinterpret_cast<u32x4*>(strip + chunk_at(c, chunk)) =
-                            u32x4{pack16<b>(t[0], t[1]), pack16<b>(t[2], t[3]), pack16<b>(t[4], t[5]), pack16<b>(t[6], t[7])};
-                    } else {
-                        *reinterpret_cast<v4f*>(strip + chunk_at(c, chunk)) = v4f{t[0], t[1], t[2], t[3]};
-                        *reinterpret_cast<v4f*>(strip + chunk_at(c, chunk + 1)) = v4f{t[4], t[5], t[6], t[7]};
-                    }
+                    for (int r = 0; r < 16; ++r) t[r] *= to;
+                    const int slot = s_slot[(wt * FT + i) * 32 + c], col = col0 + j * 32;
+                    if (h == 0 && slot >= 0 && col < N)
+                        p.out_scales[(int64_t)slot * (p.ldo / 32) + col / 32] = xs * __uint_as_float(sb << 23);
+                }
+                const int chunk = ((j - j0) * 32 + 16 * h) * kSize / 16;
+                if constexpr (k2) {
+                    constexpr bool b = decltype(bf16)::value;
+#pragma unroll
+                    for (int q = 0; q < 2; ++q)
+                        *reinterpret_cast<u32x4*>(strip + chunk_at(c, chunk + q)) =
+                            u32x4{pack16<b>(t[8 * q], t[8 * q + 1]), pack16<b>(t[8 * q + 2], t[8 * q + 3]),
+                                  pack16<b>(t[8 * q + 4], t[8 * q + 5]), pack16<b>(t[8 * q + 6], t[8 * q + 7])};
+                } else {
+#pragma unroll
+                    for (int q = 0; q < 4; ++q)
+                        *reinterpret_cast<v4f*>(strip + chunk_at(c, chunk + q)) =
+                            v4f{t[4 * q], t[4 * q + 1], t[4 * q + 2], t[4 * q + 3]};
                 }
                 __builtin_amdgcn_sched_barrier(0);
             }
@@ -455,7 +480,7 @@ __global__ void __launch_bounds__(C::kThreads * C::KS, C::EU) int8_tiles_kernel(
         if (!more) break;
         item = next_item;
         lds_barrier();                                           // nobody reads the tables any more
-        issue(slot_of(std::integral_constant<int, 1>{}), 1, 0, 1);
+        issue(slot_of(std::integral_constant<int, S - 1>{}), S - 1, 0, 1);
     }
 }
 
@@ -487,8 +512,11 @@ using Tile128x64 = Tile<4, 2, 1, 1, 4, 1, 2, true>;
 using Tile128x128 = Tile<2, 4, 2, 1, 4, 1, 2, true>;
 using Tile256x128 = Tile<4, 2, 2, 2, 3, 1, 2>;
 using Tile256x256 = Tile<2, 4, 4, 2, 2, 1, 2>;
-using Tile64x256 = Tile<1, 4, 2, 2, 2, 1, 2>;            // grouped; two a CU
-using Tile128x256 = Tile<2, 4, 2, 2, 3, 1, 2>;           // grouped
+// grouped: the layer's first and second product, blocks of 64 and 128 rows
+using First64 = Tile<1, 4, 2, 2, 2, 1, 2>;
+using Second64 = Tile<2, 4, 1, 2, 2, 1, 4>;
+using First128 = Tile<2, 4, 2, 2, 3, 1, 2>;
+using Second128 = Tile<2, 4, 2, 2, 3, 1, 2>;
 
 // The dense tile of least cost. us as measured at N = K = 4096 (the rule compares tiles at one K, as if all their costs
 // grew with it alike), by the tiles a CU has to take:
@@ -535,13 +563,12 @@ bool int8_tiles_supported(const Int8Args& a) {
 int launch_int8_tiles(const Int8Args& a, hipStream_t s) {
     const Int8Params p = int8_params(a);
     if (p.P == 0) return W4A8_OK;
-    auto grouped = [&](auto tile) -> int {
-        using C = decltype(tile);
-        if (a.dst == Out8::kSiluF32) return tiles_go<C, Out8::kSiluF32, true>(p, s);
-        if (a.dst == Out8::kSlot16) return tiles_go<C, Out8::kSlot16, true>(p, s);
-        return tiles_go<C, Out8::kSlotF32, true>(p, s);
+    auto grouped = [&](auto first, auto second) -> int {
+        if (a.dst == Out8::kSiluF32) return tiles_go<decltype(first), Out8::kSiluF32, true>(p, s);
+        if (a.dst == Out8::kSlot16) return tiles_go<decltype(second), Out8::kSlot16, true>(p, s);
+        return tiles_go<decltype(second), Out8::kSlotF32, true>(p, s);
     };
-    if (a.sorted_ids != nullptr) return a.block_m == 128 ? grouped(Tile128x256{}) : grouped(Tile64x256{});
+    if (a.sorted_ids != nullptr) return a.block_m == 128 ? grouped(First128{}, Second128{}) : grouped(First64{}, Second64{});
     return dense_go(p, s);
 }
 
