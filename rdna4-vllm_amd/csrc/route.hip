@@ -10,7 +10,9 @@
 // one, c is formed in fp64 (in fp32 two experts' c may round to one number), compared rounded to fp32 (which keeps the
 // order) and, where that is equal, by what was rounded off.
 //
-// One wave a token: lane l holds experts NV l .. NV l + NV - 1.
+// Bound: for many tokens the vector units (their logits take 4 us), for few the launch.
+#include <type_traits>
+
 #include "w4a8_common.h"
 #include "w4a8_internal.h"
 
@@ -26,6 +28,7 @@ struct RouteParams {
     int E, top_k, groups, top_groups, size;    // size: experts of a group
     int sigmoid, renorm;
     float scale;
+    int nv, vec;                               // sixteen lanes a token: experts a lane; whole pieces of 16 bytes each
 };
 
 __device__ __forceinline__ uint32_t order_key(float v) {       // larger for a larger value, 0 for none
@@ -59,14 +62,16 @@ __device__ __forceinline__ float logit_at(const void* l, int64_t i) {
     return __half2float(__ushort_as_half(v));
 }
 
+// What a wave compares groups by, in LDS: c in fp64, or the logit.
+template <int NV, bool BIAS>
+struct RouteScratch {
+    double c[BIAS ? 64 * NV : 1];
+    float l[BIAS ? 1 : 64 * NV];
+};
+
+// One token by one wave: lane l holds experts NV l .. NV l + NV - 1.
 template <int NV, int SRC, bool BIAS>
-__global__ void __launch_bounds__(256) route_topk_kernel(RouteParams p) {
-    // what groups are compared by: c in fp64, or the logit
-    __shared__ double s_c[BIAS ? 4 : 1][BIAS ? 64 * NV : 1];
-    __shared__ float s_l[BIAS ? 1 : 4][BIAS ? 1 : 64 * NV];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int64_t t = (int64_t)blockIdx.x * 4 + wave;
-    if (t >= p.T) return;                       // (no work-group barrier below)
+__device__ void route_token(const RouteParams& p, int64_t t, int lane, RouteScratch<NV, BIAS>& scratch) {
     const int E = p.E;
     float l[NV];
 #pragma unroll
@@ -74,8 +79,8 @@ __global__ void __launch_bounds__(256) route_topk_kernel(RouteParams p) {
     float m = -INFINITY;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-        // +inf as the largest finite number, NaN as -inf
-        l[i] = lane * NV + i < E && l[i] > -INFINITY ? fminf(l[i], 3.402823466e38f) : -INFINITY;
+        // +inf as the largest finite number, NaN as -inf, -0 as 0
+        l[i] = lane * NV + i < E && l[i] > -INFINITY ? fminf(l[i], 3.402823466e38f) + 0.f : -INFINITY;
         m = fmaxf(m, l[i]);
     }
     m = wave_max(m);
@@ -114,8 +119,8 @@ __global__ void __launch_bounds__(256) route_topk_kernel(RouteParams p) {
     if (p.groups > 1) {
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            if constexpr (BIAS) s_c[wave][lane * NV + i] = c[i];
-            else s_l[wave][lane * NV + i] = l[i];
+            if constexpr (BIAS) scratch.c[lane * NV + i] = c[i];
+            else scratch.l[lane * NV + i] = l[i];
         }
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
         __builtin_amdgcn_wave_barrier();
@@ -124,8 +129,8 @@ __global__ void __launch_bounds__(256) route_topk_kernel(RouteParams p) {
             double second = -INFINITY;
             for (int i = 0; i < p.size; ++i) {
                 double v;
-                if constexpr (BIAS) v = s_c[wave][lane * p.size + i];
-                else v = s_l[wave][lane * p.size + i];
+                if constexpr (BIAS) v = scratch.c[lane * p.size + i];
+                else v = scratch.l[lane * p.size + i];
                 second = fmax(second, fmin(v, score));
                 score = fmax(score, v);
             }
@@ -200,8 +205,297 @@ __global__ void __launch_bounds__(256) route_topk_kernel(RouteParams p) {
     }
 }
 
+template <int NV, int SRC, bool BIAS>
+__global__ void __launch_bounds__(256) route_topk_kernel(RouteParams p) {
+    __shared__ RouteScratch<NV, BIAS> scratch[4];
+    const int wave = threadIdx.x >> 6;
+    const int64_t t = (int64_t)blockIdx.x * 4 + wave;
+    if (t >= p.T) return;                       // (no work-group barrier below)
+    route_token<NV, SRC, BIAS>(p, t, threadIdx.x & 63, scratch[wave]);
+}
+
+// ---- four tokens a wave ----
+// Sixteen lanes a token, lane s holds experts nv s .. nv s + nv - 1 (at most 256 in all), picks up to 8. An expert's key
+// is its score in 24 bits over 255 - expert, so that one unsigned maximum finds score and expert: of 16-bit logits
+// without a bias the logit's own bits in their order (exact); else c in fp32, as a part of the token's range of c. Where
+// two keys that the choice hangs on lie nearer to each other than all roundings together may be off, the whole wave takes
+// the token again by route_token (about one token in 2000).
+constexpr int kTop = 8;
+
+__device__ __forceinline__ void order2(uint32_t& a, uint32_t& b) {
+    const uint32_t m = max(a, b);
+    b = min(a, b);
+    a = m;
+}
+__device__ __forceinline__ void sort8(uint32_t (&v)[8]) {        // descending, odd-even merges
+    order2(v[0], v[1]); order2(v[2], v[3]); order2(v[4], v[5]); order2(v[6], v[7]);
+    order2(v[0], v[2]); order2(v[1], v[3]); order2(v[4], v[6]); order2(v[5], v[7]);
+    order2(v[1], v[2]); order2(v[5], v[6]);
+    order2(v[0], v[4]); order2(v[1], v[5]); order2(v[2], v[6]); order2(v[3], v[7]);
+    order2(v[2], v[4]); order2(v[3], v[5]);
+    order2(v[1], v[2]); order2(v[3], v[4]); order2(v[5], v[6]);
+}
+__device__ __forceinline__ void merge8(uint32_t (&v)[8]) {       // a bitonic sequence, descending
+    order2(v[0], v[4]); order2(v[1], v[5]); order2(v[2], v[6]); order2(v[3], v[7]);
+    order2(v[0], v[2]); order2(v[1], v[3]); order2(v[4], v[6]); order2(v[5], v[7]);
+    order2(v[0], v[1]); order2(v[2], v[3]); order2(v[4], v[5]); order2(v[6], v[7]);
+}
+// The 8 largest of two lanes' lists, in both lanes.
+template <int S>
+__device__ __forceinline__ void join8(uint32_t (&v)[8]) {
+    uint32_t o[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) o[i] = max(v[i], dpp_step<S>(v[7 - i]));
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = o[i];
+    merge8(v);
+}
+__device__ __forceinline__ float row_max(float v) { return lane_allreduce<4>(v, MaxOp{}); }
+__device__ __forceinline__ float row_sum(float v) { return lane_allreduce<4>(v, SumOp{}); }
+struct AddU {
+    __device__ float operator()(float a, float b) const { return __uint_as_float(__float_as_uint(a) + __float_as_uint(b)); }
+};
+__device__ __forceinline__ uint32_t row_count(uint32_t v) { return __float_as_uint(lane_allreduce<4>(__uint_as_float(v), AddU{})); }
+__device__ __forceinline__ float exp_fast(float x) { return __builtin_amdgcn_exp2f(x * 1.44269504088896340736f); }
+// e^x to about two roundings: the rounding error of x log2(e) is put back.
+__device__ __forceinline__ float exp_near(float x) {
+    const float t = x * 1.44269504088896340736f;
+    const float lo = fmaf(x, 1.44269504088896340736f, -t) + x * 1.92596299112661746887e-8f;
+    const float e = __builtin_amdgcn_exp2f(t);
+    return t > -200.f ? fmaf(e * 0.69314718055994530942f, lo, e) : 0.f;
+}
+template <int R>
+__device__ __forceinline__ int larger_in_row(uint32_t v) {       // lanes of the row of sixteen that hold more than v
+    if constexpr (R == 0) return 0;
+    else return ((uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x120 + R, 0xF, 0xF, true) > v ? 1 : 0) + larger_in_row<R - 1>(v);
+}
+
+template <int NV, int SRC, bool BIAS>
+__global__ void __launch_bounds__(256) route_rows_kernel(RouteParams p) {
+    constexpr bool EXACT = !BIAS && SRC != 0;
+    __shared__ RouteScratch<4, BIAS> scratch[4];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, row = lane >> 4, sub = lane & 15;
+    const int64_t t0 = ((int64_t)blockIdx.x * 4 + wave) * 4;
+    if (t0 >= p.T) return;                      // (no work-group barrier below)
+    const int64_t t = min(t0 + row, p.T - 1), at = t * p.ldl;
+    const int nv = p.nv, e0 = sub * nv, E = p.E;
+
+    // ---- logits ----
+    float l[NV];
+    uint32_t bits[NV];                          // EXACT: the logit's own, in their order
+    auto one = [&](int i, uint32_t raw) __attribute__((always_inline)) {
+        const bool in = i < nv && e0 + i < E;
+        if constexpr (SRC == 0) l[i] = __uint_as_float(raw);
+        else if constexpr (SRC == 2) l[i] = __uint_as_float(raw << 16);
+        else l[i] = __half2float(__ushort_as_half((uint16_t)raw));
+        const bool live = in && l[i] > -INFINITY;
+        if constexpr (EXACT) {
+            const uint32_t b = raw == 0x8000u ? 0u : raw;
+            bits[i] = live ? ((b & 0x8000u) ? ~b & 0xFFFFu : b | 0x8000u) : 0u;
+        }
+        l[i] = live ? fminf(l[i], 3.402823466e38f) : -INFINITY;
+    };
+    if (p.vec) {                                // a lane's logits are whole pieces of 16 bytes
+        constexpr int per = SRC == 0 ? 4 : 8;
+        u32x4 v[(NV + per - 1) / per];
+#pragma unroll
+        for (int i = 0; i < NV; i += per)
+            v[i / per] = reinterpret_cast<const u32x4*>(reinterpret_cast<const char*>(p.logits) +
+                                                        (at + min(e0 + i, E - per)) * (SRC == 0 ? 4 : 2))[0];
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const uint32_t w = v[i / per][SRC == 0 ? i % 4 : i % 8 / 2];
+            one(i, SRC == 0 ? w : i % 2 ? w >> 16 : w & 0xFFFFu);
+        }
+    } else {
+        uint32_t v[NV];
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int64_t a = at + min(e0 + min(i, nv - 1), E - 1);
+            if constexpr (SRC == 0) v[i] = reinterpret_cast<const uint32_t*>(p.logits)[a];
+            else v[i] = reinterpret_cast<const uint16_t*>(p.logits)[a];
+        }
+#pragma unroll
+        for (int i = 0; i < NV; ++i) one(i, v[i]);
+    }
+    float m = l[0];
+#pragma unroll
+    for (int i = 1; i < NV; ++i) m = fmaxf(m, l[i]);
+    m = row_max(m);
+    if (m == -INFINITY) m = 0.f;
+
+    // ---- scores: c, off by no more than `off` ----
+    float c[NV], sum = 1.f, off = 0.f;
+    if (!p.sigmoid && (BIAS || !p.renorm)) {
+        sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            c[i] = exp_fast(l[i] - m);
+            sum += c[i];
+        }
+        sum = row_sum(sum);
+    }
+    if constexpr (BIAS) {
+        const float inv = 1.0f / sum;
+        float top = 0.f;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const float b = p.bias[min(e0 + min(i, nv - 1), E - 1)];
+            const float s = p.sigmoid ? __builtin_amdgcn_rcpf(1.0f + exp_fast(-l[i])) : c[i] * inv;
+            c[i] = l[i] > -INFINITY && s + b > -INFINITY ? s + b : -INFINITY;
+            top = fmaxf(top, fabsf(b));
+        }
+        // In units of 2^-24: e^x is off by (2 |x| + 2) e^x, a softmax's sum by as much of each term (2 |x| e^x adds up to
+        // no more than 2 ln 256 of it) and 8 of its tree, the quotient by 3 more: below 32 for p up to 1; a sigmoid by
+        // less than 8. The sum with b by half a step.
+        off = (32.f + 1.f + row_max(top)) * 0x1p-24f;
+    } else {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) c[i] = l[i];
+    }
+
+    // ---- groups: lanes of a group hold its score, and how many lanes hold a larger one ----
+    bool sure = true;
+    bool kept = true;
+    if (p.groups > 1) {
+        float first = -INFINITY, second = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            second = fmaxf(second, fminf(first, c[i]));
+            first = fmaxf(first, c[i]);
+        }
+        auto join = [&](auto step) __attribute__((always_inline)) {
+            constexpr int S = decltype(step)::value;
+            const float f = __uint_as_float(dpp_step<S>(__float_as_uint(first)));
+            const float s = __uint_as_float(dpp_step<S>(__float_as_uint(second)));
+            second = fmaxf(fminf(first, f), fmaxf(second, s));
+            first = fmaxf(first, f);
+        };
+        const int lanes = p.size / nv;          // of a group: 1, 2, 4, 8 or 16
+        if (lanes > 1) join(std::integral_constant<int, 0>{});
+        if (lanes > 2) join(std::integral_constant<int, 1>{});
+        if (lanes > 4) join(std::integral_constant<int, 2>{});
+        if (lanes > 8) join(std::integral_constant<int, 3>{});
+        const float score = first + (BIAS && second > -INFINITY ? second : 0.f);
+        uint32_t group_key = order_key(score);
+        if constexpr (EXACT) {                  // with the group's number: no two are equal
+            uint32_t top = 0;
+#pragma unroll
+            for (int i = 0; i < NV; ++i) top = max(top, bits[i]);
+            if (lanes > 1) top = max(top, dpp_step<0>(top));
+            if (lanes > 2) top = max(top, dpp_step<1>(top));
+            if (lanes > 4) top = max(top, dpp_step<2>(top));
+            if (lanes > 8) top = max(top, dpp_step<3>(top));
+            group_key = top << 8 | (uint32_t)(255 - e0 / p.size);
+        }
+        kept = larger_in_row<15>(group_key) < p.top_groups * lanes;
+        // (equal groups at the border are kept together)
+        sure = row_count(kept ? 1u : 0u) == (uint32_t)(p.top_groups * lanes);
+        if constexpr (BIAS) {
+            const float least = -row_max(kept ? -score : -INFINITY), out = row_max(kept ? -INFINITY : score);
+            sure = sure && (out == -INFINITY || least - out > 4.f * off + fabsf(least) * 0x1p-22f);
+        }
+    }
+
+    // ---- keys ----
+    uint32_t key[NV], tol = 0;
+    if constexpr (EXACT) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) key[i] = bits[i] != 0u && kept ? bits[i] << 8 | (uint32_t)(255 - e0 - i) : 0u;
+    } else {
+        float hi = -INFINITY, lo = INFINITY;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            hi = fmaxf(hi, c[i]);
+            lo = fminf(lo, c[i] > -INFINITY ? c[i] : INFINITY);
+        }
+        hi = row_max(hi);
+        lo = -row_max(-lo);
+        const float span = hi - lo;
+        sure = sure && (hi == -INFINITY || (span < 1e30f && span > 1e-30f));
+        const float f = 16777000.f / span;
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+            key[i] = c[i] > -INFINITY && kept ? ((uint32_t)((c[i] - lo) * f) + 1u) << 8 | (uint32_t)(255 - e0 - i) : 0u;
+        tol = 8u + (uint32_t)fminf(2.f * off * f, 16777216.f);   // (three units a key for the arithmetic just done)
+    }
+
+    // ---- the eight largest keys of the row, in all its lanes ----
+    uint32_t best[kTop];
+#pragma unroll
+    for (int i = 0; i < kTop; ++i) best[i] = i < NV ? key[i < NV ? i : 0] : 0u;
+    if constexpr (NV > 1) sort8(best);
+    if constexpr (NV > kTop) {
+        uint32_t more[kTop];
+#pragma unroll
+        for (int i = 0; i < kTop; ++i) more[i] = key[i + kTop < NV ? i + kTop : 0];
+        sort8(more);
+#pragma unroll
+        for (int i = 0; i < kTop; ++i) best[i] = max(best[i], more[kTop - 1 - i]);
+        merge8(best);
+    }
+    join8<0>(best);
+    join8<1>(best);
+    join8<2>(best);
+    join8<3>(best);
+    if constexpr (!EXACT) {
+        // picks in doubt among themselves, or the last of them with one that was not picked
+        uint32_t last = 0;
+#pragma unroll
+        for (int i = 0; i < kTop; ++i) {
+            if (i + 1 < kTop && i + 1 < p.top_k && best[i + 1] != 0u) sure = sure && (best[i] >> 8) - (best[i + 1] >> 8) > tol;
+            if (i + 1 == p.top_k) last = best[i];
+        }
+        uint32_t near = 0;
+        const uint32_t from = (last >> 8) > tol ? (last >> 8) - tol : 1u;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) near += (key[i] >> 8) >= from && key[i] != 0u ? 1u : 0u;
+        sure = sure && (last == 0u || row_count(near) == (uint32_t)p.top_k);
+    }
+
+    // ---- weights: lane j has pick j ----
+    uint32_t mine = 0;
+#pragma unroll
+    for (int i = 0; i < kTop; ++i) mine = sub == i && i < p.top_k ? best[i] : mine;
+    const int e = 255 - (int)(mine & 255u);
+    float w = 0.f;
+    if (mine != 0u) {
+        const float x = fminf(logit_at<SRC>(p.logits, at + e), 3.402823466e38f);
+        // (of a sigmoid the smaller of e^x and e^-x, which is a number)
+        const float ex = exp_near(p.sigmoid ? -fabsf(x) : x - m);
+        w = !p.sigmoid ? ex : x < 0.f ? ex / (1.0f + ex) : 1.0f / (1.0f + ex);
+    }
+    if (p.renorm) {
+        const float total = row_sum(w);
+        sure = sure && (total > 1e-30f || row_count(mine != 0u ? 1u : 0u) == 0u);
+        w = total > 0.f ? w / total : 0.f;
+    } else if (!p.sigmoid && mine != 0u) {
+        w /= sum;
+    }
+    // (weights near fp32's least numbers: by route_token too)
+    sure = sure && row_count(mine != 0u && !(w > 1e-30f) ? 1u : 0u) == 0u;
+    if (sure && t0 + row < p.T && sub < p.top_k) {
+        p.tw[t * p.top_k + sub] = w * p.scale;
+        p.ids[t * p.top_k + sub] = mine != 0u ? e : -1;
+    }
+    const uint64_t again = __ballot(!sure);
+    if (again == 0) return;
+    for (int r = 0; r < 4; ++r)
+        if ((again >> (16 * r) & 0xFFFF) != 0 && t0 + r < p.T) route_token<4, SRC, BIAS>(p, t0 + r, lane, scratch[wave]);
+}
+
 template <int SRC, bool BIAS>
 int route_go(const RouteParams& p, hipStream_t s) {
+    // Four tokens a wave: up to 256 experts and 8 picks, groups of whole lanes, a power of two of them.
+    const int lanes = p.size / p.nv;
+    if (p.E <= 256 && p.top_k <= kTop &&
+        (p.groups == 1 || (p.E == 16 * p.nv && p.size % p.nv == 0 && (lanes & (lanes - 1)) == 0 && lanes <= 16))) {
+        const dim3 grid((unsigned)((p.T + 15) / 16));
+        if (p.nv <= 4) launch_kernel(&route_rows_kernel<4, SRC, BIAS>, grid, dim3(256), 0, s, p);
+        else if (p.nv <= 8) launch_kernel(&route_rows_kernel<8, SRC, BIAS>, grid, dim3(256), 0, s, p);
+        else launch_kernel(&route_rows_kernel<16, SRC, BIAS>, grid, dim3(256), 0, s, p);
+        return check_launch("route_rows_kernel");
+    }
     const dim3 grid((unsigned)((p.T + 3) / 4));
     if (p.E <= 64) launch_kernel(&route_topk_kernel<1, SRC, BIAS>, grid, dim3(256), 0, s, p);
     else if (p.E <= 128) launch_kernel(&route_topk_kernel<2, SRC, BIAS>, grid, dim3(256), 0, s, p);
@@ -214,8 +508,11 @@ int route_go(const RouteParams& p, hipStream_t s) {
 }  // namespace
 
 int launch_route_topk(const RouteArgs& a, hipStream_t s) {
+    const int nv = (int)((a.E + 15) / 16), size = a.dtype == W4A8_DTYPE_F32 ? 4 : 2;
+    const bool vec = nv * size % 16 == 0 && a.E == 16 * nv && reinterpret_cast<uintptr_t>(a.logits) % 16 == 0 &&
+                     (a.ldl * size % 16 == 0 || a.T == 1);
     const RouteParams p{a.logits, a.bias, a.tw, a.ids, a.T, a.ldl, (int)a.E, (int)a.top_k, (int)a.groups, (int)a.top_groups,
-                        (int)(a.E / a.groups), a.sigmoid ? 1 : 0, a.renorm ? 1 : 0, a.scale};
+                        (int)(a.E / a.groups), a.sigmoid ? 1 : 0, a.renorm ? 1 : 0, a.scale, nv, vec ? 1 : 0};
     if (a.dtype == W4A8_DTYPE_F32) return a.bias ? route_go<0, true>(p, s) : route_go<0, false>(p, s);
     if (a.dtype == W4A8_DTYPE_F16) return a.bias ? route_go<1, true>(p, s) : route_go<1, false>(p, s);
     return a.bias ? route_go<2, true>(p, s) : route_go<2, false>(p, s);
