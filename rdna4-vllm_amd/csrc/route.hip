@@ -28,7 +28,7 @@ struct RouteParams {
     int E, top_k, groups, top_groups, size;    // size: experts of a group
     int sigmoid, renorm;
     float scale;
-    int nv, vec;                               // sixteen lanes a token: experts a lane; whole pieces of 16 bytes each
+    int nv, vec, bias_vec;                     // sixteen lanes a token: experts a lane; whole pieces of 16 bytes each
 };
 
 __device__ __forceinline__ uint32_t order_key(float v) {       // larger for a larger value, 0 for none
@@ -217,9 +217,10 @@ __global__ void __launch_bounds__(256) route_topk_kernel(RouteParams p) {
 // ---- four tokens a wave ----
 // Sixteen lanes a token, lane s holds experts nv s .. nv s + nv - 1 (at most 256 in all), picks up to 8. An expert's key
 // is its score in 24 bits over 255 - expert, so that one unsigned maximum finds score and expert: of 16-bit logits
-// without a bias the logit's own bits in their order (exact); else c in fp32, as a part of the token's range of c. Where
-// two keys that the choice hangs on lie nearer to each other than all roundings together may be off, the whole wave takes
-// the token again by route_token (about one token in 2000).
+// without a bias the logit's own bits in their order (exact); else c in fp32, as a part of its range. Picks whose keys lie
+// nearer to each other, or to one that was not picked, than all roundings together may be off are put in order by their c
+// in fp64 (about one token in 2000); where groups, several others or a softmax's sum are in doubt, the whole wave takes the
+// token again by route_token
 constexpr int kTop = 8;
 
 __device__ __forceinline__ void order2(uint32_t& a, uint32_t& b) {
@@ -325,7 +326,7 @@ __global__ void __launch_bounds__(256) route_rows_kernel(RouteParams p) {
     if (m == -INFINITY) m = 0.f;
 
     // ---- scores: c, off by no more than `off` ----
-    float c[NV], sum = 1.f, off = 0.f;
+    float c[NV], sum = 1.f, off = 0.f, top = 0.f;                // top: of the biases' magnitudes
     if (!p.sigmoid && (BIAS || !p.renorm)) {
         sum = 0.f;
 #pragma unroll
@@ -337,18 +338,30 @@ __global__ void __launch_bounds__(256) route_rows_kernel(RouteParams p) {
     }
     if constexpr (BIAS) {
         const float inv = 1.0f / sum;
-        float top = 0.f;
+        float b[NV];
+        if (nv % 4 == 0 && p.bias_vec) {
+#pragma unroll
+            for (int i = 0; i < NV; i += 4) {
+                const v4f v = *reinterpret_cast<const v4f*>(p.bias + min(e0 + i, E - 4));
+#pragma unroll
+                for (int r = 0; r < 4; ++r) b[i + r] = v[r];
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < NV; ++i) b[i] = p.bias[min(e0 + min(i, nv - 1), E - 1)];
+        }
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            const float b = p.bias[min(e0 + min(i, nv - 1), E - 1)];
             const float s = p.sigmoid ? __builtin_amdgcn_rcpf(1.0f + exp_fast(-l[i])) : c[i] * inv;
-            c[i] = l[i] > -INFINITY && s + b > -INFINITY ? s + b : -INFINITY;
-            top = fmaxf(top, fabsf(b));
+            // (a NaN counts for neither maximum nor key)
+            c[i] = l[i] > -INFINITY ? s + b[i] : -INFINITY;
+            top = fmaxf(top, i < nv ? fabsf(b[i]) < INFINITY ? fabsf(b[i]) : 0.f : 0.f);
         }
+        top = row_max(top);
         // In units of 2^-24: e^x is off by (2 |x| + 2) e^x, a softmax's sum by as much of each term (2 |x| e^x adds up to
         // no more than 2 ln 256 of it) and 8 of its tree, the quotient by 3 more: below 32 for p up to 1; a sigmoid by
         // less than 8. The sum with b by half a step.
-        off = (32.f + 1.f + row_max(top)) * 0x1p-24f;
+        off = ((p.sigmoid ? 8.f : 32.f) + 1.f + top) * 0x1p-24f;
     } else {
 #pragma unroll
         for (int i = 0; i < NV; ++i) c[i] = l[i];
@@ -401,23 +414,25 @@ __global__ void __launch_bounds__(256) route_rows_kernel(RouteParams p) {
     uint32_t key[NV], tol = 0;
     if constexpr (EXACT) {
 #pragma unroll
-        for (int i = 0; i < NV; ++i) key[i] = bits[i] != 0u && kept ? bits[i] << 8 | (uint32_t)(255 - e0 - i) : 0u;
+        for (int i = 0; i < NV; ++i) key[i] = kept ? bits[i] << 8 | (uint32_t)(255 - e0 - i) : 0u;
     } else {
-        float hi = -INFINITY, lo = INFINITY;
+        // Scores with a bias lie in [-top, 1 + top], logits are taken between the row's largest and smallest. The mapping
+        // grows with c, so that only what c is off by, and the cut to whole numbers, can hide an order.
+        float lo = -top, span = 1.f + 2.f * top;
+        if constexpr (!BIAS) {
+            lo = INFINITY;
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            hi = fmaxf(hi, c[i]);
-            lo = fminf(lo, c[i] > -INFINITY ? c[i] : INFINITY);
+            for (int i = 0; i < NV; ++i) lo = fminf(lo, c[i] > -INFINITY ? c[i] : INFINITY);
+            lo = -row_max(-lo);
+            span = m - lo;
         }
-        hi = row_max(hi);
-        lo = -row_max(-lo);
-        const float span = hi - lo;
-        sure = sure && (hi == -INFINITY || (span < 1e30f && span > 1e-30f));
-        const float f = 16777000.f / span;
+        const bool some = lo < INFINITY;
+        sure = sure && (!some || (span < 1e30f && span > 1e-30f));
+        const float f = some && kept ? 16777000.f / span : 0.f, o = some && kept ? 2.f : 0.f;
 #pragma unroll
-        for (int i = 0; i < NV; ++i)
-            key[i] = c[i] > -INFINITY && kept ? ((uint32_t)((c[i] - lo) * f) + 1u) << 8 | (uint32_t)(255 - e0 - i) : 0u;
-        tol = 8u + (uint32_t)fminf(2.f * off * f, 16777216.f);   // (three units a key for the arithmetic just done)
+        for (int i = 0; i < NV; ++i)            // (-inf and NaN become 0)
+            key[i] = (uint32_t)__builtin_amdgcn_fmed3f(fmaf(c[i] - lo, f, o), 0.f, 16777215.f) << 8 | (uint32_t)(255 - e0 - i);
+        tol = 4u + (uint32_t)fminf(2.f * off * (16777000.f / span), 16777216.f);
     }
 
     // ---- the eight largest keys of the row, in all its lanes ----
@@ -438,32 +453,67 @@ __global__ void __launch_bounds__(256) route_rows_kernel(RouteParams p) {
     join8<1>(best);
     join8<2>(best);
     join8<3>(best);
-    if constexpr (!EXACT) {
-        // picks in doubt among themselves, or the last of them with one that was not picked
-        uint32_t last = 0;
+    // lane j: pick j (a key below 256 is no expert)
+    uint32_t mine = 0, last = 0;
+    bool doubt = false;
 #pragma unroll
-        for (int i = 0; i < kTop; ++i) {
-            if (i + 1 < kTop && i + 1 < p.top_k && best[i + 1] != 0u) sure = sure && (best[i] >> 8) - (best[i + 1] >> 8) > tol;
-            if (i + 1 == p.top_k) last = best[i];
-        }
-        uint32_t near = 0;
-        const uint32_t from = (last >> 8) > tol ? (last >> 8) - tol : 1u;
-#pragma unroll
-        for (int i = 0; i < NV; ++i) near += (key[i] >> 8) >= from && key[i] != 0u ? 1u : 0u;
-        sure = sure && (last == 0u || row_count(near) == (uint32_t)p.top_k);
+    for (int i = 0; i < kTop; ++i) {
+        mine = sub == i && i < p.top_k ? best[i] : mine;
+        if (i + 1 == p.top_k) last = best[i];
+        // picks in doubt among themselves
+        if (!EXACT && i + 1 < kTop && i + 1 < p.top_k)
+            doubt = doubt || (best[i + 1] > 255u && (best[i] >> 8) - (best[i + 1] >> 8) <= tol);
     }
-
-    // ---- weights: lane j has pick j ----
-    uint32_t mine = 0;
+    if constexpr (!EXACT) {
+        // the last of them with others that were not picked: one of those is taken along
+        const uint32_t from = last > 255u ? ((last >> 8) > tol ? (last >> 8) - tol : 1u) << 8 : ~0u;
+        uint32_t near = 0, next = 0;
 #pragma unroll
-    for (int i = 0; i < kTop; ++i) mine = sub == i && i < p.top_k ? best[i] : mine;
+        for (int i = 0; i < NV; ++i) {
+            near += key[i] >= from ? 1u : 0u;
+            next = max(next, key[i] < last ? key[i] : 0u);
+        }
+        near = row_count(near);
+        if (near > (uint32_t)p.top_k && last > 255u) {
+            doubt = true;
+            sure = sure && near == (uint32_t)p.top_k + 1;
+        }
+        if (__ballot(doubt) != 0) {
+            next = __float_as_uint(lane_allreduce<4>(__uint_as_float(next), UMax{}));
+            if (doubt && near > (uint32_t)p.top_k && sub == p.top_k) mine = next;
+        }
+    }
+    mine = mine > 255u ? mine : 0u;
+
+    // ---- weights ----
     const int e = 255 - (int)(mine & 255u);
-    float w = 0.f;
+    float w = 0.f, x = -INFINITY;
     if (mine != 0u) {
-        const float x = fminf(logit_at<SRC>(p.logits, at + e), 3.402823466e38f);
+        x = fminf(logit_at<SRC>(p.logits, at + e), 3.402823466e38f);
         // (of a sigmoid the smaller of e^x and e^-x, which is a number)
         const float ex = exp_near(p.sigmoid ? -fabsf(x) : x - m);
         w = !p.sigmoid ? ex : x < 0.f ? ex / (1.0f + ex) : 1.0f / (1.0f + ex);
+    }
+    int place = sub;
+    if (!EXACT && __ballot(doubt) != 0) {
+        // In doubt: sigmoids with a bias, and logits, are compared in fp64 among the row's lanes; a softmax with a bias
+        // needs its sum in fp64 too.
+        if (BIAS && !p.sigmoid) sure = sure && !doubt;
+        double d = -INFINITY;
+        if (mine != 0u) d = !BIAS ? (double)x : 1.0 / (1.0 + exp(-(double)x)) + (double)p.bias[e];
+        int rank = 0;
+        for (int j = 0; j <= kTop; ++j) {
+            const double other = __shfl(d, row * 16 + j);
+            const int oe = __shfl(e, row * 16 + j);
+            rank += other > d || (other == d && oe < e) ? 1 : 0;
+        }
+        if (doubt) {
+            place = mine != 0u ? rank : sub;
+            if (place >= p.top_k) {
+                mine = 0u;
+                w = 0.f;
+            }
+        }
     }
     if (p.renorm) {
         const float total = row_sum(w);
@@ -474,9 +524,9 @@ __global__ void __launch_bounds__(256) route_rows_kernel(RouteParams p) {
     }
     // (weights near fp32's least numbers: by route_token too)
     sure = sure && row_count(mine != 0u && !(w > 1e-30f) ? 1u : 0u) == 0u;
-    if (sure && t0 + row < p.T && sub < p.top_k) {
-        p.tw[t * p.top_k + sub] = w * p.scale;
-        p.ids[t * p.top_k + sub] = mine != 0u ? e : -1;
+    if (sure && t0 + row < p.T && place < p.top_k) {
+        p.tw[t * p.top_k + place] = w * p.scale;
+        p.ids[t * p.top_k + place] = mine != 0u ? e : -1;
     }
     const uint64_t again = __ballot(!sure);
     if (again == 0) return;
@@ -512,7 +562,7 @@ int launch_route_topk(const RouteArgs& a, hipStream_t s) {
     const bool vec = nv * size % 16 == 0 && a.E == 16 * nv && reinterpret_cast<uintptr_t>(a.logits) % 16 == 0 &&
                      (a.ldl * size % 16 == 0 || a.T == 1);
     const RouteParams p{a.logits, a.bias, a.tw, a.ids, a.T, a.ldl, (int)a.E, (int)a.top_k, (int)a.groups, (int)a.top_groups,
-                        (int)(a.E / a.groups), a.sigmoid ? 1 : 0, a.renorm ? 1 : 0, a.scale, nv, vec ? 1 : 0};
+                        (int)(a.E / a.groups), a.sigmoid ? 1 : 0, a.renorm ? 1 : 0, a.scale, nv, vec ? 1 : 0, a.E % 4 == 0 && reinterpret_cast<uintptr_t>(a.bias) % 16 == 0 ? 1 : 0};
     if (a.dtype == W4A8_DTYPE_F32) return a.bias ? route_go<0, true>(p, s) : route_go<0, false>(p, s);
     if (a.dtype == W4A8_DTYPE_F16) return a.bias ? route_go<1, true>(p, s) : route_go<1, false>(p, s);
     return a.bias ? route_go<2, true>(p, s) : route_go<2, false>(p, s);
