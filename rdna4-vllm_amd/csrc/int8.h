@@ -76,7 +76,6 @@ struct RowsArgs {
     const int32_t* emap;         // global -> local expert, or null
     int64_t emap_len, slots, top_k;
     bool gather;                 // slot s reads x[s / top_k], else x[s]
-    bool single;                 // a work-group takes one slot, not an expert's
     Out8 dst;                    // out rows are slots (dense: rows)
     bool bf16;
     void* out;
@@ -108,7 +107,7 @@ struct RowsParams : OutParams {
     const float* xs;
     const int32_t* ids;
     const int32_t* emap;
-    int rows, slots, emap_len, single;
+    int rows, slots, emap_len, by_slot;
 };
 
 template <typename A>
@@ -132,7 +131,7 @@ inline RowsParams rows_params(const RowsArgs& a) {
     RowsParams p;
     out_params(a, p);
     p.x = a.x; p.xs = a.xs; p.ids = a.ids; p.emap = a.emap;
-    p.rows = (int)a.rows; p.slots = (int)a.slots; p.emap_len = (int)a.emap_len; p.single = a.single ? 1 : 0;
+    p.rows = (int)a.rows; p.slots = (int)a.slots; p.emap_len = (int)a.emap_len; p.by_slot = 0;
     return p;
 }
 

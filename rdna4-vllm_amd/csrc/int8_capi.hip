@@ -27,6 +27,10 @@ constexpr int64_t kMaxSide = (int64_t)1 << 24;    // rows of a weight
 constexpr int64_t kStreamRows = 16;               // dense rows up to which the weights are streamed
 constexpr int64_t kMaxRows = ((int64_t)1 << 31) - 256;
 
+// Dense rows that the product's kernel quantises itself; more take a launch of their own (4096 x 4096, us in the kernel /
+// before it: 1 row 8.9 / 10.5, 4 10.5 / 11, 16 18.7 / 11.8).
+bool quantised_in_kernel(int64_t M, int64_t K) { return M <= 4 && int8_rows_quantised_in_kernel(K); }
+
 // Sizes and pointers that every product shares.
 int check_product(const void* x, int x_dtype, const float* xs, int64_t rows, int64_t K, int64_t ldx, const int8_t* w,
                   const float* ws, int64_t E, int64_t N) {
@@ -53,7 +57,7 @@ int check_product(const void* x, int x_dtype, const float* xs, int64_t rows, int
 // Slots an expert from which tiles have 128 rows.
 constexpr int64_t kWideRows = 192;
 struct LayerPlan {
-    bool tiles, single;
+    bool tiles;
     int64_t part;                // tokens of a part
     int64_t block_m;             // tiles: rows of a block
     int64_t P, nblk;             // of a part: padded rows and blocks
@@ -62,7 +66,7 @@ struct LayerPlan {
 LayerPlan plan_layer(int64_t T, int64_t H, int64_t inter, int64_t E, int64_t top_k, int x_dtype) {
     LayerPlan pl{};
     const int64_t lim = ((int64_t)1 << 32) - 1, pad = E * 127 + 128;
-    pl.tiles = T * top_k > std::min<int64_t>(12 * E, kScanSlots) && 2 * inter * H <= lim;
+    pl.tiles = T * top_k > std::min<int64_t>(5 * E + 128, kScanSlots) && 2 * inter * H <= lim;
     const int64_t most = pl.tiles ? std::min(lim / H, (lim / inter - pad) / top_k) : kScanSlots / top_k;
     pl.part = std::min(T, std::max<int64_t>(1, most));
     const int64_t n = pl.part * top_k;
@@ -70,8 +74,6 @@ LayerPlan plan_layer(int64_t T, int64_t H, int64_t inter, int64_t E, int64_t top
     // every block in use holds a slot
     pl.P = pl.tiles ? std::min((n + E * (pl.block_m - 1) + pl.block_m - 1) / pl.block_m * pl.block_m, n * pl.block_m) : n;
     pl.nblk = pl.P / pl.block_m;
-    // few slots: hardly two of one expert
-    pl.single = n * 8 <= E;
     pl.quant_x = x_dtype != W4A8_DTYPE_INT8 && (pl.tiles || !int8_rows_quantised_in_kernel(H));
     pl.quant_h = pl.tiles || !int8_rows_quantised_in_kernel(inter);
     return pl;
@@ -154,7 +156,7 @@ int run_layer(const Layer& l, const LayerPlan& pl, const LayerScratch& m, hipStr
         g1.x = x; g1.src = pl.quant_x ? Src8::kI8 : src_of(l.x_dtype); g1.xs = xs; g1.rows = l.T; g1.K = l.H; g1.ldx = l.H;
         g1.w = l.w13; g1.ws = l.s13; g1.E = l.E; g1.N = 2 * l.inter;
         g1.ids = l.ids; g1.emap = l.emap; g1.emap_len = l.n_global; g1.slots = n; g1.top_k = l.top_k;
-        g1.gather = true; g1.single = pl.single; g1.dst = Out8::kSiluF32; g1.out = m.h; g1.ldo = l.inter;
+        g1.gather = true; g1.dst = Out8::kSiluF32; g1.out = m.h; g1.ldo = l.inter;
         if (int rc = launch_int8_rows(g1, s)) return rc;
         RowsArgs g2 = g1;
         g2.x = m.h; g2.src = Src8::kF32; g2.rows = n; g2.K = l.inter; g2.ldx = l.inter;
@@ -197,7 +199,7 @@ int w4a8_act_quant_int8(const void* x, int x_dtype, int64_t rows, int64_t K, int
 }
 
 size_t w4a8_int8_gemm_workspace_size(int x_dtype, int64_t M, int64_t K) {
-    if (x_dtype == W4A8_DTYPE_INT8 || M <= 0 || K <= 0 || (M <= kStreamRows && int8_rows_quantised_in_kernel(K))) return 0;
+    if (x_dtype == W4A8_DTYPE_INT8 || M <= 0 || K <= 0 || quantised_in_kernel(M, K)) return 0;
     WorkspaceSize s;
     s.take<int8_t>((size_t)(M * K));
     s.take<float>((size_t)M);
@@ -213,7 +215,7 @@ int w4a8_int8_gemm(const void* x, int x_dtype, const float* x_scales, int64_t M,
     if (M == 0) return W4A8_OK;
     W4A8_REQUIRE(out, "int8_gemm: null pointer");
     hipStream_t s = as_stream(stream);
-    const bool in_kernel = M <= kStreamRows && int8_rows_quantised_in_kernel(K);
+    const bool in_kernel = quantised_in_kernel(M, K);
     Src8 src = src_of(x_dtype);
     if (src != Src8::kI8 && !in_kernel) {
         Workspace ws(workspace, workspace_bytes);

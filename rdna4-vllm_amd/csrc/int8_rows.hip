@@ -5,8 +5,8 @@
 // row c, for rows and weights alike (a sum of whole numbers may take its k in any order). Weights are the first
 // operand: a lane ends up with four adjacent columns of one row.
 //
-// Grouped, a work-group finds its rows itself: it scans the routed ids for the slots of its expert (or, of few slots,
-// takes one slot), so that no launch has to sort them first.
+// Grouped, a work-group finds its rows itself: it scans the routed ids for the slots of its expert, so that no launch has
+// to sort them first.
 //
 // int8_rows_kernel holds its rows in registers (16 rows by GPW steps a wave, quantised there where they come in 16 or 32
 // bits) and walks over column fragments with D of them in flight; KS waves share K and add their sums in LDS.
@@ -30,89 +30,86 @@ __device__ __forceinline__ int expert_of(const RowsParams& p, int i) {
     if (p.emap != nullptr) e = e >= 0 && e < p.emap_len ? p.emap[e] : -1;
     return e >= 0 && e < p.E ? e : -1;
 }
-// Group g of rows: dense, all of them; with `single`, slot g; else the slots of expert g, in order, in `list`.
-// WAVES: of the work-group, all of which call this.
+// Group g of rows: dense, all of them; else the slots of one expert, in order, in `list`: of expert g, or (by_slot, for
+// fewer slots than experts) of slot g's expert, where slot g is its first. WAVES: of the work-group, all of which call
+// this.
 template <int WAVES>
 __device__ __forceinline__ Routed find_rows(const RowsParams& p, int g, uint16_t* list, int* counts) {
     if (p.ids == nullptr) return {0, p.rows};
-    if (p.single) {
-        const int e = expert_of(p, g);
-        return {e, e >= 0 ? 1 : 0};
-    }
+    const int e = p.by_slot ? __builtin_amdgcn_readfirstlane(expert_of(p, g)) : g;
+    if (e < 0) return {0, 0};
     constexpr int kMost = kScanSlots / (64 * WAVES);             // slots a lane
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int per = (p.slots + 64 * WAVES - 1) / (64 * WAVES);   // steps of 64 slots a wave
     const int first = wave * per * 64 + lane;
-    uint32_t mine = 0;                                           // bit i: slot first + 64 i
+    uint32_t mine = 0, sooner = 0;                               // bit i: slot first + 64 i
 #pragma unroll 4
     for (int i = 0; i < kMost; ++i) {
         if (i >= per) break;
         const int s = first + 64 * i;
-        if (s < p.slots && expert_of(p, s) == g) mine |= 1u << i;
+        if (s < p.slots && expert_of(p, s) == e) {
+            mine |= 1u << i;
+            sooner |= s < g ? 1u : 0u;
+        }
     }
-    int before = 0;
-    for (int i = 0; i < per; ++i) before += __popcll(__ballot(mine >> i & 1));
-    if (lane == 0) counts[wave] = before;
+    int n = 0;
+    for (int i = 0; i < per; ++i) n += __popcll(__ballot(mine >> i & 1));
+    const bool late = p.by_slot && __ballot(sooner != 0) != 0;
+    if (lane == 0) counts[wave] = late ? -1 : n;
     __syncthreads();
-    int at = 0, n = 0;
+    int at = 0;
+    n = 0;
 #pragma unroll
     for (int w = 0; w < WAVES; ++w) {
+        if (counts[w] < 0) return {e, 0};                        // (all waves)
         if (w < wave) at += counts[w];
         n += counts[w];
     }
-    if (n == 0) return {g, 0};
+    if (n == 0) return {e, 0};
     for (int i = 0; i < per; ++i) {
         const uint64_t m = __ballot(mine >> i & 1);
         if (mine >> i & 1) list[at + __popcll(m & ((1ull << lane) - 1))] = (uint16_t)(first + 64 * i);
         at += __popcll(m);
     }
     __syncthreads();
-    return {g, n};
+    return {e, n};
 }
 // Row r of the group: its slot (dense: r), -1 past the end.
-__device__ __forceinline__ int slot_at(const RowsParams& p, const Routed& d, int g, int r, const uint16_t* list) {
+__device__ __forceinline__ int slot_at(const RowsParams& p, const Routed& d, int r, const uint16_t* list) {
     if (r >= d.n) return -1;
-    return p.ids == nullptr ? r : p.single ? g : list[r];
+    return p.ids == nullptr ? r : list[r];
 }
 
 // ---- rows' values ----
 template <Src8 SRC>
 constexpr int kSrcBytes = SRC == Src8::kI8 ? 1 : SRC == Src8::kF32 ? 4 : 2;
 template <Src8 SRC>
-struct RawStep {                                                 // a lane's 32 values of one step
-    u32x4 v[2 * kSrcBytes<SRC>];
-    __device__ __forceinline__ void load(const uint8_t* row, int g, int q, int K) {
+struct Raw8 {                                                    // eight values of a row
+    u32x4 v[SRC == Src8::kF32 ? 2 : 1];
+    __device__ __forceinline__ void load(const uint8_t* row, int k) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int k = min(g * kStep + h * 64 + q * 16, K - 16);
-#pragma unroll
-            for (int b = 0; b < kSrcBytes<SRC>; ++b)
-                v[h * kSrcBytes<SRC> + b] = *reinterpret_cast<const u32x4*>(row + (int64_t)k * kSrcBytes<SRC> + 16 * b);
-        }
+        for (int b = 0; b < (SRC == Src8::kF32 ? 2 : 1); ++b)
+            v[b] = *reinterpret_cast<const u32x4*>(row + (int64_t)k * kSrcBytes<SRC> + 16 * b);
     }
-    __device__ __forceinline__ float value(int h, int t) const {
-        if constexpr (SRC == Src8::kF32) return __uint_as_float(v[h * 4 + t / 4][t % 4]);
-        const uint32_t u = v[h * 2 + t / 8][(t / 2) % 4];
+    __device__ __forceinline__ float value(int t) const {
+        if constexpr (SRC == Src8::kF32) return __uint_as_float(v[t / 4][t % 4]);
+        const uint32_t u = v[0][t / 2];
         if constexpr (SRC == Src8::kBf16) return __uint_as_float((t & 1) ? u & 0xFFFF0000u : u << 16);
         return __half2float(__ushort_as_half((uint16_t)((t & 1) ? u >> 16 : u & 0xFFFF)));
     }
-    // (what the clamped addresses past the end hold counts for no maximum, and its quotients are cleared)
     __device__ __forceinline__ uint32_t top() const {
         uint32_t m = 0;
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-            for (int t = 0; t < 16; ++t) m = max(m, abs_bits(value(h, t)));
+        for (int t = 0; t < 8; ++t) m = max(m, abs_bits(value(t)));
         return m;
     }
 };
 
-__device__ __forceinline__ uint32_t rows4_umax(uint32_t v) {    // over the four lanes that hold a row's values
-    const auto a = __builtin_amdgcn_permlane16_swap(v, v, false, false);
-    v = max(a[0], a[1]);
-    const auto b = __builtin_amdgcn_permlane32_swap(v, v, false, false);
-    return max(b[0], b[1]);
-}
+struct UMax8 {
+    __device__ float operator()(float a, float b) const {
+        return __uint_as_float(max(__float_as_uint(a), __float_as_uint(b)));
+    }
+};
 
 // CG groups of KS waves; a group walks over its own `per` column fragments (kSiluF32: fragments of the gate half, each
 // with its up fragment), D in flight.
@@ -126,7 +123,11 @@ __global__ void __launch_bounds__(64 * KS * CG, KS * CG <= 4 ? 2 : 1) int8_rows_
     __shared__ __attribute__((aligned(16))) v4i part[KS > 1 ? 2 : 1][KS > 1 ? CG : 1][KS > 1 ? D : 1][KS > 1 ? KS : 1][64];
     __shared__ uint16_t list[kScanSlots];
     __shared__ int counts[kWaves];
-    __shared__ uint32_t s_top[KS > 1 ? kWaves : 1][16];
+    // sixteen quantised rows (16 bytes apart beside their values: sixteen lanes then read different banks) and their scales
+    constexpr bool kQuant = SRC != Src8::kI8;
+    constexpr int kRowK = GPW * KS * kStep + 16;
+    __shared__ __attribute__((aligned(16))) int8_t s_x[kQuant ? 16 * kRowK : 16];
+    __shared__ uint32_t s_top[kQuant ? 16 : 1];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int ks = wave % KS, cg = wave / KS;
     const int q = lane >> 4, c = lane & 15;
@@ -160,54 +161,98 @@ __global__ void __launch_bounds__(64 * KS * CG, KS * CG <= 4 ? 2 : 1) int8_rows_
             }
     };
     Stage ring[D];
-#pragma unroll
-    for (int d = 0; d < D; ++d) load(ring[d], d);
-    __builtin_amdgcn_sched_barrier(0);
-
     const int mine = min(per, frags - f0);                       // output fragments of this group (may be <= 0)
     const int rounds = (per * kPair + D - 1) / D;                // of the work-group: the barriers agree
     for (int r0 = 0; r0 < rt.n; r0 += 16) {
         // ---- sixteen rows, held ----
-        const int slot = slot_at(p, rt, group, r0 + c, list);
-        const int row = slot < 0 ? slot_at(p, rt, group, r0, list) : slot;   // (a row that exists; never stored)
+        const int slot = slot_at(p, rt, r0 + c, list);
+        const int row = slot < 0 ? slot_at(p, rt, r0, list) : slot;   // (a row that exists; never stored)
         const int xrow = p.gather ? row / p.top_k : row;
-        const uint8_t* xp = reinterpret_cast<const uint8_t*>(p.x) + (int64_t)xrow * p.ldx * kSrcBytes<SRC>;
         u32x4 x[GPW][2];
         float xs;
-        if constexpr (SRC == Src8::kI8) {
+        auto first_weights = [&]() __attribute__((always_inline)) {
+            if (r0 > 0) return;
+#pragma unroll
+            for (int d = 0; d < D; ++d) load(ring[d], d);
+            __builtin_amdgcn_sched_barrier(0);
+        };
+        if constexpr (!kQuant) {
+            const int8_t* xp = reinterpret_cast<const int8_t*>(p.x) + (int64_t)xrow * p.ldx;
             xs = p.xs[xrow];
-#pragma unroll
-            for (int j = 0; j < GPW; ++j) {
-                RawStep<SRC> raw;
-                raw.load(xp, min(g0 + j, G - 1), q, K);
-                x[j][0] = raw.v[0];
-                x[j][1] = raw.v[1];
-            }
-        } else {
-            RawStep<SRC> raw[GPW];
-#pragma unroll
-            for (int j = 0; j < GPW; ++j) raw[j].load(xp, min(g0 + j, G - 1), q, K);
-            uint32_t top = 0;
-#pragma unroll
-            for (int j = 0; j < GPW; ++j) top = max(top, raw[j].top());
-            top = rows4_umax(top);
-            if constexpr (KS > 1) {
-                if (r0 > 0) __syncthreads();                     // (the last rows' maxima have been read)
-                if (q == 0) s_top[wave][c] = top;
-                lds_barrier();
-#pragma unroll
-                for (int w = 0; w < KS; ++w) top = max(top, s_top[cg * KS + w][c]);
-            }
-            const RowScale r = row_scale(top);
-            xs = r.s;
 #pragma unroll
             for (int j = 0; j < GPW; ++j)
 #pragma unroll
                 for (int h = 0; h < 2; ++h)
+                    x[j][h] = *reinterpret_cast<const u32x4*>(xp + min(min(g0 + j, G - 1) * kStep + h * 64 + q * 16, K - 16));
+            first_weights();
+        } else {
+            // The work-group quantises its real rows, eight values a thread and turn, into LDS, kHold turns' loads
+            // together. The first turns' values stay in registers between the maximum and the rounding; they are loaded
+            // before the weights, as loads return in order.
+            constexpr int kHold = 4, kThreads = 64 * kWaves;
+            const int live = min(16, rt.n - r0), pieces = K / 8, items = live * pieces;
+            const bool whole = pieces % 64 == 0;                 // a wave's pieces are of one row
+            Raw8<SRC> raw[kHold];
+            int rr[kHold], rk[kHold];
+            auto read = [&](int first) __attribute__((always_inline)) {
 #pragma unroll
-                    for (int d = 0; d < 4; ++d)
-                        x[j][h][d] = quant4(raw[j].value(h, 4 * d), raw[j].value(h, 4 * d + 1), raw[j].value(h, 4 * d + 2),
-                                            raw[j].value(h, 4 * d + 3), r);
+                for (int i = 0; i < kHold; ++i) {
+                    const int item = min(first + i * kThreads, items - 1);
+                    rr[i] = item / pieces;
+                    rk[i] = (item - rr[i] * pieces) * 8;
+                    const int s = slot_at(p, rt, r0 + rr[i], list);
+                    raw[i].load(reinterpret_cast<const uint8_t*>(p.x) + (int64_t)(p.gather ? s / p.top_k : s) * p.ldx * kSrcBytes<SRC>, rk[i]);
+                }
+            };
+            auto maxima = [&](int first) __attribute__((always_inline)) {
+#pragma unroll
+                for (int i = 0; i < kHold; ++i) {
+                    const int item = first + i * kThreads;
+                    if (whole) {
+                        if (item - lane >= items) break;         // (of the whole wave)
+                        const uint32_t m = __float_as_uint(lane_allreduce<6>(__uint_as_float(raw[i].top()), UMax8{}));
+                        if (lane == 0) atomicMax(&s_top[rr[i]], m);
+                    } else if (item < items) {
+                        atomicMax(&s_top[rr[i]], raw[i].top());
+                    }
+                }
+            };
+            auto put = [&](int first) __attribute__((always_inline)) {
+#pragma unroll
+                for (int i = 0; i < kHold; ++i) {
+                    if (first + i * kThreads >= items) break;
+                    const RowScale sc = row_scale(s_top[rr[i]]);
+                    *reinterpret_cast<uint2*>(s_x + rr[i] * kRowK + rk[i]) =
+                        make_uint2(quant4(raw[i].value(0), raw[i].value(1), raw[i].value(2), raw[i].value(3), sc),
+                                   quant4(raw[i].value(4), raw[i].value(5), raw[i].value(6), raw[i].value(7), sc));
+                }
+            };
+            constexpr int kTurn = kHold * kThreads;
+            read(tid);
+            __builtin_amdgcn_sched_barrier(0);
+            first_weights();
+            if (r0 > 0) __syncthreads();                         // (the last rows have been read)
+            if (tid < 16) s_top[tid] = 0;
+            lds_barrier();
+            maxima(tid);
+            for (int t = tid + kTurn; t - tid < items; t += kTurn) {
+                read(t);
+                maxima(t);
+            }
+            lds_barrier();
+            if (items > kTurn) read(tid);
+            put(tid);
+            for (int t = tid + kTurn; t - tid < items; t += kTurn) {
+                read(t);
+                put(t);
+            }
+            lds_barrier();
+            xs = row_scale(s_top[c]).s;
+#pragma unroll
+            for (int j = 0; j < GPW; ++j)
+#pragma unroll
+                for (int h = 0; h < 2; ++h)                      // (rows that are not real hold anything)
+                    x[j][h] = *reinterpret_cast<const u32x4*>(s_x + c * kRowK + (g0 + j) * kStep + h * 64 + q * 16);
         }
         // (what the clamped addresses hold counts in its own place)
 #pragma unroll
@@ -304,8 +349,8 @@ __global__ void __launch_bounds__(64 * KS) int8_stream_kernel(RowsParams p, int 
     const float* ws = p.ws + (int64_t)rt.e * p.N;
     const int G = (K + kStep - 1) / kStep, steps = (G + KS - 1) / KS;
     for (int r0 = 0; r0 < rt.n; r0 += 16) {
-        const int slot = slot_at(p, rt, group, r0 + c, list);
-        const int row = slot < 0 ? slot_at(p, rt, group, r0, list) : slot;
+        const int slot = slot_at(p, rt, r0 + c, list);
+        const int row = slot < 0 ? slot_at(p, rt, r0, list) : slot;
         const int xrow = p.gather ? row / p.top_k : row;
         const int8_t* xp = reinterpret_cast<const int8_t*>(p.x) + (int64_t)xrow * p.ldx;
         struct Stage {
@@ -374,10 +419,8 @@ int too_many() {
     set_error("int8 product: too many tiles");
     return W4A8_ERR_INVALID;
 }
-// Groups of rows that work-groups take, and how many of them hold rows.
-int64_t groups_of(const RowsParams& p) { return p.ids == nullptr ? 1 : p.single ? p.slots : p.E; }
-int64_t busy_of(const RowsParams& p) { return p.ids == nullptr ? 1 : std::min(p.slots, p.E); }
-
+// Groups of rows that work-groups take.
+int64_t groups_of(const RowsParams& p) { return p.ids == nullptr ? 1 : std::min(p.slots, p.E); }
 template <int FN, int KS, Out8 DST>
 int stream_go(const RowsParams& p, hipStream_t s) {
     constexpr bool silu = DST == Out8::kSiluF32;
@@ -407,10 +450,14 @@ template <int GPW, int KS, int CG, int D, Src8 SRC, Out8 DST>
 int rows_go(const RowsParams& p, hipStream_t s) {
     constexpr int unit = D / (DST == Out8::kSiluF32 ? 2 : 1);
     const int frags = ((DST == Out8::kSiluF32 ? p.N / 2 : p.N) + 15) / 16;
-    // One round of work-groups (eight waves a CU), each walking over what that leaves it, up to eight rings' worth.
-    const int64_t groups = (int64_t)device_cu_count() * std::max(1, 8 / (KS * CG)) * CG;
-    int64_t per = (busy_of(p) * frags + groups - 1) / groups;
-    if (per > unit) per = std::min<int64_t>((per + unit - 1) / unit, 8) * unit;
+    // As many work-groups as run at once (eight waves a CU), those of groups without rows among them, each walking over
+    // what that leaves it: some more would run behind all others. us of a layer of 256 experts (2048 x 512, 8 a token), by
+    // the first product's fragments a work-group 1 / 2 / 4 / 8 / 16 / 32 (the rule's in brackets): 8 tokens 63 / 53 / (47) /
+    // 48 / 62 / 94, 16 tokens 104 / 92 / 82 / (78) / 78 / 107, 64 tokens 229 / 194 / 176 / 170 / (168) / 165.
+    const int64_t resident = (int64_t)device_cu_count() * std::max(1, 8 / (KS * CG));
+    const int64_t slices = std::max<int64_t>(1, resident / groups_of(p));
+    int64_t per = (frags + CG * slices - 1) / (CG * slices);
+    if (per > unit) per = (per + unit - 1) / unit * unit;
     return rows_launch<GPW, KS, CG, D, SRC, DST>(p, frags, std::max<int64_t>(1, per), s);
 }
 
@@ -434,7 +481,8 @@ int rows_any(const RowsParams& p, hipStream_t s) {
 bool int8_rows_quantised_in_kernel(int64_t K) { return K <= 32 * kStep; }
 
 int launch_int8_rows(const RowsArgs& a, hipStream_t s) {
-    const RowsParams p = rows_params(a);
+    RowsParams p = rows_params(a);
+    p.by_slot = p.slots < p.E ? 1 : 0;
     if (p.rows == 0 || (p.ids != nullptr && p.slots == 0)) return W4A8_OK;
     if (p.ids != nullptr && p.slots > kScanSlots) {
         set_error("int8 product: too many slots for the streaming kernels");

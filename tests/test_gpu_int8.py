@@ -216,7 +216,7 @@ def make_routing(g, T, E, k, skew=0.0):
 
 def rows16(T, E, k, dtype):
     """Whether the layer rounds its slots' rows to 16 bits: many tokens, bf16 output."""
-    return T * k > min(12 * E, 4096) and dtype == torch.bfloat16
+    return T * k > min(5 * E + 128, 4096) and dtype == torch.bfloat16
 
 
 LAYERS = [(1, 8, 2, 64, 64), (1, 256, 8, 512, 128), (3, 16, 4, 192, 320), (5, 4, 4, 256, 64), (17, 8, 2, 64, 192), (32, 32, 4, 512, 256),
