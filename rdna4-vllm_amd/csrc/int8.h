@@ -245,6 +245,9 @@ int launch_act_quant_int8(const void* x, Rows src, int64_t rows, int64_t K, int6
 // int8_rows_quantised_in_kernel().
 bool int8_rows_quantised_in_kernel(int64_t K);
 int launch_int8_rows(const RowsArgs& a, hipStream_t s);
+// The second product (rows by slot, fp32) and the sum over each token's slots in one, rounded to 16 bits: out (T, N).
+bool int8_token_supported(int64_t slots, int64_t E, int64_t inter);
+int launch_int8_token(const RowsArgs& a, const float* topk_weights, hipStream_t s);
 // Tiles (int8_tiles.hip): sizes that 32-bit offsets reach; grouped, blocks of as many rows as a tile has: 64 or 128.
 bool int8_tiles_supported(const Int8Args& a);
 int launch_int8_tiles(const Int8Args& a, hipStream_t s);

@@ -164,8 +164,12 @@ int run_layer(const Layer& l, const LayerPlan& pl, const LayerScratch& m, hipStr
             if (int rc = launch_act_quant_int8(m.h, Rows::kF32, n, l.inter, l.inter, false, m.hq, m.hs, nullptr, nullptr, 0, s)) return rc;
             g2.x = m.hq; g2.src = Src8::kI8; g2.xs = m.hs;
         }
-        g2.w = l.w2; g2.ws = l.s2; g2.N = l.H; g2.gather = false;
-        g2.dst = Out8::kSlotF32; g2.out = m.y; g2.ldo = l.H;
+        g2.w = l.w2; g2.ws = l.s2; g2.N = l.H; g2.gather = false; g2.ldo = l.H;
+        if (int8_token_supported(n, l.E, l.inter)) {
+            g2.dst = Out8::k16; g2.out = l.out; g2.bf16 = l.bf16;
+            return launch_int8_token(g2, l.tw, s);
+        }
+        g2.dst = Out8::kSlotF32; g2.out = m.y;
         if (int rc = launch_int8_rows(g2, s)) return rc;
     }
     return launch_int8_reduce(m.y, pl.tiles && l.bf16 ? m.ys : nullptr, l.tw, l.ids, l.emap, l.n_global, l.E, l.T, l.H, l.top_k, l.out, l.bf16, s);

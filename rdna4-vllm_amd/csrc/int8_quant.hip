@@ -147,8 +147,13 @@ __global__ void __launch_bounds__(256) quant_any_kernel(QuantParams p) {
 
 template <Rows SRC, bool SILU>
 int quant_go(const QuantParams& p, bool wide, hipStream_t s) {
-    auto go = [&](auto kernel, int rows_each, int threads) {
-        launch_kernel(kernel, dim3((unsigned)((p.rows + rows_each - 1) / rows_each)), dim3(threads), 0, s, p);
+    auto go = [&](auto kernel, int rows_each, int threads) -> int {
+        const int64_t blocks = (p.rows + rows_each - 1) / rows_each;
+        if (!grid_fits(blocks, threads)) {
+            set_error("act_quant_int8: too many rows");
+            return W4A8_ERR_INVALID;
+        }
+        launch_kernel(kernel, dim3((unsigned)blocks), dim3(threads), 0, s, p);
         return check_launch("act_quant_int8");
     };
     if (!wide || p.K > 32768) return go(&quant_any_kernel<SRC, SILU>, 1, 256);
@@ -217,10 +222,6 @@ __global__ void __launch_bounds__(256) int8_reduce_kernel(const void* __restrict
 int launch_act_quant_int8(const void* x, Rows src, int64_t rows, int64_t K, int64_t ldx, bool silu, int8_t* q, float* scales,
                           const int32_t* sorted_ids, const int32_t* ntp, int64_t num_valid, hipStream_t s) {
     if (rows == 0) return W4A8_OK;
-    if (!grid_fits(rows, 1024)) {
-        set_error("act_quant_int8: too many rows");
-        return W4A8_ERR_INVALID;
-    }
     const QuantParams p{x, q, scales, sorted_ids, ntp, rows, ldx, (int)K, (int)num_valid};
     const int size = src == Rows::kF32 ? 4 : 2;
     const bool wide = K % 8 == 0 && reinterpret_cast<uintptr_t>(x) % 16 == 0 && (ldx * size % 16 == 0 || rows == 1) &&
