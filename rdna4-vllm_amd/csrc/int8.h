@@ -249,7 +249,6 @@ int launch_int8_rows(const RowsArgs& a, hipStream_t s);
 bool int8_token_supported(int64_t slots, int64_t E, int64_t inter);
 int launch_int8_token(const RowsArgs& a, const float* topk_weights, hipStream_t s);
 // Tiles (int8_tiles.hip): sizes that 32-bit offsets reach; grouped, blocks of as many rows as a tile has: 64 or 128.
-bool int8_tiles_supported(const Int8Args& a);
 int launch_int8_tiles(const Int8Args& a, hipStream_t s);
 // out[t, n] = sum over the slots j in order of tw[t, j] * y[t top_k + j, n], rounded to 16 bits; slots whose (mapped)
 // expert is not in [0, E) contribute nothing. y as kSlotF32, or with scales as kSlot16 leaves it. N % 32 == 0.

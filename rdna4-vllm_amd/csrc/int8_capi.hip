@@ -237,7 +237,18 @@ int w4a8_int8_gemm(const void* x, int x_dtype, const float* x_scales, int64_t M,
     a.w = w; a.ws = w_scales; a.E = 1; a.N = N; a.bias = bias; a.bias_f32 = bias_is_f32 != 0;
     a.P = M; a.top_k = 1; a.num_valid = M; a.block_m = 16;
     a.dst = Out8::k16; a.bf16 = out_dtype == W4A8_DTYPE_BF16; a.out = out; a.ldo = N;
-    if (M > kStreamRows && int8_tiles_supported(a)) return launch_int8_tiles(a, s);
+    // The tiles address weights and rows in 32 bits: rows past that are taken in parts.
+    const int64_t lim = ((int64_t)1 << 32) - 1, part = lim / x_stride / 256 * 256;
+    if (M > kStreamRows && N * K <= lim && part > 0) {
+        for (int64_t m = 0; m < M; m += part) {
+            a.x_rows = a.P = a.num_valid = std::min(part, M - m);
+            if (int rc = launch_int8_tiles(a, s)) return rc;
+            a.x += part * x_stride;
+            a.xs += part;
+            a.out = static_cast<uint16_t*>(a.out) + part * N;
+        }
+        return W4A8_OK;
+    }
     RowsArgs r{};
     r.x = x; r.src = src; r.xs = x_scales; r.rows = M; r.K = K; r.ldx = x_stride;
     r.w = w; r.ws = w_scales; r.E = 1; r.N = N; r.bias = bias; r.bias_f32 = a.bias_f32; r.top_k = 1;

@@ -554,12 +554,6 @@ int dense_go(const Int8Params& p, hipStream_t s) {
 
 }  // namespace
 
-bool int8_tiles_supported(const Int8Args& a) {
-    // rows and an expert's weights are addressed in 32 bits
-    const int64_t lim = (int64_t)1 << 32;
-    return a.x_rows * a.ldx < lim && a.N * a.K < lim;
-}
-
 int launch_int8_tiles(const Int8Args& a, hipStream_t s) {
     const Int8Params p = int8_params(a);
     if (p.P == 0) return W4A8_OK;

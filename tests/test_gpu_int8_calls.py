@@ -123,6 +123,19 @@ def test_dense_weights_and_outputs_past_32_bits():
         assert torch.equal(y[rows], W.int8_gemm(x[rows].contiguous(), xs[rows], w, ws))
 
 
+def test_dense_rows_past_32_bits():
+    """M K past 2^32: rows in parts."""
+    g = torch.Generator(device=DEV).manual_seed(5)
+    M, N, K = 270000, 64, 16384
+    x = torch.randint(-128, 128, (M, K), generator=g, dtype=torch.int8, device=DEV)
+    xs = torch.rand((M,), generator=g, device=DEV)
+    w = torch.randint(-128, 128, (N, K), generator=g, dtype=torch.int8, device=DEV)
+    ws = torch.rand((N,), generator=g, device=DEV) * 1e-3
+    y = W.int8_gemm(x, xs, w, ws)
+    for rows in (slice(0, 40), slice(262144 - 300, 262144 + 40), slice(M - 40, M)):
+        assert torch.equal(y[rows], W.int8_gemm(x[rows].contiguous(), xs[rows], w, ws))
+
+
 def test_many_short_rows():
     x = torch.randn((5_000_000, 16), device=DEV, dtype=torch.float16)
     q, s = W.act_quant_int8(x)
