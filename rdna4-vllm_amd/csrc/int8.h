@@ -107,7 +107,7 @@ struct RowsParams : OutParams {
     const float* xs;
     const int32_t* ids;
     const int32_t* emap;
-    int rows, slots, emap_len, by_slot;
+    int rows, slots, emap_len, one_slot;     // one_slot: each slot is a group of its own
 };
 
 template <typename A>
@@ -131,7 +131,7 @@ inline RowsParams rows_params(const RowsArgs& a) {
     RowsParams p;
     out_params(a, p);
     p.x = a.x; p.xs = a.xs; p.ids = a.ids; p.emap = a.emap;
-    p.rows = (int)a.rows; p.slots = (int)a.slots; p.emap_len = (int)a.emap_len; p.by_slot = 0;
+    p.rows = (int)a.rows; p.slots = (int)a.slots; p.emap_len = (int)a.emap_len; p.one_slot = 0;
     return p;
 }
 

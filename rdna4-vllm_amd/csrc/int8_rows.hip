@@ -5,11 +5,14 @@
 // row c, for rows and weights alike (a sum of whole numbers may take its k in any order). Weights are the first
 // operand: a lane ends up with four adjacent columns of one row.
 //
-// Grouped, a work-group finds its rows itself: it scans the routed ids for the slots of its expert, so that no launch has
-// to sort them first.
+// Grouped, a work-group counts the routed ids by expert in LDS itself, so that no launch has to sort them first, and takes an
+// equal part of what all experts with rows amount to. One or two slots of an expert, two thirds of 256 experts in use (32
+// tokens, 8 picks, 2048 x 512): the layer's two products read 510 MB in 100 of its 108 us, 5.1 TB/s (a group a work-group
+// column, whatever the number of experts in use: 128 us); reads alone, of the same pieces, reach 6.3.
 //
-// int8_rows_kernel holds its rows in registers (16 rows by GPW steps a wave, quantised there where they come in 16 or 32
-// bits) and walks over column fragments with D of them in flight; KS waves share K and add their sums in LDS.
+// int8_rows_kernel holds its rows in registers (16 rows by GPW steps a wave, quantised in LDS where they come in 16 or 32
+// bits) and walks over column fragments with D of them in flight; KS waves share K and add their sums in LDS. Four fragments
+// in flight were slower than two (64 tokens: 103 us for 93 of the first product).
 // int8_stream_kernel takes any K and reads int8 rows again for each column fragment.
 #include <algorithm>
 #include <type_traits>
@@ -19,68 +22,147 @@
 namespace w4a8 {
 namespace {
 
-// ---- a work-group's rows ----
-constexpr int kOneSlot = 2;
-struct Routed {
-    int e;            // expert
-    int n;            // its rows
-};
+// ---- groups of up to sixteen rows that share their weights ----
+constexpr int kMaxExperts = 1024;
 // The expert of slot i (an id of no local expert: -1).
 __device__ __forceinline__ int expert_of(const RowsParams& p, int i) {
     int e = p.ids[i];
     if (p.emap != nullptr) e = e >= 0 && e < p.emap_len ? p.emap[e] : -1;
     return e >= 0 && e < p.E ? e : -1;
 }
-// Group g of rows: dense, all of them; else the slots of one expert, in order, in `list`: of expert g, or (by_slot, for
-// fewer slots than experts) of slot g's expert, where slot g is its first; or slot g alone (kOneSlot). WAVES: of the work-group, all of which call
-// this.
+struct Routed {                                                  // in LDS
+    uint32_t group[kMaxExperts + kScanSlots / 16];               // expert | its first place in slots << 10 | rows << 23
+    uint32_t first[kMaxExperts + 1];                             // an expert's slots, then its first place
+    uint32_t sums[16];
+    int wide;                                                    // some expert has several groups
+    uint16_t slots[kScanSlots];                                  // by expert
+};
+// The number of groups: dense, sixteen rows each in order; one_slot, a slot each; else the slots counted by expert, their
+// experts' groups in order. WAVES: of the work-group, all of which call this.
 template <int WAVES>
-__device__ __forceinline__ Routed find_rows(const RowsParams& p, int g, uint16_t* list, int* counts) {
-    if (p.ids == nullptr) return {0, p.rows};
-    const int e = p.by_slot ? __builtin_amdgcn_readfirstlane(expert_of(p, g)) : g;
-    if (e < 0) return {0, 0};
-    if (p.by_slot == kOneSlot) return {e, 1};
-    constexpr int kMost = kScanSlots / (64 * WAVES);             // slots a lane
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int per = (p.slots + 64 * WAVES - 1) / (64 * WAVES);   // steps of 64 slots a wave
-    const int first = wave * per * 64 + lane;
-    uint32_t mine = 0, sooner = 0;                               // bit i: slot first + 64 i
-#pragma unroll 4
-    for (int i = 0; i < kMost; ++i) {
-        if (i >= per) break;
-        const int s = first + 64 * i;
-        if (s < p.slots && expert_of(p, s) == e) {
-            mine |= 1u << i;
-            sooner |= s < g ? 1u : 0u;
-        }
-    }
-    int n = 0;
-    for (int i = 0; i < per; ++i) n += __popcll(__ballot(mine >> i & 1));
-    const bool late = p.by_slot && __ballot(sooner != 0) != 0;
-    if (lane == 0) counts[wave] = late ? -1 : n;
+__device__ __forceinline__ int find_groups(const RowsParams& p, Routed& rt) {
+    if (p.ids == nullptr) return (p.rows + 15) / 16;
+    if (p.one_slot) return p.slots;
+    constexpr int kThreads = 64 * WAVES, kMost = kScanSlots / kThreads, kEach = kMaxExperts / kThreads, kAhead = 4;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    uint32_t mine[kMost];                                        // expert << 16 | its slots before this one
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) rt.first[tid + j * kThreads] = 0;
+    if (tid == 0) rt.wide = 0;
     __syncthreads();
-    int at = 0;
-    n = 0;
+#pragma unroll
+    for (int i0 = 0; i0 < kMost; i0 += kAhead)
+        if (i0 * kThreads < p.slots) {
+            int e[kAhead];
+#pragma unroll
+            for (int i = 0; i < kAhead; ++i) e[i] = expert_of(p, min(tid + (i0 + i) * kThreads, p.slots - 1));
+#pragma unroll
+            for (int i = 0; i < kAhead; ++i) {
+                mine[i0 + i] = ~0u;
+                if (e[i] >= 0 && tid + (i0 + i) * kThreads < p.slots)
+                    mine[i0 + i] = (uint32_t)e[i] << 16 | atomicAdd(&rt.first[e[i]], 1u);
+            }
+        }
+    __syncthreads();
+    // slots | groups << 16 of the experts before
+    uint32_t n[kEach], all = 0;
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) {
+        n[j] = rt.first[tid * kEach + j];
+        all += n[j] | (n[j] + 15) / 16 << 16;
+        if (n[j] > 16) rt.wide = 1;
+    }
+    uint32_t upto = all;
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+        const uint32_t o = (uint32_t)__shfl_up((int)upto, d);
+        upto += lane >= d ? o : 0u;
+    }
+    if (lane == 63) rt.sums[wave] = upto;
+    __syncthreads();
+    uint32_t at = upto - all, total = 0;
 #pragma unroll
     for (int w = 0; w < WAVES; ++w) {
-        if (counts[w] < 0) return {e, 0};                        // (all waves)
-        if (w < wave) at += counts[w];
-        n += counts[w];
+        at += w < wave ? rt.sums[w] : 0u;
+        total += rt.sums[w];
     }
-    if (n == 0) return {e, 0};
-    for (int i = 0; i < per; ++i) {
-        const uint64_t m = __ballot(mine >> i & 1);
-        if (mine >> i & 1) list[at + __popcll(m & ((1ull << lane) - 1))] = (uint16_t)(first + 64 * i);
-        at += __popcll(m);
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) {
+        const uint32_t e = tid * kEach + j;
+        rt.first[e] = at & 0xFFFFu;
+        for (uint32_t r = 0; r < n[j]; r += 16) {
+            rt.group[at >> 16] = e | ((at & 0xFFFFu) + r) << 10 | min(16u, n[j] - r) << 23;
+            at += 1u << 16;
+        }
+        at += n[j];
     }
+    if (tid == kThreads - 1) rt.first[kMaxExperts] = at & 0xFFFFu;
     __syncthreads();
-    return {e, n};
+#pragma unroll
+    for (int i = 0; i < kMost; ++i)
+        if (i * kThreads < p.slots && mine[i] != ~0u)
+            rt.slots[rt.first[mine[i] >> 16] + (mine[i] & 0xFFFFu)] = (uint16_t)(tid + i * kThreads);
+    __syncthreads();
+    if (rt.wide) {
+        // Work-groups have counted an expert's slots in orders of their own, but each has to find the same ones in each of
+        // its groups: they are put in order.
+#pragma unroll
+        for (int i = 0; i < kMost; ++i)
+            if (i * kThreads < p.slots && mine[i] != ~0u) {
+                const uint32_t e = mine[i] >> 16, from = rt.first[e], to = rt.first[e + 1];
+                uint32_t rank = 0;
+                if (to - from > 16)
+                    for (uint32_t j = from; j < to; ++j) rank += rt.slots[j] < tid + i * kThreads ? 1u : 0u;
+                else
+                    rank = mine[i] & 0xFFFFu;
+                mine[i] = from + rank;
+            }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < kMost; ++i)
+            if (i * kThreads < p.slots && mine[i] != ~0u) rt.slots[mine[i]] = (uint16_t)(tid + i * kThreads);
+        __syncthreads();
+    }
+    return __builtin_amdgcn_readfirstlane(total >> 16);
 }
-// Row r of the group: its slot (dense: r), -1 past the end.
-__device__ __forceinline__ int slot_at(const RowsParams& p, const Routed& d, int g, int r, const uint16_t* list) {
-    if (r >= d.n) return -1;
-    return p.ids == nullptr ? r : p.by_slot == kOneSlot ? g : list[r];
+struct Group {
+    int e;            // expert
+    int n;            // rows: 0 to 16
+    int at;           // the first one's place
+    bool listed;      // places are of Routed's slots, else slots (dense: rows)
+};
+__device__ __forceinline__ Group group_at(const RowsParams& p, const Routed& rt, int g) {
+    if (p.ids == nullptr) return {0, min(16, p.rows - 16 * g), 16 * g, false};
+    if (p.one_slot) {
+        const int e = __builtin_amdgcn_readfirstlane(expert_of(p, g));
+        return {e, e < 0 ? 0 : 1, g, false};
+    }
+    const uint32_t v = __builtin_amdgcn_readfirstlane(rt.group[g]);
+    return {(int)(v & 1023u), (int)(v >> 23), (int)(v >> 10 & 8191u), true};
 }
+__device__ __forceinline__ int slot_at(const Routed& rt, const Group& g, int i) { return g.listed ? rt.slots[g.at + i] : g.at + i; }
+// The units (a group by an output fragment) of a work-group: of one group where that leaves it no more than an eighth over
+// an equal part of all, else such a part, those of a group one after another.
+struct Walk {
+    int left, g, f;
+    __device__ __forceinline__ Walk(int groups, int frags) {
+        const uint32_t W = gridDim.x, b = blockIdx.x, n = (uint32_t)groups, units = n * (uint32_t)frags;
+        const uint32_t s = n > 0 ? W / n : 0;                    // work-groups a group
+        const uint32_t per = s > 0 ? ((uint32_t)frags + s - 1) / s : 0;
+        if (s > 0 && (uint64_t)per * W * 8 <= (uint64_t)units * 9) {
+            g = (int)(b / s);
+            f = (int)((b - g * s) * per);
+            left = g < groups ? min((int)per, frags - f) : 0;
+        } else {
+            const uint32_t each = units / W, more = units - each * W, u = b * each + min(b, more);
+            left = (int)(each + (b < more ? 1u : 0u));
+            g = (int)(u / (uint32_t)frags);
+            f = (int)(u - (uint32_t)g * (uint32_t)frags);
+        }
+    }
+    __device__ __forceinline__ int here(int frags) const { return min(left, frags - f); }
+    __device__ __forceinline__ void next(int n) { left -= n; ++g; f = 0; }
+};
 
 // ---- rows' values ----
 template <Src8 SRC>
@@ -113,18 +195,17 @@ struct UMax8 {
     }
 };
 
-// CG groups of KS waves; a group walks over its own `per` column fragments (kSiluF32: fragments of the gate half, each
-// with its up fragment), D in flight.
+// CG groups of KS waves share a work-group's fragments (kSiluF32: fragments of the gate half, each with its up fragment),
+// D in flight.
 template <int GPW, int KS, int CG, int D, Src8 SRC, Out8 DST>
-__global__ void __launch_bounds__(64 * KS * CG, KS * CG <= 4 ? 2 : 1) int8_rows_kernel(RowsParams p, int slices, int per) {
+__global__ void __launch_bounds__(64 * KS * CG, KS * CG <= 4 ? 2 : 1) int8_rows_kernel(RowsParams p) {
     constexpr bool kSilu = DST == Out8::kSiluF32;
     constexpr int kPair = kSilu ? 2 : 1;                         // fragments of one output fragment
     static_assert(D % kPair == 0, "an output fragment's parts are in flight together");
     constexpr int kUnits = D / kPair;                            // output fragments of one round
     constexpr int kWaves = KS * CG;
     __shared__ __attribute__((aligned(16))) v4i part[KS > 1 ? 2 : 1][KS > 1 ? CG : 1][KS > 1 ? D : 1][KS > 1 ? KS : 1][64];
-    __shared__ uint16_t list[kScanSlots];
-    __shared__ int counts[kWaves];
+    __shared__ Routed rt;
     // sixteen quantised rows (16 bytes apart beside their values: sixteen lanes then read different banks) and their scales
     constexpr bool kQuant = SRC != Src8::kI8;
     constexpr int kRowK = GPW * KS * kStep + 16;
@@ -133,76 +214,122 @@ __global__ void __launch_bounds__(64 * KS * CG, KS * CG <= 4 ? 2 : 1) int8_rows_
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int ks = wave % KS, cg = wave / KS;
     const int q = lane >> 4, c = lane & 15;
-    const int group = blockIdx.x / slices, sl = blockIdx.x % slices;
-    const Routed rt = find_rows<kWaves>(p, group, list, counts);
-    if (rt.n == 0) return;
     const int half = p.N / 2;
     const int cols = kSilu ? half : p.N;
     const int K = p.K, G = (K + kStep - 1) / kStep;
     const int frags = (cols + 15) / 16;
-    const int f0 = (sl * CG + cg) * per;                         // first output fragment of this group
     const int g0 = ks * GPW;                                     // first step of this wave
-    const int8_t* we = p.w + (int64_t)rt.e * p.N * K;
-    const float* wse = p.ws + (int64_t)rt.e * p.N;
 
-    // ---- weights: step i is fragment f0 + i / kPair of the gate (i even) or the up half ----
+    // ---- what these KS waves take of a group: `per` output fragments from f0 on ----
+    struct Part {
+        const int8_t* w;
+        const float* ws;
+        int f0, per;
+    };
+    auto part_of = [&](int e, int f, int here) __attribute__((always_inline)) {
+        const int per = (here + CG - 1) / CG;
+        return Part{p.w + (int64_t)e * p.N * K, p.ws + (int64_t)e * p.N, f + cg * per, per};
+    };
+    // weights: step i is fragment f0 + i / kPair of the gate (i even) or the up half; on: 0 for a load of no use, of one
+    // address
     struct Stage {
         u32x4 w[GPW][2];
     };
-    auto load = [&](Stage& s, int i) __attribute__((always_inline)) {
-        const int f = min(f0 + min(i / kPair, per - 1), frags - 1);
+    auto load = [&](Stage& s, const Part& a, int i, int on) __attribute__((always_inline)) {
+        const int f = min(a.f0 + min(i / kPair, a.per - 1), frags - 1);
         const int up = kSilu && (i & 1) ? half : 0;
         // (columns past the end read the last one; never stored)
-        const int8_t* wr = we + (int64_t)(up + min(f * 16 + c, cols - 1)) * K;
+        const int8_t* wr = a.w + (int64_t)((up + min(f * 16 + c, cols - 1)) & on) * K;
 #pragma unroll
         for (int j = 0; j < GPW; ++j)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 const int k = min(min(g0 + j, G - 1) * kStep + h * 64 + q * 16, K - 16);
-                s.w[j][h] = *reinterpret_cast<const u32x4*>(wr + k);
+                s.w[j][h] = *reinterpret_cast<const u32x4*>(wr + (k & on));
             }
     };
+    // Scales of the columns that a wave stores in a round (unit u of it: output fragment f0 + it kUnits + u). Loads return
+    // in order: those of the layer are loaded before the round's weights, so that nothing waits for later ones.
+    constexpr int kMine = KS == 1 ? kUnits : 1;
+    static_assert(KS == 1 || kUnits <= KS, "a wave a unit");
+    constexpr bool kEarly = DST != Out8::k16;                    // (whole fragments)
+    using v4f1 = float __attribute__((ext_vector_type(4), aligned(4)));
+    struct Cols {
+        v4f ws[kMine], up[kSilu ? kMine : 1];
+    };
+    auto load_cols = [&](Cols& t, const Part& a, int it) __attribute__((always_inline)) {
+        if constexpr (kEarly)
+#pragma unroll
+            for (int i = 0; i < kMine; ++i) {
+                const int n = min((a.f0 + it * kUnits + (KS == 1 ? i : ks)) * 16, cols - 16) + 4 * q;
+                t.ws[i] = *reinterpret_cast<const v4f1*>(a.ws + n);
+                if constexpr (kSilu) t.up[i] = *reinterpret_cast<const v4f1*>(a.ws + half + n);
+            }
+    };
+
     Stage ring[D];
-    const int mine = min(per, frags - f0);                       // output fragments of this group (may be <= 0)
-    const int rounds = (per * kPair + D - 1) / D;                // of the work-group: the barriers agree
-    for (int r0 = 0; r0 < rt.n; r0 += 16) {
+    Cols now;
+    bool again = false, ahead = false;                           // ahead: the first weights of this part are in flight
+    Walk walk(find_groups<kWaves>(p, rt), frags);
+    for (; walk.left > 0; walk.next(walk.here(frags))) {
+        const Group gr = group_at(p, rt, walk.g);
+        if (gr.n == 0) {
+            ahead = false;
+            continue;
+        }
+        const int here = walk.here(frags);
+        const Part cur = part_of(gr.e, walk.f, here);
+        const int mine = min(cur.per, walk.f + here - cur.f0);   // real fragments (may be <= 0)
+        const int rounds = (cur.per * kPair + D - 1) / D;        // of the work-group: the barriers agree
+        Part nxt = cur;                                          // what follows
+        bool follows = false;
+        if (walk.left > here) {
+            const Group gn = group_at(p, rt, walk.g + 1);
+            follows = gn.n > 0;
+            if (follows) nxt = part_of(gn.e, 0, min(walk.left - here, frags));
+        }
         // ---- sixteen rows, held ----
-        const int slot = slot_at(p, rt, group, r0 + c, list);
-        const int row = slot < 0 ? slot_at(p, rt, group, r0, list) : slot;   // (a row that exists; never stored)
+        const int slot = c < gr.n ? slot_at(rt, gr, c) : -1;
+        const int row = slot < 0 ? slot_at(rt, gr, 0) : slot;    // (a row that exists; never stored)
         const int xrow = p.gather ? row / p.top_k : row;
         u32x4 x[GPW][2];
         float xs;
         auto first_weights = [&]() __attribute__((always_inline)) {
-            if (r0 > 0) return;
+            __builtin_amdgcn_sched_barrier(0);
+            load_cols(now, cur, 0);
 #pragma unroll
-            for (int d = 0; d < D; ++d) load(ring[d], d);
+            for (int d = 0; d < D; ++d) load(ring[d], cur, d, -1);
             __builtin_amdgcn_sched_barrier(0);
         };
         if constexpr (!kQuant) {
-            const int8_t* xp = reinterpret_cast<const int8_t*>(p.x) + (int64_t)xrow * p.ldx;
-            xs = p.xs[xrow];
+            auto read = [&]() __attribute__((always_inline)) {
+                const int8_t* xp = reinterpret_cast<const int8_t*>(p.x) + (int64_t)xrow * p.ldx;
+                xs = p.xs[xrow];
 #pragma unroll
-            for (int j = 0; j < GPW; ++j)
+                for (int j = 0; j < GPW; ++j)
 #pragma unroll
-                for (int h = 0; h < 2; ++h)
-                    x[j][h] = *reinterpret_cast<const u32x4*>(xp + min(min(g0 + j, G - 1) * kStep + h * 64 + q * 16, K - 16));
-            first_weights();
+                    for (int h = 0; h < 2; ++h)
+                        x[j][h] = *reinterpret_cast<const u32x4*>(xp + min(min(g0 + j, G - 1) * kStep + h * 64 + q * 16, K - 16));
+            };
+            read();
+            if (!ahead) first_weights();
         } else {
             // The work-group quantises its real rows, eight values a thread and turn, into LDS, kHold turns' loads
             // together. The first turns' values stay in registers between the maximum and the rounding; they are loaded
             // before the weights, as loads return in order.
             constexpr int kHold = 4, kThreads = 64 * kWaves;
-            const int live = min(16, rt.n - r0), pieces = K / 8, items = live * pieces;
+            const int pieces = K / 8, items = gr.n * pieces;
             const bool whole = pieces % 64 == 0;                 // a wave's pieces are of one row
+            const float each = 1.0f / (float)pieces;
             Raw8<SRC> raw[kHold];
             int rr[kHold], rk[kHold];
             auto read = [&](int first) __attribute__((always_inline)) {
 #pragma unroll
                 for (int i = 0; i < kHold; ++i) {
                     const int item = min(first + i * kThreads, items - 1);
-                    rr[i] = item / pieces;
+                    rr[i] = (int)(((float)item + 0.5f) * each);  // (item / pieces: both below 2^13)
                     rk[i] = (item - rr[i] * pieces) * 8;
-                    const int s = slot_at(p, rt, group, r0 + rr[i], list);
+                    const int s = slot_at(rt, gr, rr[i]);
                     raw[i].load(reinterpret_cast<const uint8_t*>(p.x) + (int64_t)(p.gather ? s / p.top_k : s) * p.ldx * kSrcBytes<SRC>, rk[i]);
                 }
             };
@@ -230,13 +357,18 @@ __global__ void __launch_bounds__(64 * KS * CG, KS * CG <= 4 ? 2 : 1) int8_rows_
                 }
             };
             constexpr int kTurn = kHold * kThreads;
-            read(tid);
-            __builtin_amdgcn_sched_barrier(0);
-            first_weights();
-            if (r0 > 0) __syncthreads();                         // (the last rows have been read)
+            if (again) lds_barrier();                            // (the last group's rows have been read)
             if (tid < 16) s_top[tid] = 0;
-            lds_barrier();
-            maxima(tid);
+            read(tid);
+            // (the maxima twice: each side then waits for as many loads as it has behind them)
+            if (!ahead) {
+                first_weights();
+                lds_barrier();
+                maxima(tid);
+            } else {
+                lds_barrier();
+                maxima(tid);
+            }
             for (int t = tid + kTurn; t - tid < items; t += kTurn) {
                 read(t);
                 maxima(t);
@@ -265,7 +397,13 @@ __global__ void __launch_bounds__(64 * KS * CG, KS * CG <= 4 ? 2 : 1) int8_rows_
         __builtin_amdgcn_sched_barrier(0);
 
         for (int it = 0; it < rounds; ++it) {
+            const bool end = it + 1 == rounds;                   // behind the last round: the first of what follows
+            const Part to{end ? nxt.w : cur.w, end ? nxt.ws : cur.ws, end ? nxt.f0 : cur.f0, end ? nxt.per : cur.per};
+            const int first = end ? 0 : (it + 1) * D, on = !end || follows ? -1 : 0;
             v4i run[D];
+            Cols next_cols;
+            load_cols(next_cols, to, end ? 0 : it + 1);
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int d = 0; d < D; ++d) {
                 run[d] = v4i{0, 0, 0, 0};
@@ -274,85 +412,87 @@ __global__ void __launch_bounds__(64 * KS * CG, KS * CG <= 4 ? 2 : 1) int8_rows_
 #pragma unroll
                     for (int h = 0; h < 2; ++h) run[d] = mfma_i8(ring[d].w[j][h], x[j][h], run[d]);
                 __builtin_amdgcn_sched_barrier(0);
-                // (behind the last round: the first fragments again, for the next sixteen rows)
-                const int next = (it + 1) * D + d;
-                load(ring[d], it + 1 < rounds ? next : d);
+                load(ring[d], to, first + d, on);
                 __builtin_amdgcn_sched_barrier(0);
             }
             // unit u of the round: an output fragment
-            auto put = [&](int u, const v4i& a, const v4i& b) __attribute__((always_inline)) {
+            auto put = [&](int u, int i, const v4i& a, const v4i& b) __attribute__((always_inline)) {
                 const int of = it * kUnits + u;
-                const int col = (f0 + of) * 16 + 4 * q;
+                const int col = (cur.f0 + of) * 16 + 4 * q;
                 if (of >= mine || slot < 0 || col >= cols) return;
                 v4f t;
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    const int n = min(col + r, cols - 1);
-                    const float f = xs * wse[n];
-                    if constexpr (kSilu) t[r] = silu_mul((float)a[r] * f, (float)b[r] * (xs * wse[half + n]));
-                    else if constexpr (DST == Out8::k16) t[r] = fmaf((float)a[r], f, bias_at(p, n));
-                    else t[r] = (float)a[r] * f;
+                    if constexpr (kSilu) {
+                        t[r] = silu_mul((float)a[r] * (xs * now.ws[i][r]), (float)b[r] * (xs * now.up[i][r]));
+                    } else if constexpr (DST == Out8::k16) {
+                        const int n = min(col + r, cols - 1);
+                        t[r] = fmaf((float)a[r], xs * cur.ws[n], bias_at(p, n));
+                    } else {
+                        t[r] = (float)a[r] * (xs * now.ws[i][r]);
+                    }
                 }
                 if constexpr (DST == Out8::k16) store16(p, slot, col, t);
                 else *reinterpret_cast<v4f*>(reinterpret_cast<float*>(p.out) + (int64_t)slot * p.ldo + col) = t;
             };
             if constexpr (KS == 1) {
 #pragma unroll
-                for (int u = 0; u < kUnits; ++u) put(u, run[u * kPair], run[u * kPair + kPair - 1]);
+                for (int u = 0; u < kUnits; ++u) put(u, u, run[u * kPair], run[u * kPair + kPair - 1]);
             } else {
                 auto& buf = part[it & 1][cg];
 #pragma unroll
                 for (int d = 0; d < D; ++d) buf[d][ks][lane] = run[d];
                 lds_barrier();
                 // (the next round writes the other buffer; this one is written again behind its barrier)
-#pragma unroll
-                for (int u0 = 0; u0 < kUnits; u0 += KS) {
-                    const int u = u0 + ks;
-                    if (kUnits % KS != 0 && u >= kUnits) break;
+                if (ks < kUnits) {
                     auto total = [&](int d) __attribute__((always_inline)) {
                         v4i t = buf[d][0][lane];
 #pragma unroll
                         for (int w = 1; w < KS; ++w) t += buf[d][w][lane];
                         return t;
                     };
-                    const v4i t = total(u * kPair);
-                    if constexpr (kSilu) put(u, t, total(u * kPair + 1));
-                    else put(u, t, t);
+                    const v4i t = total(ks * kPair);
+                    if constexpr (kSilu) put(ks, 0, t, total(ks * kPair + 1));
+                    else put(ks, 0, t, t);
                 }
             }
+            now = next_cols;
         }
         if (KS > 1) lds_barrier();                               // (an odd number of rounds: the first buffer is read)
+        again = true;
+        ahead = follows;
     }
 }
 
 // Any K, int8 rows: KS waves take the steps of K in turn (what they read at one time is contiguous along K).
-constexpr int kRing = 3;          // steps of a wave in flight
+constexpr int kRing = 3;          // steps of a wave in flight: two work-groups a CU have registers (four, with one: 14.4 us for 13.6)
 template <int FN, int KS, Out8 DST>
-__global__ void __launch_bounds__(64 * KS) int8_stream_kernel(RowsParams p, int slices) {
+__global__ void __launch_bounds__(64 * KS) int8_stream_kernel(RowsParams p) {
     constexpr bool kSilu = DST == Out8::kSiluF32;
     constexpr int kCols = kSilu ? FN / 2 : FN;                   // column fragments of the output
     __shared__ __attribute__((aligned(16))) v4i part[KS][FN][64];
-    __shared__ uint16_t list[kScanSlots];
-    __shared__ int counts[KS];
+    __shared__ Routed rt;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int q = lane >> 4, c = lane & 15;
-    const int group = blockIdx.x / slices, sl = blockIdx.x % slices;
-    const Routed rt = find_rows<KS>(p, group, list, counts);
-    if (rt.n == 0) return;
     const int half = p.N / 2;
     const int cols = kSilu ? half : p.N;
     const int K = p.K;
-    const int8_t* wp[FN];
-#pragma unroll
-    for (int j = 0; j < FN; ++j) {
-        const int f = (sl * kCols + j % kCols) * 16, up = kSilu && j >= kCols ? half : 0;
-        wp[j] = p.w + ((int64_t)rt.e * p.N + up + min(f + c, cols - 1)) * K;
-    }
-    const float* ws = p.ws + (int64_t)rt.e * p.N;
     const int G = (K + kStep - 1) / kStep, steps = (G + KS - 1) / KS;
-    for (int r0 = 0; r0 < rt.n; r0 += 16) {
-        const int slot = slot_at(p, rt, group, r0 + c, list);
-        const int row = slot < 0 ? slot_at(p, rt, group, r0, list) : slot;
+    const int frags = (cols + kCols * 16 - 1) / (kCols * 16);    // of kCols column fragments
+    bool again = false;
+    Walk walk(find_groups<KS>(p, rt), frags);
+    for (; walk.left > 0; --walk.left, walk.f + 1 < frags ? ++walk.f : (++walk.g, walk.f = 0)) {
+        const Group gr = group_at(p, rt, walk.g);
+        if (gr.n == 0) continue;
+        const int8_t* wp[FN];
+#pragma unroll
+        for (int j = 0; j < FN; ++j) {
+            const int f = (walk.f * kCols + j % kCols) * 16, up = kSilu && j >= kCols ? half : 0;
+            wp[j] = p.w + ((int64_t)gr.e * p.N + up + min(f + c, cols - 1)) * K;
+        }
+        const float* ws = p.ws + (int64_t)gr.e * p.N;
+        const int slot = c < gr.n ? slot_at(rt, gr, c) : -1;
+        const int row = slot < 0 ? slot_at(rt, gr, 0) : slot;
         const int xrow = p.gather ? row / p.top_k : row;
         const int8_t* xp = reinterpret_cast<const int8_t*>(p.x) + (int64_t)xrow * p.ldx;
         struct Stage {
@@ -387,13 +527,14 @@ __global__ void __launch_bounds__(64 * KS) int8_stream_kernel(RowsParams p, int 
                 __builtin_amdgcn_sched_barrier(0);
             }
         }
-        if (r0 > 0) __syncthreads();                             // (the last rows' sums have been read)
+        if (again) __syncthreads();                              // (the last sums have been read)
+        again = true;
 #pragma unroll
         for (int j = 0; j < FN; ++j) part[wave][j][lane] = run[j];
         __syncthreads();
         // wave j joins column fragment j (four adjacent columns of a row a lane)
         static_assert(kCols <= KS, "a wave a fragment");
-        const int col = (sl * kCols + wave) * 16 + 4 * q;
+        const int col = (walk.f * kCols + wave) * 16 + 4 * q;
         if (wave >= kCols || slot < 0 || col >= cols) continue;
         auto total = [&](int f) __attribute__((always_inline)) {
             v4i t = part[0][f][lane];
@@ -531,48 +672,44 @@ int too_many() {
     return W4A8_ERR_INVALID;
 }
 // Groups of rows that work-groups take.
-int64_t groups_of(const RowsParams& p) { return p.ids == nullptr ? 1 : std::min(p.slots, p.E); }
+int64_t groups_of(const RowsParams& p) {
+    return p.ids == nullptr ? ((int64_t)p.rows + 15) / 16 : std::min(p.slots, p.E + p.slots / 16);
+}
 template <int FN, int KS, Out8 DST>
 int stream_go(const RowsParams& p, hipStream_t s) {
     constexpr bool silu = DST == Out8::kSiluF32;
     const int cols = silu ? p.N / 2 : p.N, per = 16 * (silu ? FN / 2 : FN);
-    const int slices = (cols + per - 1) / per;
-    const int64_t grid = groups_of(p) * slices;
-    if (!grid_fits(grid, 64 * KS)) return too_many();
-    launch_kernel(&int8_stream_kernel<FN, KS, DST>, dim3((unsigned)grid), dim3(64 * KS), 0, s, p, slices);
+    // (two work-groups a CU run at once; several rounds of them even out their ends)
+    const int64_t units = groups_of(p) * ((cols + per - 1) / per), grid = std::min<int64_t>(units, (int64_t)device_cu_count() * 16);
+    if (units >= (int64_t)1 << 31) return too_many();
+    launch_kernel(&int8_stream_kernel<FN, KS, DST>, dim3((unsigned)grid), dim3(64 * KS), 0, s, p);
     return check_launch("int8_stream_kernel");
 }
 
-// per: output fragments a group of waves walks over. The kernel loads D fragments beforehand whatever `per` is, so few of
+// per: output fragments that KS waves walk over. The kernel loads D fragments beforehand whatever `per` is, so few of
 // them take a variant with a smaller D.
 template <int GPW, int KS, int CG, int D, Src8 SRC, Out8 DST>
-int rows_launch(const RowsParams& p, int frags, int64_t per, hipStream_t s) {
+int rows_launch(const RowsParams& p, int64_t grid, int64_t per, hipStream_t s) {
     constexpr int pair = DST == Out8::kSiluF32 ? 2 : 1;
     if constexpr (D > pair)
-        if (per * pair <= D / 2) return rows_launch<GPW, KS, CG, D / 2, SRC, DST>(p, frags, per, s);
-    const int slices = (int)((frags + per * CG - 1) / (per * CG));
-    const int64_t grid = groups_of(p) * slices;
-    if (!grid_fits(grid, 64 * KS * CG)) return too_many();
-    launch_kernel(&int8_rows_kernel<GPW, KS, CG, D, SRC, DST>, dim3((unsigned)grid), dim3(64 * KS * CG), 0, s, p, slices, (int)per);
+        if (per * pair <= D / 2) return rows_launch<GPW, KS, CG, D / 2, SRC, DST>(p, grid, per, s);
+    launch_kernel(&int8_rows_kernel<GPW, KS, CG, D, SRC, DST>, dim3((unsigned)grid), dim3(64 * KS * CG), 0, s, p);
     return check_launch("int8_rows_kernel");
 }
 
 template <int GPW, int KS, int CG, int D, Src8 SRC, Out8 DST>
 int rows_go(const RowsParams& p, hipStream_t s) {
-    constexpr int unit = D / (DST == Out8::kSiluF32 ? 2 : 1);
-    const int frags = ((DST == Out8::kSiluF32 ? p.N / 2 : p.N) + 15) / 16;
-    // As many work-groups as run at once (eight waves a CU), those of groups without rows among them, each walking over
-    // what that leaves it: some more would run behind all others. us of a layer of 256 experts (2048 x 512, 8 a token), by
-    // the first product's fragments a work-group 1 / 2 / 4 / 8 / 16 / 32 (the rule's in brackets): 8 tokens 63 / 53 / (47) /
-    // 48 / 62 / 94, 16 tokens 104 / 92 / 82 / (78) / 78 / 107, 64 tokens 229 / 194 / 176 / 170 / (168) / 165.
+    const int64_t frags = ((DST == Out8::kSiluF32 ? p.N / 2 : p.N) + 15) / 16, units = groups_of(p) * frags;
+    if (units >= (int64_t)1 << 31) return too_many();
+    // As many work-groups as run at once (eight waves a CU).
     const int64_t resident = (int64_t)device_cu_count() * std::max(1, 8 / (KS * CG));
-    const int64_t slices = std::max<int64_t>(1, resident / groups_of(p));
-    int64_t per = (frags + CG * slices - 1) / (CG * slices);
-    if (per > unit) per = (per + unit - 1) / unit * unit;
-    return rows_launch<GPW, KS, CG, D, SRC, DST>(p, frags, std::max<int64_t>(1, per), s);
+    const int64_t grid = std::min(resident, (units + CG - 1) / CG);
+    return rows_launch<GPW, KS, CG, D, SRC, DST>(p, grid, (units + grid * CG - 1) / (grid * CG), s);
 }
 
 // The wave split by the number of steps: a wave holds the rows' values of up to four of them, up to eight waves share K.
+// (Sixteen waves of one step each less, or two column fragments, of longer K: 15.7 and 19.8 us for 13.5, 8 rows of 4096 x
+// 12288.)
 template <Src8 SRC, Out8 DST>
 int rows_any(const RowsParams& p, hipStream_t s) {
     const int G = (p.K + kStep - 1) / kStep;
@@ -611,7 +748,7 @@ int launch_int8_token(const RowsArgs& a, const float* topk_weights, hipStream_t 
 
 int launch_int8_rows(const RowsArgs& a, hipStream_t s) {
     RowsParams p = rows_params(a);
-    p.by_slot = few_slots(p.slots, p.E) ? kOneSlot : p.slots < p.E ? 1 : 0;
+    p.one_slot = few_slots(p.slots, p.E) ? 1 : 0;
     if (p.rows == 0 || (p.ids != nullptr && p.slots == 0)) return W4A8_OK;
     if (p.ids != nullptr && p.slots > kScanSlots) {
         set_error("int8 product: too many slots for the streaming kernels");
