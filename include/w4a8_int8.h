@@ -37,7 +37,7 @@ W4A8_API int w4a8_act_quant_int8(const void* x, int x_dtype, int64_t rows, int64
  * bf16 (x_scales unused): quantised in the call, as w4a8_act_quant_int8 does. K a multiple of 16 up to 131071; rows of x
  * start at multiples of 16 bytes; x and w aligned to 16 bytes. bias (N,): null, fp32 (bias_is_f32 != 0) or of out's
  * type. */
-W4A8_API size_t w4a8_int8_gemm_workspace_size(int x_dtype, int64_t M, int64_t K);
+W4A8_API size_t w4a8_int8_gemm_workspace_size(int x_dtype, int64_t M, int64_t K, int64_t N);
 W4A8_API int w4a8_int8_gemm(const void* x, int x_dtype, const float* x_scales, int64_t M, int64_t K, int64_t x_stride,
                             const int8_t* w, const float* w_scales, int64_t N, const void* bias, int bias_is_f32, void* out,
                             int out_dtype, void* workspace, size_t workspace_bytes, void* stream);

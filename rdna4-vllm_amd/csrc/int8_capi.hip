@@ -24,12 +24,16 @@ Src8 src_of(int dt) { return dt == W4A8_DTYPE_INT8 ? Src8::kI8 : dt == W4A8_DTYP
 Rows rows_of(int dt) { return dt == W4A8_DTYPE_BF16 ? Rows::kBf16 : Rows::kF16; }
 
 constexpr int64_t kMaxSide = (int64_t)1 << 24;    // rows of a weight
-constexpr int64_t kStreamRows = 16;               // dense rows up to which the weights are streamed
+// Dense rows and K up to which the weights are streamed, else tiles. us streamed / tiles, 8 rows: 2048 x 2048 4.4 / 5.1,
+// one row: 229376 x 2048 82 / 84, 229376 x 512 29 / 34; but 4096 x 4096 7.3 / 6.8, 12288 x 4096 13.0 / 10.0, 28672 x 8192 63 / 44.
+constexpr int64_t kStreamRows = 16, kStreamK = 2048;
 constexpr int64_t kMaxRows = ((int64_t)1 << 31) - 256;
 
-// Dense rows that the product's kernel quantises itself; more take a launch of their own (4096 x 4096, us in the kernel /
-// before it: 1 row 8.9 / 10.5, 4 10.5 / 11, 16 18.7 / 11.8).
-bool quantised_in_kernel(int64_t M, int64_t K) { return M <= 4 && int8_rows_quantised_in_kernel(K); }
+// Dense rows that the product's kernel quantises itself; more take a launch of their own. us in the kernel / before tiles,
+// 4096 x 4096: 1 row 7.7 / 8.8, 4 rows 8.9 / 9.1; but 12288 x 4096, 1 row 14.3 / 12.1.
+bool quantised_in_kernel(int64_t M, int64_t K, int64_t N) {
+    return M <= 4 && int8_rows_quantised_in_kernel(K) && (K <= kStreamK || N * K <= (int64_t)1 << 25);
+}
 
 // Sizes and pointers that every product shares.
 int check_product(const void* x, int x_dtype, const float* xs, int64_t rows, int64_t K, int64_t ldx, const int8_t* w,
@@ -202,8 +206,8 @@ int w4a8_act_quant_int8(const void* x, int x_dtype, int64_t rows, int64_t K, int
                                  as_stream(stream));
 }
 
-size_t w4a8_int8_gemm_workspace_size(int x_dtype, int64_t M, int64_t K) {
-    if (x_dtype == W4A8_DTYPE_INT8 || M <= 0 || K <= 0 || quantised_in_kernel(M, K)) return 0;
+size_t w4a8_int8_gemm_workspace_size(int x_dtype, int64_t M, int64_t K, int64_t N) {
+    if (x_dtype == W4A8_DTYPE_INT8 || M <= 0 || K <= 0 || N <= 0 || quantised_in_kernel(M, K, N)) return 0;
     WorkspaceSize s;
     s.take<int8_t>((size_t)(M * K));
     s.take<float>((size_t)M);
@@ -219,7 +223,7 @@ int w4a8_int8_gemm(const void* x, int x_dtype, const float* x_scales, int64_t M,
     if (M == 0) return W4A8_OK;
     W4A8_REQUIRE(out, "int8_gemm: null pointer");
     hipStream_t s = as_stream(stream);
-    const bool in_kernel = quantised_in_kernel(M, K);
+    const bool in_kernel = quantised_in_kernel(M, K, N);
     Src8 src = src_of(x_dtype);
     if (src != Src8::kI8 && !in_kernel) {
         Workspace ws(workspace, workspace_bytes);
@@ -239,7 +243,7 @@ int w4a8_int8_gemm(const void* x, int x_dtype, const float* x_scales, int64_t M,
     a.dst = Out8::k16; a.bf16 = out_dtype == W4A8_DTYPE_BF16; a.out = out; a.ldo = N;
     // The tiles address weights and rows in 32 bits: rows past that are taken in parts.
     const int64_t lim = ((int64_t)1 << 32) - 1, part = lim / x_stride / 256 * 256;
-    if (M > kStreamRows && N * K <= lim && part > 0) {
+    if ((M > kStreamRows || K > kStreamK) && src == Src8::kI8 && N * K <= lim && part > 0) {
         for (int64_t m = 0; m < M; m += part) {
             a.x_rows = a.P = a.num_valid = std::min(part, M - m);
             if (int rc = launch_int8_tiles(a, s)) return rc;

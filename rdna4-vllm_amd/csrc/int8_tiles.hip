@@ -7,6 +7,10 @@
 //
 // Work-groups are persistent: a tile's ids are read under the one before, its first steps are loaded under the one
 // before's epilogue.
+//
+// Bound: of few rows HBM (77 rows of 12288 x 4096: 13.6 us, 4 TB/s), of many the matrix cores' power (see dense_go). Of a
+// layer's 32768 slots over 256 experts (2048 x 512, rows skewed) the first product takes 170 us (537 MB of weights at
+// 3.2 TB/s, x and h beside them), the second 123 (268 MB, and 134 MB of slots' rows written).
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -56,7 +60,6 @@ struct Tile {
     static constexpr int PX = BT * 8 / kThreads, PW = BN * 8 / kThreads;   // 16-byte pieces a thread
     static constexpr int kLoads = PX + PW;                       // of a wave and step
     static_assert(PX * kThreads == BT * 8 && PW * kThreads == BN * 8, "pieces divide");
-    static_assert(kThreads % 128 == 0, "a thread's pieces are the same one of their rows");
     static_assert(S >= 2 && S <= 6 && (!DEEP || S % 2 == 0), "two to six slots, for two sets of fragments in turn");
     static_assert(kLoads * (S - 1) < 64, "loads in flight can be counted");
 };
@@ -108,7 +111,7 @@ __global__ void __launch_bounds__(C::kThreads * C::KS, C::EU) int8_tiles_kernel(
         const int pl = (tid + i * C::kThreads) >> 3;
         return pl ^ ((pl >> 3) & 1);
     };
-    const int piece_k = ((tid & 7) ^ (piece_row(0) & 7)) * 16;
+    auto piece_k = [&](int i) __attribute__((always_inline)) { return ((tid & 7) ^ (piece_row(i) & 7)) * 16; };
     // The column behind row r of the slot's BN: of each 32, MFMA row 8 a + 4 b + d is column 16 b + 4 a + d. kSilu takes
     // FN / 2 fragments of the gate half and the same of the up half.
     const int half = N / 2;
@@ -156,9 +159,9 @@ __global__ void __launch_bounds__(C::kThreads * C::KS, C::EU) int8_tiles_kernel(
         we = p.w + (int64_t)e * N * K;
 #pragma unroll
         for (int i = 0; i < C::PX; ++i)
-            xoff[i] = xrow_of(row0 + piece_row(i), GROUPED ? ids[i] : 0) * (uint32_t)p.ldx + (uint32_t)piece_k;
+            xoff[i] = xrow_of(row0 + piece_row(i), GROUPED ? ids[i] : 0) * (uint32_t)p.ldx + (uint32_t)piece_k(i);
 #pragma unroll
-        for (int i = 0; i < C::PW; ++i) woff[i] = (uint32_t)col_of(ct, piece_row(i)) * (uint32_t)K + (uint32_t)piece_k;
+        for (int i = 0; i < C::PW; ++i) woff[i] = (uint32_t)col_of(ct, piece_row(i)) * (uint32_t)K + (uint32_t)piece_k(i);
         // the tile's scales, for its epilogue
 #pragma unroll
         for (int i = 0; i < NX; ++i) {
@@ -195,18 +198,18 @@ __global__ void __launch_bounds__(C::kThreads * C::KS, C::EU) int8_tiles_kernel(
         const int8_t* wg = reinterpret_cast<const int8_t*>(((reinterpret_cast<uint64_t>(we) + at) & far) | z);
         asm volatile("" : "+s"(xg), "+s"(wg));                   // (scalar bases, 32-bit offsets)
         int8_t *xd = slot + wave * 1024, *wd = slot + C::kW + wave * 1024;
-        auto src = [&](const int8_t* base, uint32_t off) __attribute__((always_inline)) {
+        auto src = [&](const int8_t* base, uint32_t off, int i) __attribute__((always_inline)) {
             const int8_t* at = base + opaque_u32(off & on);
             if constexpr (TAIL)
-                if (gg * kStep + piece_k >= K) at = zeros;
+                if (gg * kStep + piece_k(i) >= K) at = zeros;
             return at;
         };
 #pragma unroll
         for (int i = 0; i < C::PX; ++i)
-            if (i * parts / C::kLoads == some) dma(src(xg, xoff[i]), xd + i * C::kThreads * 16);
+            if (i * parts / C::kLoads == some) dma(src(xg, xoff[i], i), xd + i * C::kThreads * 16);
 #pragma unroll
         for (int i = 0; i < C::PW; ++i)
-            if ((C::PX + i) * parts / C::kLoads == some) dma(src(wg, woff[i]), wd + i * C::kThreads * 16);
+            if ((C::PX + i) * parts / C::kLoads == some) dma(src(wg, woff[i], i), wd + i * C::kThreads * 16);
     };
 
     // ---- fragments: lane (h, c) reads piece 2 s + h of row c of each 32, sub-step s of four ----
@@ -506,6 +509,7 @@ int tiles_go(const Int8Params& p, hipStream_t s) {
 }
 
 //                      WT WN FT FN S KS EU
+using Tile32x32K4 = Tile<1, 1, 1, 1, 4, 4, 1, true>;
 using Tile64x32K2 = Tile<2, 1, 1, 1, 4, 2, 1, true>;
 using Tile64x64 = Tile<2, 2, 1, 1, 4, 1, 2, true>;       // two work-groups a CU, the others one
 using Tile128x64 = Tile<4, 2, 1, 1, 4, 1, 2, true>;
@@ -521,34 +525,37 @@ using Second128 = Tile<2, 4, 2, 2, 3, 1, 2>;
 // The dense tile of least cost. us as measured at N = K = 4096 (the rule compares tiles at one K, as if all their costs
 // grew with it alike), by the tiles a CU has to take:
 //                            1/4   1/2   3/4     1   1.5     2     3     4
+//   32 x 32, K in four             7.0         14.3*
 //   64 x 32, K in two        8.3   8.4         14.7*
 //   64 x 64                  9.3   9.4  ...    10.0  14.8  15.6  21.8  28.5
 //   128 x 64                10.2  11.5  12.1   13.7  23.4  25.5  36.8  49.8
 //   128 x 128               15.0  15.8  18.1   21.2  35.3  40.7        79.2
 //   256 x 128               25.5  27.3  30.4   35.9        71.7       218 (6)
 //   256 x 256               42.9  44.5         59.0       190.7 (3)
-// (* two a CU do not run beside each other.) What a CU loads into LDS bounds the small ones: about 95 bytes a
-// nanosecond with all CUs at it, 120 with few. The largest does 2.3 PFLOP/s (4096^3), where MFMAs alone on such data, by
-// the card's power, do 3.4.
+// (* two a CU do not run beside each other.) 8 rows of K = 12288, N = 4096: 32 x 32 11.8, 64 x 32 13.7. What a CU loads into
+// LDS bounds the small ones: about 95 bytes a nanosecond with all CUs at it, 120 with few. The largest does 2.25e15
+// operations a second (4096 x 12288 x 4096: 183 us), where MFMAs alone on such data, by the card's power, do 3.4e15.
 int dense_go(const Int8Params& p, hipStream_t s) {
     const float cus = (float)device_cu_count();
     auto share = [&](int bt, int bn) { return (float)((int64_t)((p.P + bt - 1) / bt) * ((p.N + bn - 1) / bn)) / cus; };
     auto cost = [](float f, float base, float slope, float least, float each) {   // f: tiles a CU
         return f <= 1.f ? std::max(least, base + slope * f) : each * std::ceil(f);
     };
-    const float f32 = share(64, 32), f64 = share(64, 64);
+    const float f32x32 = share(32, 32), f32 = share(64, 32), f64 = share(64, 64);
+    const float c32x32 = f32x32 <= 1.f ? 7.4f : 1e9f;
     const float c32 = f32 <= 1.f ? 8.4f : 1e9f;
     const float c64 = f64 <= 1.f ? 9.7f : 2.2f + 6.7f * std::ceil(f64);
     const float c128x64 = cost(share(128, 64), 10.4f, 3.2f, 0.f, 12.5f);
     const float c128 = cost(share(128, 128), 10.4f, 10.8f, 15.2f, 20.f);
     const float c256x128 = cost(share(256, 128), 18.f, 18.f, 26.5f, 36.f);
     const float c256 = cost(share(256, 256), 30.f, 29.f, 43.f, 62.f);
-    const float best = std::min({c32, c64, c128x64, c128, c256x128, c256});
+    const float best = std::min({c32x32, c32, c64, c128x64, c128, c256x128, c256});
     if (c256 == best) return tiles_go<Tile256x256, Out8::k16, false>(p, s);
     if (c256x128 == best) return tiles_go<Tile256x128, Out8::k16, false>(p, s);
     if (c128 == best) return tiles_go<Tile128x128, Out8::k16, false>(p, s);
     if (c128x64 == best) return tiles_go<Tile128x64, Out8::k16, false>(p, s);
     if (c64 == best) return tiles_go<Tile64x64, Out8::k16, false>(p, s);
+    if (c32x32 == best) return tiles_go<Tile32x32K4, Out8::k16, false>(p, s);
     return tiles_go<Tile64x32K2, Out8::k16, false>(p, s);
 }
 

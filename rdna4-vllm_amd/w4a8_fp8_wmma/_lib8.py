@@ -19,7 +19,7 @@ SIGNATURES = {
     "w4a8_int8_abi_version": (_int, []),
     "w4a8_int8_last_error": (ctypes.c_char_p, []),
     "w4a8_act_quant_int8": (_int, [_p, _int, _i64, _i64, _i64, _int, _p, _p, _p]),
-    "w4a8_int8_gemm_workspace_size": (_size, [_int, _i64, _i64]),
+    "w4a8_int8_gemm_workspace_size": (_size, [_int, _i64, _i64, _i64]),
     "w4a8_int8_gemm": (_int, [_p, _int, _p, _i64, _i64, _i64, _p, _p, _i64, _p, _int, _p, _int, _p, _size, _p]),
     "w4a8_moe_int8_workspace_size": (_size, [_i64, _i64, _i64, _i64, _i64]),
     "w4a8_moe_int8_apply": (_int, [_p, _int, _p, _i64, _i64, _i64, _i64, _i64, _p, _p, _p, _p, _p, _p, _p, _i64, _p,

@@ -112,7 +112,7 @@ def int8_gemm(x: torch.Tensor, x_scales: torch.Tensor | None, w: torch.Tensor, w
     _same_device(dev, xs, w, ws, bias)
     x = _mfma_rows(x, "x")
     out = torch.empty((M, N), dtype=dt, device=dev)
-    nbytes = 0 if xs is not None else lib.w4a8_int8_gemm_workspace_size(_DT[x.dtype], M, K)
+    nbytes = 0 if xs is not None else lib.w4a8_int8_gemm_workspace_size(_DT[x.dtype], M, K, N)
     work = _workspace(nbytes, dev) if nbytes else None
     with _on(dev):
         check(lib.w4a8_int8_gemm(

@@ -70,8 +70,9 @@ def test_dense_refusals(bad, says):
 
 def test_dense_workspace():
     size = L.w4a8_int8_gemm_workspace_size
-    assert size(INT8, 0, 4096) == 0 and size(BF16, 0, 128) == 0
-    need = size(BF16, 4097, 400)
+    assert size(INT8, 0, 4096, 64) == 0 and size(BF16, 0, 128, 64) == 0
+    assert size(BF16, 1, 4096, 4096) == 0 and size(BF16, 1, 4096, 65536) >= 4096 + 4
+    need = size(BF16, 4097, 400, 64)
     assert need >= 4097 * 400 + 4097 * 4
     assert gemm(xd=BF16, xs=None, M=4097, K=400, ldx=400) == WORKSPACE and "workspace" in err()
     assert gemm(xd=BF16, xs=None, M=4097, K=400, ldx=400, work=P16, nb=need - 1) == WORKSPACE
