@@ -10,7 +10,8 @@
 // one, c is formed in fp64 (in fp32 two experts' c may round to one number), compared rounded to fp32 (which keeps the
 // order) and, where that is equal, by what was rounded off.
 //
-// Bound: for many tokens the vector units (their logits take 4 us), for few the launch.
+// Bound: for many tokens the vector units: 16384 tokens of 256 experts, 8 picks in 4 of 8 groups, sigmoid with a bias, take
+// 13.1 us with the call (one token a wave: 39), where their logits' bytes take 4; for few the launch, 4.5 us.
 #include <type_traits>
 
 #include "w4a8_common.h"
