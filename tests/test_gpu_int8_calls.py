@@ -70,6 +70,27 @@ def test_layer_skewed(T):
     layer_ok(T, 16, 2, 128, 64, skew=4.0)
 
 
+@pytest.mark.parametrize("T,E,k,kind", [(50, 64, 8, "one"), (50, 64, 8, "two"), (2, 256, 8, "one"), (33, 1024, 8, "one"), (512, 1024, 8, "few"),
+                                        (512, 1024, 8, "all"), (16, 1, 8, "one"), (50, 64, 8, "none"), (3, 256, 8, "none"), (50, 64, 8, "odd")])
+def test_layer_ids(T, E, k, kind):
+    """Every slot at one expert or at few, an expert several times among a token's picks, no slot at all, ids of no expert."""
+    H, I = 128, 64
+    g = gen(T, E, k, 47)
+    w13, w2, s13, s2 = make_layer(g, E, H, I)
+    tw = torch.rand((T, k), generator=g)
+    pick = {"one": [E - 1], "two": [0, E - 1], "few": [1, 7, 500, 1023], "all": list(range(E)), "none": [-1], "odd": [-5, 3, E, 2 ** 31 - 1]}[kind]
+    ids = torch.tensor(pick)[torch.randint(0, len(pick), (T, k), generator=g)].to(torch.int32)
+    x = hidden(g, T, H, torch.bfloat16)
+    args = on(x, w13, w2, s13, s2, tw, ids)
+    y = W.moe_int8_apply(*args)
+    live = torch.where((ids >= 0) & (ids < E), ids, -1)
+    ref, tol = O.layer(*O.quantise(f64(x)), f64(w13), s13.numpy(), f64(w2), s2.numpy(), tw.numpy(), live.numpy(),
+                       rows16=rows16(T, E, k, torch.bfloat16))
+    assert_close(y, ref, tol, torch.bfloat16)
+    for _ in range(5):
+        assert torch.equal(W.moe_int8_apply(*args), y)
+
+
 def test_layer_many_tokens_of_wide_experts():
     layer_ok(3000, 4, 2, 192, 704, part=40)
 
