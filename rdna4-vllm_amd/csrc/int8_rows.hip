@@ -561,7 +561,7 @@ __global__ void __launch_bounds__(64 * KS) int8_stream_kernel(RowsParams p) {
 // The layer's second product and its sum over a token's slots, for hardly two slots of one expert: a work-group takes a
 // token and FN column fragments, wave w the token's slots w, w + 8, ... in turn. A wave quantises its slot's row of h (fp32)
 // alone, multiplies by its expert's weights, and the slots are added in order through LDS. Saves a launch and the slots'
-// rows (one token of 256 experts, 2048 x 512: 18.3 -> 16.4 us).
+// rows.
 constexpr int kTokenWaves = 8;
 constexpr int kTokenK = 4096;
 template <int FN>
@@ -728,15 +728,17 @@ int rows_any(const RowsParams& p, hipStream_t s) {
 
 bool int8_rows_quantised_in_kernel(int64_t K) { return K <= 32 * kStep; }
 
-// Hardly two slots of one expert, whose weights would be read twice: no scan for them, either (one token of 256 experts,
-// 2048 x 512: 16.4 -> 15.6 us).
-bool few_slots(int64_t slots, int64_t E) { return slots * 8 <= E; }
+// Hardly two slots of one expert, whose weights would be read twice: no count, and one launch less. us as ever / with it:
+// 256 experts of 2048 x 512, 8 picks, 1 token 18.4 / 14.2, 4 tokens 30.4 / 25.9, 8 tokens 45.3 / 44.3; 64 experts of 4096 x
+// 1024, 6 picks, 2 tokens 45.1 / 36.5.
+bool few_slots(int64_t slots, int64_t E) { return slots * 4 <= E; }
 bool int8_token_supported(int64_t slots, int64_t E, int64_t inter) { return few_slots(slots, E) && inter <= kTokenK; }
 
 int launch_int8_token(const RowsArgs& a, const float* topk_weights, hipStream_t s) {
     const RowsParams p = rows_params(a);
     const int frags = (p.N + 15) / 16, tokens = p.slots / p.top_k;
-    // one fragment a work-group while those run at once (four a CU), else two
+    // one fragment a work-group while those run at once (four a CU), else two (us with one / two, 2048 x 512: 1 token 14.2 /
+    // 17.0, 4 tokens 25.9 / 25.1)
     const bool two = (int64_t)tokens * frags > 4 * (int64_t)device_cu_count();
     const int slices = two ? (frags + 1) / 2 : frags;
     const int64_t grid = (int64_t)tokens * slices;

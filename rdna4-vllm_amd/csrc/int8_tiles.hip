@@ -516,7 +516,9 @@ using Tile128x64 = Tile<4, 2, 1, 1, 4, 1, 2, true>;
 using Tile128x128 = Tile<2, 4, 2, 1, 4, 1, 2, true>;
 using Tile256x128 = Tile<4, 2, 2, 2, 3, 1, 2>;
 using Tile256x256 = Tile<2, 4, 4, 2, 2, 1, 2>;
-// grouped: the layer's first and second product, blocks of 64 and 128 rows
+// grouped: the layer's first and second product, blocks of 64 and 128 rows. The first product's waves hold gate and up
+// fragments of the same columns; the second one's steps are few, so that waves (eight, two work-groups a CU) hide its
+// prologue and stores: with four waves a layer of 4096 tokens, 256 experts of 2048 x 512, took 350 us for 335.
 using First64 = Tile<1, 4, 2, 2, 2, 1, 2>;
 using Second64 = Tile<2, 4, 1, 2, 2, 1, 4>;
 using First128 = Tile<2, 4, 2, 2, 3, 1, 2>;
