@@ -25,8 +25,6 @@ enum class Out8 : int {
     k16 = 0,        // out[row, n] rounded to fp16 or bf16
     kSiluF32 = 1,   // out[row, n] = silu(gate) * up in fp32, N = [gate | up] halves
     kSlotF32 = 2,   // out[slot, n] in fp32
-    kSlot16 = 3,    // out[slot, n] in fp16 with a scale per row and 32 columns (out_scales: the row's times a power of
-                    // two), so that no value overflows and none loses bits to a fixed range
 };
 
 // What the streaming kernels read their rows from.
@@ -57,7 +55,6 @@ struct Int8Args {
     Out8 dst;
     bool bf16;                   // k16: bf16, else fp16
     void* out;
-    float* out_scales;
     int64_t ldo;
 };
 
@@ -99,7 +96,6 @@ struct Int8Params : OutParams {
     const int32_t* sorted_ids;
     const int32_t* expert_ids;
     const int32_t* ntp;
-    float* out_scales;
     int P, x_rows, num_valid, block_m;
 };
 struct RowsParams : OutParams {
@@ -123,7 +119,6 @@ inline Int8Params int8_params(const Int8Args& a) {
     Int8Params p;
     out_params(a, p);
     p.x = a.x; p.xs = a.xs; p.sorted_ids = a.sorted_ids; p.expert_ids = a.expert_ids; p.ntp = a.ntp;
-    p.out_scales = a.out_scales;
     p.P = (int)a.P; p.x_rows = (int)a.x_rows; p.num_valid = (int)a.num_valid; p.block_m = (int)a.block_m;
     return p;
 }
@@ -251,8 +246,8 @@ int launch_int8_token(const RowsArgs& a, const float* topk_weights, hipStream_t 
 // Tiles (int8_tiles.hip): sizes that 32-bit offsets reach; grouped, blocks of as many rows as a tile has: 64 or 128.
 int launch_int8_tiles(const Int8Args& a, hipStream_t s);
 // out[t, n] = sum over the slots j in order of tw[t, j] * y[t top_k + j, n], rounded to 16 bits; slots whose (mapped)
-// expert is not in [0, E) contribute nothing. y as kSlotF32, or with scales as kSlot16 leaves it. N % 32 == 0.
-int launch_int8_reduce(const void* y, const float* y_scales, const float* tw, const int32_t* ids, const int32_t* emap, int64_t emap_len, int64_t E,
+// expert is not in [0, E) contribute nothing. N % 8 == 0.
+int launch_int8_reduce(const float* y, const float* tw, const int32_t* ids, const int32_t* emap, int64_t emap_len, int64_t E,
                        int64_t T, int64_t N, int64_t top_k, void* out, bool bf16, hipStream_t s);
 
 }  // namespace w4a8

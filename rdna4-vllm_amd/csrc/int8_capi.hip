@@ -54,12 +54,12 @@ int check_product(const void* x, int x_dtype, const float* xs, int64_t rows, int
 
 // ---- the gated layer ----
 // Few rows an expert: the streaming kernels, which find their rows in the routed ids (h and the slots' rows in fp32, by
-// slot). Else tiles: rows quantised beforehand, slots aligned to blocks of the rows that a tile has. The slots' rows
-// are rounded before the sum only where that is lost in the output's own rounding: for bf16 output they are fp16 with
-// a power of two for 32 columns (an eighth of its step), for fp16 output fp32. Tokens are taken in parts of as many as
-// either can address.
+// slot). Else tiles: rows quantised beforehand, slots aligned to blocks of the rows that a tile has. The slots' rows are
+// fp32 in every schedule and summed in the slots' order, so that a token's output has the same bits in any batch (in fp16
+// they are half the bytes, but where slots cancel their roundings are all that is left). Tokens are taken in parts of as
+// many as either can address.
 // Slots an expert from which tiles have 128 rows (us with 64 / 128: 64 experts of 4096 x 1024, 6 picks: 96 slots an expert
-// 310 / 310, 192 462 / 431, 384 800 / 769; but 256 experts of 2048 x 512, skewed, 128 slots an expert: 348 / 407).
+// 281 / 278, 192 410 / 373, 384 686 / 639; but 256 experts of 2048 x 512, skewed, 128 slots an expert: 376 / 419).
 constexpr int64_t kWideRows = 192;
 struct LayerPlan {
     bool tiles;
@@ -71,9 +71,9 @@ struct LayerPlan {
 LayerPlan plan_layer(int64_t T, int64_t H, int64_t inter, int64_t E, int64_t top_k, int x_dtype) {
     LayerPlan pl{};
     const int64_t lim = ((int64_t)1 << 32) - 1, pad = E * 127 + 128;
-    // (us streamed / tiles: 256 experts of 2048 x 512, 8 picks, 100 tokens 158 / 175, 176 172 / 181, 256 187 / 184, skewed 176
-    // 183 / 160, 256 236 / 172; 32 experts, 4 picks, 64 tokens 41 / 49, 90 54 / 50; 8 experts, 2 picks, 40 tokens 31 / 35, 90
-    // 38 / 35.)
+    // (us streamed / tiles: 256 experts of 2048 x 512, 8 picks, 100 tokens 158 / 178, 176 172 / 183, 256 189 / 187, skewed 176
+    // 187 / 163, 256 236 / 175; 32 experts, 4 picks, 64 tokens 38 / 41, 90 53 / 41; 8 experts, 2 picks, 40 tokens 30 / 35, 90
+    // 39 / 37.)
     pl.tiles = T * top_k > std::min<int64_t>(5 * E + 128, kScanSlots) && 2 * inter * H <= lim;
     const int64_t most = pl.tiles ? std::min(lim / H, (lim / inter - pad) / top_k) : kScanSlots / top_k;
     pl.part = std::min(T, std::max<int64_t>(1, most));
@@ -92,7 +92,6 @@ struct LayerScratch {
     size_t align_bytes;
     int8_t *xq, *hq;
     float *xs, *hs, *h, *y;
-    float* ys;                   // y in fp16: its scales, behind it
 };
 template <typename WS>
 void carve_layer(WS& w, const LayerPlan& pl, int64_t H, int64_t inter, int64_t E, int64_t top_k, LayerScratch& m) {
@@ -115,7 +114,6 @@ void carve_layer(WS& w, const LayerPlan& pl, int64_t H, int64_t inter, int64_t E
         m.hs = w.template take<float>((size_t)pl.P);
     }
     m.y = w.template take<float>((size_t)(n * H));
-    m.ys = m.y + n * H / 2;
 }
 struct Layer {
     const void* x;
@@ -157,7 +155,7 @@ int run_layer(const Layer& l, const LayerPlan& pl, const LayerScratch& m, hipStr
         Int8Args g2 = g1;
         g2.x = m.hq; g2.xs = m.hs; g2.x_rows = pl.P; g2.K = l.inter; g2.ldx = l.inter;
         g2.w = l.w2; g2.ws = l.s2; g2.N = l.H; g2.gather = false;
-        g2.dst = l.bf16 ? Out8::kSlot16 : Out8::kSlotF32; g2.out = m.y; g2.out_scales = m.ys; g2.ldo = l.H;
+        g2.dst = Out8::kSlotF32; g2.out = m.y; g2.ldo = l.H;
         if (int rc = launch_int8_tiles(g2, s)) return rc;
     } else {
         RowsArgs g1{};
@@ -180,7 +178,7 @@ int run_layer(const Layer& l, const LayerPlan& pl, const LayerScratch& m, hipStr
         g2.dst = Out8::kSlotF32; g2.out = m.y;
         if (int rc = launch_int8_rows(g2, s)) return rc;
     }
-    return launch_int8_reduce(m.y, pl.tiles && l.bf16 ? m.ys : nullptr, l.tw, l.ids, l.emap, l.n_global, l.E, l.T, l.H, l.top_k, l.out, l.bf16, s);
+    return launch_int8_reduce(m.y, l.tw, l.ids, l.emap, l.n_global, l.E, l.T, l.H, l.top_k, l.out, l.bf16, s);
 }
 struct SizeProbe {
     WorkspaceSize s;

@@ -3,7 +3,7 @@
 //
 // Bound: memory. A row is read once: W waves hold it in registers (eight values a lane and piece) between its
 // largest magnitude and its rounding. 32768 rows of 512 fp32 values: 17 us, 4.9 TB/s; the sum of 4096 tokens' eight rows of
-// 2048 in fp16 25 us, 6 TB/s.
+// 2048 48 us, 5.9 TB/s.
 #include <algorithm>
 
 #include "int8.h"
@@ -167,51 +167,37 @@ int quant_go(const QuantParams& p, bool wide, hipStream_t s) {
     return go(&quant_rows_kernel<SRC, SILU, 16, 4>, 1, 1024);
 }
 
-// Eight columns a lane; a token's slots in order, their rows requested together. SCALED: fp16 rows with a scale
-// for 32 columns; a value is scaled back before its weight, as their scale times the weight can leave fp32's range where
-// the product of all three does not.
-template <bool BF16, bool SCALED>
-__global__ void __launch_bounds__(256) int8_reduce_kernel(const void* __restrict__ y, const float* __restrict__ ys,
-                                                         const float* __restrict__ tw, const int32_t* __restrict__ ids,
-                                                         const int32_t* __restrict__ emap, int emap_len, int E, int N, int top_k,
-                                                         int64_t pieces, uint16_t* __restrict__ out) {
+// Eight columns a lane; a token's slots in order, their rows requested four at a time.
+template <bool BF16>
+__global__ void __launch_bounds__(256) int8_reduce_kernel(const float* __restrict__ y, const float* __restrict__ tw,
+                                                         const int32_t* __restrict__ ids, const int32_t* __restrict__ emap,
+                                                         int emap_len, int E, int N, int top_k, int64_t pieces,
+                                                         uint16_t* __restrict__ out) {
     const int64_t piece = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (piece >= pieces) return;
     const int per = N / 8;
     const int64_t t = piece / per;
     const int n = (int)(piece - t * per) * 8;
     float sum[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    constexpr int kAt = SCALED ? 8 : 4;        // slots read together
+    constexpr int kAt = 4;                     // slots read together
     for (int j0 = 0; j0 < top_k; j0 += kAt) {
-        u32x4 v[kAt][SCALED ? 1 : 2];
-        float w[kAt], sc[kAt];
+        v4f v[kAt][2];
+        float w[kAt];
         int e[kAt];
 #pragma unroll
         for (int i = 0; i < kAt; ++i) {
             const int64_t slot = t * top_k + min(j0 + i, top_k - 1);
             e[i] = ids[slot];
             w[i] = tw[slot];
-            if constexpr (SCALED) {
-                v[i][0] = *reinterpret_cast<const u32x4*>(reinterpret_cast<const uint16_t*>(y) + slot * N + n);
-                sc[i] = ys[slot * (N / 32) + n / 32];
-            } else {
-                v[i][0] = *reinterpret_cast<const u32x4*>(reinterpret_cast<const float*>(y) + slot * N + n);
-                v[i][1] = *reinterpret_cast<const u32x4*>(reinterpret_cast<const float*>(y) + slot * N + n + 4);
-            }
+            v[i][0] = *reinterpret_cast<const v4f*>(y + slot * N + n);
+            v[i][1] = *reinterpret_cast<const v4f*>(y + slot * N + n + 4);
         }
 #pragma unroll
         for (int i = 0; i < kAt; ++i) {
             if (emap != nullptr) e[i] = e[i] >= 0 && e[i] < emap_len ? emap[e[i]] : -1;
             if (j0 + i >= top_k || e[i] < 0 || e[i] >= E) continue;
 #pragma unroll
-            for (int r = 0; r < 8; ++r) {
-                float f;
-                if constexpr (SCALED)
-                    f = __half2float(__ushort_as_half((uint16_t)(v[i][0][r / 2] >> (r % 2 * 16)))) * sc[i];
-                else
-                    f = __uint_as_float(v[i][r / 4][r % 4]);
-                sum[r] = fmaf(w[i], f, sum[r]);
-            }
+            for (int r = 0; r < 8; ++r) sum[r] = fmaf(w[i], v[i][r / 4][r % 4], sum[r]);
         }
     }
     *reinterpret_cast<uint4*>(out + t * N + n) = make_uint4(pack16<BF16>(sum[0], sum[1]), pack16<BF16>(sum[2], sum[3]),
@@ -232,8 +218,8 @@ int launch_act_quant_int8(const void* x, Rows src, int64_t rows, int64_t K, int6
     return silu ? quant_go<Rows::kF16, true>(p, wide, s) : quant_go<Rows::kF16, false>(p, wide, s);
 }
 
-int launch_int8_reduce(const void* y, const float* y_scales, const float* tw, const int32_t* ids, const int32_t* emap,
-                       int64_t emap_len, int64_t E, int64_t T, int64_t N, int64_t top_k, void* out, bool bf16, hipStream_t s) {
+int launch_int8_reduce(const float* y, const float* tw, const int32_t* ids, const int32_t* emap, int64_t emap_len, int64_t E,
+                       int64_t T, int64_t N, int64_t top_k, void* out, bool bf16, hipStream_t s) {
     if (T == 0) return W4A8_OK;
     const int64_t pieces = T * (N / 8), blocks = (pieces + 255) / 256;
     if (!grid_fits(blocks, 256)) {
@@ -241,12 +227,11 @@ int launch_int8_reduce(const void* y, const float* y_scales, const float* tw, co
         return W4A8_ERR_INVALID;
     }
     auto go = [&](auto kernel) {
-        launch_kernel(kernel, dim3((unsigned)blocks), dim3(256), 0, s, y, y_scales, tw, ids, emap, (int)emap_len, (int)E, (int)N,
-                      (int)top_k, pieces, static_cast<uint16_t*>(out));
+        launch_kernel(kernel, dim3((unsigned)blocks), dim3(256), 0, s, y, tw, ids, emap, (int)emap_len, (int)E, (int)N, (int)top_k,
+                      pieces, static_cast<uint16_t*>(out));
         return check_launch("int8_reduce_kernel");
     };
-    if (y_scales != nullptr) return bf16 ? go(&int8_reduce_kernel<true, true>) : go(&int8_reduce_kernel<false, true>);
-    return bf16 ? go(&int8_reduce_kernel<true, false>) : go(&int8_reduce_kernel<false, false>);
+    return bf16 ? go(&int8_reduce_kernel<true>) : go(&int8_reduce_kernel<false>);
 }
 
 }  // namespace w4a8

@@ -9,8 +9,8 @@
 // before's epilogue.
 //
 // Bound: of few rows HBM (77 rows of 12288 x 4096: 13.6 us, 4 TB/s), of many the matrix cores' power (see dense_go). Of a
-// layer's 32768 slots over 256 experts (2048 x 512, rows skewed) the first product takes 170 us (537 MB of weights at
-// 3.2 TB/s, x and h beside them), the second 123 (268 MB, and 134 MB of slots' rows written).
+// layer's 32768 slots over 256 experts (2048 x 512, rows skewed) the first product takes 173 us (537 MB of weights at
+// 3.1 TB/s, x and h beside them), the second 135 (268 MB, and 268 MB of slots' rows written: 4 TB/s).
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -365,7 +365,7 @@ __global__ void __launch_bounds__(C::kThreads * C::KS, C::EU) int8_tiles_kernel(
         // chunks of 16 bytes, chunk i of row r at i ^ (r & 15) (rows of 256 bytes or more), i ^ (r / 2 & 7) (of 128) or
         // i ^ (r / 4 & 3) (of 64): sixteen lanes then write to different banks.
         // 16-bit rows of all the wave's columns, fp32 rows of a fragment's.
-        constexpr bool k2 = DST == Out8::k16 || DST == Out8::kSlot16;
+        constexpr bool k2 = DST == Out8::k16;
         constexpr int kFrags = kSilu ? FN / 2 : FN, kAt = k2 ? kFrags : 1, kSize = k2 ? 2 : 4;
         constexpr int kRowBytes = kAt * 32 * kSize, kChunks = kRowBytes / 16;
         static_assert(kChunks >= 4, "a row is 64 bytes or more");
@@ -403,28 +403,7 @@ __global__ void __launch_bounds__(C::kThreads * C::KS, C::EU) int8_tiles_kernel(
                     if constexpr (kSilu)
                         t[r] = silu_mul(v * (xs * ws_at(j, r)), (float)run[i][j + FN / 2][r] * (xs * ws_at(j + FN / 2, r)));
                     else if constexpr (DST == Out8::k16) t[r] = fmaf(v, xs * ws_at(j, r), bias_at(j, r));
-                    else if constexpr (DST == Out8::kSlot16) t[r] = v * ws_at(j, r);
                     else t[r] = v * (xs * ws_at(j, r));
-                }
-                if constexpr (DST == Out8::kSlot16) {
-                    // the largest finite value of these 32 columns to [2^14, 2^15): infinities, NaN and zeros as they are
-                    auto largest = [&](auto real) __attribute__((always_inline)) {
-                        float m = 0.f;
-#pragma unroll
-                        for (int r = 0; r < 16; ++r)
-                            m = fmaxf(m, !decltype(real)::value || fabsf(t[r]) < INFINITY ? fabsf(t[r]) : 0.f);
-                        const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(m), __float_as_uint(m), false, false);
-                        return max(both[0], both[1]) >> 23;
-                    };
-                    uint32_t eb = largest(std::false_type{});
-                    if (__ballot(eb == 255) != 0) eb = largest(std::true_type{});
-                    const uint32_t sb = eb == 0 ? 127u : eb > 15 ? eb - 14 : 1u;
-                    const float to = __uint_as_float((254u - sb) << 23);
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) t[r] *= to;
-                    const int slot = s_slot[(wt * FT + i) * 32 + c], col = col0 + j * 32;
-                    if (h == 0 && slot >= 0 && col < N)
-                        p.out_scales[(int64_t)slot * (p.ldo / 32) + col / 32] = xs * __uint_as_float(sb << 23);
                 }
                 const int chunk = ((j - j0) * 32 + 16 * h) * kSize / 16;
                 if constexpr (k2) {
@@ -453,11 +432,11 @@ __global__ void __launch_bounds__(C::kThreads * C::KS, C::EU) int8_tiles_kernel(
                 const int r = r0 + lane / kChunks, chunk = lane % kChunks;
                 const u32x4 v = *reinterpret_cast<const u32x4*>(strip + chunk_at(r, chunk));
                 const int slot = s_slot[(wt * FT + i) * 32 + r];
-                const int64_t row = DST == Out8::kSlotF32 || DST == Out8::kSlot16 ? slot : r0_now + (wt * FT + i) * 32 + r;
+                const int64_t row = DST == Out8::kSlotF32 ? slot : r0_now + (wt * FT + i) * 32 + r;
                 const int col = col0 + j0 * 32 + chunk * 16 / kSize;
                 if (slot < 0 || col >= (kSilu ? half : N)) continue;
                 if constexpr (k2) {
-                    if (DST == Out8::kSlot16 || (p.out16 && col + 8 <= N)) {
+                    if (p.out16 && col + 8 <= N) {
                         *reinterpret_cast<u32x4*>(reinterpret_cast<uint16_t*>(p.out) + row * p.ldo + col) = v;
                     } else {
                         const uint32_t w[4] = {v[0], v[1], v[2], v[3]};
@@ -518,7 +497,7 @@ using Tile256x128 = Tile<4, 2, 2, 2, 3, 1, 2>;
 using Tile256x256 = Tile<2, 4, 4, 2, 2, 1, 2>;
 // grouped: the layer's first and second product, blocks of 64 and 128 rows. The first product's waves hold gate and up
 // fragments of the same columns; the second one's steps are few, so that waves (eight, two work-groups a CU) hide its
-// prologue and stores: with four waves a layer of 4096 tokens, 256 experts of 2048 x 512, took 350 us for 335.
+// prologue and stores (with four a layer of 4096 tokens, 256 experts of 2048 x 512, takes as long, 371 us).
 using First64 = Tile<1, 4, 2, 2, 2, 1, 2>;
 using Second64 = Tile<2, 4, 1, 2, 2, 1, 4>;
 using First128 = Tile<2, 4, 2, 2, 3, 1, 2>;
@@ -568,7 +547,6 @@ int launch_int8_tiles(const Int8Args& a, hipStream_t s) {
     if (p.P == 0) return W4A8_OK;
     auto grouped = [&](auto first, auto second) -> int {
         if (a.dst == Out8::kSiluF32) return tiles_go<decltype(first), Out8::kSiluF32, true>(p, s);
-        if (a.dst == Out8::kSlot16) return tiles_go<decltype(second), Out8::kSlot16, true>(p, s);
         return tiles_go<decltype(second), Out8::kSlotF32, true>(p, s);
     };
     if (a.sorted_ids != nullptr) return a.block_m == 128 ? grouped(First128{}, Second128{}) : grouped(First64{}, Second64{});
