@@ -354,8 +354,8 @@ __global__ void __launch_bounds__(256) route_rows_kernel(RouteParams p) {
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const float s = p.sigmoid ? __builtin_amdgcn_rcpf(1.0f + exp_fast(-l[i])) : c[i] * inv;
-            // (a NaN counts for neither maximum nor key)
-            c[i] = l[i] > -INFINITY ? s + b[i] : -INFINITY;
+            // (a NaN is -inf: left as it is, the smaller of it and a group's best were that best, a second time)
+            c[i] = l[i] > -INFINITY && s + b[i] > -INFINITY ? s + b[i] : -INFINITY;
             top = fmaxf(top, i < nv ? fabsf(b[i]) < INFINITY ? fabsf(b[i]) : 0.f : 0.f);
         }
         top = row_max(top);
@@ -431,7 +431,7 @@ __global__ void __launch_bounds__(256) route_rows_kernel(RouteParams p) {
         sure = sure && (!some || (span < 1e30f && span > 1e-30f));
         const float f = some && kept ? 16777000.f / span : 0.f, o = some && kept ? 2.f : 0.f;
 #pragma unroll
-        for (int i = 0; i < NV; ++i)            // (-inf and NaN become 0)
+        for (int i = 0; i < NV; ++i)            // (-inf, and its product with 0, become 0)
             key[i] = (uint32_t)__builtin_amdgcn_fmed3f(fmaf(c[i] - lo, f, o), 0.f, 16777215.f) << 8 | (uint32_t)(255 - e0 - i);
         tol = 4u + (uint32_t)fminf(2.f * off * (16777000.f / span), 16777216.f);
     }
