@@ -165,11 +165,12 @@ __device__ __forceinline__ uint32_t quant4(float a, float b, float c, float d, c
 // border between two whole numbers (in the layer each such move costs up to a step). e^-g is the hardware's
 // 2^t, t = -g log2(e) with its rounding error put back, and 1 / (1 + e^-g) the hardware's reciprocal corrected
 // once. Below -80 e^-g may be no normal number, and u as large as fp32 numbers are: silu(g) = g e^g to 35 digits
-// there, as two factors e^(g / 2).
+// there, as two factors e^(g / 2). Past 128 silu(g) is g, and t is that of 128: g log2(e) may be past fp32's numbers.
 __device__ __forceinline__ float silu_mul(float g, float u) {
     constexpr float l2e = 1.44269504088896340736f, l2e_lo = 1.92596299112661746887e-8f;
-    const float t = -g * l2e;
-    const float lo = fmaf(-g, l2e, -t) - g * l2e_lo;
+    const float e = fminf(g, 128.f);
+    const float t = -e * l2e;
+    const float lo = fmaf(-e, l2e, -t) - e * l2e_lo;
     const float p2 = __builtin_amdgcn_exp2f(t);
     const float d = 1.0f + fmaf(p2 * 0.69314718055994530942f, lo, p2);
     float r = __builtin_amdgcn_rcpf(d);
