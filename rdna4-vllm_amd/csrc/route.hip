@@ -63,6 +63,15 @@ __device__ __forceinline__ float logit_at(const void* l, int64_t i) {
     return __half2float(__ushort_as_half(v));
 }
 
+// e^(a - b), a not above b, to about two roundings: what a - b and its product with log2(e) round off is put back.
+__device__ __forceinline__ float exp_near(float a, float b) {
+    const float x = a - b, y = x - a, off = (a - (x - y)) - (b + y);
+    const float t = x * 1.44269504088896340736f;
+    const float lo = fmaf(x, 1.44269504088896340736f, -t) + fmaf(off, 1.44269504088896340736f, x * 1.92596299112661746887e-8f);
+    const float e = __builtin_amdgcn_exp2f(t);
+    return t > -200.f ? fmaf(e * 0.69314718055994530942f, lo, e) : 0.f;
+}
+
 // What a wave compares groups by, in LDS: c in fp64, or the logit.
 template <int NV, bool BIAS>
 struct RouteScratch {
@@ -107,13 +116,12 @@ __device__ void route_token(const RouteParams& p, int64_t t, int lane, RouteScra
             key[i] = c[i] > -INFINITY ? order_key((float)c[i]) : 0u;
         }
     } else {
-        float s = 0.f;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             key[i] = l[i] > -INFINITY ? order_key(l[i]) : 0u;
-            s += expf(l[i] - m);
+            sum += (double)exp_near(l[i], m);
         }
-        sum = (double)wave_sum(s);
+        sum = wave_sum64(sum);
     }
 
     // ---- groups: lane g scores group g, and its rank says whether it stays ----
@@ -253,19 +261,17 @@ __device__ __forceinline__ void join8(uint32_t (&v)[8]) {
     merge8(v);
 }
 __device__ __forceinline__ float row_max(float v) { return lane_allreduce<4>(v, MaxOp{}); }
-__device__ __forceinline__ float row_sum(float v) { return lane_allreduce<4>(v, SumOp{}); }
+template <int S>
+__device__ __forceinline__ double row_add64(double v) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    return v + __builtin_bit_cast(double, (uint64_t)dpp_step<S>((uint32_t)(b >> 32)) << 32 | dpp_step<S>((uint32_t)b));
+}
+__device__ __forceinline__ double row_sum64(double v) { return row_add64<3>(row_add64<2>(row_add64<1>(row_add64<0>(v)))); }
 struct AddU {
     __device__ float operator()(float a, float b) const { return __uint_as_float(__float_as_uint(a) + __float_as_uint(b)); }
 };
 __device__ __forceinline__ uint32_t row_count(uint32_t v) { return __float_as_uint(lane_allreduce<4>(__uint_as_float(v), AddU{})); }
 __device__ __forceinline__ float exp_fast(float x) { return __builtin_amdgcn_exp2f(x * 1.44269504088896340736f); }
-// e^x to about two roundings: the rounding error of x log2(e) is put back.
-__device__ __forceinline__ float exp_near(float x) {
-    const float t = x * 1.44269504088896340736f;
-    const float lo = fmaf(x, 1.44269504088896340736f, -t) + x * 1.92596299112661746887e-8f;
-    const float e = __builtin_amdgcn_exp2f(t);
-    return t > -200.f ? fmaf(e * 0.69314718055994530942f, lo, e) : 0.f;
-}
 template <int R>
 __device__ __forceinline__ int larger_in_row(uint32_t v) {       // lanes of the row of sixteen that hold more than v
     if constexpr (R == 0) return 0;
@@ -327,18 +333,19 @@ __global__ void __launch_bounds__(256) route_rows_kernel(RouteParams p) {
     if (m == -INFINITY) m = 0.f;
 
     // ---- scores: c, off by no more than `off` ----
-    float c[NV], sum = 1.f, off = 0.f, top = 0.f;                // top: of the biases' magnitudes
+    float c[NV], off = 0.f, top = 0.f;                           // top: of the biases' magnitudes
+    double sum = 1.0;
     if (!p.sigmoid && (BIAS || !p.renorm)) {
-        sum = 0.f;
+        sum = 0.0;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            c[i] = exp_fast(l[i] - m);
-            sum += c[i];
+            c[i] = exp_near(l[i], m);
+            sum += (double)c[i];
         }
-        sum = row_sum(sum);
+        sum = row_sum64(sum);
     }
     if constexpr (BIAS) {
-        const float inv = 1.0f / sum;
+        const float inv = 1.0f / (float)sum;
         float b[NV];
         if (nv % 4 == 0 && p.bias_vec) {
 #pragma unroll
@@ -355,14 +362,13 @@ __global__ void __launch_bounds__(256) route_rows_kernel(RouteParams p) {
         for (int i = 0; i < NV; ++i) {
             const float s = p.sigmoid ? __builtin_amdgcn_rcpf(1.0f + exp_fast(-l[i])) : c[i] * inv;
             // (a NaN is -inf: left as it is, the smaller of it and a group's best were that best, a second time)
-            c[i] = l[i] > -INFINITY && s + b[i] > -INFINITY ? s + b[i] : -INFINITY;
+            c[i] = fmaxf(l[i] > -INFINITY ? s + b[i] : -INFINITY, -INFINITY);
             top = fmaxf(top, i < nv ? fabsf(b[i]) < INFINITY ? fabsf(b[i]) : 0.f : 0.f);
         }
         top = row_max(top);
-        // In units of 2^-24: e^x is off by (2 |x| + 2) e^x, a softmax's sum by as much of each term (2 |x| e^x adds up to
-        // no more than 2 ln 256 of it) and 8 of its tree, the quotient by 3 more: below 32 for p up to 1; a sigmoid by
-        // less than 8. The sum with b by half a step.
-        off = ((p.sigmoid ? 8.f : 32.f) + 1.f + top) * 0x1p-24f;
+        // In units of 2^-24: a softmax's e^x and its sum are off by 3 each, the inverse and the product by 4 more: below 16
+        // for p up to 1; a sigmoid, whose e^x is off by (2 |x| + 2) e^x, by less than 8. The sum with b by half a step.
+        off = ((p.sigmoid ? 8.f : 16.f) + 1.f + top) * 0x1p-24f;
     } else {
 #pragma unroll
         for (int i = 0; i < NV; ++i) c[i] = l[i];
@@ -486,14 +492,14 @@ __global__ void __launch_bounds__(256) route_rows_kernel(RouteParams p) {
     }
     mine = mine > 255u ? mine : 0u;
 
-    // ---- weights ----
+    // ---- weights, in fp64 as route_token's ----
     const int e = 255 - (int)(mine & 255u);
-    float w = 0.f, x = -INFINITY;
+    float x = -INFINITY;
+    double w = 0.0;
     if (mine != 0u) {
         x = fminf(logit_at<SRC>(p.logits, at + e), 3.402823466e38f);
-        // (of a sigmoid the smaller of e^x and e^-x, which is a number)
-        const float ex = exp_near(p.sigmoid ? -fabsf(x) : x - m);
-        w = !p.sigmoid ? ex : x < 0.f ? ex / (1.0f + ex) : 1.0f / (1.0f + ex);
+        w = exp(p.sigmoid ? -(double)x : (double)x - (double)m);
+        if (p.sigmoid) w = 1.0 / (1.0 + w);
     }
     int place = sub;
     if (!EXACT && __ballot(doubt) != 0) {
@@ -501,7 +507,7 @@ __global__ void __launch_bounds__(256) route_rows_kernel(RouteParams p) {
         // needs its sum in fp64 too.
         if (BIAS && !p.sigmoid) sure = sure && !doubt;
         double d = -INFINITY;
-        if (mine != 0u) d = !BIAS ? (double)x : 1.0 / (1.0 + exp(-(double)x)) + (double)p.bias[e];
+        if (mine != 0u) d = !BIAS ? (double)x : w + (double)p.bias[e];
         int rank = 0;
         for (int j = 0; j <= kTop; ++j) {
             const double other = __shfl(d, row * 16 + j);
@@ -512,21 +518,18 @@ __global__ void __launch_bounds__(256) route_rows_kernel(RouteParams p) {
             place = mine != 0u ? rank : sub;
             if (place >= p.top_k) {
                 mine = 0u;
-                w = 0.f;
+                w = 0.0;
             }
         }
     }
     if (p.renorm) {
-        const float total = row_sum(w);
-        sure = sure && (total > 1e-30f || row_count(mine != 0u ? 1u : 0u) == 0u);
-        w = total > 0.f ? w / total : 0.f;
+        const double total = row_sum64(w);
+        w = total > 0.0 ? w / total : 0.0;
     } else if (!p.sigmoid && mine != 0u) {
         w /= sum;
     }
-    // (weights near fp32's least numbers: by route_token too)
-    sure = sure && row_count(mine != 0u && !(w > 1e-30f) ? 1u : 0u) == 0u;
     if (sure && t0 + row < p.T && place < p.top_k) {
-        p.tw[t * p.top_k + place] = w * p.scale;
+        p.tw[t * p.top_k + place] = (float)(w * (double)p.scale);
         p.ids[t * p.top_k + place] = mine != 0u ? e : -1;
     }
     const uint64_t again = __ballot(!sure);
