@@ -332,8 +332,8 @@ __global__ void __launch_bounds__(256) route_rows_kernel(RouteParams p) {
     m = row_max(m);
     if (m == -INFINITY) m = 0.f;
 
-    // ---- scores: c, off by no more than `off` ----
-    float c[NV], off = 0.f, top = 0.f;                           // top: of the biases' magnitudes
+    // ---- scores ----
+    float c[NV];
     double sum = 1.0;
     if (!p.sigmoid && (BIAS || !p.renorm)) {
         sum = 0.0;
@@ -363,20 +363,21 @@ __global__ void __launch_bounds__(256) route_rows_kernel(RouteParams p) {
             const float s = p.sigmoid ? __builtin_amdgcn_rcpf(1.0f + exp_fast(-l[i])) : c[i] * inv;
             // (a NaN is -inf: left as it is, the smaller of it and a group's best were that best, a second time)
             c[i] = fmaxf(l[i] > -INFINITY ? s + b[i] : -INFINITY, -INFINITY);
-            top = fmaxf(top, i < nv ? fabsf(b[i]) < INFINITY ? fabsf(b[i]) : 0.f : 0.f);
         }
-        top = row_max(top);
-        // In units of 2^-24: a softmax's e^x and its sum are off by 3 each, the inverse and the product by 4 more: below 16
-        // for p up to 1; a sigmoid, whose e^x is off by (2 |x| + 2) e^x, by less than 8. The sum with b by half a step.
-        off = ((p.sigmoid ? 8.f : 16.f) + 1.f + top) * 0x1p-24f;
     } else {
 #pragma unroll
         for (int i = 0; i < NV; ++i) c[i] = l[i];
     }
 
+    // With a bias c is off by no more than (slack + |c|) 2^-24. In units of 2^-24: a softmax's e^x and its sum are off by 3
+    // each, the inverse and the product by 4 more: below 16 for p up to 1; a sigmoid, whose e^x is off by (2 |x| + 2) e^x, by
+    // less than 8; the sum with b by half a step.
+    const float slack = !BIAS ? 0.f : p.sigmoid ? 9.f : 17.f;
+
     // ---- groups: lanes of a group hold its score, and how many lanes hold a larger one ----
     bool sure = true;
     bool kept = true;
+    float most = -INFINITY;                     // of the lane's scores
     if (p.groups > 1) {
         float first = -INFINITY, second = -INFINITY;
 #pragma unroll
@@ -384,6 +385,7 @@ __global__ void __launch_bounds__(256) route_rows_kernel(RouteParams p) {
             second = fmaxf(second, fminf(first, c[i]));
             first = fmaxf(first, c[i]);
         }
+        most = first;
         auto join = [&](auto step) __attribute__((always_inline)) {
             constexpr int S = decltype(step)::value;
             const float f = __uint_as_float(dpp_step<S>(__float_as_uint(first)));
@@ -396,7 +398,8 @@ __global__ void __launch_bounds__(256) route_rows_kernel(RouteParams p) {
         if (lanes > 2) join(std::integral_constant<int, 1>{});
         if (lanes > 4) join(std::integral_constant<int, 2>{});
         if (lanes > 8) join(std::integral_constant<int, 3>{});
-        const float score = first + (BIAS && second > -INFINITY ? second : 0.f);
+        const bool two = BIAS && second > -INFINITY;
+        const float score = first + (two ? second : 0.f);
         uint32_t group_key = order_key(score);
         if constexpr (EXACT) {                  // with the group's number: no two are equal
             uint32_t top = 0;
@@ -412,9 +415,15 @@ __global__ void __launch_bounds__(256) route_rows_kernel(RouteParams p) {
         // (equal groups at the border are kept together)
         sure = row_count(kept ? 1u : 0u) == (uint32_t)(p.top_groups * lanes);
         if constexpr (BIAS) {
-            const float least = -row_max(kept ? -score : -INFINITY), out = row_max(kept ? -INFINITY : score);
-            sure = sure && (out == -INFINITY || least - out > 4.f * off + fabsf(least) * 0x1p-22f);
+            // two scores and their sum's rounding, and that of what follows
+            const float size = fabsf(first) + (two ? fabsf(second) : 0.f);
+            const float off = size < INFINITY ? (2.f * slack + 4.f * size) * 0x1p-24f : 0.f;
+            const float least = -row_max(kept ? off - score : -INFINITY), out = row_max(kept ? -INFINITY : score + off);
+            sure = sure && (out == -INFINITY || least > out);
         }
+    } else {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) most = fmaxf(most, c[i]);
     }
 
     // ---- keys ----
@@ -423,21 +432,34 @@ __global__ void __launch_bounds__(256) route_rows_kernel(RouteParams p) {
 #pragma unroll
         for (int i = 0; i < NV; ++i) key[i] = kept ? bits[i] << 8 | (uint32_t)(255 - e0 - i) : 0u;
     } else {
-        // Scores with a bias lie in [-top, 1 + top], logits are taken between the row's largest and smallest. The mapping
-        // grows with c, so that only what c is off by, and the cut to whole numbers, can hide an order.
-        float lo = -top, span = 1.f + 2.f * top;
-        if constexpr (!BIAS) {
-            lo = INFINITY;
+        // Scores are taken between the row's largest, hi, and a little below the top_k-th largest of its lanes' largest,
+        // which no pick lies below: experts masked by a low number, or far above the others, then leave the others their
+        // bits (taken between the row's largest and smallest, tokens with such a mask all went through route_token: 85 us
+        // for 23, 65536 tokens of 256 experts). Few lanes, or equal ones: down to the smallest score that is no such mask.
+        // The mapping grows with c, so that only what c is off by, and the cut to whole numbers, can hide an order. What c
+        // is off by is that of numbers up to three times the range's; of a c far below it is less than its distance.
+        if (!kept) most = -INFINITY;
+        const float hi = row_max(most);
+        float lo = -row_max(larger_in_row<15>(order_key(most)) < max(p.top_k, 2) ? -most : -INFINITY);
+        float off = BIAS ? (slack + 3.f * fmaxf(fabsf(lo), fabsf(hi))) * 0x1p-24f : 0.f;
+        const bool few = !(lo > -1e30f) || (!BIAS && lo == hi);
+        lo -= fmaxf(0.125f * (hi - lo), 16.f * off);
+        if (__ballot(few) != 0) {
+            float least = INFINITY;
 #pragma unroll
-            for (int i = 0; i < NV; ++i) lo = fminf(lo, c[i] > -INFINITY ? c[i] : INFINITY);
-            lo = -row_max(-lo);
-            span = m - lo;
+            for (int i = 0; i < NV; ++i) least = fminf(least, kept && c[i] > -1e30f ? c[i] : INFINITY);
+            least = -row_max(-least);
+            if (few) {
+                lo = least;
+                off = BIAS ? (slack + 3.f * fmaxf(fabsf(lo), fabsf(hi))) * 0x1p-24f : 0.f;
+            }
         }
-        const bool some = lo < INFINITY;
-        sure = sure && (!some || (span < 1e30f && span > 1e-30f));
+        const float span = hi - lo;
+        const bool some = span < 1e30f && span > 1e-30f;
+        sure = sure && (some || hi == -INFINITY);
         const float f = some && kept ? 16777000.f / span : 0.f, o = some && kept ? 2.f : 0.f;
 #pragma unroll
-        for (int i = 0; i < NV; ++i)            // (-inf, and its product with 0, become 0)
+        for (int i = 0; i < NV; ++i)            // (-inf, and its product with 0, become 0, as what lies below the range)
             key[i] = (uint32_t)__builtin_amdgcn_fmed3f(fmaf(c[i] - lo, f, o), 0.f, 16777215.f) << 8 | (uint32_t)(255 - e0 - i);
         tol = 4u + (uint32_t)fminf(2.f * off * (16777000.f / span), 16777216.f);
     }
@@ -484,6 +506,15 @@ __global__ void __launch_bounds__(256) route_rows_kernel(RouteParams p) {
         if (near > (uint32_t)p.top_k && last > 255u) {
             doubt = true;
             sure = sure && near == (uint32_t)p.top_k + 1;
+        }
+        // next to the range's end, or no pick: what lies below it may be one
+        const bool low = (last >> 8) <= tol;
+        if (__ballot(low) != 0) {
+            bool cut = false;
+#pragma unroll
+            for (int i = 0; i < NV; ++i) cut = cut || (kept && c[i] > -INFINITY && key[i] < 256u);
+            cut = row_count(cut ? 1u : 0u) != 0u;
+            sure = sure && !(low && cut);
         }
         if (__ballot(doubt) != 0) {
             next = __float_as_uint(lane_allreduce<4>(__uint_as_float(next), UMax{}));
