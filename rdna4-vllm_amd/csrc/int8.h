@@ -30,7 +30,7 @@ enum class Out8 : int {
 // What the streaming kernels read their rows from.
 enum class Src8 : int {
     kI8 = 0,        // int8 rows with their scales
-    kF16 = 1,       // fp16 / bf16 / fp32 rows, quantised in registers
+    kF16 = 1,       // fp16, bf16 or fp32 rows, which the kernel quantises into LDS
     kBf16 = 2,
     kF32 = 3,
 };

@@ -465,7 +465,9 @@ __global__ void __launch_bounds__(64 * KS * CG, KS * CG <= 4 ? 2 : 1) int8_rows_
 }
 
 // Any K, int8 rows: KS waves take the steps of K in turn (what they read at one time is contiguous along K).
-constexpr int kRing = 3;          // steps of a wave in flight: two work-groups a CU have registers (four, with one: 14.4 us for 13.6)
+// Steps of a wave in flight. 8 tokens, 2 picks, half of them among 8 experts of 8192 x 2048: 66 us (two: 61, four: 73); 40
+// tokens, 8 picks, 64 experts of 7168 x 2048: 684 us, 4.1 TB/s (632, 737).
+constexpr int kRing = 3;
 template <int FN, int KS, Out8 DST>
 __global__ void __launch_bounds__(64 * KS) int8_stream_kernel(RowsParams p) {
     constexpr bool kSilu = DST == Out8::kSiluF32;
@@ -708,8 +710,8 @@ int rows_go(const RowsParams& p, hipStream_t s) {
 }
 
 // The wave split by the number of steps: a wave holds the rows' values of up to four of them, up to eight waves share K.
-// (Sixteen waves of one step each less, or two column fragments, of longer K: 15.7 and 19.8 us for 13.5, 8 rows of 4096 x
-// 12288.)
+// (Longer K by sixteen waves, or by twice the column fragments: 972 and 719 us for 684, 40 tokens, 8 picks, 64 experts of
+// 7168 x 2048.)
 template <Src8 SRC, Out8 DST>
 int rows_any(const RowsParams& p, hipStream_t s) {
     const int G = (p.K + kStep - 1) / kStep;
@@ -756,7 +758,8 @@ int launch_int8_rows(const RowsArgs& a, hipStream_t s) {
         set_error("int8 product: too many slots for the streaming kernels");
         return W4A8_ERR_INVALID;
     }
-    if (a.dst == Out8::kSlotF32) return a.src == Src8::kI8 ? rows_any<Src8::kI8, Out8::kSlotF32>(p, s) : rows_any<Src8::kF32, Out8::kSlotF32>(p, s);
+    // (h in int8 is of rows that are too long to be quantised in the kernel)
+    if (a.dst == Out8::kSlotF32) return a.src == Src8::kI8 ? stream_go<1, 8, Out8::kSlotF32>(p, s) : rows_any<Src8::kF32, Out8::kSlotF32>(p, s);
     auto from = [&](auto dst) -> int {
         constexpr Out8 DST = decltype(dst)::value;
         switch (a.src) {

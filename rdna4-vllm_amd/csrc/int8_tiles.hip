@@ -60,7 +60,7 @@ struct Tile {
     static constexpr int PX = BT * 8 / kThreads, PW = BN * 8 / kThreads;   // 16-byte pieces a thread
     static constexpr int kLoads = PX + PW;                       // of a wave and step
     static_assert(PX * kThreads == BT * 8 && PW * kThreads == BN * 8, "pieces divide");
-    static_assert(S >= 2 && S <= 6 && (!DEEP || S % 2 == 0), "two to six slots, for two sets of fragments in turn");
+    static_assert(S >= 2 && S <= 4 && (!DEEP || S % 2 == 0), "two to four slots, for two sets of fragments in turn");
     static_assert(kLoads * (S - 1) < 64, "loads in flight can be counted");
 };
 
@@ -74,10 +74,8 @@ __global__ void __launch_bounds__(C::kThreads * C::KS, C::EU) int8_tiles_kernel(
     __shared__ __attribute__((aligned(1024))) int8_t slots1[KS * C::kSlot];
     __shared__ __attribute__((aligned(1024))) int8_t slots2[S > 2 ? KS * C::kSlot : 16];
     __shared__ __attribute__((aligned(1024))) int8_t slots3[S > 3 ? KS * C::kSlot : 16];
-    __shared__ __attribute__((aligned(1024))) int8_t slots4[S > 4 ? KS * C::kSlot : 16];
-    __shared__ __attribute__((aligned(1024))) int8_t slots5[S > 5 ? KS * C::kSlot : 16];
     // Tables for the epilogue, in the last slot between a tile's last step and the next one's loads into it.
-    int8_t* const aside = S == 2 ? slots1 : S == 3 ? slots2 : S == 4 ? slots3 : S == 5 ? slots4 : slots5;
+    int8_t* const aside = S == 2 ? slots1 : S == 3 ? slots2 : slots3;
     float *const s_xs = reinterpret_cast<float*>(aside), *const s_ws = s_xs + BT, *const s_bias = s_ws + BN;
     int* const s_slot = reinterpret_cast<int*>(s_bias + BN);
 
@@ -100,7 +98,7 @@ __global__ void __launch_bounds__(C::kThreads * C::KS, C::EU) int8_tiles_kernel(
     const int G1 = (G + KS - 1) / KS, g_first = part * G1;       // steps of a part, the first of them
     auto slot_of = [&](auto i) __attribute__((always_inline)) {      // slot i % S
         constexpr int n = decltype(i)::value % S;
-        int8_t* const all = n == 0 ? slots0 : n == 1 ? slots1 : n == 2 ? slots2 : n == 3 ? slots3 : n == 4 ? slots4 : slots5;
+        int8_t* const all = n == 0 ? slots0 : n == 1 ? slots1 : n == 2 ? slots2 : slots3;
         return all + part * C::kSlot;
     };
 
@@ -279,8 +277,6 @@ __global__ void __launch_bounds__(C::kThreads * C::KS, C::EU) int8_tiles_kernel(
         f(std::integral_constant<int, 1>{});
         if constexpr (S > 2) f(std::integral_constant<int, 2>{});
         if constexpr (S > 3) f(std::integral_constant<int, 3>{});
-        if constexpr (S > 4) f(std::integral_constant<int, 4>{});
-        if constexpr (S > 5) f(std::integral_constant<int, 5>{});
     };
     each_slot([&](auto i) __attribute__((always_inline)) { issue(slot_of(i), decltype(i)::value, 0, 1); });
     for (;;) {
