@@ -122,6 +122,13 @@ def int8_gemm(x: torch.Tensor, x_scales: torch.Tensor | None, w: torch.Tensor, w
     return out
 
 
+def _ids32(ids):
+    """Expert ids in 32 bits. Numbers past those name no expert, whatever their low words are."""
+    if ids.dtype == torch.int64:
+        ids = ids.clamp(-1, (1 << 31) - 1)
+    return ids.to(torch.int32).contiguous()
+
+
 def moe_int8_apply(x: torch.Tensor, w13: torch.Tensor, w2: torch.Tensor, w13_scales: torch.Tensor,
                    w2_scales: torch.Tensor, topk_weights: torch.Tensor, topk_ids: torch.Tensor,
                    x_scales: torch.Tensor | None = None, expert_map: torch.Tensor | None = None,
@@ -152,7 +159,7 @@ def moe_int8_apply(x: torch.Tensor, w13: torch.Tensor, w2: torch.Tensor, w13_sca
     if expert_map is not None:
         if expert_map.dim() != 1:
             _fail("expert_map must be 1-d (global_num_experts,)")
-        emap = expert_map.to(device=dev, dtype=torch.int32).contiguous()
+        emap = _ids32(expert_map.to(device=dev))
     n_global = E if emap is None else emap.numel()
     if global_num_experts is not None and int(global_num_experts) != n_global:
         _fail(f"global_num_experts={global_num_experts} differs from the expert count {n_global}"
@@ -163,7 +170,7 @@ def moe_int8_apply(x: torch.Tensor, w13: torch.Tensor, w2: torch.Tensor, w13_sca
     if not x.is_contiguous():
         x = x.contiguous()
     tw = topk_weights.to(torch.float32).contiguous()
-    ids = topk_ids.to(torch.int32).contiguous()
+    ids = _ids32(topk_ids)
     out = torch.empty((T, H), dtype=dt, device=dev)
     nbytes = lib.w4a8_moe_int8_workspace_size(T, H, inter, E, top_k)
     work = _workspace(nbytes, dev)
