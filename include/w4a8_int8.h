@@ -8,7 +8,7 @@
  *
  * Rows are int8 with one fp32 scale each, weights (N, K) or (E, N, K) int8 with one fp32 scale per output channel:
  *   out[m, n] = xs[m] * ws[n] * sum_k x[m, k] w[n, k],
- * the sum in whole numbers, the rest in fp32. Quantisation: a = max(absmax, 127 * 2^-100), q = the whole number nearest
+ * the sum in whole numbers, the rest in fp32 (xs * ws first). Quantisation: a = max(absmax, 127 * 2^-100), q = the whole number nearest
  * to 127 v / a (ties to even), scale = a / 127; a row that holds an infinity or a NaN gets the scale NaN. No reference
  * counterpart (the reference serves int4 and E2M1 weights).
  */
@@ -45,7 +45,8 @@ W4A8_API int w4a8_int8_gemm(const void* x, int x_dtype, const float* x_scales, i
 /* The gated expert layer: out (T, H) = sum over a token's slots of topk_weights * (silu(gate) * up, quantised) times w2
  * transposed. x as above, rows contiguous; w13 (E, 2 inter, H) = [gate | up], w2 (E, H, inter); H and inter multiples of
  * 64. topk_ids (T, top_k) are global expert ids; with expert_map (num_global_experts entries, -1 = not local) they are
- * mapped to the E local experts. Slots without one contribute nothing. */
+ * mapped to the E local experts. Slots without one contribute nothing. The slots' rows are summed in fp32, in the slots'
+ * order: a token's output has the same bits in any batch. */
 W4A8_API size_t w4a8_moe_int8_workspace_size(int64_t T, int64_t H, int64_t inter, int64_t E, int64_t top_k);
 W4A8_API int w4a8_moe_int8_apply(const void* x, int x_dtype, const float* x_scales, int64_t T, int64_t H, int64_t inter,
                                  int64_t E, int64_t top_k, const int8_t* w13, const float* w13_scales, const int8_t* w2,

@@ -58,8 +58,8 @@ def expert(q, xs, w13, s13, w2, s2):
 
 
 def layer(q, xs, w13, s13, w2, s2, tw, ids, expert_map=None, rows16=False):
-    """(out, how far fp32 arithmetic may be off); ids without a local expert contribute nothing. rows16: each slot's
-    row is rounded to fp16 before the sum, times a power of two that puts the largest of 32 columns into [2^14, 2^15):
+    """(out, how far fp32 arithmetic may be off); ids without a local expert contribute nothing. rows16: for slots'
+    rows that are rounded to fp16 before the sum (no schedule of the layer does so), times a power of two that puts the largest of 32 columns into [2^14, 2^15):
     off by 2^-11 of a value, and by 2^-25 (half of fp16's least step) of 2^-14 of that largest one."""
     T, k = ids.shape
     out, tol = np.zeros((T, w2.shape[1])), np.zeros((T, w2.shape[1]))

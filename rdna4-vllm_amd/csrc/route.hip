@@ -10,8 +10,9 @@
 // one, c is formed in fp64 (in fp32 two experts' c may round to one number), compared rounded to fp32 (which keeps the
 // order) and, where that is equal, by what was rounded off.
 //
-// Bound: for many tokens the vector units: 16384 tokens of 256 experts, 8 picks in 4 of 8 groups, sigmoid with a bias, take
-// 13.1 us with the call (one token a wave: 39), where their logits' bytes take 4; for few the launch, 4.5 us.
+// Bound: for many tokens the vector units (busy 0.79 of the time): 16384 tokens of 256 experts, 8 picks in 4 of 8 groups,
+// sigmoid with a bias, take 11.5 to 14.0 us with the call (one token a wave: 39), where their logits' bytes take 4; for few
+// the launch, 4 us, and with a bias fp64's latency, 6.
 #include <type_traits>
 
 #include "w4a8_common.h"
@@ -228,8 +229,9 @@ __global__ void __launch_bounds__(256) route_topk_kernel(RouteParams p) {
 // is its score in 24 bits over 255 - expert, so that one unsigned maximum finds score and expert: of 16-bit logits
 // without a bias the logit's own bits in their order (exact); else c in fp32, as a part of its range. Picks whose keys lie
 // nearer to each other, or to one that was not picked, than all roundings together may be off are put in order by their c
-// in fp64 (about one token in 2000); where groups, several others or a softmax's sum are in doubt, the whole wave takes the
-// token again by route_token
+// in fp64 (about one token in 1500, by sigmoids with a bias); where groups, several others or a softmax's sum are in doubt
+// (with a bias one token in 400 to 700), the whole wave takes the token again by route_token. Weights are formed in fp64 by
+// both: in fp32 a token had other last bits by the one than by the other (65536 tokens, sigmoid, bias: 36.5 us for 35.4).
 constexpr int kTop = 8;
 
 __device__ __forceinline__ void order2(uint32_t& a, uint32_t& b) {

@@ -95,7 +95,8 @@ def int8_gemm(x: torch.Tensor, x_scales: torch.Tensor | None, w: torch.Tensor, w
     """Dense layer x (M, K) times w (N, K) transposed, with scales of rows and channels, -> (M, N).
 
     x is int8 with x_scales (M,) or (M, 1), or fp16 / bf16 with ``x_scales=None``: rows that the call quantises as
-    ``act_quant_int8`` does. The sum is exact; scales and bias (N,) (fp32 or out_dtype) are applied in fp32.
+    ``act_quant_int8`` does. The sum is exact; scales and bias (N,) (fp32 or out_dtype) are applied in fp32 (the product
+    of a row's and a channel's scale is formed first, and has to be a number of its range).
     out_dtype: fp16 or bf16 (default: x's, bf16 for int8 x). K must be a multiple of 16, up to 131071."""
     xs = _check_rows(x, x_scales)
     M, K = x.shape
@@ -139,7 +140,8 @@ def moe_int8_apply(x: torch.Tensor, w13: torch.Tensor, w2: torch.Tensor, w13_sca
     int8 with scales (E, 2 inter) and (E, H); H and inter multiples of 64. Between the products h = silu(gate) * up
     stays fp32 until each slot's row is quantised. topk_ids (T, top_k) hold global expert ids; with expert_map
     (global_num_experts entries, -1 = not local) they are mapped to the E local experts. Ids that name no local
-    expert (-1 among them) contribute nothing. out_dtype: x's, bf16 for int8 x."""
+    expert (-1 among them) contribute nothing. The slots' rows are summed in fp32, in the slots' order: a token's
+    output has the same bits in any batch. out_dtype: x's, bf16 for int8 x."""
     xs = _check_rows(x, x_scales)
     T, H = x.shape
     if w13.dim() != 3 or w2.dim() != 3 or w13.shape[1] % 2 != 0:
