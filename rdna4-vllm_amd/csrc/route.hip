@@ -12,7 +12,7 @@
 //
 // Bound: for many tokens the vector units (busy 0.79 of the time): 16384 tokens of 256 experts, 8 picks in 4 of 8 groups,
 // sigmoid with a bias, take 11.5 to 14.0 us with the call (one token a wave: 39), where their logits' bytes take 4; for few
-// the launch, 4 us, and with a bias fp64's latency, 6.
+// the launch and the steps' latency, 4 to 6 us.
 #include <type_traits>
 
 #include "w4a8_common.h"
@@ -437,7 +437,7 @@ __global__ void __launch_bounds__(256) route_rows_kernel(RouteParams p) {
         // Scores are taken between the row's largest, hi, and a little below the top_k-th largest of its lanes' largest,
         // which no pick lies below: experts masked by a low number, or far above the others, then leave the others their
         // bits (taken between the row's largest and smallest, tokens with such a mask all went through route_token: 85 us
-        // for 23, 65536 tokens of 256 experts). Few lanes, or equal ones: down to the smallest score that is no such mask.
+        // for 24, 65536 tokens of 256 experts). Few lanes, or equal ones: down to the smallest score that is no such mask.
         // The mapping grows with c, so that only what c is off by, and the cut to whole numbers, can hide an order. What c
         // is off by is that of numbers up to three times the range's; of a c far below it is less than its distance.
         if (!kept) most = -INFINITY;
